@@ -28,3 +28,4 @@ c10::optional<Tensor> linear_swiglu(const Tensor& x, const Tensor& w, bool few, 
 Tensor gemv(const Tensor& x, const Tensor& w, const c10::optional<Tensor>& residual);
 
 void bind_native_autograd(pybind11::module_& m);
+void bind_paged(pybind11::module_& m);

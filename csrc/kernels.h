@@ -202,4 +202,39 @@ void flash_attn_bwd(const void* go, const void* q, const void* k, const void* v,
                     int Hkv, int S_pad, const long* gs, const long* qs, const long* ks, const long* vs, const long* os,
                     const long* dqs, const long* dks, const long* dvs, float scale, bool causal, cudaStream_t st);
 
+// ---- key/value cache in pages (paged.cu)
+// Attention of W new tokens per sequence over pages.  Rows: query row r of a (sequence, key/value head) is token r / G, head r % G of the group.
+struct PagedAttn {
+  const void *q, *k, *v;
+  void* out;
+  const int* table;                  // [B, cols] page of keys [i * ps, (i + 1) * ps); entries outside [0, pages) are holes: nobody sees their keys
+  const int* shared_pages;           // pages of keys [0, shared) of every sequence
+  const long* positions;             // [B] index of a row's first new token; negative: an idle row
+  const long* lens;                  // [B] new tokens of a row, or null: W
+  float *part_o, *part_ml;           // parts of pairs that several blocks walk: [slot][rows of a block][D], [slot][rows](maximum, sum)
+  float *pre_o, *pre_ml;             // parts over the shared pages: [split][Hkv][pre_rows][D]
+  int B, W, G, Hkv, cols, ps, pages, shared;      // shared: keys in shared pages
+  int row_blocks;                    // of the rows of one (sequence, key/value head)
+  int pre_splits, pre_rows;
+  long q_sb, q_sw, q_sh, o_sb, o_sw, o_sh, table_sb;
+  long k_sp, k_sr, k_sh, v_sp, v_sr, v_sh;        // strides of pages, rows in a page, heads
+  float scale_log2;
+};
+
+// How a launch is dealt out; what it leaves in workspaces follows from it
+struct PagedPlan {
+  int row_tiles;                     // blocks of eight query rows that one walk over the keys serves
+  int grid, pre_splits, pre_rows;
+};
+PagedPlan paged_plan(int B, int W, int G, int Hkv, int shared);
+void paged_attention(PagedAttn p, const PagedPlan& plan, int D, int dt, cudaStream_t st);
+// strides s: (b, w, h) of q, k, v; cs: (page, row, head) of the caches; q_out: heads and columns contiguous
+void paged_append(const void* q, const void* k, const void* v, const long* positions, const long* lens, const float* cos_t, const float* sin_t,
+                  void* q_out, void* kc, void* vc, const int* table, int B, int W, int H, int Hkv, int D, int rows, int cols, int ps, int pages,
+                  long table_sb, const long (*s)[3], long o_sb, long o_sw, const long (*cs)[3], int dt, cudaStream_t st);
+
+// ---- drafted tokens against the target's probabilities (verify.cu); strides of rows in elements, dt of both sides
+void verify_drafts(const long* tokens, const void* draft, const void* target, const float* accept, const float* sample, long* out, long* accepted,
+                   int B, int K, int V, const long* draft_s, const long* target_s, int dt, cudaStream_t st);
+
 }  // namespace nxd
