@@ -203,7 +203,7 @@ void flash_attn_bwd(const void* go, const void* q, const void* k, const void* v,
                     const long* dqs, const long* dks, const long* dvs, float scale, bool causal, cudaStream_t st);
 
 // ---- key/value cache in pages (paged.cu)
-// Attention of W new tokens per sequence over pages.  Rows: query row r of a (sequence, key/value head) is token r / G, head r % G of the group.
+// Attention of W new tokens per sequence over pages.  Query row r of a (sequence, key/value head) is token r / G, head r % G of the group.
 struct PagedAttn {
   const void *q, *k, *v;
   void* out;
@@ -211,23 +211,25 @@ struct PagedAttn {
   const int* shared_pages;           // pages of keys [0, shared) of every sequence
   const long* positions;             // [B] index of a row's first new token; negative: an idle row
   const long* lens;                  // [B] new tokens of a row, or null: W
-  float *part_o, *part_ml;           // parts of pairs that several blocks walk: [slot][rows of a block][D], [slot][rows](maximum, sum)
-  float *pre_o, *pre_ml;             // parts over the shared pages: [split][Hkv][pre_rows][D]
+  float *part_o, *part_ml;           // parts of pairs (paged.cuh): [slot][tile_rows][D] sums, [slot][tile_rows] (maximum, sum of weights)
+  float *pre_o, *pre_ml;             // the same over the shared pages
   int B, W, G, Hkv, cols, ps, pages, shared;      // shared: keys in shared pages
-  int row_blocks;                    // of the rows of one (sequence, key/value head)
-  int pre_splits, pre_rows;
+  int row_tiles, tile_rows, tile_keys, min_tiles; // how rows and keys are cut, and a block's least share of tiles
+  int cluster;                       // blocks that share a pair, none of them with others (0: dealt out)
+  int pre_row_tiles, pre_tile_rows, pre_tiles, pre_per;      // the same over the shared pages: rows of the whole batch; key tiles of a pair and of a block
   long q_sb, q_sw, q_sh, o_sb, o_sw, o_sh, table_sb;
   long k_sp, k_sr, k_sh, v_sp, v_sr, v_sh;        // strides of pages, rows in a page, heads
   float scale_log2;
 };
-
-// How a launch is dealt out; what it leaves in workspaces follows from it
+// How a launch is dealt out (rows: few, the kernel of paged.cu, or tiles of 128, paged_attention_sm100.cu); workspaces follow from it
 struct PagedPlan {
-  int row_tiles;                     // blocks of eight query rows that one walk over the keys serves
-  int grid, pre_splits, pre_rows;
+  bool tiles, pre_tiles;             // whether the tile kernel has the rows, and those over the shared pages
+  int grid, pre_grid;                // blocks of each walk
+  long slots, pre_slots;             // rows of parts that each leaves
 };
-PagedPlan paged_plan(int B, int W, int G, int Hkv, int shared);
-void paged_attention(PagedAttn p, const PagedPlan& plan, int D, int dt, cudaStream_t st);
+PagedPlan paged_plan(PagedAttn& p);  // fills in p's cuts
+void paged_attention(const PagedAttn& p, const PagedPlan& plan, int D, int dt, cudaStream_t st);
+void paged_tiles(const PagedAttn& p, int grid, bool over_shared, int D, int dt, cudaStream_t st);       // paged_attention_sm100.cu
 // strides s: (b, w, h) of q, k, v; cs: (page, row, head) of the caches; q_out: heads and columns contiguous
 void paged_append(const void* q, const void* k, const void* v, const long* positions, const long* lens, const float* cos_t, const float* sin_t,
                   void* q_out, void* kc, void* vc, const int* table, int B, int W, int H, int Hkv, int D, int rows, int cols, int ps, int pages,

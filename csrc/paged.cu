@@ -5,6 +5,7 @@
 #include "common.cuh"
 #include "kernels.h"
 #include "paged.cuh"
+#include "sm100_ptx.cuh"
 
 namespace nxd {
 
@@ -85,11 +86,13 @@ __global__ void __launch_bounds__(256) paged_append_kernel(
 }
 
 // ------------------------------------------------------------------------------------------------------- attention, few rows
+using namespace paged;
+
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kKeys = 16;                                  // keys of a warp's tile
 constexpr int kTileKeys = kWarps * kKeys;                  // keys of a block's tile
 constexpr int kStages = 3;
-constexpr int kMinTiles = 4;                               // a block's share of a launch is no less: 256 keys
+constexpr int kCluster8 = 8;                               // blocks of a cluster at most
 template <int D> constexpr int kPitch = D + 4;             // of the rows in which warps leave their sums: no bank twice
 template <int D> constexpr int rows_smem() { return kWarps * kStages * 2 * kKeys * D * 2 + kWarps * 8 * kPitch<D> * 4; }
 
@@ -120,176 +123,103 @@ template <> NXD_DEVICE void mma16816<__half>(float (&d)[4], const uint32_t (&a)[
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-template <typename T> NXD_DEVICE uint32_t pack16(float lo, float hi);
-template <> NXD_DEVICE uint32_t pack16<__nv_bfloat16>(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-template <> NXD_DEVICE uint32_t pack16<__half>(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
+NXD_DEVICE float remote(const float* at, int rank) {       // the same place in another block's shared memory
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(mapa_shared(smem_u32(at), rank)) : "memory");
+  return v;
 }
 
-// A pair is a (sequence, key/value head, block of query rows); its tiles are those of the sequence's keys behind the shared pages.  All tiles
-// of a launch, pair after pair, are dealt out evenly: block c takes `per` of them from c * per on, wherever that lies.  Each block finds its
-// place from the positions alone, so that nothing about lengths has to be known on the host.
-NXD_DEVICE int own_tiles(const PagedAttn& p, int b) {
-  const int n = paged_keys(p, b) - p.shared;
-  return n > 0 ? (n + kTileKeys - 1) / kTileKeys : 0;
-}
+// How a block gets its work (paged.cuh): dealt out; one pair for the blocks of a cluster, which take its tiles in turn and join their sums in shared
+// memory; dealt out over the shared pages, with the rows of the whole batch (8 R at most), all of whose results are parts
+enum Deal { kDealt, kCluster, kShared };
 
-// Sum of a launch's tiles, and where `at` lies in them: sequence and tile within it (128 threads, all of them call).  b = B: behind the last.
-struct Place { int b; long tile; };
-NXD_DEVICE long find_place(const PagedAttn& p, int grid, long& per, int block, Place& out) {
-  __shared__ long sums[kWarps];
-  __shared__ long found[2];
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int each = (p.B + kThreads - 1) / kThreads, b0 = min(p.B, (int)threadIdx.x * each), b1 = min(p.B, b0 + each);
-  long mine = 0;
-  for (int b = b0; b < b1; ++b) mine += own_tiles(p, b);
-  long scan = mine;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const long x = __shfl_up_sync(0xffffffffu, scan, o);
-    if (lane >= o) scan += x;
-  }
-  if (lane == 31) sums[warp] = scan;
-  if (threadIdx.x == 0) { found[0] = p.B; found[1] = 0; }
-  __syncthreads();
-  long before = scan - mine, total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) {
-    if (w < warp) before += sums[w];
-    total += sums[w];
-  }
-  const long pairs = (long)p.Hkv * p.row_blocks;
-  total *= pairs;
-  per = max((long)kMinTiles, (total + grid - 1) / grid);
-  long left = block * per - before * pairs;
-  if (left >= 0 && left < mine * pairs) {
-    for (int b = b0; b < b1; ++b) {
-      const long t = own_tiles(p, b) * pairs;
-      if (left < t) { found[0] = b; found[1] = left; break; }
-      left -= t;
-    }
-  }
-  __syncthreads();
-  out.b = (int)found[0];
-  out.tile = found[1];
-  return total;
-}
-
-// Where a block reads next: keys of one pair
-struct Cursor { int b, pair, tile, tiles, n; };
-
-NXD_DEVICE void next_tile(const PagedAttn& p, Cursor& c) {
-  if (++c.tile < c.tiles) return;
-  c.tile = 0;
-  if (++c.pair < p.Hkv * p.row_blocks) return;
-  c.pair = 0;
-  do {
-    ++c.b;
-    c.tiles = c.b < p.B ? own_tiles(p, c.b) : 1;
-  } while (c.tiles == 0);
-  c.n = c.b < p.B ? paged_keys(p, c.b) : 0;
-}
-
-// Sum over the shared pages' parts of one row, relative to their joint maximum: columns c0 .. c0 + C of the row
-template <int D, int C>
-NXD_DEVICE void add_shared(const PagedAttn& p, int b, int kvh, int row, int c0, float& m, float& l, float (&acc)[C]) {
-  const long at = (long)kvh * p.pre_rows + (long)b * p.W * p.G + row, step = (long)p.Hkv * p.pre_rows;
-  for (int s = 0; s < p.pre_splits; ++s) {
-    const float2 ml = reinterpret_cast<const float2*>(p.pre_ml)[at + s * step];
-    const float* o = p.pre_o + (at + s * step) * D + c0;
-    const float mn = fmaxf(m, ml.x);
-    const float f = m == -INFINITY ? 0.f : exp2f(m - mn), g = ml.x == -INFINITY ? 0.f : exp2f(ml.x - mn);
-#pragma unroll
-    for (int i = 0; i < C; ++i) acc[i] = acc[i] * f + (g != 0.f ? o[i] * g : 0.f);
-    l = l * f + ml.y * g;
-    m = mn;
-  }
-}
-
-// One block per share of the tiles; SHARED: one per (key/value head and block of rows of the whole batch, stretch of the shared pages).
 // Bound by HBM: 4 D bytes per key and key/value head.  A warp walks 16-key tiles of its own through its own ring of cp.async stages, which runs
 // ahead over the ends of pairs.  Scores Sᵀ = K Qᵀ and sums Oᵀ += Vᵀ Pᵀ by mma.sync with the keys, then the head's columns, as the 16 rows of the
 // instruction and 8 R query rows as its columns, so that a group of up to 8 heads wastes nothing; the accumulator of Sᵀ becomes the operand Pᵀ by an
 // 8 x 8 transposition in registers.  Probabilities are rounded to the cache's type for the second product: half a step of 2^-8 (2^-11) each, which average out over
 // the keys; row sums are those of the unrounded ones.
-template <typename T, int D, int R, bool SHARED>
+template <typename T, int D, int R, Deal DEAL>
 __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn p) {
+  constexpr bool SHARED = DEAL == kShared;
   constexpr int CH = D / 8, KS = D / 16, PITCH = kPitch<D>;
   constexpr int STAGE = 2 * kKeys * D * 2;
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float sm_m[kWarps][8 * R], sm_l[kWarps][8 * R];
+  __shared__ float sm_m[kWarps][8 * R], sm_l[kWarps][8 * R], sm_bm[8 * R], sm_bl[8 * R];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hq = lane >> 2, quad = lane & 3;
-  pdl_trigger();                                           // the merge's blocks may take their places; they wait for this grid
+  const int rows = SHARED ? p.B * p.W * p.G : p.W * p.G;
+  auto keys_of = [&](int e) { return SHARED ? p.shared : e < p.B ? all_keys(p, e) : 0; };
   pdl_wait();
-  const int tokens = SHARED ? p.B * p.W : p.W, rows = tokens * p.G, pairs = p.Hkv * p.row_blocks;
-  Cursor cur;
+  pdl_trigger();                                           // the merge's blocks may take their places; they wait for this grid
+  // Pages of this warp's keys in 32 tiles of a pair from tile t0 on, one a lane: -1 where there is none
+  const int step = DEAL == kCluster ? p.cluster : 1;
+  auto fetch_pages = [&](int e, int t0) {
+    const unsigned i = ((SHARED ? 0u : (unsigned)p.shared) + (unsigned)(t0 + lane * step) * kTileKeys + warp * kKeys) / (unsigned)p.ps;
+    if (i >= (unsigned)(SHARED ? p.shared / p.ps : p.cols)) return -1;
+    const int page = SHARED ? p.shared_pages[i] : p.table[e * p.table_sb + i];
+    return (unsigned)page < (unsigned)p.pages ? page : -1;
+  };
+  struct { Walk w; int n; } cur;
   long left;                                               // tiles of this block
-  if constexpr (SHARED) {
-    const int tiles = (p.shared + kTileKeys - 1) / kTileKeys;
-    const int per = (tiles + gridDim.y - 1) / gridDim.y, t0 = blockIdx.y * per;
-    cur = Cursor{0, (int)blockIdx.x, t0, min(tiles, t0 + per), p.shared};
-    left = cur.tiles - t0;
+  int pages = -1, next_page = 0;
+  if constexpr (DEAL == kCluster) {
+    const int pair = blockIdx.x / p.cluster, rank = blockIdx.x % p.cluster;
+    pages = fetch_pages(pair / p.Hkv, rank);               // beside the positions: it needs none of them
+    cur.w = Walk{pair / p.Hkv, pair % p.Hkv, rank, entry_tiles(p, pair / p.Hkv)};
+    cur.n = keys_of(cur.w.e);
+    left = cur.w.tiles > rank ? (cur.w.tiles - rank + step - 1) / step : 0;
   } else {
-    long per;
-    Place at;
-    const long total = find_place(p, gridDim.x, per, blockIdx.x, at);
-    left = min(per, total - blockIdx.x * per);
-    if (left <= 0) return;
-    cur.b = at.b;
-    cur.tiles = own_tiles(p, at.b);
-    cur.pair = (int)(at.tile / cur.tiles);
-    cur.tile = (int)(at.tile % cur.tiles);
-    cur.n = paged_keys(p, at.b);
+    const Place at = find_place<kThreads, SHARED>(p, gridDim.x, blockIdx.x);
+    left = min(at.per, at.total - blockIdx.x * at.per);
+    if (left > 0) {
+      cur.w.e = at.e;
+      cur.w.tiles = walk_tiles<SHARED>(p, at.e);
+      cur.w.head = (int)(at.tile / cur.w.tiles);
+      cur.w.tile = (int)(at.tile % cur.w.tiles);
+      cur.n = keys_of(at.e);
+      pages = fetch_pages(at.e, cur.w.tile);
+    }
   }
   const T* const kc = reinterpret_cast<const T*>(p.k);
   const T* const vc = reinterpret_cast<const T*>(p.v);
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (kStages * STAGE);
   float* const sm_o = reinterpret_cast<float*>(smem + kWarps * kStages * STAGE);       // [warp][8 rows][PITCH]
+  float* const sm_b = reinterpret_cast<float*>(smem);      // a cluster's block: its sums [8 R][D], over the ring that has been read
 
-  // page of this warp's 16 keys at a cursor: -1 where there is none
-  auto page_at = [&](const Cursor& c) {
-    const int key = (SHARED ? 0 : p.shared) + c.tile * kTileKeys + warp * kKeys;
-    if (key >= c.n) return -1;
-    const int page = SHARED ? p.shared_pages[key / p.ps] : p.table[c.b * p.table_sb + key / p.ps];
-    return (unsigned)page < (unsigned)p.pages ? page : -1;
-  };
   // CH lanes copy one row, 16-byte chunk c of row r lands at chunk (c ^ (r & 7)): both ways of reading are conflict-free
-  auto load_tile = [&](const Cursor& c, int page, int stage) {
+  auto load_tile = [&](const Walk& c, int n, int page, int stage) {
     constexpr int PASS = 32 / CH;
-    const int key = (SHARED ? 0 : p.shared) + c.tile * kTileKeys + warp * kKeys, kvh = c.pair / p.row_blocks;
+    const int key = (SHARED ? 0 : p.shared) + c.tile * kTileKeys + warp * kKeys;
     const int row0 = key % p.ps, cc = lane % CH;
     const long at = page < 0 ? 0 : page;
-    const T* kb = kc + at * p.k_sp + kvh * p.k_sh + cc * 8;
-    const T* vb = vc + at * p.v_sp + kvh * p.v_sh + cc * 8;
+    const T* kb = kc + at * p.k_sp + c.head * p.k_sh + cc * 8;
+    const T* vb = vc + at * p.v_sp + c.head * p.v_sh + cc * 8;
     const uint32_t dst = ring + stage * STAGE;
 #pragma unroll
     for (int i = 0; i < kKeys / PASS; ++i) {
       const int r = i * PASS + lane / CH;
-      const bool live = page >= 0 && key + r < c.n;
+      const bool live = page >= 0 && key + r < n;
       const uint32_t off = r * (D * 2) + ((cc ^ (r & 7)) << 4);
       cp_async16(dst + off, kb + (row0 + r) * p.k_sr, live);
       cp_async16(dst + kKeys * D * 2 + off, vb + (row0 + r) * p.v_sr, live);
     }
   };
 
-  Cursor ahead = cur;
+  auto ahead = cur;
   long asked = 0;
-  int page = left > 0 ? page_at(ahead) : -1;
-  // pages of tiles that have been asked for, stage by stage: the products skip holes
-  uint32_t holes = 0;                                      // bit s: the tile in stage s is a hole
+  uint32_t holes = 0;                                      // bit s: none of the warp's keys in stage s is there
   auto ask = [&](int stage) {
     if (asked < left) {
-      load_tile(ahead, page, stage);
+      if (next_page == 32) { pages = fetch_pages(ahead.w.e, ahead.w.tile); next_page = 0; }
+      const int page = __shfl_sync(0xffffffffu, pages, next_page++);
+      load_tile(ahead.w, ahead.n, page, stage);
       holes = (holes & ~(1u << stage)) | (page < 0 ? 1u << stage : 0u);
       if (++asked < left) {
-        if constexpr (SHARED) ++ahead.tile; else next_tile(p, ahead);
-        page = page_at(ahead);
+        ahead.w.tile += step;
+        if (DEAL != kCluster && ahead.w.tile == ahead.w.tiles) {
+          next_pair<SHARED>(p, ahead.w);
+          if (ahead.w.head == 0) ahead.n = keys_of(ahead.w.e);
+          next_page = 32;
+        }
       }
     }
     cp_async_commit();
@@ -303,19 +233,19 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn
   bool whole = false;                                      // the pair begins in this block
   auto row_token = [&](int row, int& b, int& w) {          // of the pair's row
     const int t = row / p.G;
-    b = SHARED ? t / p.W : cur.b;
+    b = SHARED ? t / p.W : cur.w.e;
     w = SHARED ? t % p.W : t;
   };
   auto begin = [&]() {
-    const int kvh = cur.pair / p.row_blocks, r0 = (cur.pair % p.row_blocks) * 8 * R;
-    whole = SHARED || cur.tile == 0;
-    lim_all = SHARED ? 0 : (int)min(p.positions[cur.b] + r0 / p.G + 1, (long)cur.n);
+    const int kvh = cur.w.head;
+    whole = DEAL == kCluster || cur.w.tile == 0;
+    lim_all = SHARED ? 0 : min(visible_keys(p, cur.w.e, 0), cur.n);
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       int b, w;
-      const int row = r0 + i * 8 + hq;
+      const int row = i * 8 + hq;
       row_token(row, b, w);
-      const bool live = row < rows && w < paged_new_tokens(p, b);
+      const bool live = row < rows && w < new_tokens(p, b);
       const T* qp = reinterpret_cast<const T*>(p.q) + (live ? b * p.q_sb + w * p.q_sw + (long)(kvh * p.G + row % p.G) * p.q_sh : 0) + quad * 2;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
@@ -326,10 +256,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn
       }
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int r = r0 + i * 8 + quad * 2 + e;
+        const int r = i * 8 + quad * 2 + e;
         row_token(r, b, w);
-        const bool on = r < rows && w < paged_new_tokens(p, b);
-        lim[i][e] = on ? (int)min(p.positions[b] + w + 1, (long)cur.n) : 0;
+        lim[i][e] = r < rows && w < new_tokens(p, b) ? min(visible_keys(p, b, w), cur.n) : 0;
         m[i][e] = -INFINITY;
         l[i][e] = 0.f;
       }
@@ -338,7 +267,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn
 
   // the four warps' sums of the pair, to the output or to a part
   auto finish = [&](bool last) {
-    const int kvh = cur.pair / p.row_blocks, r0 = (cur.pair % p.row_blocks) * 8 * R;
+    const int kvh = cur.w.head;
+    const bool direct = !SHARED && p.shared == 0 && whole && last;
 #pragma unroll
     for (int i = 0; i < R; ++i)
 #pragma unroll
@@ -361,44 +291,41 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn
       constexpr int PER = kThreads / D;                    // rows at a time
 #pragma unroll
       for (int x = 0; x < 8 / PER; ++x) {
-        const int rr = x * PER + (int)threadIdx.x / D, col = threadIdx.x % D, row = r0 + i * 8 + rr, rs = i * 8 + rr;
+        const int rr = x * PER + (int)threadIdx.x / D, col = threadIdx.x % D, row = i * 8 + rr;
         if (row >= rows) break;
-        float mn = fmaxf(fmaxf(sm_m[0][rs], sm_m[1][rs]), fmaxf(sm_m[2][rs], sm_m[3][rs])), ls = 0.f, acc[1] = {0.f};
+        float mn = fmaxf(fmaxf(sm_m[0][row], sm_m[1][row]), fmaxf(sm_m[2][row], sm_m[3][row])), ls = 0.f, acc = 0.f;
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
-          const float c = mn == -INFINITY ? 0.f : exp2f(sm_m[w][rs] - mn);
-          acc[0] += sm_o[(w * 8 + rr) * PITCH + col] * c;
-          ls += sm_l[w][rs] * c;
+          const float c = mn == -INFINITY ? 0.f : exp2f(sm_m[w][row] - mn);
+          acc += sm_o[(w * 8 + rr) * PITCH + col] * c;
+          ls += sm_l[w][row] * c;
         }
-        if constexpr (SHARED) {
-          const long at = ((long)blockIdx.y * p.Hkv + kvh) * p.pre_rows + row;
-          p.pre_o[at * D + col] = acc[0];
-          if (col == 0) { p.pre_ml[at * 2] = mn; p.pre_ml[at * 2 + 1] = ls; }
-        } else if (whole && last) {
-          if (p.pre_splits) add_shared<D>(p, cur.b, kvh, row, col, mn, ls, acc);
+        if (DEAL == kCluster && p.cluster > 1) {
+          sm_b[row * D + col] = acc;
+          if (col == 0) { sm_bm[row] = mn; sm_bl[row] = ls; }
+        } else if (direct) {
           int b, w;
           row_token(row, b, w);
-          const bool live = w < paged_new_tokens(p, b) && !(ls == 0.f);
-          reinterpret_cast<T*>(p.out)[b * p.o_sb + w * p.o_sw + (long)(kvh * p.G + row % p.G) * p.o_sh + col] = from_f32<T>(live ? acc[0] / ls : 0.f);
+          const bool live = w < new_tokens(p, b) && !(ls == 0.f);
+          reinterpret_cast<T*>(p.out)[b * p.o_sb + w * p.o_sw + (long)(kvh * p.G + row % p.G) * p.o_sh + col] = from_f32<T>(live ? acc / ls : 0.f);
         } else {
-          const long at = (long)(blockIdx.x * 2 + (whole ? 1 : 0)) * (8 * R) + rs;
-          p.part_o[at * D + col] = acc[0];
-          if (col == 0) { p.part_ml[at * 2] = mn; p.part_ml[at * 2 + 1] = ls; }
+          const long slot = part_slot<SHARED>(p, (long)cur.w.e * p.Hkv + kvh, blockIdx.x, whole) * (8 * R) + row;
+          (SHARED ? p.pre_o : p.part_o)[slot * D + col] = acc;
+          if (col == 0) *reinterpret_cast<float2*>((SHARED ? p.pre_ml : p.part_ml) + slot * 2) = make_float2(mn, ls);
         }
       }
     }
     __syncthreads();                                       // the sums have been read
   };
 
-  if (left > 0) begin();
-  else if constexpr (SHARED) { cur.n = 0; begin(); finish(true); return; }    // a stretch behind the shared keys
+  if (DEAL == kCluster || left > 0) begin();
   for (long t = 0; t < left; ++t) {
     const int stage = (int)(t % kStages);
     cp_async_wait<kStages - 2>();
     __syncwarp();                                          // tile t of all lanes is there; all lanes are done with tile t - 1
     const bool hole = holes >> stage & 1;
     ask((int)((t + kStages - 1) % kStages));
-    const int key = (SHARED ? 0 : p.shared) + cur.tile * kTileKeys + warp * kKeys;
+    const int key = (SHARED ? 0 : p.shared) + cur.w.tile * kTileKeys + warp * kKeys;
     if (!hole) {
       const uint32_t ks = ring + stage * STAGE, vs = ks + kKeys * D * 2;
       float s[R][4];
@@ -465,126 +392,197 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn
         for (int i = 0; i < R; ++i) mma16816<T>(o[i][k], a, pf[i][0], pf[i][1]);
       }
     }
-    const bool end = cur.tile + 1 == cur.tiles;
-    if (end || t + 1 == left) {
+    const bool end = cur.w.tile + 1 == cur.w.tiles;
+    if (DEAL != kCluster && (end || t + 1 == left)) {
       finish(end);
       if (t + 1 < left) {
-        next_tile(p, cur);
+        next_pair<SHARED>(p, cur.w);
+        if (cur.w.head == 0) cur.n = keys_of(cur.w.e);
         begin();
       }
     } else {
-      ++cur.tile;
+      cur.w.tile += step;
     }
   }
+  if constexpr (DEAL == kCluster) {
+    finish(true);
+    if (p.cluster > 1) {
+      cluster_sync_all();
+      constexpr int PER = kThreads / D;
+      const int rank = blockIdx.x % p.cluster, col = threadIdx.x % D;
+      for (int row = rank * PER + (int)threadIdx.x / D; row < rows; row += p.cluster * PER) {
+        float mb[kCluster8], lb[kCluster8], ob[kCluster8], mn = -INFINITY, ls = 0.f, acc = 0.f;
+#pragma unroll
+        for (int x = 0; x < kCluster8; ++x) {
+          const int from = x < p.cluster ? x : 0;
+          mb[x] = x < p.cluster ? remote(sm_bm + row, from) : -INFINITY;
+          lb[x] = remote(sm_bl + row, from);
+          ob[x] = remote(sm_b + row * D + col, from);
+          mn = fmaxf(mn, mb[x]);
+        }
+#pragma unroll
+        for (int x = 0; x < kCluster8; ++x) {
+          if (x >= p.cluster) break;
+          const float c = mn == -INFINITY ? 0.f : exp2f(mb[x] - mn);
+          acc += ob[x] * c;
+          ls += lb[x] * c;
+        }
+        int b, w;
+        row_token(row, b, w);
+        const bool live = w < new_tokens(p, b) && !(ls == 0.f);
+        reinterpret_cast<T*>(p.out)[b * p.o_sb + w * p.o_sw + (long)(cur.w.head * p.G + row % p.G) * p.o_sh + col] = from_f32<T>(live ? acc / ls : 0.f);
+      }
+      cluster_sync_all();                                  // nobody reads a block's sums any more
+    }
+  }
+  if (DEAL == kDealt && p.shared == 0)
+    for (int e = blockIdx.x; e < p.B; e += gridDim.x)
+      if (entry_tiles(p, e) == 0) finish_idle<T, D, kThreads>(p, e, threadIdx.x);
 }
 
-// Rows whose pair several blocks walked, or that see no key of their own: a warp joins the parts of one row.
-template <typename T, int D, int R>
+// Pairs that are cut: block (c − 1, ·) has the one that is cut first in front of block c's share, and a warp of it joins the parts of two rows.
+template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const PagedAttn p, int grid) {
-  constexpr int C = D / 32;
+  const int block = blockIdx.x + 1;
+  const Place at = find_place<kThreads, false>(p, grid, block);        // the kernel before this one waited for all that positions come from
   pdl_trigger();
   pdl_wait();
-  const int b = blockIdx.x / (p.Hkv * p.row_blocks), pair = blockIdx.x % (p.Hkv * p.row_blocks);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  // tiles of the sequences before this one, and of all
-  __shared__ long sums[2][kWarps];
-  long before = 0, total = 0;
-  for (int i = threadIdx.x; i < p.B; i += kThreads) {
-    const int t = own_tiles(p, i);
-    total += t;
-    if (i < b) before += t;
+  if (at.e >= p.B * p.row_tiles) return;
+  const int tiles = entry_tiles(p, at.e), head = (int)(at.tile / tiles);
+  const long off = at.tile % tiles, t0 = block * at.per - off;
+  if (off == 0 || off > at.per) return;                    // not cut here, or before
+  const int b = at.e / p.row_tiles, n = (int)((t0 + tiles - 1) / at.per) - (block - 1) + 1;
+  {
+    const int rs = blockIdx.y * kWarps + (threadIdx.x >> 5), row = at.e % p.row_tiles * p.tile_rows + rs, w = row / p.G;
+    if (rs >= p.tile_rows || row >= p.W * p.G) return;
+    Joined<D> sum;
+    if (w < new_tokens(p, b))
+      sum.add(p.part_o, p.part_ml, n, [&](int x) { return part_slot<false>(p, 0, block - 1 + x, x == 0) * p.tile_rows + rs; });
+    sum.store(reinterpret_cast<T*>(p.out) + b * p.o_sb + w * p.o_sw + (long)(head * p.G + row % p.G) * p.o_sh);
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    before += __shfl_xor_sync(0xffffffffu, before, o);
-    total += __shfl_xor_sync(0xffffffffu, total, o);
-  }
-  if (lane == 0) { sums[0][warp] = before; sums[1][warp] = total; }
-  __syncthreads();
-  before = total = 0;
-#pragma unroll
-  for (int w = 0; w < kWarps; ++w) { before += sums[0][w]; total += sums[1][w]; }
-  const long pairs = (long)p.Hkv * p.row_blocks;
-  const long per = max((long)kMinTiles, (total * pairs + grid - 1) / grid);
-  const int tiles = own_tiles(p, b);
-  const long t0 = before * pairs + (long)pair * tiles;
-  const int c0 = (int)(t0 / per), c1 = tiles ? (int)((t0 + tiles - 1) / per) : c0;
-  if (tiles && c0 == c1) return;                           // one block had the whole pair
-  const int rs = blockIdx.y * kWarps + warp, row = (pair % p.row_blocks) * 8 * R + rs, kvh = pair / p.row_blocks;
-  if (row >= p.W * p.G) return;
-  const int w = row / p.G, c = lane * C;
-  float m = -INFINITY, l = 0.f, acc[C];
-#pragma unroll
-  for (int i = 0; i < C; ++i) acc[i] = 0.f;
-  if (tiles) {
-    const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
-    auto slot = [&](int x) { return (long)(2 * (c0 + x) + (x == 0)) * (8 * R) + rs; };
-    const int n = c1 - c0 + 1;
-    for (int x = lane; x < n; x += 32) m = fmaxf(m, ml[slot(x)].x);
-    m = warp_max(m);
-    for (int x0 = 0; x0 < n; x0 += 32) {
-      const float2 a = x0 + lane < n ? ml[slot(x0 + lane)] : make_float2(-INFINITY, 0.f);
-      const float f = a.x == -INFINITY ? 0.f : exp2f(a.x - m);
-      l += warp_sum(a.y * f);
-      const int here = min(32, n - x0);
-#pragma unroll 8
-      for (int x = 0; x < here; ++x) {
-        const float g = __shfl_sync(0xffffffffu, f, x);
-        const float* src = p.part_o + slot(x0 + x) * D + c;
-        float v[C];
-        if constexpr (C == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
-        else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
-#pragma unroll
-        for (int i = 0; i < C; ++i) acc[i] += v[i] * g;
-      }
-    }
-  }
-  const bool live = w < paged_new_tokens(p, b);
-  if (live && p.pre_splits) add_shared<D>(p, b, kvh, row, c, m, l, acc);
-  T* dst = reinterpret_cast<T*>(p.out) + b * p.o_sb + w * p.o_sw + (long)(kvh * p.G + row % p.G) * p.o_sh + c;
-#pragma unroll
-  for (int i = 0; i < C; ++i) dst[i] = from_f32<T>(live && !(l == 0.f) ? acc[i] / l : 0.f);
 }
 
-template <typename T, int D, int R>
-void launch_rows(const PagedAttn& p, int grid, cudaStream_t st) {
-  if (p.pre_splits) {
-    PagedAttn s = p;
-    s.row_blocks = (p.B * p.W * p.G + 8 * R - 1) / (8 * R);
-    NXD_ALLOW_SMEM((paged_rows_kernel<T, D, R, true>), rows_smem<D>());
-    launch_dependent(paged_rows_kernel<T, D, R, true>, dim3(p.Hkv * s.row_blocks, p.pre_splits), kThreads, rows_smem<D>(), st, s);
+// With shared pages: every row's parts over its own pages and over the shared ones.  Block (entry, ·), a warp per row and key/value head.
+template <typename T, int D>
+__global__ void __launch_bounds__(kThreads) paged_join_kernel(const PagedAttn p, int grid) {
+  __shared__ long sums[2][kWarps];
+  const int e = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, entries = p.B * p.row_tiles;
+  int before = 0, all = 0;
+  for (int i = threadIdx.x; i < entries; i += kThreads) {
+    const int t = entry_tiles(p, i);
+    all += t;
+    if (i < e) before += t;
   }
-  NXD_ALLOW_SMEM((paged_rows_kernel<T, D, R, false>), rows_smem<D>());
-  launch_dependent(paged_rows_kernel<T, D, R, false>, grid, kThreads, rows_smem<D>(), st, p);
-  launch_dependent(paged_merge_kernel<T, D, R>, dim3(p.B * p.Hkv * p.row_blocks, 2 * R), kThreads, 0, st, p, grid);
+  const int w0 = __reduce_add_sync(0xffffffffu, before), w1 = __reduce_add_sync(0xffffffffu, all);
+  if (lane == 0) { sums[0][warp] = w0; sums[1][warp] = w1; }
+  __syncthreads();
+  long first = 0, total = 0;
+#pragma unroll
+  for (int x = 0; x < kWarps; ++x) { first += sums[0][x]; total += sums[1][x]; }
+  const long per = max((long)p.min_tiles, (total * p.Hkv + grid - 1) / grid);
+  const int tiles = entry_tiles(p, e), b = e / p.row_tiles, row0 = e % p.row_tiles * p.tile_rows, rows = min(p.tile_rows, p.W * p.G - row0);
+  pdl_trigger();
+  pdl_wait();
+  const int item = blockIdx.y * kWarps + warp;
+  if (item >= rows * p.Hkv) return;
+  const int head = item / rows, rs = item % rows, row = row0 + rs, w = row / p.G;
+  Joined<D> sum;
+  if (w < new_tokens(p, b)) {
+    const long r = (long)b * p.W * p.G + row, pre = r / p.pre_tile_rows * p.Hkv + head, s0 = pre * p.pre_tiles;
+    const int c0 = (int)(s0 / p.pre_per), at = (int)(r % p.pre_tile_rows);
+    sum.add(p.pre_o, p.pre_ml, (int)((s0 + p.pre_tiles - 1) / p.pre_per) - c0 + 1,
+            [&](int x) { return part_slot<true>(p, pre, c0 + x, x == 0) * p.pre_tile_rows + at; });
+    if (tiles) {
+      const long t0 = first * p.Hkv + (long)head * tiles;
+      const int b0 = (int)(t0 / per);
+      sum.add(p.part_o, p.part_ml, (int)((t0 + tiles - 1) / per) - b0 + 1,
+              [&](int x) { return part_slot<false>(p, (long)e * p.Hkv + head, b0 + x, x == 0) * p.tile_rows + rs; });
+    }
+  }
+  sum.store(reinterpret_cast<T*>(p.out) + b * p.o_sb + w * p.o_sw + (long)(head * p.G + row % p.G) * p.o_sh);
+}
+
+template <typename T, int D, int R, Deal DEAL>
+void launch_rows(const PagedAttn& p, int grid, cudaStream_t st) {
+  NXD_ALLOW_SMEM((paged_rows_kernel<T, D, R, DEAL>), rows_smem<D>());
+  if (DEAL != kCluster || p.cluster == 1) return launch_dependent(paged_rows_kernel<T, D, R, DEAL>, grid, kThreads, rows_smem<D>(), st, p);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid; cfg.blockDim = kThreads; cfg.dynamicSmemBytes = rows_smem<D>(); cfg.stream = st;
+  cudaLaunchAttribute attr[2]{};
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = p.cluster;
+  attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr; cfg.numAttrs = 2;
+  NXD_CUDA_CHECK(cudaLaunchKernelEx(&cfg, paged_rows_kernel<T, D, R, DEAL>, p));
+}
+template <typename T, int D>
+void launch(const PagedAttn& p, const PagedPlan& plan, int dt, cudaStream_t st) {
+  if (p.shared) {
+    if (plan.pre_tiles) paged_tiles(p, plan.pre_grid, true, D, dt, st);
+    else if (p.pre_tile_rows == 8) launch_rows<T, D, 1, kShared>(p, plan.pre_grid, st);
+    else launch_rows<T, D, 2, kShared>(p, plan.pre_grid, st);
+  }
+  if (p.cluster) return p.tile_rows == 8 ? launch_rows<T, D, 1, kCluster>(p, plan.grid, st) : launch_rows<T, D, 2, kCluster>(p, plan.grid, st);
+  if (plan.tiles) paged_tiles(p, plan.grid, false, D, dt, st);
+  else if (p.tile_rows == 8) launch_rows<T, D, 1, kDealt>(p, plan.grid, st);
+  else launch_rows<T, D, 2, kDealt>(p, plan.grid, st);
+  const int rows = std::min(p.tile_rows, p.W * p.G);
+  if (p.shared)
+    launch_dependent(paged_join_kernel<T, D>, dim3(p.B * p.row_tiles, (rows * p.Hkv + kWarps - 1) / kWarps), kThreads, 0, st, p, plan.grid);
+  else if (plan.grid > 1)
+    launch_dependent(paged_merge_kernel<T, D>, dim3(plan.grid - 1, (rows + kWarps - 1) / kWarps), kThreads, 0, st, p, plan.grid);
 }
 
 }  // namespace
 
 int device_sm_count();
 
-// Blocks of the few-row kernel, rows of a block, stretches of the shared pages
-PagedPlan paged_plan(int B, int W, int G, int Hkv, int shared) {
-  PagedPlan plan;
-  plan.row_tiles = W * G > 8 ? 2 : 1;
-  plan.grid = 2 * device_sm_count();
-  plan.pre_rows = (int)(((long)B * W * G + 15) / 16 * 16);
-  plan.pre_splits = 0;
-  if (shared > 0) {
-    const long pairs = (long)Hkv * (((long)B * W * G + 8 * plan.row_tiles - 1) / (8 * plan.row_tiles));
-    plan.pre_splits = (int)std::max(1l, std::min({(2l * plan.grid + pairs - 1) / pairs, (shared + 255l) / 256, 64l}));
+// Up to 16 query rows of a sequence and key/value head go to the kernel above, more to tiles of 128 or 256 rows on the tensor memory.
+PagedPlan paged_plan(PagedAttn& p) {
+  PagedPlan plan{};
+  const int sms = device_sm_count();
+  // rows, → (kernel, rows of a tile)
+  auto cut = [](long rows, int& tile_rows) {
+    tile_rows = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 128 ? 128 : 256;
+    return rows > 16;
+  };
+  const long rows = (long)p.W * p.G, all = rows * p.B;
+  plan.tiles = cut(rows, p.tile_rows);
+  p.row_tiles = (int)((rows + p.tile_rows - 1) / p.tile_rows);
+  p.tile_keys = plan.tiles ? 128 : kTileKeys;
+  p.min_tiles = plan.tiles ? 2 : 4;                        // 256 keys
+  plan.grid = plan.tiles ? sms : 2 * sms;
+  // A cluster per pair, as many blocks in it as the GPU takes at once, has neither a search for places nor a second launch (us, dealt out / cluster:
+  // 1 sequence of 1000 keys, 8 heads, 19 / 9.8; 64 of 300 to 600, 8 heads, 36 / 28; 16 of 4096 to 8192, 8 heads, 72 / 68), but the longest
+  // sequence lasts as long as its own blocks take, at 47 GB/s each: 2048 keys, 22 us, at most.
+  const long pairs = (long)p.B * p.Hkv, cap = (long)p.cols * p.ps;
+  if (!plan.tiles && !p.shared) {
+    int size = 1;
+    while (size < kCluster8 && ((cap > 256l * size && pairs * size * 2 <= 2 * sms) || cap > 2048l * size)) size *= 2;
+    if (cap <= 2048l * size && pairs * size < (1l << 30)) {
+      p.cluster = size;
+      plan.grid = (int)(pairs * size);
+      return plan;
+    }
+  }
+  plan.slots = (p.shared ? (long)p.B * p.row_tiles * p.Hkv + plan.grid : 2l * plan.grid) * p.tile_rows;
+  if (p.shared) {
+    plan.pre_tiles = cut(all, p.pre_tile_rows);
+    p.pre_row_tiles = (int)((all + p.pre_tile_rows - 1) / p.pre_tile_rows);
+    p.pre_tiles = (p.shared + (plan.pre_tiles ? 128 : kTileKeys) - 1) / (plan.pre_tiles ? 128 : kTileKeys);
+    const long total = (long)p.pre_row_tiles * p.Hkv * p.pre_tiles, most = plan.pre_tiles ? sms : 2 * sms;
+    p.pre_per = (int)std::max((total + most - 1) / most, plan.pre_tiles ? 1l : 4l);
+    plan.pre_grid = (int)((total + p.pre_per - 1) / p.pre_per);
+    plan.pre_slots = ((long)p.pre_row_tiles * p.Hkv + plan.pre_grid) * p.pre_tile_rows;
   }
   return plan;
 }
 
-void paged_attention(PagedAttn p, const PagedPlan& plan, int D, int dt, cudaStream_t st) {
-  p.row_blocks = (p.W * p.G + 8 * plan.row_tiles - 1) / (8 * plan.row_tiles);
-  p.pre_splits = plan.pre_splits;
-  p.pre_rows = plan.pre_rows;
-#define NXD_PAGED(T, Dv) do { if (plan.row_tiles == 1) launch_rows<T, Dv, 1>(p, plan.grid, st); else launch_rows<T, Dv, 2>(p, plan.grid, st); } while (0)
-  if (dt == kBF16) { if (D == 128) NXD_PAGED(__nv_bfloat16, 128); else NXD_PAGED(__nv_bfloat16, 64); }
-  else { if (D == 128) NXD_PAGED(__half, 128); else NXD_PAGED(__half, 64); }
-#undef NXD_PAGED
+void paged_attention(const PagedAttn& p, const PagedPlan& plan, int D, int dt, cudaStream_t st) {
+  if (dt == kBF16) { if (D == 128) launch<__nv_bfloat16, 128>(p, plan, dt, st); else launch<__nv_bfloat16, 64>(p, plan, dt, st); }
+  else { if (D == 128) launch<__half, 128>(p, plan, dt, st); else launch<__half, 64>(p, plan, dt, st); }
 }
 
 void paged_append(const void* q, const void* k, const void* v, const long* positions, const long* lens, const float* cos_t, const float* sin_t,

@@ -1,20 +1,178 @@
-// What the kernels of a paged key/value cache share (PagedAttn: kernels.h).
+// How the attention kernels of a paged cache deal out their work (PagedAttn: kernels.h).
+//
+// A sequence's query rows (its tokens times the heads of a group) are cut into row tiles, its keys behind the shared pages into key tiles.  An entry
+// is a (sequence, row tile), a pair an (entry, key/value head); a pair's key tiles are those that its newest token sees.  All key tiles of a
+// launch, pair after pair, are dealt out evenly: block c takes `per` of them from c * per on, wherever that lies, so that long and short
+// sequences in one batch fill the GPU alike.  Each block finds its place from the positions alone: nothing about lengths has to be known on the
+// host.  A pair that lies within one block is finished there; of one that is cut every block leaves its part in a workspace (slot 2 c + 1 if the pair
+// begins in block c, 2 c if it began before), and a second launch joins them.  Where there are shared pages, their rows are those of the whole
+// batch, cut and dealt out in the same way by a launch of their own; then all results of either are parts (slot: the pair's number, or the
+// number of pairs + c), and the last launch joins both kinds.
 #pragma once
 #include "common.cuh"
 #include "kernels.h"
 
 namespace nxd {
+namespace paged {
 
-NXD_DEVICE int paged_new_tokens(const PagedAttn& p, int b) {
+NXD_DEVICE int new_tokens(const PagedAttn& p, int b) {
   const long n = p.lens ? p.lens[b] : p.W;
   return p.positions[b] < 0 ? 0 : (int)(n < 0 ? 0 : n > p.W ? p.W : n);
 }
-// One past the last key that a sequence's newest token sees; what lies behind the page table's end nobody sees
-NXD_DEVICE int paged_keys(const PagedAttn& p, int b) {
-  const int m = paged_new_tokens(p, b);
-  if (m == 0) return 0;
-  const long n = p.positions[b] + m, cap = (long)p.cols * p.ps;
+// Keys that token w of sequence b sees; what lies behind the page table's end nobody sees
+NXD_DEVICE int visible_keys(const PagedAttn& p, int b, int w) {
+  const long n = p.positions[b] + w + 1, cap = (long)p.cols * p.ps;
   return (int)(n < cap ? n : cap);
 }
+// One past the last key of the sequence: none of its tokens sees more
+NXD_DEVICE int all_keys(const PagedAttn& p, int b) {
+  const int m = new_tokens(p, b);
+  return m ? visible_keys(p, b, m - 1) : 0;
+}
+// Key tiles that rows [row0, row1) of a sequence see behind the shared pages
+NXD_DEVICE int row_key_tiles(const PagedAttn& p, int b, int row0, int row1) {
+  const int m = new_tokens(p, b);
+  if (row0 / p.G >= m) return 0;
+  const int n = visible_keys(p, b, min(m, (row1 + p.G - 1) / p.G) - 1) - p.shared;
+  return n > 0 ? (n + p.tile_keys - 1) / p.tile_keys : 0;
+}
+NXD_DEVICE int entry_tiles(const PagedAttn& p, int e) {
+  const int row0 = e % p.row_tiles * p.tile_rows;
+  return row_key_tiles(p, e / p.row_tiles, row0, row0 + p.tile_rows);
+}
 
+// SHARED, here and below: the rows of the whole batch as one sequence's, over the shared pages; the cuts are the host's
+template <bool SHARED> NXD_DEVICE int walk_tiles(const PagedAttn& p, int e) { return SHARED ? p.pre_tiles : entry_tiles(p, e); }
+
+struct Place { int e; long tile; long per, total; };
+
+// Where tile block * per lies: entry (all of them behind the last tile) and tile within the entry's pairs.  All THREADS threads call it.
+template <int THREADS, bool SHARED>
+NXD_DEVICE Place find_place(const PagedAttn& p, int grid, int block) {
+  if constexpr (SHARED) {
+    const long t = (long)p.Hkv * p.pre_tiles, first = (long)block * p.pre_per;
+    return Place{(int)(first / t), first % t, p.pre_per, t * p.pre_row_tiles};
+  } else {
+    __shared__ long sums[THREADS / 32];
+    __shared__ long found[2];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, entries = p.B * p.row_tiles;
+    const int each = (entries + THREADS - 1) / THREADS, e0 = min(entries, (int)threadIdx.x * each), e1 = min(entries, e0 + each);
+    long mine = 0;
+    for (int e = e0; e < e1; ++e) mine += entry_tiles(p, e);
+    long scan = mine;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const long x = __shfl_up_sync(0xffffffffu, scan, o);
+      if (lane >= o) scan += x;
+    }
+    if (lane == 31) sums[warp] = scan;
+    if (threadIdx.x == 0) { found[0] = entries; found[1] = 0; }
+    __syncthreads();
+    Place at;
+    long before = scan - mine;
+    at.total = 0;
+#pragma unroll
+    for (int w = 0; w < THREADS / 32; ++w) {
+      if (w < warp) before += sums[w];
+      at.total += sums[w];
+    }
+    at.total *= p.Hkv;
+    at.per = max((long)p.min_tiles, (at.total + grid - 1) / grid);
+    long left = block * at.per - before * p.Hkv;
+    if (left >= 0 && left < mine * p.Hkv) {
+      for (int e = e0; e < e1; ++e) {
+        const long t = (long)entry_tiles(p, e) * p.Hkv;
+        if (left < t) { found[0] = e; found[1] = left; break; }
+        left -= t;
+      }
+    }
+    __syncthreads();
+    at.e = (int)found[0];
+    at.tile = found[1];
+    return at;
+  }
+}
+
+// A block's walk over its share: the pair and the tile in it
+struct Walk { int e, head, tile, tiles; };
+
+template <bool SHARED>
+NXD_DEVICE void next_pair(const PagedAttn& p, Walk& w) {
+  w.tile = 0;
+  if (++w.head < p.Hkv) return;
+  w.head = 0;
+  ++w.e;
+  if constexpr (!SHARED)
+    while ((w.tiles = w.e < p.B * p.row_tiles ? entry_tiles(p, w.e) : 1) == 0) ++w.e;
+}
+
+// Slot of the part that block `block` leaves of pair `pair`
+template <bool SHARED>
+NXD_DEVICE long part_slot(const PagedAttn& p, long pair, int block, bool begins) {
+  if (!SHARED && p.shared == 0) return 2l * block + begins;
+  return begins ? pair : (long)p.Hkv * (SHARED ? p.pre_row_tiles : p.B * p.row_tiles) + block;
+}
+
+// Joins parts: sums relative to their joint maximum, D / 32 columns a lane.  slot(x), x < n, is the row of part x.
+template <int D>
+struct Joined {
+  static constexpr int C = D / 32;
+  float m = -INFINITY, l = 0.f, acc[C] = {};
+  template <typename F>
+  NXD_DEVICE void add(const float* o, const float* stats, int n, F slot) {
+    const int lane = threadIdx.x & 31;
+    const float2* ml = reinterpret_cast<const float2*>(stats);
+    for (int x0 = 0; x0 < n; x0 += 32) {
+      const float2 a = x0 + lane < n ? ml[slot(x0 + lane)] : make_float2(-INFINITY, 0.f);
+      const float mn = fmaxf(m, warp_max(a.x)), old = m == -INFINITY ? 0.f : exp2f(m - mn), f = a.x == -INFINITY ? 0.f : exp2f(a.x - mn);
+      l = l * old + warp_sum(a.y * f);
+      m = mn;
+#pragma unroll
+      for (int j = 0; j < C; ++j) acc[j] *= old;
+      const int here = min(32, n - x0);
+#pragma unroll 8
+      for (int x = 0; x < here; ++x) {
+        const float g = __shfl_sync(0xffffffffu, f, x);
+        const float* src = o + slot(x0 + x) * D + lane * C;
+        float v[C];
+        if constexpr (C == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
+        else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+#pragma unroll
+        for (int j = 0; j < C; ++j) acc[j] += g == 0.f ? 0.f : v[j] * g;        // a part without weights has no sums
+      }
+    }
+  }
+  template <typename T>
+  NXD_DEVICE void store(T* row) const {
+    T* dst = row + (threadIdx.x & 31) * C;
+#pragma unroll
+    for (int j = 0; j < C; ++j) dst[j] = from_f32<T>(l == 0.f ? 0.f : acc[j] / l);
+  }
+};
+
+// Rows of an entry none of whose tokens sees a key, or counts: zeros.  (With shared pages the last launch writes all rows.)
+template <typename T, int D, int THREADS>
+NXD_DEVICE void finish_idle(const PagedAttn& p, int e, int thread) {
+  const int b = e / p.row_tiles, row0 = e % p.row_tiles * p.tile_rows, rows = min(p.tile_rows, p.W * p.G - row0);
+  for (int i = thread >> 5; i < rows * p.Hkv; i += THREADS / 32) {
+    const int row = row0 + i % rows, head = i / rows;
+    T* dst = reinterpret_cast<T*>(p.out) + b * p.o_sb + row / p.G * p.o_sw + (long)(head * p.G + row % p.G) * p.o_sh + (thread & 31) * (D / 32);
+#pragma unroll
+    for (int j = 0; j < D / 32; ++j) dst[j] = from_f32<T>(0.f);
+  }
+}
+
+template <typename T> NXD_DEVICE uint32_t pack16(float lo, float hi);
+template <> NXD_DEVICE uint32_t pack16<__nv_bfloat16>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <> NXD_DEVICE uint32_t pack16<__half>(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+}  // namespace paged
 }  // namespace nxd

@@ -62,7 +62,11 @@ bool paged_attention_ok(const Tensor& q, const Tensor& kc, const Tensor& vc) {
   return q.dim() == 4 && kc.dim() == 4 && vc.dim() == 4 && half_type(q) && (q.size(3) == 64 || q.size(3) == 128) && packets(kc) && packets(vc);
 }
 
-Tensor rows_out(const Tensor& q) { return at::empty({q.size(1), q.size(0), q.size(2), q.size(3)}, q.options()).transpose(0, 1); }
+// [B, W, H, D] with tokens first in memory, as the layers around take and leave it
+Tensor rows_out(const Tensor& q) {
+  const int64_t B = q.size(0), W = q.size(1), H = q.size(2), D = q.size(3);
+  return at::empty_strided({B, W, H, D}, {H * D, B * H * D, D, 1}, q.options());
+}
 
 Tensor paged_append(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& positions, const Tensor& cos_t, const Tensor& sin_t, Tensor kc,
                     Tensor vc, const Tensor& table, const c10::optional<Tensor>& lens) {
@@ -100,25 +104,18 @@ Tensor paged_attention(const Tensor& q_, const Tensor& kc, const Tensor& vc, con
     shared = shared_pages->size(0) * ps;
     CHECK_ARG(shared_pages->size(0) <= table.size(1), "more shared pages than a sequence has: " + std::to_string(shared_pages->size(0)) + ", page_table of " + std::to_string(table.size(1)));
   }
+  CHECK_ARG(scale > 0 && scale < 1e30, "the scale of the scores is positive");
   c10::cuda::CUDAGuard guard(q_.device());
   const Tensor q = as_packets(q_);
   Tensor out = rows_out(q);
   if (q.numel() == 0) return out;
   const int64_t B = q.size(0), W = q.size(1), H = q.size(2), D = q.size(3), Hkv = kc.size(2);
-  const nxd::PagedPlan plan = nxd::paged_plan((int)B, (int)W, (int)(H / Hkv), (int)Hkv, (int)shared);
   nxd::PagedAttn p{};
   p.q = q.data_ptr(); p.k = kc.data_ptr(); p.v = vc.data_ptr(); p.out = out.data_ptr();
   p.table = table.data_ptr<int>();
   p.shared_pages = shared ? shared_pages->data_ptr<int>() : nullptr;
   p.positions = positions.data_ptr<long>();
   p.lens = lens.has_value() ? lens->data_ptr<long>() : nullptr;
-  // one workspace: parts of pairs, then parts over the shared pages, each sums and statistics
-  const int64_t part = (int64_t)plan.grid * 2 * plan.row_tiles * 8, pre = (int64_t)plan.pre_splits * Hkv * plan.pre_rows;
-  Tensor work = at::empty({(part + pre) * (D + 2)}, q.options().dtype(at::kFloat));
-  p.part_o = work.data_ptr<float>();
-  p.pre_o = p.part_o + part * D;
-  p.part_ml = p.pre_o + pre * D;
-  p.pre_ml = p.part_ml + part * 2;
   p.B = (int)B; p.W = (int)W; p.G = (int)(H / Hkv); p.Hkv = (int)Hkv; p.cols = (int)table.size(1); p.ps = (int)ps; p.pages = (int)kc.size(0);
   p.shared = (int)shared;
   p.q_sb = q.stride(0); p.q_sw = q.stride(1); p.q_sh = q.stride(2);
@@ -126,6 +123,14 @@ Tensor paged_attention(const Tensor& q_, const Tensor& kc, const Tensor& vc, con
   p.table_sb = table.stride(0);
   p.k_sp = kc.stride(0); p.k_sr = kc.stride(1); p.k_sh = kc.stride(2);
   p.v_sp = vc.stride(0); p.v_sr = vc.stride(1); p.v_sh = vc.stride(2);
+  const nxd::PagedPlan plan = nxd::paged_plan(p);
+  // one workspace: parts of pairs that are cut, then parts over the shared pages, each sums and statistics
+  Tensor work;
+  if (plan.slots + plan.pre_slots > 0) work = at::empty({(plan.slots + plan.pre_slots) * (D + 2)}, q.options().dtype(at::kFloat));
+  p.part_o = work.defined() ? work.data_ptr<float>() : nullptr;
+  p.pre_o = p.part_o + plan.slots * D;
+  p.part_ml = p.pre_o + plan.pre_slots * D;
+  p.pre_ml = p.part_ml + plan.slots * 2;
   p.scale_log2 = (float)(scale * 1.4426950408889634);
   nxd::paged_attention(p, plan, (int)D, dt_code(q), stream());
   return out;

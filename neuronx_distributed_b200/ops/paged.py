@@ -115,6 +115,8 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pag
         _ext.count_launch(2 if shared_pages is None else 3)
         return _ext.ext().paged_attention(q, k_cache, v_cache, page_table, positions, scale, lens, shared_pages)
     _check(q, k_cache, v_cache, page_table, positions, lens)
+    if not 0 < scale < 1e30:
+        raise ValueError("the scale of the scores is positive")
     if shared_pages is not None:
         if shared_pages.dim() != 1 or shared_pages.device != q.device or shared_pages.shape[0] > page_table.shape[1]:
             raise ValueError("shared_pages is a list of no more pages than page_table has, on the queries' device")

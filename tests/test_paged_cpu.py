@@ -93,6 +93,9 @@ def test_refuses_gradients_lens_and_shared_pages():
         ops.paged.attention(*attention, shared_pages=torch.zeros(3, dtype=torch.int32))
     with pytest.raises(ValueError):
         ops.paged.attention(*attention, shared_pages=torch.zeros(1, 1, dtype=torch.int32))
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        with pytest.raises(ValueError):
+            ops.paged.attention(*attention, scale=scale)
     for args, call in ((append, ops.paged.rope_append), (attention, ops.paged.attention)):
         args[0] = args[0].clone().requires_grad_(True)
         with pytest.raises(RuntimeError):

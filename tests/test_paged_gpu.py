@@ -89,6 +89,30 @@ def test_windows(W, H, Hkv):
     check(d, attend(d))
 
 
+@pytest.mark.parametrize("W, H, Hkv", [(5, 8, 1), (3, 16, 2), (20, 8, 1), (40, 8, 1)])
+@pytest.mark.parametrize("shared", [0, 3])
+def test_windows_of_many_lengths(W, H, Hkv, shared):
+    """Every number of key tiles in a block's pieces, odd ones before even ones and ones of a single tile among them."""
+    g = torch.Generator().manual_seed(W)
+    for most in (130, 700, 4000):
+        positions = (96 + torch.randint(0, most, (60,), generator=g)).tolist()
+        lens = torch.randint(1, W + 1, (60,), generator=g).tolist()
+        d = make(6, "cuda", BF16, 60, W, H, Hkv, 64, 32, positions, lens, shared)
+        got = attend(d)
+        one = [ops.paged.attention(d["q"][b:b + 1], d["k_cache"], d["v_cache"], d["table"][b:b + 1], d["positions"][b:b + 1], lens=d["lens"][b:b + 1])
+               for b in range(60)]
+        # other cuts of the same sums: weights rounded relative to other maxima, results rounded once each
+        size = oracle_size(d)
+        assert bool(((got - torch.cat(one)).double().abs() <= 2 * bound(BF16, got.double(), size)).all())
+        assert torch.equal(got, attend(d))
+
+
+def oracle_size(d):
+    """A bound of the weighted average of the values' magnitudes, without its softmax: the largest that a row sees."""
+    v = d["v_cache"].double().nan_to_num(0.0)
+    return v.abs().amax()
+
+
 @pytest.mark.parametrize("dtype, D", [(FP16, 128), (BF16, 64), (FP16, 64)])
 @pytest.mark.parametrize("W", [4, 40, 200])
 def test_windows_of_other_types(dtype, D, W):
@@ -108,6 +132,42 @@ def test_long_and_short_sequences_together():
     positions = [9000, 3, -1, 40, 4000, 0, 700, 701, 702, 703]
     d = make(8, "cuda", BF16, len(positions), 1, 8, 1, 128, 16, positions)
     check(d, attend(d))
+
+
+def widen(d, keys):
+    """The same sequences in tables for ones of `keys` tokens: few-row launches are dealt out then, not given to clusters."""
+    ps = d["k_cache"].shape[1]
+    more = keys // ps - d["table"].shape[1]
+    d["table"] = torch.cat([d["table"], torch.full((d["table"].shape[0], more), -1, dtype=torch.int32, device="cuda")], 1)
+    return d
+
+
+@pytest.mark.parametrize("dtype, D", [(BF16, 128), (FP16, 64)])
+@pytest.mark.parametrize("H, Hkv", HEADS)
+@pytest.mark.parametrize("positions", [[0, 15, 16, 257, 700], [9000, 3, -1, 40, 4000, 0, 700, 701, 702, 703], [-1, -1], [5]])
+def test_dealt_out(dtype, D, H, Hkv, positions):
+    d = make(8, "cuda", dtype, len(positions), 1, H, Hkv, D, 16, positions)
+    near = attend(d)
+    d = widen(d, 20000)
+    check(d, attend(d))
+    assert torch.equal(near == 0, attend(d) == 0)
+
+
+@pytest.mark.parametrize("W", [2, 8])
+def test_dealt_out_windows(W):
+    d = widen(make(8, "cuda", BF16, 5, W, 4, 2, 128, 48, [3000, -1, 47, 0, 900], [W, W, 0, 1, W]), 48 * 500)
+    check(d, attend(d))
+
+
+def test_dealt_out_many():
+    """More sequences than threads that look for places."""
+    B = 1100
+    positions = [(37 * b) % 190 - 1 for b in range(B)]
+    d = make(9, "cuda", BF16, B, 1, 2, 1, 64, 16, positions)
+    want = attend(d)
+    got = attend(widen(d, 20000))
+    assert bool(((got - want).double().abs() <= 2 * bound(BF16, got.double(), oracle_size(d))).all())
+    check({**d, **{k: d[k][-40:] for k in ("q", "table", "positions")}}, got[-40:])
 
 
 @pytest.mark.parametrize("B", [129, 300])
