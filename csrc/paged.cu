@@ -545,14 +545,15 @@ PagedPlan paged_plan(PagedAttn& p) {
   const int sms = device_sm_count();
   // rows, → (kernel, rows of a tile)
   auto cut = [](long rows, int& tile_rows) {
-    tile_rows = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 128 ? 128 : 256;
+    tile_rows = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
     return rows > 16;
   };
   const long rows = (long)p.W * p.G, all = rows * p.B;
   plan.tiles = cut(rows, p.tile_rows);
   p.row_tiles = (int)((rows + p.tile_rows - 1) / p.tile_rows);
-  p.tile_keys = plan.tiles ? 128 : kTileKeys;
-  p.min_tiles = plan.tiles ? 2 : 4;                        // 256 keys
+  auto tile_keys = [](int tile_rows) { return tile_rows == 256 ? 128 : kTileKeys; };
+  p.tile_keys = tile_keys(p.tile_rows);
+  p.min_tiles = 256 / p.tile_keys;
   plan.grid = plan.tiles ? sms : 2 * sms;
   // A cluster per pair, as many blocks in it as the GPU takes at once, has neither a search for places nor a second launch (us, dealt out / cluster:
   // 1 sequence of 1000 keys, 8 heads, 19 / 9.8; 64 of 300 to 600, 8 heads, 36 / 28; 16 of 4096 to 8192, 8 heads, 72 / 68), but the longest
@@ -571,9 +572,10 @@ PagedPlan paged_plan(PagedAttn& p) {
   if (p.shared) {
     plan.pre_tiles = cut(all, p.pre_tile_rows);
     p.pre_row_tiles = (int)((all + p.pre_tile_rows - 1) / p.pre_tile_rows);
-    p.pre_tiles = (p.shared + (plan.pre_tiles ? 128 : kTileKeys) - 1) / (plan.pre_tiles ? 128 : kTileKeys);
+    const int keys = tile_keys(p.pre_tile_rows);
+    p.pre_tiles = (p.shared + keys - 1) / keys;
     const long total = (long)p.pre_row_tiles * p.Hkv * p.pre_tiles, most = plan.pre_tiles ? sms : 2 * sms;
-    p.pre_per = (int)std::max((total + most - 1) / most, plan.pre_tiles ? 1l : 4l);
+    p.pre_per = (int)std::max((total + most - 1) / most, 256l / keys);
     plan.pre_grid = (int)((total + p.pre_per - 1) / p.pre_per);
     plan.pre_slots = ((long)p.pre_row_tiles * p.Hkv + plan.pre_grid) * p.pre_tile_rows;
   }

@@ -46,17 +46,21 @@ template <bool SHARED> NXD_DEVICE int walk_tiles(const PagedAttn& p, int e) { re
 
 struct Place { int e; long tile; long per, total; };
 
-// Where tile block * per lies: entry (all of them behind the last tile) and tile within the entry's pairs.  All THREADS threads call it.
-template <int THREADS, bool SHARED>
+// Where tile block * per lies: entry (all of them behind the last tile) and tile within the entry's pairs.  THREADS threads from FIRST on call it.
+template <int THREADS, bool SHARED, int FIRST = 0>
 NXD_DEVICE Place find_place(const PagedAttn& p, int grid, int block) {
+  auto sync = [] {
+    if constexpr (FIRST == 0) __syncthreads();
+    else asm volatile("bar.sync 1, %0;" ::"n"(THREADS) : "memory");
+  };
   if constexpr (SHARED) {
     const long t = (long)p.Hkv * p.pre_tiles, first = (long)block * p.pre_per;
     return Place{(int)(first / t), first % t, p.pre_per, t * p.pre_row_tiles};
   } else {
     __shared__ long sums[THREADS / 32];
     __shared__ long found[2];
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, entries = p.B * p.row_tiles;
-    const int each = (entries + THREADS - 1) / THREADS, e0 = min(entries, (int)threadIdx.x * each), e1 = min(entries, e0 + each);
+    const int lane = threadIdx.x & 31, thread = threadIdx.x - FIRST, warp = thread >> 5, entries = p.B * p.row_tiles;
+    const int each = (entries + THREADS - 1) / THREADS, e0 = min(entries, thread * each), e1 = min(entries, e0 + each);
     long mine = 0;
     for (int e = e0; e < e1; ++e) mine += entry_tiles(p, e);
     long scan = mine;
@@ -66,8 +70,8 @@ NXD_DEVICE Place find_place(const PagedAttn& p, int grid, int block) {
       if (lane >= o) scan += x;
     }
     if (lane == 31) sums[warp] = scan;
-    if (threadIdx.x == 0) { found[0] = entries; found[1] = 0; }
-    __syncthreads();
+    if (thread == 0) { found[0] = entries; found[1] = 0; }
+    sync();
     Place at;
     long before = scan - mine;
     at.total = 0;
@@ -86,7 +90,7 @@ NXD_DEVICE Place find_place(const PagedAttn& p, int grid, int block) {
         left -= t;
       }
     }
-    __syncthreads();
+    sync();
     at.e = (int)found[0];
     at.tile = found[1];
     return at;
