@@ -212,7 +212,8 @@ struct PagedAttn {
   const long* positions;             // [B] index of a row's first new token; negative: an idle row
   const long* lens;                  // [B] new tokens of a row, or null: W
   float *part_o, *part_ml;           // parts of pairs (paged.cuh): [slot][tile_rows][D] sums, [slot][tile_rows] (maximum, sum of weights)
-  float *pre_o, *pre_ml;             // the same over the shared pages
+  float *pre_o, *pre_ml;             // the same over the shared pages, behind them: `slots` rows on
+  long slots;
   int B, W, G, Hkv, cols, ps, pages, shared;      // shared: keys in shared pages
   int row_tiles, tile_rows, tile_keys, min_tiles; // how rows and keys are cut, and a block's least share of tiles
   int cluster;                       // blocks that share a pair, none of them with others (0: dealt out)

@@ -148,8 +148,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hq = lane >> 2, quad = lane & 3;
   const int rows = SHARED ? p.B * p.W * p.G : p.W * p.G;
   auto keys_of = [&](int e) { return SHARED ? p.shared : e < p.B ? all_keys(p, e) : 0; };
-  pdl_wait();
-  pdl_trigger();                                           // the merge's blocks may take their places; they wait for this grid
+  const bool late = !SHARED && p.shared > 0;               // the launch over the shared pages is in front (paged.cuh)
+  if (!late) pdl_wait();
+  pdl_trigger();                                           // the last launch's blocks may take their places; they wait for this grid
   // Pages of this warp's keys in 32 tiles of a pair from tile t0 on, one a lane: -1 where there is none
   const int step = DEAL == kCluster ? p.cluster : 1;
   auto fetch_pages = [&](int e, int t0) {
@@ -427,6 +428,12 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn
           acc += ob[x] * c;
           ls += lb[x] * c;
         }
+        if (p.shared) {
+          const long slot = part_slot<false>(p, (long)cur.w.e * p.Hkv + cur.w.head, 0, true) * (8 * R) + row;
+          p.part_o[slot * D + col] = acc;
+          if (col == 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(mn, ls);
+          continue;
+        }
         int b, w;
         row_token(row, b, w);
         const bool live = w < new_tokens(p, b) && !(ls == 0.f);
@@ -438,6 +445,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn
   if (DEAL == kDealt && p.shared == 0)
     for (int e = blockIdx.x; e < p.B; e += gridDim.x)
       if (entry_tiles(p, e) == 0) finish_idle<T, D, kThreads>(p, e, threadIdx.x);
+  if (late) pdl_wait();
 }
 
 // Pairs that are cut: block (c − 1, ·) has the one that is cut first in front of block c's share, and a warp of it joins the parts of two rows.
@@ -452,54 +460,52 @@ __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const PagedAttn p
   const long off = at.tile % tiles, t0 = block * at.per - off;
   if (off == 0 || off > at.per) return;                    // not cut here, or before
   const int b = at.e / p.row_tiles, n = (int)((t0 + tiles - 1) / at.per) - (block - 1) + 1;
-  {
-    const int rs = blockIdx.y * kWarps + (threadIdx.x >> 5), row = at.e % p.row_tiles * p.tile_rows + rs, w = row / p.G;
-    if (rs >= p.tile_rows || row >= p.W * p.G) return;
-    Joined<D> sum;
-    if (w < new_tokens(p, b))
-      sum.add(p.part_o, p.part_ml, n, [&](int x) { return part_slot<false>(p, 0, block - 1 + x, x == 0) * p.tile_rows + rs; });
-    sum.store(reinterpret_cast<T*>(p.out) + b * p.o_sb + w * p.o_sw + (long)(head * p.G + row % p.G) * p.o_sh);
-  }
+  const int rs = blockIdx.y * kWarps + (threadIdx.x >> 5), row = at.e % p.row_tiles * p.tile_rows + rs, w = row / p.G;
+  if (rs >= p.tile_rows || row >= p.W * p.G) return;
+  join_parts<T, D>(p, w < new_tokens(p, b) ? n : 0, [&](int x) { return part_slot<false>(p, 0, block - 1 + x, x == 0) * p.tile_rows + rs; },
+                   reinterpret_cast<T*>(p.out) + b * p.o_sb + w * p.o_sw + (long)(head * p.G + row % p.G) * p.o_sh);
 }
 
-// With shared pages: every row's parts over its own pages and over the shared ones.  Block (entry, ·), a warp per row and key/value head.
+// With shared pages: every row's parts over the shared pages and over its own.  Block (entry, ·), a warp per row and key/value head.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) paged_join_kernel(const PagedAttn p, int grid) {
   __shared__ long sums[2][kWarps];
   const int e = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, entries = p.B * p.row_tiles;
-  int before = 0, all = 0;
-  for (int i = threadIdx.x; i < entries; i += kThreads) {
-    const int t = entry_tiles(p, i);
-    all += t;
-    if (i < e) before += t;
-  }
-  const int w0 = __reduce_add_sync(0xffffffffu, before), w1 = __reduce_add_sync(0xffffffffu, all);
-  if (lane == 0) { sums[0][warp] = w0; sums[1][warp] = w1; }
-  __syncthreads();
-  long first = 0, total = 0;
+  const int b = e / p.row_tiles, row0 = e % p.row_tiles * p.tile_rows, rows = min(p.tile_rows, p.W * p.G - row0);
+  const int item = blockIdx.y * kWarps + warp, head = item / rows, rs = item % rows, row = row0 + rs, w = row / p.G;
+  // parts over its own pages: a cluster leaves one, a launch that is dealt out as many as the pair was cut into
+  int own = 1, b0 = 0;
+  if (p.cluster == 0) {
+    int before = 0, all = 0;
+    for (int i = threadIdx.x; i < entries; i += kThreads) {
+      const int t = entry_tiles(p, i);
+      all += t;
+      if (i < e) before += t;
+    }
+    const int w0 = __reduce_add_sync(0xffffffffu, before), w1 = __reduce_add_sync(0xffffffffu, all);
+    if (lane == 0) { sums[0][warp] = w0; sums[1][warp] = w1; }
+    __syncthreads();
+    long first = 0, total = 0;
 #pragma unroll
-  for (int x = 0; x < kWarps; ++x) { first += sums[0][x]; total += sums[1][x]; }
-  const long per = max((long)p.min_tiles, (total * p.Hkv + grid - 1) / grid);
-  const int tiles = entry_tiles(p, e), b = e / p.row_tiles, row0 = e % p.row_tiles * p.tile_rows, rows = min(p.tile_rows, p.W * p.G - row0);
+    for (int x = 0; x < kWarps; ++x) { first += sums[0][x]; total += sums[1][x]; }
+    const long per = max((long)p.min_tiles, (total * p.Hkv + grid - 1) / grid);
+    const int tiles = entry_tiles(p, e);
+    const long t0 = first * p.Hkv + (long)head * tiles;
+    b0 = (int)(t0 / per);
+    own = tiles ? (int)((t0 + tiles - 1) / per) - b0 + 1 : 0;
+  }
+  const bool live = item < rows * p.Hkv && w < new_tokens(p, b);
+  const long r = (long)b * p.W * p.G + row, pre = r / p.pre_tile_rows * p.Hkv + head, s0 = pre * p.pre_tiles;
+  const int c0 = (int)(s0 / p.pre_per), over = (int)((s0 + p.pre_tiles - 1) / p.pre_per) - c0 + 1, at = (int)(r % p.pre_tile_rows);
   pdl_trigger();
   pdl_wait();
-  const int item = blockIdx.y * kWarps + warp;
   if (item >= rows * p.Hkv) return;
-  const int head = item / rows, rs = item % rows, row = row0 + rs, w = row / p.G;
-  Joined<D> sum;
-  if (w < new_tokens(p, b)) {
-    const long r = (long)b * p.W * p.G + row, pre = r / p.pre_tile_rows * p.Hkv + head, s0 = pre * p.pre_tiles;
-    const int c0 = (int)(s0 / p.pre_per), at = (int)(r % p.pre_tile_rows);
-    sum.add(p.pre_o, p.pre_ml, (int)((s0 + p.pre_tiles - 1) / p.pre_per) - c0 + 1,
-            [&](int x) { return part_slot<true>(p, pre, c0 + x, x == 0) * p.pre_tile_rows + at; });
-    if (tiles) {
-      const long t0 = first * p.Hkv + (long)head * tiles;
-      const int b0 = (int)(t0 / per);
-      sum.add(p.part_o, p.part_ml, (int)((t0 + tiles - 1) / per) - b0 + 1,
-              [&](int x) { return part_slot<false>(p, (long)e * p.Hkv + head, b0 + x, x == 0) * p.tile_rows + rs; });
-    }
-  }
-  sum.store(reinterpret_cast<T*>(p.out) + b * p.o_sb + w * p.o_sw + (long)(head * p.G + row % p.G) * p.o_sh);
+  join_parts<T, D>(p, live ? over + own : 0,
+                   [&](int x) {
+                     return x < over ? p.slots + part_slot<true>(p, pre, c0 + x, x == 0) * p.pre_tile_rows + at
+                                     : part_slot<false>(p, (long)e * p.Hkv + head, b0 + x - over, x == over) * p.tile_rows + rs;
+                   },
+                   reinterpret_cast<T*>(p.out) + b * p.o_sb + w * p.o_sw + (long)(head * p.G + row % p.G) * p.o_sh);
 }
 
 template <typename T, int D, int R, Deal DEAL>
@@ -524,14 +530,15 @@ void launch(const PagedAttn& p, const PagedPlan& plan, int dt, cudaStream_t st) 
     else if (p.pre_tile_rows == 8) launch_rows<T, D, 1, kShared>(p, plan.pre_grid, st);
     else launch_rows<T, D, 2, kShared>(p, plan.pre_grid, st);
   }
-  if (p.cluster) return p.tile_rows == 8 ? launch_rows<T, D, 1, kCluster>(p, plan.grid, st) : launch_rows<T, D, 2, kCluster>(p, plan.grid, st);
-  if (plan.tiles) paged_tiles(p, plan.grid, false, D, dt, st);
+  if (p.cluster && p.tile_rows == 8) launch_rows<T, D, 1, kCluster>(p, plan.grid, st);
+  else if (p.cluster) launch_rows<T, D, 2, kCluster>(p, plan.grid, st);
+  else if (plan.tiles) paged_tiles(p, plan.grid, false, D, dt, st);
   else if (p.tile_rows == 8) launch_rows<T, D, 1, kDealt>(p, plan.grid, st);
   else launch_rows<T, D, 2, kDealt>(p, plan.grid, st);
   const int rows = std::min(p.tile_rows, p.W * p.G);
   if (p.shared)
     launch_dependent(paged_join_kernel<T, D>, dim3(p.B * p.row_tiles, (rows * p.Hkv + kWarps - 1) / kWarps), kThreads, 0, st, p, plan.grid);
-  else if (plan.grid > 1)
+  else if (!p.cluster && plan.grid > 1)
     launch_dependent(paged_merge_kernel<T, D>, dim3(plan.grid - 1, (rows + kWarps - 1) / kWarps), kThreads, 0, st, p, plan.grid);
 }
 
@@ -558,17 +565,20 @@ PagedPlan paged_plan(PagedAttn& p) {
   // A cluster per pair, as many blocks in it as the GPU takes at once, has neither a search for places nor a second launch (us, dealt out / cluster:
   // 1 sequence of 1000 keys, 8 heads, 19 / 9.8; 64 of 300 to 600, 8 heads, 36 / 28; 16 of 4096 to 8192, 8 heads, 72 / 68), but the longest
   // sequence lasts as long as its own blocks take, at 47 GB/s each: 2048 keys, 22 us, at most.
-  const long pairs = (long)p.B * p.Hkv, cap = (long)p.cols * p.ps;
-  if (!plan.tiles && !p.shared) {
+  // A cluster per pair, as many blocks in it as the GPU takes at once, has neither a search for places nor a second launch (us, dealt out / cluster:
+  // 1 sequence of 1000 keys, 8 heads, 19 / 9.8; 64 of 300 to 600, 8 heads, 36 / 28; 16 of 4096 to 8192, 8 heads, 72 / 68), but the longest
+  // sequence lasts as long as its own blocks take, at 47 GB/s each: 2048 keys, 22 us, at most.
+  const long pairs = (long)p.B * p.Hkv, cap = (long)p.cols * p.ps - p.shared;
+  if (!plan.tiles) {
     int size = 1;
     while (size < kCluster8 && ((cap > 256l * size && pairs * size * 2 <= 2 * sms) || cap > 2048l * size)) size *= 2;
     if (cap <= 2048l * size && pairs * size < (1l << 30)) {
       p.cluster = size;
       plan.grid = (int)(pairs * size);
-      return plan;
     }
   }
-  plan.slots = (p.shared ? (long)p.B * p.row_tiles * p.Hkv + plan.grid : 2l * plan.grid) * p.tile_rows;
+  plan.slots = (p.shared ? (long)p.B * p.row_tiles * p.Hkv + (p.cluster ? 0 : plan.grid) : p.cluster ? 0l : 2l * plan.grid) * p.tile_rows;
+  p.slots = plan.slots;
   if (p.shared) {
     plan.pre_tiles = cut(all, p.pre_tile_rows);
     p.pre_row_tiles = (int)((all + p.pre_tile_rows - 1) / p.pre_tile_rows);

@@ -7,7 +7,9 @@
 // host.  A pair that lies within one block is finished there; of one that is cut every block leaves its part in a workspace (slot 2 c + 1 if the pair
 // begins in block c, 2 c if it began before), and a second launch joins them.  Where there are shared pages, their rows are those of the whole
 // batch, cut and dealt out in the same way by a launch of their own; then all results of either are parts (slot: the pair's number, or the
-// number of pairs + c), and the last launch joins both kinds.
+// number of pairs + c), and the last launch joins both kinds.  The launch over the shared pages goes first.  Its blocks let the next launch start
+// when they have waited for everything before them, and that one, which reads nothing that they write, waits for them at its end alone: the two
+// share the GPU.
 #pragma once
 #include "common.cuh"
 #include "kernels.h"
@@ -117,42 +119,47 @@ NXD_DEVICE long part_slot(const PagedAttn& p, long pair, int block, bool begins)
   return begins ? pair : (long)p.Hkv * (SHARED ? p.pre_row_tiles : p.B * p.row_tiles) + block;
 }
 
-// Joins parts: sums relative to their joint maximum, D / 32 columns a lane.  slot(x), x < n, is the row of part x.
-template <int D>
-struct Joined {
-  static constexpr int C = D / 32;
+// Joins n parts of a row, D / 32 columns a lane; slot(x) is the row of part x among all parts' rows.  The first eight are asked for before their weights
+// are known.
+template <typename T, int D, typename F>
+NXD_DEVICE void join_parts(const PagedAttn& p, int n, F slot, T* row) {
+  constexpr int C = D / 32, AHEAD = 8;
+  const int lane = threadIdx.x & 31;
+  const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
   float m = -INFINITY, l = 0.f, acc[C] = {};
-  template <typename F>
-  NXD_DEVICE void add(const float* o, const float* stats, int n, F slot) {
-    const int lane = threadIdx.x & 31;
-    const float2* ml = reinterpret_cast<const float2*>(stats);
-    for (int x0 = 0; x0 < n; x0 += 32) {
-      const float2 a = x0 + lane < n ? ml[slot(x0 + lane)] : make_float2(-INFINITY, 0.f);
-      const float mn = fmaxf(m, warp_max(a.x)), old = m == -INFINITY ? 0.f : exp2f(m - mn), f = a.x == -INFINITY ? 0.f : exp2f(a.x - mn);
-      l = l * old + warp_sum(a.y * f);
-      m = mn;
+  for (int x0 = 0; x0 < n; x0 += 32) {
+    const int here = min(32, n - x0);
+    float v[AHEAD][C];
+    auto ask = [&](int x1) {
 #pragma unroll
-      for (int j = 0; j < C; ++j) acc[j] *= old;
-      const int here = min(32, n - x0);
-#pragma unroll 8
-      for (int x = 0; x < here; ++x) {
-        const float g = __shfl_sync(0xffffffffu, f, x);
-        const float* src = o + slot(x0 + x) * D + lane * C;
-        float v[C];
-        if constexpr (C == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(src);
-        else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(src);
+      for (int x = 0; x < AHEAD; ++x)
+        if (x1 + x < here) {
+          const float* src = p.part_o + slot(x0 + x1 + x) * D + lane * C;
+          if constexpr (C == 4) *reinterpret_cast<float4*>(v[x]) = *reinterpret_cast<const float4*>(src);
+          else *reinterpret_cast<float2*>(v[x]) = *reinterpret_cast<const float2*>(src);
+        }
+    };
+    ask(0);
+    const float2 a = lane < here ? ml[slot(x0 + lane)] : make_float2(-INFINITY, 0.f);
+    const float mn = fmaxf(m, warp_max(a.x)), old = m == -INFINITY ? 0.f : exp2f(m - mn), f = a.x == -INFINITY ? 0.f : exp2f(a.x - mn);
+    l = l * old + warp_sum(a.y * f);
+    m = mn;
 #pragma unroll
-        for (int j = 0; j < C; ++j) acc[j] += g == 0.f ? 0.f : v[j] * g;        // a part without weights has no sums
+    for (int j = 0; j < C; ++j) acc[j] *= old;
+    for (int x1 = 0; x1 < here; x1 += AHEAD) {
+      if (x1) ask(x1);
+#pragma unroll
+      for (int x = 0; x < AHEAD; ++x) {
+        const float g = __shfl_sync(0xffffffffu, f, (x1 + x) & 31);
+#pragma unroll
+        for (int j = 0; j < C; ++j) acc[j] += x1 + x >= here || g == 0.f ? 0.f : v[x][j] * g;        // a part without weights has no sums
       }
     }
   }
-  template <typename T>
-  NXD_DEVICE void store(T* row) const {
-    T* dst = row + (threadIdx.x & 31) * C;
+  T* dst = row + lane * C;
 #pragma unroll
-    for (int j = 0; j < C; ++j) dst[j] = from_f32<T>(l == 0.f ? 0.f : acc[j] / l);
-  }
-};
+  for (int j = 0; j < C; ++j) dst[j] = from_f32<T>(l == 0.f ? 0.f : acc[j] / l);
+}
 
 // Rows of an entry none of whose tokens sees a key, or counts: zeros.  (With shared pages the last launch writes all rows.)
 template <typename T, int D, int THREADS>

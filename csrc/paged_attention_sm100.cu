@@ -223,9 +223,10 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
 
   // registers: 128 a thread at launch, 2 x 168 + 88 + 88 = 4 x 128 from here on
   Place at;
+  const bool late = !SHARED && p.shared > 0;       // the launch in front has waited for what is read here, and writes none of it (paged.cuh)
   if (warp >= 8) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-    pdl_wait();
+    if (!late) pdl_wait();
     pdl_trigger();                                 // behind the allocation; the last launch waits for this grid
     at = find_place<256, SHARED, 256>(p, gridDim.x, blockIdx.x);
   }
@@ -378,9 +379,9 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       load_q(it, q, tile, own);
     };
     Item it = next_item();
-    if (it.n > 0)                                  // the first piece's rows: the softmax warps brought them
+    if (it.n > 0)
       for (int t = 0; t < (PAIR ? 2 : 1); ++t)
-        if (!PAIR || (t ? it.n1 : it.n0) > 0) q_loads ^= 1u << t;
+        if (!PAIR || (t ? it.n1 : it.n0) > 0) load_rows(it, t, t);
     for (int il = 0; it.n > 0; ++il) {
       const Item nx = next_item();
       // the next item's rows before this one's sums: the products wait for those rows before they have issued the last of this item's
@@ -542,8 +543,9 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     const uint64_t sl2_2 = pack2(sl2, sl2);
     int g = 0, items = 0, pos0 = 0, tile0 = 0;
     // A piece of one step in front of the first works on whatever there is and leaves nothing behind (its weights go over the sums, which the first
-    // product does not add to): a step's 15 KB of instructions come from memory while the place is found and the first keys come.  Without it the
-    // first step took 3 to 5 us.
+    // product does not add to): a step's 10 KB of instructions come from memory, a part by each warp, while the place is found and the first keys
+    // come.  Without it the first step took 3 to 5 us.
+    const int part_of_step = warp;
     bool dry = true;
     Item it{};
     it.n0 = it.n1 = 1;
@@ -558,7 +560,6 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       const int sees_lo = __reduce_min_sync(0xffffffffu, sees);
       const bool rows_here = dry || __any_sync(0xffffffffu, live);             // otherwise the warp lets the scores be what they are
       float m_ref = -INFINITY, l = 0.f;
-      if (!dry && piece == 1 && (PAIR || t == 0)) load_q(it, t, t, own);       // the first piece's rows, which nobody else brings
       for (int j = 0; j < nt; ++j) {
         const int jt = PAIR ? j : 2 * j + t, key0 = key_at(it.j0 + jt), pos = pos0 + ring_at(t, j);
         if (!dry) wait(my_s, (uint32_t)(g++ & 1));
@@ -567,37 +568,33 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         const uint32_t tP = dry ? tO : tS;
         uint32_t hole;                             // written before the keys' barrier, which the products waited for
         asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(hole) : "r"(holes + ((tile0 + jt) % kHoles) * 4) : "memory");
+        const int lim = sees - 1 - key0;           // last column that this row sees
+        if (sees_lo - key0 < KEYS || (hole != 0 && !dry)) {
+          // what is not seen becomes -inf where the scores lie, sixteen columns at a time: seldom, and few instructions to have at hand
+          const int from = hole ? 0 : max(0, sees_lo - key0) >> 4;
+#pragma unroll 1
+          for (int c = from; c < KEYS / 16; ++c) {
+            uint32_t r[16];
+            tcgen05_ld_32x16(tS + c * 16, r);
+            tcgen05_wait_ld();
+            const int end = hole >> (c * 16 / box) & 1 ? -1 : lim - c * 16;
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+              if (i > end) r[i] = 0xff800000u;
+            tcgen05_st_32x16(tS + c * 16, r);
+          }
+          tcgen05_wait_st();
+        }
         uint32_t sr[Q][32];
 #pragma unroll
         for (int c = 0; c < Q; ++c) tcgen05_ld_32x32(tS + c * 32, sr[c]);
         tcgen05_wait_ld();
-        if (dry) hole = 0;
-        const int lim = sees - 1 - key0, lim_lo = sees_lo - 1 - key0;            // last column that is seen
-        if (lim_lo < KEYS - 1) {
-#pragma unroll
-          for (int c = 0; c < Q; ++c)
-            if (lim_lo < c * 32 + 31) fwd_mask(sr[c], lim - c * 32);
-        }
-        if (hole) {
-#pragma unroll
-          for (int c = 0; c < Q; ++c)
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (hole >> ((c * 32 + i) / box) & 1) sr[c][i] = 0xff800000u;
-        }
-        if (j == 0) {
-          float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int i = 0; i < 32; i += 2)
-#pragma unroll
-            for (int c = 0; c < Q; ++c) m4[c] = max3(m4[c], __uint_as_float(sr[c][i]), __uint_as_float(sr[c][i + 1]));
-          m_ref = fmaxf(max3(m4[0], m4[1], m4[2]), m4[3]);
-        }
-        float base = m_ref == -INFINITY ? 0.f : m_ref;       // a row that has seen nothing yet
+        float base = m_ref == -INFINITY ? 0.f : m_ref;       // a row that has seen nothing yet: its first quarter is done again below
         uint64_t shift = pack2(-base * sl2, -base * sl2), sum[Q] = {};
         float mx, unused;
-        exps<T, Q, true>(sr, 0, sl2_2, shift, sum[0], mx);
-        const bool need = !dry && ((mx - base) * sl2 > 8.f || (m_ref == -INFINITY && mx > -INFINITY));
+        mx = -INFINITY;
+        if (!dry || part_of_step == 0) exps<T, Q, true>(sr, 0, sl2_2, shift, sum[0], mx);
+        const bool need = dry ? part_of_step == 4 : (mx - base) * sl2 > 8.f || (m_ref == -INFINITY && mx > -INFINITY);
         if (__any_sync(0xffffffffu, need)) {
           const float f = !need ? 1.f : m_ref == -INFINITY ? 0.f : ex2((m_ref - mx) * sl2);
           if (need) m_ref = base = mx;
@@ -616,12 +613,6 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
           }
           tcgen05_ld_32x32(tS, sr[0]);
           tcgen05_wait_ld();
-          if (lim_lo < 31) fwd_mask(sr[0], lim);
-          if (hole) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (hole >> (i / box) & 1) sr[0][i] = 0xff800000u;
-          }
           sum[0] = 0ull;
           exps<T, Q, false>(sr, 0, sl2_2, shift, sum[0], unused);
         }
@@ -629,6 +620,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         tcgen05_st_32x16p(tP, sr[0]);
 #pragma unroll
         for (int c = 1; c < Q; ++c) {
+          if (dry && part_of_step != c) continue;
           exps<T, Q, false>(sr, c, sl2_2, shift, sum[c], unused);
           tcgen05_st_32x16p(tP + c * 16, sr[c]);
         }
@@ -661,12 +653,13 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       }
       }
       if (!dry) { pos0 += 2 * it.n; tile0 += it.n; }
-      if (dry) pdl_wait();
+      if (dry && !late) pdl_wait();
       dry = false;
       it = next_item();
       if (it.n == 0) break;
     }
   }
+  if (late) pdl_wait();
   tcgen05_fence_before();
   __syncthreads();
   if (warp == 13) tcgen05_dealloc(tmem_base, 512);

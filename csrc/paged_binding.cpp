@@ -128,7 +128,7 @@ Tensor paged_attention(const Tensor& q_, const Tensor& kc, const Tensor& vc, con
   Tensor work;
   if (plan.slots + plan.pre_slots > 0) work = at::empty({(plan.slots + plan.pre_slots) * (D + 2)}, q.options().dtype(at::kFloat));
   p.part_o = work.defined() ? work.data_ptr<float>() : nullptr;
-  p.pre_o = p.part_o + plan.slots * D;
+  p.pre_o = p.part_o + plan.slots * D;             // join_parts counts on this order
   p.part_ml = p.pre_o + plan.pre_slots * D;
   p.pre_ml = p.part_ml + plan.slots * 2;
   p.scale_log2 = (float)(scale * 1.4426950408889634);
