@@ -9,80 +9,75 @@
 
 namespace nxd {
 
+int device_sm_count();
+
 namespace {
 
 // ---------------------------------------------------------------------------------------------------------------- append
 // x' = (a cos − b sin, b cos + a sin), a and b the halves of a head, angle by the token's position: q to q_out, k into its page, v as it is
-// beside it.  Bound by HBM: every number is read and written once; a thread turns 16 bytes of each half.
+// beside it.  Bound by HBM: every number is read and written once.  A thread has 16 bytes of each half of one head, a block as many as it can of one
+// token, whose position, page, cosines and sines its threads share in L1.
+struct AppendArgs {
+  const void *q, *k, *v;
+  const long *positions, *lens;
+  const float *cos_t, *sin_t;
+  void *q_out, *kc, *vc;
+  const int* table;
+  int B, W, H, Hkv, half, rows, cols, ps, pages, parts;    // parts: blocks of a token
+  long table_sb, q_sb, q_sw, q_sh, k_sb, k_sw, k_sh, v_sb, v_sw, v_sh, o_sb, o_sw, kc_sp, kc_sr, kc_sh, vc_sp, vc_sr, vc_sh;
+};
+constexpr int kAppendThreads = 128;
 template <typename T>
-__global__ void __launch_bounds__(256) paged_append_kernel(
-    const T* q, const T* k, const T* v, const long* positions, const long* lens, const float* cos_t, const float* sin_t, T* q_out, T* kc, T* vc,
-    const int* table, int B, int W, int H, int Hkv, int half, int rows, int cols, int ps, int pages, long table_sb, long q_sb, long q_sw, long q_sh,
-    long k_sb, long k_sw, long k_sh, long v_sb, long v_sw, long v_sh, long o_sb, long o_sw, long kc_sp, long kc_sr, long kc_sh, long vc_sp, long vc_sr,
-    long vc_sh, long items) {
+__global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const AppendArgs p) {
   constexpr int N = Pack16<T>::N;
   pdl_trigger();
+  const unsigned t = blockIdx.x / p.parts, item = blockIdx.x % p.parts * kAppendThreads + threadIdx.x, chunks = p.half / N;
+  const int h = (int)(item / chunks), c = (int)(item % chunks) * N;
+  const int w = (int)(t / p.B), b = (int)(t % p.B);        // tokens of all sequences beside one another, as projections leave them
   pdl_wait();
-  const long i = (long)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= items) return;
-  const int per_head = half / N, heads = H + 2 * Hkv;
-  const int c = (int)(i % per_head) * N;
-  const long j = i / per_head;
-  const int h = (int)(j % heads);
-  const long t = j / heads;
-  const int b = (int)(t % B), w = (int)(t / B);            // tokens of all sequences beside one another, as projections leave them
-  const long first = positions[b];
-  const long m = lens ? lens[b] : W, pos = first + w;
-  const bool live = first >= 0 && w < m && pos < rows;
+  if (h >= p.H + 2 * p.Hkv) return;
+  const long first = p.positions[b], m = p.lens ? p.lens[b] : p.W, pos = first + w;
+  const bool live = first >= 0 && w < m && pos < p.rows, query = h < p.H, key = h < p.H + p.Hkv;
+  T* const q_out = (T*)p.q_out + b * p.o_sb + w * p.o_sw + (long)h * (2 * p.half) + c;
   Pack16<T> lo, hi;
-  if (h < H) {
-    T* dst = q_out + b * o_sb + w * o_sw + (long)h * (2 * half) + c;
-    if (!live) {
+  if (!live) {
+    if (query) {
 #pragma unroll
       for (int e = 0; e < N; ++e) { lo.set(e, 0.f); hi.set(e, 0.f); }
-      lo.store(dst);
-      hi.store(dst + half);
-      return;
+      lo.store(q_out);
+      hi.store(q_out + p.half);
     }
-    const T* src = q + b * q_sb + w * q_sw + h * q_sh + c;
-    lo.load(src);
-    hi.load(src + half);
-    const float *cs = cos_t + pos * half + c, *sn = sin_t + pos * half + c;
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const float x = lo.f(e), y = hi.f(e);
-      lo.set(e, x * cs[e] - y * sn[e]);
-      hi.set(e, y * cs[e] + x * sn[e]);
-    }
-    lo.store(dst);
-    hi.store(dst + half);
     return;
   }
-  if (!live || pos / ps >= cols) return;
-  const int page = table[b * table_sb + pos / ps], row = (int)(pos % ps);
-  if (page < 0 || page >= pages) return;
-  if (h < H + Hkv) {
-    const T* src = k + b * k_sb + w * k_sw + (h - H) * k_sh + c;
-    T* dst = kc + page * kc_sp + row * kc_sr + (h - H) * kc_sh + c;
-    lo.load(src);
-    hi.load(src + half);
-    const float *cs = cos_t + pos * half + c, *sn = sin_t + pos * half + c;
-#pragma unroll
-    for (int e = 0; e < N; ++e) {
-      const float x = lo.f(e), y = hi.f(e);
-      lo.set(e, x * cs[e] - y * sn[e]);
-      hi.set(e, y * cs[e] + x * sn[e]);
-    }
-    lo.store(dst);
-    hi.store(dst + half);
-  } else {
-    const T* src = v + b * v_sb + w * v_sw + (h - H - Hkv) * v_sh + c;
-    T* dst = vc + page * vc_sp + row * vc_sr + (h - H - Hkv) * vc_sh + c;
-    lo.load(src);
-    hi.load(src + half);
-    lo.store(dst);
-    hi.store(dst + half);
+  const T* const src = (query ? (const T*)p.q + b * p.q_sb + w * p.q_sw + h * p.q_sh
+                        : key ? (const T*)p.k + b * p.k_sb + w * p.k_sw + (h - p.H) * p.k_sh
+                              : (const T*)p.v + b * p.v_sb + w * p.v_sw + (h - p.H - p.Hkv) * p.v_sh) + c;
+  lo.load(src);
+  hi.load(src + p.half);
+  T* dst = q_out;
+  if (!query) {
+    const int column = (int)pos / p.ps, row = (int)pos - column * p.ps;            // positions with a place in the tables fit
+    const int page = column < p.cols ? p.table[b * p.table_sb + column] : -1;
+    if (page < 0 || page >= p.pages) return;
+    dst = key ? (T*)p.kc + page * p.kc_sp + row * p.kc_sr + (h - p.H) * p.kc_sh + c
+              : (T*)p.vc + page * p.vc_sp + row * p.vc_sr + (h - p.H - p.Hkv) * p.vc_sh + c;
   }
+  if (key) {
+    const float *cs = p.cos_t + pos * p.half + c, *sn = p.sin_t + pos * p.half + c;
+#pragma unroll
+    for (int e = 0; e < N; e += 4) {
+      const float4 co = *reinterpret_cast<const float4*>(cs + e), si = *reinterpret_cast<const float4*>(sn + e);
+      const float cf[4] = {co.x, co.y, co.z, co.w}, sf[4] = {si.x, si.y, si.z, si.w};
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float x = lo.f(e + i), y = hi.f(e + i);
+        lo.set(e + i, x * cf[i] - y * sf[i]);
+        hi.set(e + i, y * cf[i] + x * sf[i]);
+      }
+    }
+  }
+  lo.store(dst);
+  hi.store(dst + p.half);
 }
 
 // ------------------------------------------------------------------------------------------------------- attention, few rows
@@ -544,8 +539,6 @@ void launch(const PagedAttn& p, const PagedPlan& plan, int dt, cudaStream_t st) 
 
 }  // namespace
 
-int device_sm_count();
-
 // Up to 16 query rows of a sequence and key/value head go to the kernel above, more to tiles of 128 or 256 rows on the tensor memory.
 PagedPlan paged_plan(PagedAttn& p) {
   PagedPlan plan{};
@@ -601,16 +594,16 @@ void paged_append(const void* q, const void* k, const void* v, const long* posit
                   void* q_out, void* kc, void* vc, const int* table, int B, int W, int H, int Hkv, int D, int rows, int cols, int ps, int pages,
                   long table_sb, const long (*s)[3], long o_sb, long o_sw, const long (*cs)[3], int dt, cudaStream_t st) {
   const int half = D / 2;
-  const long items = (long)B * W * (H + 2 * Hkv) * (half / (dt == kF32 ? 4 : 8));
-  if (items == 0) return;
-#define NXD_APPEND(T)                                                                                                                              \
-  launch_dependent(paged_append_kernel<T>, (unsigned)((items + 255) / 256), 256, 0, st, (const T*)q, (const T*)k, (const T*)v, positions, lens,      \
-                   cos_t, sin_t, (T*)q_out, (T*)kc, (T*)vc, table, B, W, H, Hkv, half, rows, cols, ps, pages, table_sb, s[0][0], s[0][1], s[0][2],   \
-                   s[1][0], s[1][1], s[1][2], s[2][0], s[2][1], s[2][2], o_sb, o_sw, cs[0][0], cs[0][1], cs[0][2], cs[1][0], cs[1][1], cs[1][2], items)
-  if (dt == kBF16) NXD_APPEND(__nv_bfloat16);
-  else if (dt == kF16) NXD_APPEND(__half);
-  else NXD_APPEND(float);
-#undef NXD_APPEND
+  const long tokens = (long)B * W, items = (long)(H + 2 * Hkv) * (half / (dt == kF32 ? 4 : 8)), parts = (items + kAppendThreads - 1) / kAppendThreads;
+  if (tokens == 0) return;
+  if (tokens * parts >= (1l << 31)) nxd_throw("paged_append: too many tokens", __FILE__, __LINE__);
+  const AppendArgs a{q, k, v, positions, lens, cos_t, sin_t, q_out, kc, vc, table, B, W, H, Hkv, half, rows, cols, ps, pages, (int)parts,
+                     table_sb, s[0][0], s[0][1], s[0][2], s[1][0], s[1][1], s[1][2], s[2][0], s[2][1], s[2][2], o_sb, o_sw,
+                     cs[0][0], cs[0][1], cs[0][2], cs[1][0], cs[1][1], cs[1][2]};
+  const unsigned grid = (unsigned)(tokens * parts);
+  if (dt == kBF16) launch_dependent(paged_append_kernel<__nv_bfloat16>, grid, kAppendThreads, 0, st, a);
+  else if (dt == kF16) launch_dependent(paged_append_kernel<__half>, grid, kAppendThreads, 0, st, a);
+  else launch_dependent(paged_append_kernel<float>, grid, kAppendThreads, 0, st, a);
 }
 
 }  // namespace nxd

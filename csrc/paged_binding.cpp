@@ -53,6 +53,13 @@ void check_cache(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tens
   CHECK_ARG(q.size(0) < (1 << 20) && q.size(1) < (1 << 24) && q.size(0) * q.size(1) * q.size(2) < (1ll << 30), "too many query rows: " + list(q.sizes()));
 }
 
+// Numbers of another type, or not one after the other, are converted
+Tensor ints(const Tensor& t, at::ScalarType type) { return t.scalar_type() == type && t.is_contiguous() ? t : t.to(type).contiguous(); }
+c10::optional<Tensor> ints(const c10::optional<Tensor>& t, at::ScalarType type) { return t.has_value() ? c10::optional<Tensor>(ints(*t, type)) : t; }
+Tensor as_table(const Tensor& t) {
+  return t.scalar_type() == at::kInt && (t.dim() != 2 || t.size(1) <= 1 || t.stride(1) == 1) ? t : t.to(at::kInt).contiguous();
+}
+
 // Whether the append kernel takes these: 32- or 16-bit types, halves of heads and cache rows of whole 16-byte packets
 bool paged_append_ok(const Tensor& q, const Tensor& kc, const Tensor& vc) {
   return q.dim() == 4 && kc.dim() == 4 && vc.dim() == 4 && (half_type(q) || q.scalar_type() == at::kFloat) && q.size(3) * q.element_size() % 32 == 0 && packets(kc) && packets(vc);
@@ -68,8 +75,10 @@ Tensor rows_out(const Tensor& q) {
   return at::empty_strided({B, W, H, D}, {H * D, B * H * D, D, 1}, q.options());
 }
 
-Tensor paged_append(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& positions, const Tensor& cos_t, const Tensor& sin_t, Tensor kc,
-                    Tensor vc, const Tensor& table, const c10::optional<Tensor>& lens) {
+Tensor paged_append(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& positions_, const Tensor& cos_t, const Tensor& sin_t, Tensor kc,
+                    Tensor vc, const Tensor& table_, const c10::optional<Tensor>& lens_) {
+  const Tensor positions = ints(positions_, at::kLong), table = as_table(table_);
+  const c10::optional<Tensor> lens = ints(lens_, at::kLong);
   check_cache(q_, kc, vc, table, positions, lens);
   CHECK_ARG(k_.sizes() == v_.sizes() && k_.dim() == 4 && k_.size(0) == q_.size(0) && k_.size(1) == q_.size(1) && k_.size(2) == kc.size(2) &&
             k_.size(3) == q_.size(3), "new keys and values must be " + list({q_.size(0), q_.size(1), kc.size(2), q_.size(3)}));
@@ -80,20 +89,22 @@ Tensor paged_append(const Tensor& q_, const Tensor& k_, const Tensor& v_, const 
             "cos and sin must be contiguous float32 tables [positions, " + std::to_string(q_.size(3) / 2) + "]");
   CHECK_ARG(q_.is_cuda() && paged_append_ok(q_, kc, vc), "the kernel takes caches of whole 16-byte packets");
   c10::cuda::CUDAGuard guard(q_.device());
-  const Tensor q = as_packets(q_), k = as_packets(k_), v = as_packets(v_);
+  const Tensor q = as_packets(q_), k = as_packets(k_), v = as_packets(v_), cos_p = as_packets(cos_t), sin_p = as_packets(sin_t);
   Tensor out = rows_out(q);
   if (q.size(0) == 0 || q.size(1) == 0) return out;
   const long s[3][3] = {{q.stride(0), q.stride(1), q.stride(2)}, {k.stride(0), k.stride(1), k.stride(2)}, {v.stride(0), v.stride(1), v.stride(2)}};
   const long cs[2][3] = {{kc.stride(0), kc.stride(1), kc.stride(2)}, {vc.stride(0), vc.stride(1), vc.stride(2)}};
   nxd::paged_append(q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr<long>(), lens.has_value() ? lens->data_ptr<long>() : nullptr,
-                    cos_t.data_ptr<float>(), sin_t.data_ptr<float>(), out.data_ptr(), kc.data_ptr(), vc.data_ptr(), table.data_ptr<int>(), (int)q.size(0),
+                    cos_p.data_ptr<float>(), sin_p.data_ptr<float>(), out.data_ptr(), kc.data_ptr(), vc.data_ptr(), table.data_ptr<int>(), (int)q.size(0),
                     (int)q.size(1), (int)q.size(2), (int)kc.size(2), (int)q.size(3), (int)cos_t.size(0), (int)table.size(1), (int)kc.size(1),
                     (int)kc.size(0), table.stride(0), s, out.stride(0), out.stride(1), cs, dt_code(q), stream());
   return out;
 }
 
-Tensor paged_attention(const Tensor& q_, const Tensor& kc, const Tensor& vc, const Tensor& table, const Tensor& positions, double scale,
-                       const c10::optional<Tensor>& lens, const c10::optional<Tensor>& shared_pages) {
+Tensor paged_attention(const Tensor& q_, const Tensor& kc, const Tensor& vc, const Tensor& table_, const Tensor& positions_, double scale,
+                       const c10::optional<Tensor>& lens_, const c10::optional<Tensor>& shared_pages_) {
+  const Tensor positions = ints(positions_, at::kLong), table = as_table(table_);
+  const c10::optional<Tensor> lens = ints(lens_, at::kLong), shared_pages = ints(shared_pages_, at::kInt);
   check_cache(q_, kc, vc, table, positions, lens);
   CHECK_ARG(q_.is_cuda() && paged_attention_ok(q_, kc, vc), "the kernels take 16-bit types, heads of 64 or 128 numbers and caches of whole 16-byte packets");
   const int64_t ps = kc.size(1);

@@ -14,34 +14,34 @@ namespace nxd {
 
 namespace {
 
-constexpr int kThreads = 512, kWarps = kThreads / 32;
+constexpr int kThreads = 256, kWarps = kThreads / 32;
+constexpr int kAhead = 4;                                  // steps of a warp whose numbers are asked for at once
+constexpr int kParts = 32 / kWarps;                        // sums that a warp keeps: one for each lane of a block's search
 
+// N numbers of p and of q (0 where there is none, or behind the row's end)
 template <typename T, int N>
-NXD_DEVICE void load_weights(const T* p, const T* q, int v, int V, bool packets, double (&w)[N], double& plain) {
-  float a[N], b[N];
-  if (packets) {
-    Pack16<T> x;
-    x.load(p + v);
+struct Pair {
+  Pack16<T> a, b;
+  NXD_DEVICE void load(const T* p, const T* q, int v, int V, bool packets) {
+    if (packets && v < V) {
+      a.load(p + v);
+      if (q) b.load(q + v);
+    } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) a[i] = x.f(i);
-    if (q) x.load(q + v);
-#pragma unroll
-    for (int i = 0; i < N; ++i) b[i] = q ? x.f(i) : 0.f;
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      a[i] = v + i < V ? to_f32<T>(p[v + i]) : 0.f;
-      b[i] = q && v + i < V ? to_f32<T>(q[v + i]) : 0.f;
+      for (int i = 0; i < N; ++i) {
+        a.v[i] = v + i < V ? p[v + i] : from_f32<T>(0.f);
+        b.v[i] = q && v + i < V ? q[v + i] : from_f32<T>(0.f);
+      }
     }
-  }
-  plain = 0;
+    if (!q)
 #pragma unroll
-  for (int i = 0; i < N; ++i) {
-    const double x = (double)a[i], d = x - (double)b[i];
-    w[i] = d > 0 ? d : 0;                                  // NaN: 0
-    plain += x > 0 ? x : 0;
+      for (int i = 0; i < N; ++i) b.v[i] = from_f32<T>(0.f);
   }
-}
+  NXD_DEVICE double weight(int i) const {
+    const double d = (double)a.f(i) - (double)b.f(i);
+    return d > 0 ? d : 0;                                  // NaN: 0
+  }
+};
 
 NXD_DEVICE double warp_sum64(double v) {
 #pragma unroll
@@ -55,15 +55,16 @@ NXD_DEVICE double remote_double(const double* at, int rank) {
   return v;
 }
 
-// One cluster per sequence: each block sums a stretch of the vocabulary, each warp a stretch of the block's; where the drawn share of the sum lies
-// is found from the sums, and the one warp that has it walks its stretch again (out of L2).  Bound by HBM: one row of p and one of q; one
-// sequence alone by its chain of drafted tokens, their probabilities, the walk and the exchange.
+// One cluster per sequence: each block sums a stretch of the vocabulary in 32 parts; where the drawn share of the sum lies is found from the sums,
+// and a warp walks the one part that has it again (out of L2).  Bound by HBM, one row of p and one of q, and by its chain: the drafted tokens, their
+// probabilities, the walk, the exchange of sums, the second walk.  Blocks of 256 threads, so that all of a batch of 64 are there at once: with 512
+// they came in two to four rounds and 64 x 7 drafts over 100352 tokens took 24 to 47 us.
 template <typename T>
-__global__ void __launch_bounds__(kThreads) verify_kernel(const long* tokens, const T* draft, const T* target, const float* accept, const float* sample,
+__global__ void __launch_bounds__(kThreads, 4) verify_kernel(const long* tokens, const T* draft, const T* target, const float* accept, const float* sample,
                                                           long* out, long* accepted, int K, int V, long d_sb, long d_sk, long t_sb, long t_sk) {
   constexpr int N = Pack16<T>::N, STEP = 32 * N;
-  __shared__ double sums[2][kWarps];                       // of max(p − q, 0) and of p
-  __shared__ double block_sums[2];
+  __shared__ double sums[32];
+  __shared__ double block_sum;
   __shared__ int refused, bonus;
   const int rank = (int)cluster_ctarank(), size = (int)gridDim.x, b = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_trigger();
@@ -90,89 +91,100 @@ __global__ void __launch_bounds__(kThreads) verify_kernel(const long* tokens, co
   __syncthreads();
   const int n = refused;
   const T* const p = target + b * t_sb + n * t_sk;
-  const T* const q = bonus ? nullptr : draft + b * d_sb + n * d_sk;
+  const T* q = bonus ? nullptr : draft + b * d_sb + n * d_sk;
   const bool packets = (uintptr_t)p % 16 == 0 && (uintptr_t)q % 16 == 0 && V % N == 0;
-  // steps of STEP numbers, the same number for every warp of the cluster
-  const int steps = (V + STEP - 1) / STEP, per = (steps + size * kWarps - 1) / (size * kWarps), s0 = (rank * kWarps + warp) * per, s1 = min(steps, s0 + per);
-  double sum = 0, sum_p = 0;
-#pragma unroll 4
-  for (int s = s0; s < s1; ++s) {
-    const int v = s * STEP + lane * N;
-    if (v < V) {
-      double w[N], all;
-      load_weights<T, N>(p, q, v, V, packets, w, all);
+  // steps of STEP numbers: `per` to a part, the same number for every part of the cluster
+  const int steps = (V + STEP - 1) / STEP, all = size * 32, per = (steps + all - 1) / all;
+  auto first_step = [&](int part) { return min((long)steps, (long)(rank * 32 + part) * per); };
+  // sum of this block's weights, by parts; q null: of p alone
+  auto add_up = [&](const T* q) {
+#pragma unroll 1
+    for (int i = 0; i < kParts; ++i) {
+      const int part = warp * kParts + i, s1 = (int)first_step(part + 1);
+      double sum = 0;
+      for (int s = (int)first_step(part); s < s1; s += kAhead) {
+        Pair<T, N> x[kAhead];
 #pragma unroll
-      for (int i = 0; i < N; ++i) sum += w[i];
-      sum_p += all;
+        for (int a = 0; a < kAhead; ++a) x[a].load(p, q, s + a < s1 ? (s + a) * STEP + lane * N : V, V, packets);
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a)
+#pragma unroll
+          for (int j = 0; j < N; ++j) sum += x[a].weight(j);
+      }
+      sum = warp_sum64(sum);
+      if (lane == 0) sums[part] = sum;
     }
+    __syncthreads();
+    if (warp == 0) {
+      const double x = warp_sum64(sums[lane]);
+      if (lane == 0) block_sum = x;
+    }
+    cluster_sync_all();
+    double total = 0;
+    for (int r = 0; r < size; ++r) total += remote_double(&block_sum, r);
+    return total;
+  };
+  double total = add_up(q);
+  if (q && !(total > 0)) {                                 // nothing is left of p - q: from p itself
+    cluster_sync_all();                                    // every block has read the sums
+    q = nullptr;
+    total = add_up(q);
   }
-  sum = warp_sum64(sum);
-  sum_p = warp_sum64(sum_p);
-  if (lane == 0) { sums[0][warp] = sum; sums[1][warp] = sum_p; }
-  __syncthreads();
-  if (threadIdx.x < 2) {
-    double x = 0;
-#pragma unroll
-    for (int w = 0; w < kWarps; ++w) x += sums[threadIdx.x][w];
-    block_sums[threadIdx.x] = x;
-  }
-  cluster_sync_all();
   if (warp == 0) {
-    double total[2] = {0, 0};
-    for (int r = 0; r < size; ++r) {
-      total[0] += remote_double(&block_sums[0], r);
-      total[1] += remote_double(&block_sums[1], r);
-    }
-    const int which = total[0] > 0 ? 0 : 1;                // nothing left of p - q: from p itself
-    const double want = (double)sample[b] * total[which];
-    // the block, then the warp, in which the running sum passes `want`; if roundings leave none, the last that has anything
+    const double want = (double)sample[b] * total;
+    // the block, then the part, in which the running sum passes `want`; if roundings leave none, the last that has anything
     double before = 0, base = 0;
     int mine = -1;
     for (int r = 0; r < size; ++r) {
-      const double x = remote_double(&block_sums[which], r);
+      const double x = remote_double(&block_sum, r);
       if (x > 0) { mine = r; base = before; }
       before += x;
       if (x > 0 && before > want) break;
     }
     if (mine == rank) {
-      int at = -1;
-      double start = base;
-      before = base;
-      for (int w = 0; w < kWarps; ++w) {
-        const double x = sums[which][w];
-        if (x > 0) { at = w; start = before; }
-        before += x;
-        if (x > 0 && before > want) break;
+      const double x = sums[lane];
+      double scan = x;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const double y = __shfl_up_sync(0xffffffffu, scan, o);
+        if (lane >= o) scan += y;
       }
-      const T* const qq = which ? nullptr : q;
-      const int f0 = (rank * kWarps + at) * per, f1 = min(steps, f0 + per);
+      const unsigned some = __ballot_sync(0xffffffffu, x > 0), past = __ballot_sync(0xffffffffu, x > 0 && base + scan > want);
+      const int at = past ? __ffs(past) - 1 : 31 - __clz(some);
+      double start = base + __shfl_sync(0xffffffffu, scan - x, at);
+      const int f0 = (int)first_step(at), f1 = (int)first_step(at + 1);
       long chosen = -1, last = -1;
-      for (int s = f0; s < f1 && chosen < 0; ++s) {
-        const int v = s * STEP + lane * N;
-        double w[N], all, part = 0;
+      for (int s = f0; s < f1 && chosen < 0; s += kAhead) {
+        Pair<T, N> x[kAhead];
 #pragma unroll
-        for (int i = 0; i < N; ++i) w[i] = 0;
-        if (v < V) load_weights<T, N>(p, qq, v, V, packets, w, all);
-        int hit = -1, tail = -1;
+        for (int i = 0; i < kAhead; ++i) x[i].load(p, q, s + i < f1 ? (s + i) * STEP + lane * N : V, V, packets);
 #pragma unroll
-        for (int i = 0; i < N; ++i) part += w[i];
-        double scan = part;
+        for (int i = 0; i < kAhead; ++i) {
+          double part = 0;
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const double x = __shfl_up_sync(0xffffffffu, scan, o);
-          if (lane >= o) scan += x;
+          for (int j = 0; j < N; ++j) part += x[i].weight(j);
+          double scan = part;
+#pragma unroll
+          for (int o = 1; o < 32; o <<= 1) {
+            const double y = __shfl_up_sync(0xffffffffu, scan, o);
+            if (lane >= o) scan += y;
+          }
+          double run = start + (scan - part);
+          int hit = -1, tail = -1;
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            const double w = x[i].weight(j);
+            run += w;
+            if (w > 0) tail = j;
+            if (hit < 0 && w > 0 && run > want) hit = j;
+          }
+          const int v = (s + i) * STEP;
+          const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), tails = __ballot_sync(0xffffffffu, tail >= 0);
+          const int first = __ffs(hits) - 1, end = 31 - __clz(tails);
+          if (chosen < 0 && hits) chosen = v + first * N + __shfl_sync(0xffffffffu, hit, first);
+          if (tails) last = v + end * N + __shfl_sync(0xffffffffu, tail, end);
+          start += __shfl_sync(0xffffffffu, scan, 31);
         }
-        double run = start + (scan - part);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-          run += w[i];
-          if (w[i] > 0) tail = v + i;
-          if (hit < 0 && w[i] > 0 && run > want) hit = v + i;
-        }
-        const unsigned hits = __ballot_sync(0xffffffffu, hit >= 0), tails = __ballot_sync(0xffffffffu, tail >= 0);
-        if (hits) chosen = __shfl_sync(0xffffffffu, hit, __ffs(hits) - 1);
-        else if (tails) last = __shfl_sync(0xffffffffu, tail, 31 - __clz(tails));
-        start += __shfl_sync(0xffffffffu, scan, 31);
       }
       if (lane == 0) out[(long)b * (K + 1) + n] = chosen >= 0 ? chosen : last;
     }
@@ -193,9 +205,9 @@ int device_sm_count();
 void verify_drafts(const long* tokens, const void* draft, const void* target, const float* accept, const float* sample, long* out, long* accepted,
                    int B, int K, int V, const long* draft_s, const long* target_s, int dt, cudaStream_t st) {
   if (B == 0) return;
-  // about two blocks per SM in all, and no block with less than a step for every second warp
+  // two blocks per SM and more, and no block with less than a step for every second warp
   int size = 1;
-  while (size < 8 && (long)B * size < device_sm_count() && V / (2 * size) >= 4096) size *= 2;
+  while (size < 8 && (long)B * size < 2 * device_sm_count() && V / (2 * size) >= 2048) size *= 2;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(size, B);
   cfg.blockDim = kThreads;

@@ -63,11 +63,11 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     to the pages, in one launch.  ``cos`` / ``sin [positions, D / 2]`` fp32: :func:`ops.rope.rope_tables`.  Tokens that do not count, or that stand
     behind the tables' end, come back as zeros and are not written; tokens behind the page table's end are not written."""
     _no_gradient("rope_append", q, k, v, k_cache, v_cache)
-    positions, page_table = _ints(positions, torch.long), _table(page_table)
-    lens = None if lens is None else _ints(lens, torch.long)
-    if _ext.use_cuda(q, k_cache, v_cache) and _ext._load().paged_append_ok(q, k_cache, v_cache):
+    if _ext.use_cuda(q) and _ext._load().paged_append_ok(q, k_cache, v_cache):
         _ext.count_launch()
         return _ext.ext().paged_append(q, k, v, positions, cos, sin, k_cache, v_cache, page_table, lens)
+    positions, page_table = _ints(positions, torch.long), _table(page_table)
+    lens = None if lens is None else _ints(lens, torch.long)
     _check(q, k_cache, v_cache, page_table, positions, lens)
     B, W, H, D = q.shape
     if k.shape != v.shape or tuple(k.shape) != (B, W, k_cache.shape[2], D):
@@ -107,13 +107,13 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pag
     first ``n`` columns of ``page_table`` are not looked at."""
     _no_gradient("paged attention", q, k_cache, v_cache)
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
+    if _ext.use_cuda(q) and _ext._load().paged_attention_ok(q, k_cache, v_cache):
+        _ext.count_launch(2 if shared_pages is None else 3)
+        return _ext.ext().paged_attention(q, k_cache, v_cache, page_table, positions, scale, lens, shared_pages)
     positions, page_table = _ints(positions, torch.long), _table(page_table)
     lens = None if lens is None else _ints(lens, torch.long)
     if shared_pages is not None:
         shared_pages = _ints(shared_pages, torch.int32)
-    if _ext.use_cuda(q, k_cache, v_cache) and _ext._load().paged_attention_ok(q, k_cache, v_cache):
-        _ext.count_launch(2 if shared_pages is None else 3)
-        return _ext.ext().paged_attention(q, k_cache, v_cache, page_table, positions, scale, lens, shared_pages)
     _check(q, k_cache, v_cache, page_table, positions, lens)
     if not 0 < scale < 1e30:
         raise ValueError("the scale of the scores is positive")

@@ -62,6 +62,9 @@ def test_append_takes_sections_and_odd_views():
         a = ops.paged.rope_append(q, k, v, positions, cos, sin, caches[0], caches[1], table)
         b = ops.paged.rope_append(q.contiguous(), k.contiguous(), v.contiguous(), positions, cos, sin, caches[2], caches[3], table)
         assert torch.equal(a, b) and torch.equal(caches[0], caches[2]) and torch.equal(caches[1], caches[3])
+        odd = torch.zeros(cos.numel() + 1, device="cuda")
+        odd[1:] = cos.flatten()
+        assert torch.equal(a, ops.paged.rope_append(q, k, v, positions, odd[1:].view_as(cos), sin, caches[2], caches[3], table))
 
 
 # --------------------------------------------------------------------------------------------------------------- attention
