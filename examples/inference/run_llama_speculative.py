@@ -4,6 +4,7 @@ forward — counterpart of the reference's ``examples/inference/run_llama_specul
 
   python examples/inference/run_llama_speculative.py --model tiny --speculation_length 4
   torchrun --nproc-per-node 8 examples/inference/run_llama_speculative.py --model 13b --draft_layers 4 --tp_degree 8
+  python examples/inference/run_llama_speculative.py --model tiny --page_size 32 --temperature 0.8 --batch_size 4
 """
 import argparse
 import os
@@ -20,7 +21,7 @@ sys.path.insert(0, os.path.join(ROOT, "examples", "training"))
 from neuronx_distributed_b200.models.llama import LlamaConfig, llama2_13b_config, llama2_7b_config  # noqa: E402
 from neuronx_distributed_b200.models.llama_inference import LlamaForInference  # noqa: E402
 from neuronx_distributed_b200.parallel_layers import parallel_state as ps  # noqa: E402
-from neuronx_distributed_b200.utils.speculative import speculative_generate  # noqa: E402
+from neuronx_distributed_b200.utils.speculative import speculative_generate, speculative_sample  # noqa: E402
 from training_utils import init_distributed  # noqa: E402
 
 
@@ -32,6 +33,9 @@ def main():
     p.add_argument("--prompt_length", type=int, default=32)
     p.add_argument("--max_new_tokens", type=int, default=32)
     p.add_argument("--speculation_length", type=int, default=4)
+    p.add_argument("--page_size", type=int, default=0, help="keep keys and values in pages of that many tokens (0: contiguous rows)")
+    p.add_argument("--temperature", type=float, default=0.0, help="above 0: sampled tokens, accepted against the target's probabilities")
+    p.add_argument("--batch_size", type=int, default=1, help="rows of the batch (sampling only)")
     a = p.parse_args()
     dev = init_distributed()
     ps.initialize_model_parallel(tensor_model_parallel_size=a.tp_degree)
@@ -41,11 +45,22 @@ def main():
     mk = {"7b": llama2_7b_config, "13b": llama2_13b_config}.get(a.model, lambda **k: LlamaConfig(
         vocab_size=4096, hidden_size=256, intermediate_size=704, num_hidden_layers=4, num_attention_heads=8, **k))
     torch.manual_seed(0)
-    target = LlamaForInference(mk(**kw), batch_size=1, max_seq_len=L).eval()
+    sampled = a.temperature > 0
+    how = dict(batch_size=a.batch_size if sampled else 1, max_seq_len=L, page_size=a.page_size or None, on_device_sampling=not sampled)
+    target = LlamaForInference(mk(**kw), **how).eval()
     dcfg = mk(**kw)
     dcfg.num_hidden_layers = a.draft_layers
     torch.manual_seed(0)        # same seed: the draft's layers start as a prefix of the target's (a crude "distilled" draft)
-    draft = LlamaForInference(dcfg, batch_size=1, max_seq_len=L).eval()
+    draft = LlamaForInference(dcfg, **how).eval()
+    if sampled:
+        prompt = torch.randint(0, target.cfg.vocab_size, (a.batch_size, a.prompt_length), device=dev)
+        t0 = time.perf_counter()
+        out, acc = speculative_sample(target, draft, prompt, a.max_new_tokens, a.speculation_length, a.temperature)
+        if dist.get_rank() == 0:
+            print(f"sampled {tuple(out.shape)}; accepted draft tokens / target forward: {acc:.2f}; {1e3 * (time.perf_counter() - t0):.1f} ms", flush=True)
+        dist.barrier()
+        dist.destroy_process_group()
+        return
     prompt = torch.randint(0, target.cfg.vocab_size, (1, a.prompt_length), device=dev)
     t0 = time.perf_counter()
     ref = target.generate(prompt, a.max_new_tokens)

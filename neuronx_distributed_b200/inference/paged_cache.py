@@ -1,0 +1,93 @@
+"""Key/value cache in pages: one pool per layer ``[pages, page_size, H_kv_local, D]``, a table of pages per batch row, and a prefix that all rows
+share.  Beside ``kv_cache.py``, whose rows are contiguous and as long as the longest sequence may get, rows here hold as many pages as they need,
+and what they begin alike is there once.  The pages themselves are written and read by ``ops.paged`` (``csrc/paged.cu``); this class says
+whose they are.  Tables live on the device at fixed addresses (CUDA graphs read them as they are at the replay); pages are handed out on the host."""
+from __future__ import annotations
+
+from typing import List, Optional
+
+import torch
+
+
+class PagedKVCacheManager:
+    def __init__(self, num_layers: int, batch_size: int, max_seq_len: int, num_kv_heads_local: int, head_dim: int, page_size: int = 32,
+                 num_pages: Optional[int] = None, dtype: torch.dtype = torch.bfloat16, device=None):
+        """``num_pages``: of the pool (default: enough for every row to be ``max_seq_len`` long)."""
+        if page_size < 16 or page_size % 16:
+            raise ValueError(f"a page holds a multiple of 16 tokens, got {page_size}")
+        self.num_layers, self.batch_size, self.max_seq_len, self.page_size = num_layers, batch_size, max_seq_len, page_size
+        self.columns = (max_seq_len + page_size - 1) // page_size
+        self.num_pages = batch_size * self.columns if num_pages is None else num_pages
+        if self.num_pages < 1:
+            raise ValueError("a pool without pages")
+        shape = (self.num_pages, page_size, num_kv_heads_local, head_dim)
+        self.k: List[torch.Tensor] = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(num_layers)]
+        self.v: List[torch.Tensor] = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(num_layers)]
+        self.page_table = torch.full((batch_size, self.columns), -1, dtype=torch.int32, device=device)
+        self.shared_pages: Optional[torch.Tensor] = None      # [n] int32: what every row begins with
+        self._shared: List[int] = []
+        self._rows: List[List[int]] = [[] for _ in range(batch_size)]       # pages of a row behind the shared ones
+        self._free: List[int] = list(range(self.num_pages))[::-1]
+
+    @property
+    def shared_tokens(self) -> int:
+        return len(self._shared) * self.page_size
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    def _take(self, n: int) -> List[int]:
+        if n > len(self._free):
+            raise RuntimeError(f"the key/value pool has {len(self._free)} pages left, {n} are needed")
+        return [self._free.pop() for _ in range(n)]
+
+    def reserve(self, row: int, tokens: int) -> None:
+        """Room for a sequence of ``tokens`` tokens in all, the shared ones among them.  Tokens without room are not kept."""
+        if tokens > self.columns * self.page_size:
+            raise ValueError(f"a sequence of {tokens} tokens is longer than max_seq_len {self.max_seq_len}")
+        held = len(self._shared) + len(self._rows[row])
+        pages = self._take(max(0, (tokens + self.page_size - 1) // self.page_size - held))
+        if pages:
+            self._rows[row] += pages
+            self.page_table[row, held:held + len(pages)] = torch.tensor(pages, dtype=torch.int32, device=self.page_table.device)
+
+    def reserve_rows(self, rows: int, tokens: int) -> None:
+        """:meth:`reserve` for the first ``rows`` rows: all of them, or, where the pool has not as much, none."""
+        want = max(0, (tokens + self.page_size - 1) // self.page_size - len(self._shared))
+        need = sum(max(0, want - len(self._rows[r])) for r in range(rows))
+        if tokens <= self.columns * self.page_size and need > len(self._free):
+            raise RuntimeError(f"the key/value pool has {len(self._free)} pages left, {need} are needed")
+        for r in range(rows):
+            self.reserve(r, tokens)
+
+    def release(self, row: int) -> None:
+        """The row's own pages go back to the pool; the shared ones stay."""
+        if self._rows[row]:
+            self._free += self._rows[row][::-1]
+            self._rows[row] = []
+            self.page_table[row, len(self._shared):] = -1
+
+    def take_shared(self, tokens: int) -> torch.Tensor:
+        """Pages for a prefix of ``tokens`` tokens that every row begins with, in place of the one before → ``[n]`` int32 (who asked fills them).  All
+        rows start anew."""
+        if tokens % self.page_size:
+            raise ValueError(f"a shared prefix fills whole pages of {self.page_size} tokens, got {tokens}")
+        if tokens > self.columns * self.page_size:
+            raise ValueError(f"a prefix of {tokens} tokens is longer than max_seq_len {self.max_seq_len}")
+        n = tokens // self.page_size
+        if n > self.num_pages:
+            raise RuntimeError(f"the key/value pool has {self.num_pages} pages, {n} are needed")
+        for row in range(self.batch_size):
+            self.release(row)
+        self._free += self._shared[::-1]
+        self._shared = self._take(n)
+        pages = torch.tensor(self._shared, dtype=torch.int32, device=self.page_table.device)
+        self.page_table[:] = -1
+        self.page_table[:, :n] = pages
+        self.shared_pages = pages if n else None
+        return pages
+
+    def reset(self) -> None:
+        """All pages go back to the pool, the shared ones too."""
+        self.take_shared(0)

@@ -13,6 +13,7 @@ from torch.nn.modules.module import _global_forward_hooks, _global_forward_pre_h
 
 from .. import ops
 from ..inference.kv_cache import KVCacheManager
+from ..inference.paged_cache import PagedKVCacheManager
 from ..utils.sampling import Sampler
 from ..modules.rms_norm import RMSNorm
 from ..parallel_layers.layers import column_swiglu
@@ -21,9 +22,11 @@ from .llama import LlamaConfig, LlamaForCausalLM
 
 class LlamaForInference(nn.Module):
     def __init__(self, cfg: LlamaConfig, batch_size: int = 1, max_seq_len: int = 2048, on_device_sampling: bool = True,
-                 sampler: Optional[Sampler] = None, lm_cls=None, flash_decoding: bool = False):
+                 sampler: Optional[Sampler] = None, lm_cls=None, flash_decoding: bool = False, page_size: Optional[int] = None,
+                 num_pages: Optional[int] = None):
         """``lm_cls``: any decoder built from Llama attention blocks (``LlamaForCausalLM`` default; ``MixtralForCausalLM`` for
-        the MoE families — its layers' ``mlp`` returns ``(y, router_logits)``, handled in ``_body``)."""
+        the MoE families — its layers' ``mlp`` returns ``(y, router_logits)``, handled in ``_body``).  ``page_size``: the cache
+        lies in pages of that many tokens (``inference/paged_cache.py``), ``num_pages`` of them; without it, in contiguous rows."""
         super().__init__()
         cfg.sequence_parallel_enabled = False
         cfg.activation_checkpointing = "none"
@@ -42,8 +45,16 @@ class LlamaForInference(nn.Module):
                 "flash decoding needs replicated KV heads (tensor-parallel size > number of KV heads)"
             shards, self.kv_rank = dist.get_world_size(self.kv_group), dist.get_rank(self.kv_group)
             assert max_seq_len % shards == 0, f"max_seq_len {max_seq_len} must divide by the KV replication factor {shards}"
-        self.kv = KVCacheManager(cfg.num_hidden_layers, batch_size, max_seq_len, attn0.num_kv_heads_local, cfg.head_dim,
-                                 dtype=cfg.dtype, device=cfg.device, num_cores_per_group=shards)
+        self.paged = page_size is not None
+        self._rows = None                                # rows of a prompt in a paged cache: first position, lengths, tables, shared pages
+        if self.paged:
+            if flash_decoding:
+                raise ValueError("flash decoding shards contiguous cache rows; it does not go with pages")
+            self.kv = PagedKVCacheManager(cfg.num_hidden_layers, batch_size, max_seq_len, attn0.num_kv_heads_local, cfg.head_dim,
+                                          page_size=page_size, num_pages=num_pages, dtype=cfg.dtype, device=cfg.device)
+        else:
+            self.kv = KVCacheManager(cfg.num_hidden_layers, batch_size, max_seq_len, attn0.num_kv_heads_local, cfg.head_dim,
+                                     dtype=cfg.dtype, device=cfg.device, num_cores_per_group=shards)
         self.sampler = sampler or Sampler(top_k=1, vocab_parallel=True)
         self.on_device_sampling = on_device_sampling
         cos, sin = ops.rope.rope_tables(max_seq_len, cfg.head_dim, cfg.rope_theta, cfg.device, 0, cfg.rope_scaling_factor)
@@ -72,7 +83,15 @@ class LlamaForInference(nn.Module):
         q = q.reshape(S, B, att.num_heads_local, D).transpose(0, 1)
         k = k.reshape(S, B, att.num_kv_heads_local, D).transpose(0, 1)
         v = v.reshape(S, B, att.num_kv_heads_local, D).transpose(0, 1)      # a view: caches and kernels take its strides
-        if self.flash_decoding and not prefill:
+        if self.paged:
+            if tree is not None:
+                raise ValueError("candidate trees need contiguous cache rows (accepted nodes move inside them)")
+            # one launch: rotation of q and k and the new rows of the pages; prompts, windows and single tokens read them there
+            first, lens, table, shared = self._rows if prefill else (positions.long(), None, self.kv.page_table[:B], self.kv.shared_pages)
+            kc, vc = self.kv.k[layer_idx], self.kv.v[layer_idx]
+            q = ops.paged.rope_append(q, k, v, first, self.rope_cos, self.rope_sin, kc, vc, table, lens=lens)
+            o = ops.paged.attention(q, kc, vc, table, first, lens=lens, shared_pages=shared)
+        elif self.flash_decoding and not prefill:
             v = v.contiguous()
             assert S == 1 and tree is None, "flash decoding serves plain token generation (no speculation window)"
             from ..modules.attention.flash_decode import flash_decode_attention, write_decode_sharded
@@ -200,10 +219,35 @@ class LlamaForInference(nn.Module):
 
     # ------------------------------------------------------------------ entry points
     @torch.no_grad()
+    def share_prefix(self, prefix_ids: torch.Tensor) -> None:
+        """A prefix ``[n]`` (whole pages) that every sequence begins with from now on: it is encoded once and kept once, prompts go on
+        behind it, and single tokens and windows of all rows read it together.  All rows start anew; ``n = 0`` ends it."""
+        if not self.paged:
+            raise ValueError("a shared prefix needs a cache in pages (page_size)")
+        ids = prefix_ids.reshape(1, -1)
+        pages = self.kv.take_shared(ids.shape[1])
+        if ids.shape[1]:
+            self._rows = (torch.zeros(1, dtype=torch.long, device=ids.device), None, pages.view(1, -1), None)
+            try:
+                self._body(ids, None, True, None)
+            finally:
+                self._rows = None
+
+    @torch.no_grad()
     def context_encoding(self, input_ids: torch.Tensor, last_token_index: Optional[torch.Tensor] = None) -> torch.Tensor:
-        """``input_ids`` [B, S_bucket] (right-padded) → next token ids [B] (or vocab-parallel logits)."""
-        h = self._body(input_ids, None, True, None)                              # [S, B, H]
+        """``input_ids`` [B, S_bucket] (right-padded) → next token ids [B] (or vocab-parallel logits).  In a paged cache the prompts stand
+        behind the shared prefix, in pages that are reserved for all of ``S_bucket``."""
         B = input_ids.shape[0]
+        if self.paged:
+            shared = self.kv.shared_tokens
+            self.kv.reserve_rows(B, shared + input_ids.shape[1])
+            first = torch.full((B,), shared, dtype=torch.long, device=input_ids.device)
+            lens = None if last_token_index is None else last_token_index.long() + 1
+            self._rows = (first, lens, self.kv.page_table[:B], self.kv.shared_pages)
+        try:
+            h = self._body(input_ids, None, True, None)                          # [S, B, H]
+        finally:
+            self._rows = None
         if last_token_index is None:
             last = h[-1]
         else:
@@ -213,7 +257,8 @@ class LlamaForInference(nn.Module):
 
     @torch.no_grad()
     def token_generation(self, input_ids: torch.Tensor, positions: torch.Tensor, kv_len: Optional[int] = None) -> torch.Tensor:
-        """``input_ids`` [B, 1], ``positions`` [B] → next token ids [B]."""
+        """``input_ids`` [B, 1], ``positions`` [B] → next token ids [B].  Positions count the shared prefix of a paged cache; its rows need
+        pages for them (``kv.reserve``), and one at -1 is idle."""
         h = self._body(input_ids, positions, False, kv_len)
         logits = self.lm.lm_head(h)[0].float()
         return self.sampler.sample(logits) if self.on_device_sampling else logits
@@ -237,9 +282,12 @@ class LlamaForInference(nn.Module):
     def generate(self, prompt_ids: torch.Tensor, max_new_tokens: int, prompt_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
         B, S = prompt_ids.shape
         lens = prompt_lens if prompt_lens is not None else torch.full((B,), S, device=prompt_ids.device, dtype=torch.long)
+        pos = lens.clone()
+        if self.paged:
+            self.kv.reserve_rows(B, self.kv.shared_tokens + S + max(0, max_new_tokens - 1))
+            pos = pos + self.kv.shared_tokens
         tok = self.context_encoding(prompt_ids, lens - 1)
         out = [tok]
-        pos = lens.clone()
         for _ in range(max_new_tokens - 1):
             tok = self.token_generation(tok.view(B, 1), pos)
             out.append(tok)
