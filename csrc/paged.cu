@@ -437,9 +437,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn
       cluster_sync_all();                                  // nobody reads a block's sums any more
     }
   }
-  if (DEAL == kDealt && p.shared == 0)
-    for (int e = blockIdx.x; e < p.B; e += gridDim.x)
-      if (entry_tiles(p, e) == 0) finish_idle<T, D, kThreads>(p, e, threadIdx.x);
+  if (DEAL == kDealt && p.shared == 0) finish_idle<T, D, kThreads>(p, threadIdx.x);
   if (late) pdl_wait();
 }
 

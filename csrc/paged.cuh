@@ -161,15 +161,21 @@ NXD_DEVICE void join_parts(const PagedAttn& p, int n, F slot, T* row) {
   for (int j = 0; j < C; ++j) dst[j] = from_f32<T>(l == 0.f ? 0.f : acc[j] / l);
 }
 
-// Rows of an entry none of whose tokens sees a key, or counts: zeros.  (With shared pages the last launch writes all rows.)
+// Zeros for the rows of entries none of whose tokens sees a key, or counts, sixteen rows of an entry at a time, dealt out over the blocks.  (With shared
+// pages the last launch writes all rows.)
 template <typename T, int D, int THREADS>
-NXD_DEVICE void finish_idle(const PagedAttn& p, int e, int thread) {
-  const int b = e / p.row_tiles, row0 = e % p.row_tiles * p.tile_rows, rows = min(p.tile_rows, p.W * p.G - row0);
-  for (int i = thread >> 5; i < rows * p.Hkv; i += THREADS / 32) {
-    const int row = row0 + i % rows, head = i / rows;
-    T* dst = reinterpret_cast<T*>(p.out) + b * p.o_sb + row / p.G * p.o_sw + (long)(head * p.G + row % p.G) * p.o_sh + (thread & 31) * (D / 32);
-#pragma unroll
-    for (int j = 0; j < D / 32; ++j) dst[j] = from_f32<T>(0.f);
+NXD_DEVICE void finish_idle(const PagedAttn& p, int thread) {
+  const int chunks = (p.tile_rows + 15) / 16;
+  for (long i = blockIdx.x; i < (long)p.B * p.row_tiles * chunks; i += gridDim.x) {
+    const int e = (int)(i / chunks);
+    if (entry_tiles(p, e) > 0) continue;
+    const int b = e / p.row_tiles, row0 = e % p.row_tiles * p.tile_rows + (int)(i % chunks) * 16;
+    const int rows = min(min(16, p.tile_rows), p.W * p.G - row0);
+    for (int x = thread; x < rows * p.Hkv * (D / 8); x += THREADS) {
+      const int c = x % (D / 8), y = x / (D / 8), head = y % p.Hkv, row = row0 + y / p.Hkv;
+      *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + b * p.o_sb + row / p.G * p.o_sw + (long)(head * p.G + row % p.G) * p.o_sh + c * 8) =
+          make_uint4(0, 0, 0, 0);
+    }
   }
 }
 

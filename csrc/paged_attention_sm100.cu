@@ -528,9 +528,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       }
       it = nx;
     }
-    if (!SHARED && p.shared == 0)
-      for (int e = blockIdx.x; e < p.B * p.row_tiles; e += gridDim.x)
-        if (entry_tiles(p, e) == 0) finish_idle<T, D, 128>(p, e, threadIdx.x - 256);
+    if (!SHARED && p.shared == 0) finish_idle<T, D, 128>(p, threadIdx.x - 256);
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     const int t = warp >= 4;                       // stream of this warpgroup
