@@ -86,10 +86,13 @@ using namespace paged;
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 constexpr int kKeys = 16;                                  // keys of a warp's tile
 constexpr int kTileKeys = kWarps * kKeys;                  // keys of a block's tile
-constexpr int kStages = 3;
+constexpr float kNone = -1e30f;                            // the maximum of a row that has seen no key: below every score, and finite
 constexpr int kCluster8 = 8;                               // blocks of a cluster at most
 template <int D> constexpr int kPitch = D + 4;             // of the rows in which warps leave their sums: no bank twice
-template <int D> constexpr int rows_smem() { return kWarps * kStages * 2 * kKeys * D * 2 + kWarps * 8 * kPitch<D> * 4; }
+template <int D> constexpr int kSums = kWarps * 8 * kPitch<D> * 4;          // bytes of them
+// two blocks an SM, three stages of 8 KB a warp: three blocks with two took 28.7 us for 26.7 (64 sequences of 300 to 600 keys, 8 heads), 74 for 66 (16 to 8192)
+constexpr int kStages = 3;
+template <int D> constexpr int rows_smem(bool cluster) { return kWarps * kStages * 2 * kKeys * D * 2 + (cluster ? 0 : kSums<D>); }
 
 NXD_DEVICE void cp_async16(uint32_t dst, const void* src, bool live) {    // not live: 16 zero bytes, nothing is read
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
@@ -178,8 +181,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn
   const T* const kc = reinterpret_cast<const T*>(p.k);
   const T* const vc = reinterpret_cast<const T*>(p.v);
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (kStages * STAGE);
-  float* const sm_o = reinterpret_cast<float*>(smem + kWarps * kStages * STAGE);       // [warp][8 rows][PITCH]
-  float* const sm_b = reinterpret_cast<float*>(smem);      // a cluster's block: its sums [8 R][D], over the ring that has been read
+  // sums of the warps [warp][8 rows][PITCH] and of a cluster's block [8 R][D]: a cluster's lie over the ring, which has been read by then
+  float* const sm_o = reinterpret_cast<float*>(smem + (DEAL == kCluster ? 0 : kWarps * kStages * STAGE));
+  float* const sm_b = reinterpret_cast<float*>(smem + kSums<D>);
 
   // CH lanes copy one row, 16-byte chunk c of row r lands at chunk (c ^ (r & 7)): both ways of reading are conflict-free
   auto load_tile = [&](const Walk& c, int n, int page, int stage) {
@@ -255,7 +259,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn
         const int r = i * 8 + quad * 2 + e;
         row_token(r, b, w);
         lim[i][e] = r < rows && w < new_tokens(p, b) ? min(visible_keys(p, b, w), cur.n) : 0;
-        m[i][e] = -INFINITY;
+        m[i][e] = kNone;
         l[i][e] = 0.f;
       }
     }
@@ -265,6 +269,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn
   auto finish = [&](bool last) {
     const int kvh = cur.w.head;
     const bool direct = !SHARED && p.shared == 0 && whole && last;
+    if (DEAL == kCluster) __syncthreads();
 #pragma unroll
     for (int i = 0; i < R; ++i)
 #pragma unroll
@@ -275,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn
 #pragma unroll
       for (int i = 0; i < R; ++i)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) { sm_m[warp][i * 8 + quad * 2 + e] = m[i][e]; sm_l[warp][i * 8 + quad * 2 + e] = l[i][e]; }
+        for (int e = 0; e < 2; ++e) { sm_m[warp][i * 8 + quad * 2 + e] = m[i][e] == kNone ? -INFINITY : m[i][e]; sm_l[warp][i * 8 + quad * 2 + e] = l[i][e]; }
 #pragma unroll
     for (int i = 0; i < R; ++i) {
       if (i) __syncthreads();
@@ -324,11 +329,11 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn
     const int key = (SHARED ? 0 : p.shared) + cur.w.tile * kTileKeys + warp * kKeys;
     if (!hole) {
       const uint32_t ks = ring + stage * STAGE, vs = ks + kKeys * D * 2;
-      float s[R][4];
+      float s[R][4], s1[R][4];                             // two chains of products: a warp waits for one most of its time
 #pragma unroll
       for (int i = 0; i < R; ++i)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
+        for (int e = 0; e < 4; ++e) s[i][e] = s1[i][e] = 0.f;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         // matrices: keys 0-7 / columns 16 k.., keys 8-15 / 16 k.., keys 0-7 / 16 k + 8.., keys 8-15 / 16 k + 8..
@@ -336,43 +341,44 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn
         uint32_t a[4];
         ldmatrix_x4(a, ks + r * (D * 2) + ((c ^ (r & 7)) << 4));
 #pragma unroll
-        for (int i = 0; i < R; ++i) mma16816<T>(s[i], a, qf[i][k][0], qf[i][k][1]);
+        for (int i = 0; i < R; ++i) mma16816<T>(k & 1 ? s1[i] : s[i], a, qf[i][k][0], qf[i][k][1]);
       }
       const bool masked = key + kKeys > lim_all;
       uint32_t pf[R][2];
 #pragma unroll
       for (int i = 0; i < R; ++i) {
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {                      // key hq + 8 (e / 2), row 2 quad + e % 2
-          s[i][e] *= p.scale_log2;
+        for (int e = 0; e < 4; ++e) s[i][e] += s1[i][e];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)                        // key hq + 8 (e / 2), row 2 quad + e % 2
           if (masked && key + hq + (e >> 1) * 8 >= lim[i][e & 1]) s[i][e] = -INFINITY;
-        }
-        float mx[2], f[2];
-        bool grew = false;
+        // Weights relative to a maximum that is at most 2^8 behind: it is looked for among the eight lanes of a row when one of them finds it passed
+        float x[4];
+        bool passed = false;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          mx[e] = fmaxf(s[i][e], s[i][e + 2]);
-#pragma unroll
-          for (int x = 4; x < 32; x <<= 1) mx[e] = fmaxf(mx[e], __shfl_xor_sync(0xffffffffu, mx[e], x));
-          grew = grew || mx[e] > m[i][e];
+        for (int e = 0; e < 4; ++e) {
+          x[e] = fmaf(s[i][e], p.scale_log2, -m[i][e & 1]);
+          passed = passed || x[e] > 8.f;
         }
-        if (__any_sync(0xffffffffu, grew)) {
+        if (__any_sync(0xffffffffu, passed)) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
-            const float mn = fmaxf(m[i][e], mx[e]);
-            f[e] = mx[e] > m[i][e] ? exp2f(m[i][e] - mn) : 1.f;       // m = -inf: 0
+            float mx = fmaxf(s[i][e], s[i][e + 2]) * p.scale_log2;
+#pragma unroll
+            for (int y = 4; y < 32; y <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, y));
+            const float mn = fmaxf(m[i][e], mx), f = exp2f(m[i][e] - mn);      // none before: 0
             m[i][e] = mn;
-            l[i][e] *= f[e];
+            l[i][e] *= f;
+#pragma unroll
+            for (int k = 0; k < KS; ++k) { o[i][k][e] *= f; o[i][k][e + 2] *= f; }
           }
 #pragma unroll
-          for (int k = 0; k < KS; ++k)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) o[i][k][e] *= f[e & 1];
+          for (int e = 0; e < 4; ++e) x[e] = fmaf(s[i][e], p.scale_log2, -m[i][e & 1]);
         }
         float pr[4];
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          pr[e] = exp2f(s[i][e] - (m[i][e & 1] == -INFINITY ? 0.f : m[i][e & 1]));
+          pr[e] = exp2f(x[e]);
           l[i][e & 1] += pr[e];
         }
         pf[i][0] = transpose8x8(pack16<T>(pr[0], pr[1]));
@@ -503,10 +509,12 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const PagedAttn p,
 
 template <typename T, int D, int R, Deal DEAL>
 void launch_rows(const PagedAttn& p, int grid, cudaStream_t st) {
-  NXD_ALLOW_SMEM((paged_rows_kernel<T, D, R, DEAL>), rows_smem<D>());
-  if (DEAL != kCluster || p.cluster == 1) return launch_dependent(paged_rows_kernel<T, D, R, DEAL>, grid, kThreads, rows_smem<D>(), st, p);
+  constexpr int smem = rows_smem<D>(DEAL == kCluster);
+  static_assert(DEAL != kCluster || kSums<D> + 8 * R * D * 4 <= smem, "a cluster's sums lie over the ring");
+  NXD_ALLOW_SMEM((paged_rows_kernel<T, D, R, DEAL>), smem);
+  if (DEAL != kCluster || p.cluster == 1) return launch_dependent(paged_rows_kernel<T, D, R, DEAL>, grid, kThreads, smem, st, p);
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = grid; cfg.blockDim = kThreads; cfg.dynamicSmemBytes = rows_smem<D>(); cfg.stream = st;
+  cfg.gridDim = grid; cfg.blockDim = kThreads; cfg.dynamicSmemBytes = smem; cfg.stream = st;
   cudaLaunchAttribute attr[2]{};
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -541,13 +549,17 @@ void launch(const PagedAttn& p, const PagedPlan& plan, int dt, cudaStream_t st) 
 PagedPlan paged_plan(PagedAttn& p) {
   PagedPlan plan{};
   const int sms = device_sm_count();
-  // rows, → (kernel, rows of a tile)
-  auto cut = [](long rows, int& tile_rows) {
-    tile_rows = rows <= 8 ? 8 : rows <= 16 ? 16 : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
-    return rows > 16;
+  // rows, the most that go to the few-row kernel → whether there are more; rows of a tile
+  auto cut = [](long rows, int few, int& tile_rows) {
+    tile_rows = rows <= few ? (rows <= 8 ? 8 : 16) : rows <= 64 ? 64 : rows <= 128 ? 128 : 256;
+    return rows > few;
   };
   const long rows = (long)p.W * p.G, all = rows * p.B;
-  plan.tiles = cut(rows, p.tile_rows);
+  // Nine to sixteen rows of long sequences, enough of them to fill the GPU, are the tensor memory's, too: there the few-row kernel is bound by its
+  // instructions (us, few rows / tiles: 16 sequences to 3000 keys, 16 rows, 8 heads, 50 / 45; 4 to 8000 50 / 34; 8 to 4000 38 / 35; but 1 to 2000
+  // 11 / 18, 32 to 1000 33 / 43).
+  const long pairs = (long)p.B * p.Hkv, cap = (long)p.cols * p.ps - p.shared;
+  plan.tiles = cut(rows, cap > 2048 && pairs * cap > 131072 ? 8 : 16, p.tile_rows);
   p.row_tiles = (int)((rows + p.tile_rows - 1) / p.tile_rows);
   auto tile_keys = [](int tile_rows) { return tile_rows == 256 ? 128 : kTileKeys; };
   p.tile_keys = tile_keys(p.tile_rows);
@@ -556,10 +568,6 @@ PagedPlan paged_plan(PagedAttn& p) {
   // A cluster per pair, as many blocks in it as the GPU takes at once, has neither a search for places nor a second launch (us, dealt out / cluster:
   // 1 sequence of 1000 keys, 8 heads, 19 / 9.8; 64 of 300 to 600, 8 heads, 36 / 28; 16 of 4096 to 8192, 8 heads, 72 / 68), but the longest
   // sequence lasts as long as its own blocks take, at 47 GB/s each: 2048 keys, 22 us, at most.
-  // A cluster per pair, as many blocks in it as the GPU takes at once, has neither a search for places nor a second launch (us, dealt out / cluster:
-  // 1 sequence of 1000 keys, 8 heads, 19 / 9.8; 64 of 300 to 600, 8 heads, 36 / 28; 16 of 4096 to 8192, 8 heads, 72 / 68), but the longest
-  // sequence lasts as long as its own blocks take, at 47 GB/s each: 2048 keys, 22 us, at most.
-  const long pairs = (long)p.B * p.Hkv, cap = (long)p.cols * p.ps - p.shared;
   if (!plan.tiles) {
     int size = 1;
     while (size < kCluster8 && ((cap > 256l * size && pairs * size * 2 <= 2 * sms) || cap > 2048l * size)) size *= 2;
@@ -571,12 +579,12 @@ PagedPlan paged_plan(PagedAttn& p) {
   plan.slots = (p.shared ? (long)p.B * p.row_tiles * p.Hkv + (p.cluster ? 0 : plan.grid) : p.cluster ? 0l : 2l * plan.grid) * p.tile_rows;
   p.slots = plan.slots;
   if (p.shared) {
-    plan.pre_tiles = cut(all, p.pre_tile_rows);
+    plan.pre_tiles = cut(all, 16, p.pre_tile_rows);
     p.pre_row_tiles = (int)((all + p.pre_tile_rows - 1) / p.pre_tile_rows);
     const int keys = tile_keys(p.pre_tile_rows);
     p.pre_tiles = (p.shared + keys - 1) / keys;
     const long total = (long)p.pre_row_tiles * p.Hkv * p.pre_tiles, most = plan.pre_tiles ? sms : 2 * sms;
-    p.pre_per = (int)std::max((total + most - 1) / most, 256l / keys);
+    p.pre_per = (int)std::max((total + most - 1) / most, 384l / keys);
     plan.pre_grid = (int)((total + p.pre_per - 1) / p.pre_per);
     plan.pre_slots = ((long)p.pre_row_tiles * p.Hkv + plan.pre_grid) * p.pre_tile_rows;
   }

@@ -651,7 +651,10 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       }
       }
       if (!dry) { pos0 += 2 * it.n; tile0 += it.n; }
-      if (dry && !late) pdl_wait();
+      if (dry) {
+        if (!late) pdl_wait();
+        pdl_trigger();
+      }
       dry = false;
       it = next_item();
       if (it.n == 0) break;
