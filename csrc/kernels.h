@@ -208,13 +208,14 @@ struct PagedAttn {
   const void *q, *k, *v;
   void* out;
   const int* table;                  // [B, cols] page of keys [i * ps, (i + 1) * ps); entries outside [0, pages) are holes: nobody sees their keys
-  const int* shared_pages;           // pages of keys [0, shared) of every sequence
+  const int* shared_pages;           // the first shared_cols pages of every sequence, in place of the table's
   const long* positions;             // [B] index of a row's first new token; negative: an idle row
   const long* lens;                  // [B] new tokens of a row, or null: W
   float *part_o, *part_ml;           // parts of pairs (paged.cuh): [slot][tile_rows][D] sums, [slot][tile_rows] (maximum, sum of weights)
   float *pre_o, *pre_ml;             // the same over the shared pages, behind them: `slots` rows on
   long slots;
-  int B, W, G, Hkv, cols, ps, pages, shared;      // shared: keys in shared pages
+  int B, W, G, Hkv, cols, ps, pages, shared_cols;
+  int shared;                        // keys in shared pages, if those are walked for the whole batch at once; otherwise 0
   int row_tiles, tile_rows, tile_keys, min_tiles; // how rows and keys are cut, and a block's least share of tiles
   int cluster;                       // blocks that share a pair, none of them with others (0: dealt out)
   int pre_row_tiles, pre_tile_rows, pre_tiles, pre_per;      // the same over the shared pages: rows of the whole batch; key tiles of a pair and of a block

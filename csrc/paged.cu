@@ -16,7 +16,8 @@ namespace {
 // ---------------------------------------------------------------------------------------------------------------- append
 // x' = (a cos − b sin, b cos + a sin), a and b the halves of a head, angle by the token's position: q to q_out, k into its page, v as it is
 // beside it.  Bound by HBM: every number is read and written once.  A thread has 16 bytes of each half of one head, a block as many as it can of one
-// token, whose position, page, cosines and sines its threads share in L1.
+// token, whose position, page, cosines and sines its threads share in L1.  4 x 2000 tokens, 64 heads on 8: 49 us, 5.0 TB/s (threads that go through
+// heads with their cosines and sines in registers: 99, too few of them at a time); one token 2.6.
 struct AppendArgs {
   const void *q, *k, *v;
   const long *positions, *lens;
@@ -37,7 +38,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
   pdl_wait();
   if (h >= p.H + 2 * p.Hkv) return;
   const long first = p.positions[b], m = p.lens ? p.lens[b] : p.W, pos = first + w;
-  const bool live = first >= 0 && w < m && pos < p.rows, query = h < p.H, key = h < p.H + p.Hkv;
+  const bool live = first >= 0 && first < p.rows && w < m && pos < p.rows, query = h < p.H, key = h < p.H + p.Hkv;
   T* const q_out = (T*)p.q_out + b * p.o_sb + w * p.o_sw + (long)h * (2 * p.half) + c;
   Pack16<T> lo, hi;
   if (!live) {
@@ -135,7 +136,8 @@ enum Deal { kDealt, kCluster, kShared };
 // ahead over the ends of pairs.  Scores Sᵀ = K Qᵀ and sums Oᵀ += Vᵀ Pᵀ by mma.sync with the keys, then the head's columns, as the 16 rows of the
 // instruction and 8 R query rows as its columns, so that a group of up to 8 heads wastes nothing; the accumulator of Sᵀ becomes the operand Pᵀ by an
 // 8 x 8 transposition in registers.  Probabilities are rounded to the cache's type for the second product: half a step of 2^-8 (2^-11) each, which average out over
-// the keys; row sums are those of the unrounded ones.
+// the keys; row sums are those of the unrounded ones.  One token of 16 sequences to 8192 keys, 32 heads on 8: 66 us, 6.0 TB/s; of 6 to 2500, 40 single
+// heads: 40 us; of one to 300: 6.7.
 template <typename T, int D, int R, Deal DEAL>
 __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn p) {
   constexpr bool SHARED = DEAL == kShared;
@@ -153,8 +155,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn
   const int step = DEAL == kCluster ? p.cluster : 1;
   auto fetch_pages = [&](int e, int t0) {
     const unsigned i = ((SHARED ? 0u : (unsigned)p.shared) + (unsigned)(t0 + lane * step) * kTileKeys + warp * kKeys) / (unsigned)p.ps;
-    if (i >= (unsigned)(SHARED ? p.shared / p.ps : p.cols)) return -1;
-    const int page = SHARED ? p.shared_pages[i] : p.table[e * p.table_sb + i];
+    if (i >= (unsigned)(SHARED ? p.shared_cols : p.cols)) return -1;
+    const int page = i < (unsigned)p.shared_cols ? p.shared_pages[i] : p.table[e * p.table_sb + i];
     return (unsigned)page < (unsigned)p.pages ? page : -1;
   };
   struct { Walk w; int n; } cur;
@@ -555,6 +557,8 @@ PagedPlan paged_plan(PagedAttn& p) {
     return rows > few;
   };
   const long rows = (long)p.W * p.G, all = rows * p.B;
+  // Portions of prompts, whose own rows fill the row tiles, gain nothing from the batch's: the shared pages are the first of their own
+  p.shared = rows <= 128 ? p.shared_cols * p.ps : 0;
   // Nine to sixteen rows of long sequences, enough of them to fill the GPU, are the tensor memory's, too: there the few-row kernel is bound by its
   // instructions (us, few rows / tiles: 16 sequences to 3000 keys, 16 rows, 8 heads, 50 / 45; 4 to 8000 50 / 34; 8 to 4000 38 / 35; but 1 to 2000
   // 11 / 18, 32 to 1000 33 / 43).

@@ -23,8 +23,8 @@ NXD_DEVICE int new_tokens(const PagedAttn& p, int b) {
 }
 // Keys that token w of sequence b sees; what lies behind the page table's end nobody sees
 NXD_DEVICE int visible_keys(const PagedAttn& p, int b, int w) {
-  const long n = p.positions[b] + w + 1, cap = (long)p.cols * p.ps;
-  return (int)(n < cap ? n : cap);
+  const long cap = (long)p.cols * p.ps, first = p.positions[b];
+  return (int)(first < cap && first + w + 1 < cap ? first + w + 1 : cap);
 }
 // One past the last key of the sequence: none of its tokens sees more
 NXD_DEVICE int all_keys(const PagedAttn& p, int b) {

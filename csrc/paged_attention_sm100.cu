@@ -128,6 +128,9 @@ NXD_DEVICE Item make_item(const PagedAttn& p, const Walk& w, long left) {
   return it;
 }
 
+// PAIR: a step of two row tiles and 128 keys takes 2.2 us: exponentials 1.05, products 1.05 (heads of 128 numbers), which overlap little.  2 x 1000 tokens (a
+// quarter padding) behind 6000 keys, 48 heads of 64 on 8: 158 us, 470 TFLOP/s.  Otherwise: two tiles of 64 keys in 1.7 us, 5 TB/s over the GPU; windows of 5
+// tokens of 8 sequences to 6000 keys, 64 heads on 8: 43 us, of which 7 are the start and 5 the launch that joins parts.
 template <typename T, int D, bool PAIR, int ROWS, bool SHARED>
 __global__ void __launch_bounds__(kRowsThreads, 1)
 paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const PagedAttn p, int box) {
@@ -238,10 +241,11 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       const int boxes = KEYS / box, round = 32 / boxes;
       for (Item it = next_item(); it.n > 0; it = next_item()) {
         const int n = it.keys;
-        const int* table = SHARED ? p.shared_pages : p.table + it.e / row_tiles * p.table_sb;
+        const int* table = p.table + (SHARED ? 0 : it.e / row_tiles * p.table_sb);
         auto look_up = [&](int j) {
           const int at = j + lane / boxes, key = key_at(it.j0 + at) + lane % boxes * box;
-          return at < it.n && key < n ? table[key / p.ps] : -1;
+          const int i = key / p.ps;
+          return at >= it.n || key >= n ? -1 : i < p.shared_cols ? p.shared_pages[i] : table[i];
         };
         int found = look_up(0), next = look_up(round);
         for (int j = 0; j < it.n; ++j, ++tile) {
@@ -550,105 +554,105 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     while (true) {
       const int nt = t ? it.n1 : it.n0;
       if (nt > 0) {
-      int b = 0, w = 0;
-      const int row = first_row(it) + (PAIR ? t * kRows : 0) + own, n = it.keys;
-      const bool live = !dry && row_token(it, row, b, w);
-      // keys that this row sees (one that does not count: all, whatever comes of it), and the fewest of the warp's rows
-      const int sees = live ? min(visible_keys(p, b, w), n) : 0x7fffffff;
-      const int sees_lo = __reduce_min_sync(0xffffffffu, sees);
-      const bool rows_here = dry || __any_sync(0xffffffffu, live);             // otherwise the warp lets the scores be what they are
-      float m_ref = -INFINITY, l = 0.f;
-      for (int j = 0; j < nt; ++j) {
-        const int jt = PAIR ? j : 2 * j + t, key0 = key_at(it.j0 + jt), pos = pos0 + ring_at(t, j);
-        if (!dry) wait(my_s, (uint32_t)(g++ & 1));
-        tcgen05_fence_after();
-        if (rows_here) {
-        const uint32_t tP = dry ? tO : tS;
-        uint32_t hole;                             // written before the keys' barrier, which the products waited for
-        asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(hole) : "r"(holes + ((tile0 + jt) % kHoles) * 4) : "memory");
-        const int lim = sees - 1 - key0;           // last column that this row sees
-        if (sees_lo - key0 < KEYS || (hole != 0 && !dry)) {
-          // what is not seen becomes -inf where the scores lie, sixteen columns at a time: seldom, and few instructions to have at hand
-          const int from = hole ? 0 : max(0, sees_lo - key0) >> 4;
+        int b = 0, w = 0;
+        const int row = first_row(it) + (PAIR ? t * kRows : 0) + own, n = it.keys;
+        const bool live = !dry && row_token(it, row, b, w);
+        // keys that this row sees (one that does not count: all, whatever comes of it), and the fewest of the warp's rows
+        const int sees = live ? min(visible_keys(p, b, w), n) : 0x7fffffff;
+        const int sees_lo = __reduce_min_sync(0xffffffffu, sees);
+        const bool rows_here = dry || __any_sync(0xffffffffu, live);             // otherwise the warp lets the scores be what they are
+        float m_ref = -INFINITY, l = 0.f;
+        for (int j = 0; j < nt; ++j) {
+          const int jt = PAIR ? j : 2 * j + t, key0 = key_at(it.j0 + jt), pos = pos0 + ring_at(t, j);
+          if (!dry) wait(my_s, (uint32_t)(g++ & 1));
+          tcgen05_fence_after();
+          if (rows_here) {
+            const uint32_t tP = dry ? tO : tS;
+            uint32_t hole;                             // written before the keys' barrier, which the products waited for
+            asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(hole) : "r"(holes + ((tile0 + jt) % kHoles) * 4) : "memory");
+            const int lim = sees - 1 - key0;           // last column that this row sees
+            if (sees_lo - key0 < KEYS || (hole != 0 && !dry)) {
+              // what is not seen becomes -inf where the scores lie, sixteen columns at a time: seldom, and few instructions to have at hand
+              const int from = hole ? 0 : max(0, sees_lo - key0) >> 4;
 #pragma unroll 1
-          for (int c = from; c < KEYS / 16; ++c) {
-            uint32_t r[16];
-            tcgen05_ld_32x16(tS + c * 16, r);
-            tcgen05_wait_ld();
-            const int end = hole >> (c * 16 / box) & 1 ? -1 : lim - c * 16;
+              for (int c = from; c < KEYS / 16; ++c) {
+                uint32_t r[16];
+                tcgen05_ld_32x16(tS + c * 16, r);
+                tcgen05_wait_ld();
+                const int end = hole >> (c * 16 / box) & 1 ? -1 : lim - c * 16;
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (i > end) r[i] = 0xff800000u;
-            tcgen05_st_32x16(tS + c * 16, r);
+                for (int i = 0; i < 16; ++i)
+                  if (i > end) r[i] = 0xff800000u;
+                tcgen05_st_32x16(tS + c * 16, r);
+              }
+              tcgen05_wait_st();
+            }
+            uint32_t sr[Q][32];
+#pragma unroll
+            for (int c = 0; c < Q; ++c) tcgen05_ld_32x32(tS + c * 32, sr[c]);
+            tcgen05_wait_ld();
+            float base = m_ref == -INFINITY ? 0.f : m_ref;       // a row that has seen nothing yet: its first quarter is done again below
+            uint64_t shift = pack2(-base * sl2, -base * sl2), sum[Q] = {};
+            float mx, unused;
+            mx = -INFINITY;
+            if (!dry || part_of_step == 0) exps<T, Q, true>(sr, 0, sl2_2, shift, sum[0], mx);
+            const bool need = dry ? part_of_step == 4 : (mx - base) * sl2 > 8.f || (m_ref == -INFINITY && mx > -INFINITY);
+            if (__any_sync(0xffffffffu, need)) {
+              const float f = !need ? 1.f : m_ref == -INFINITY ? 0.f : ex2((m_ref - mx) * sl2);
+              if (need) m_ref = base = mx;
+              l *= f;
+              shift = pack2(-base * sl2, -base * sl2);
+              if (j > 0) {                             // PV of the step before is done (these scores came after it): O is quiescent
+#pragma unroll 1
+                for (int c = 0; c < D / 16; ++c) {
+                  uint32_t r[16];
+                  tcgen05_ld_32x16(tO + c * 16, r);
+                  tcgen05_wait_ld();
+#pragma unroll
+                  for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
+                  tcgen05_st_32x16(tO + c * 16, r);
+                }
+              }
+              tcgen05_ld_32x32(tS, sr[0]);
+              tcgen05_wait_ld();
+              sum[0] = 0ull;
+              exps<T, Q, false>(sr, 0, sl2_2, shift, sum[0], unused);
+            }
+            if (!(mx < INFINITY)) l = __int_as_float(0x7fffffff);        // NaN or +inf among the scores: a row of NaN
+            tcgen05_st_32x16p(tP, sr[0]);
+#pragma unroll
+            for (int c = 1; c < Q; ++c) {
+              if (dry && part_of_step != c) continue;
+              exps<T, Q, false>(sr, c, sl2_2, shift, sum[c], unused);
+              tcgen05_st_32x16p(tP + c * 16, sr[c]);
+            }
+            float part = 0.f;
+#pragma unroll
+            for (int c = 0; c < Q; ++c) { float x, y; unpack2(sum[c], x, y); part += x + y; }
+            l += part;
+          }
+          if (!dry && key0 + KEYS > n) {
+            // behind the last key: the rest of its page may hold anything, and 0 times NaN is NaN
+            wait(bar_kvf + 8 * ((pos + 1) % SLOTS), (uint32_t)(((pos + 1) / SLOTS) & 1));
+            if (own < KEYS && key0 + own >= n) {
+              const uint32_t dst = sKV + (pos + 1) % SLOTS * TILE + own * 128;
+#pragma unroll
+              for (int c = 0; c < D / 8; ++c)
+                asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + (c >> 3) * C::HALF + (c & 7) * 16), "r"(0u) : "memory");
+            }
+            fence_async_smem();
           }
           tcgen05_wait_st();
+          tcgen05_fence_before();
+          if (!dry) mbar_arrive(my_p);
         }
-        uint32_t sr[Q][32];
-#pragma unroll
-        for (int c = 0; c < Q; ++c) tcgen05_ld_32x32(tS + c * 32, sr[c]);
-        tcgen05_wait_ld();
-        float base = m_ref == -INFINITY ? 0.f : m_ref;       // a row that has seen nothing yet: its first quarter is done again below
-        uint64_t shift = pack2(-base * sl2, -base * sl2), sum[Q] = {};
-        float mx, unused;
-        mx = -INFINITY;
-        if (!dry || part_of_step == 0) exps<T, Q, true>(sr, 0, sl2_2, shift, sum[0], mx);
-        const bool need = dry ? part_of_step == 4 : (mx - base) * sl2 > 8.f || (m_ref == -INFINITY && mx > -INFINITY);
-        if (__any_sync(0xffffffffu, need)) {
-          const float f = !need ? 1.f : m_ref == -INFINITY ? 0.f : ex2((m_ref - mx) * sl2);
-          if (need) m_ref = base = mx;
-          l *= f;
-          shift = pack2(-base * sl2, -base * sl2);
-          if (j > 0) {                             // PV of the step before is done (these scores came after it): O is quiescent
-#pragma unroll 1
-            for (int c = 0; c < D / 16; ++c) {
-              uint32_t r[16];
-              tcgen05_ld_32x16(tO + c * 16, r);
-              tcgen05_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 16; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * f);
-              tcgen05_st_32x16(tO + c * 16, r);
-            }
-          }
-          tcgen05_ld_32x32(tS, sr[0]);
-          tcgen05_wait_ld();
-          sum[0] = 0ull;
-          exps<T, Q, false>(sr, 0, sl2_2, shift, sum[0], unused);
+        // ---- maximum (in units of the exponent) and row sum to the output warps
+        if (!dry) {
+          wait(bar_le + 8 * t, (uint32_t)((items & 1) ^ 1));
+          ++items;
+          asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(sStat + t * 1024 + own * 8), "f"(m_ref * sl2), "f"(l) : "memory");
+          mbar_arrive(bar_lf + 8 * t);
         }
-        if (!(mx < INFINITY)) l = __int_as_float(0x7fffffff);        // NaN or +inf among the scores: a row of NaN
-        tcgen05_st_32x16p(tP, sr[0]);
-#pragma unroll
-        for (int c = 1; c < Q; ++c) {
-          if (dry && part_of_step != c) continue;
-          exps<T, Q, false>(sr, c, sl2_2, shift, sum[c], unused);
-          tcgen05_st_32x16p(tP + c * 16, sr[c]);
-        }
-        float part = 0.f;
-#pragma unroll
-        for (int c = 0; c < Q; ++c) { float x, y; unpack2(sum[c], x, y); part += x + y; }
-        l += part;
-        }
-        if (!dry && key0 + KEYS > n) {
-          // behind the last key: the rest of its page may hold anything, and 0 times NaN is NaN
-          wait(bar_kvf + 8 * ((pos + 1) % SLOTS), (uint32_t)(((pos + 1) / SLOTS) & 1));
-          if (own < KEYS && key0 + own >= n) {
-            const uint32_t dst = sKV + (pos + 1) % SLOTS * TILE + own * 128;
-#pragma unroll
-            for (int c = 0; c < D / 8; ++c)
-              asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(dst + (c >> 3) * C::HALF + (c & 7) * 16), "r"(0u) : "memory");
-          }
-          fence_async_smem();
-        }
-        tcgen05_wait_st();
-        tcgen05_fence_before();
-        if (!dry) mbar_arrive(my_p);
-      }
-      // ---- maximum (in units of the exponent) and row sum to the output warps
-      if (!dry) {
-        wait(bar_le + 8 * t, (uint32_t)((items & 1) ^ 1));
-        ++items;
-        asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(sStat + t * 1024 + own * 8), "f"(m_ref * sl2), "f"(l) : "memory");
-        mbar_arrive(bar_lf + 8 * t);
-      }
       }
       if (!dry) { pos0 += 2 * it.n; tile0 += it.n; }
       if (dry) {

@@ -44,7 +44,8 @@ void check_cache(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tens
             "heads do not match: queries " + list(q.sizes()) + ", keys " + list(kc.sizes()) + ", values " + list(vc.sizes()));
   CHECK_ARG(q.scalar_type() == kc.scalar_type() && q.scalar_type() == vc.scalar_type(), "queries and caches are of one type");
   CHECK_ARG(kc.device() == q.device() && vc.device() == q.device(), "queries and caches are on one device");
-  CHECK_ARG(kc.size(0) > 0 && kc.size(1) > 0 && kc.size(0) < (1ll << 31) && kc.size(1) % 16 == 0, "a page holds a multiple of 16 tokens, got " + std::to_string(kc.size(1)));
+  CHECK_ARG(kc.size(0) > 0 && kc.size(1) > 0 && kc.size(0) < (1ll << 31) && kc.size(1) % 16 == 0,
+            "a page holds a multiple of 16 tokens, got " + std::to_string(kc.size(1)));
   CHECK_ARG(table.dim() == 2 && table.size(0) == q.size(0) && table.scalar_type() == at::kInt && table.device() == q.device() &&
             (table.size(1) <= 1 || table.stride(1) == 1) && table.size(1) * kc.size(1) < (1ll << 31),
             "page_table must be an int32 tensor [" + std::to_string(q.size(0)) + ", pages of a sequence] on the queries' device");
@@ -62,7 +63,8 @@ Tensor as_table(const Tensor& t) {
 
 // Whether the append kernel takes these: 32- or 16-bit types, halves of heads and cache rows of whole 16-byte packets
 bool paged_append_ok(const Tensor& q, const Tensor& kc, const Tensor& vc) {
-  return q.dim() == 4 && kc.dim() == 4 && vc.dim() == 4 && (half_type(q) || q.scalar_type() == at::kFloat) && q.size(3) * q.element_size() % 32 == 0 && packets(kc) && packets(vc);
+  return q.dim() == 4 && kc.dim() == 4 && vc.dim() == 4 && (half_type(q) || q.scalar_type() == at::kFloat) &&
+         q.size(3) * q.element_size() % 32 == 0 && packets(kc) && packets(vc);
 }
 // Whether the attention kernels take these: 16-bit types, heads of 64 or 128 numbers, cache rows of whole 16-byte packets
 bool paged_attention_ok(const Tensor& q, const Tensor& kc, const Tensor& vc) {
@@ -108,12 +110,13 @@ Tensor paged_attention(const Tensor& q_, const Tensor& kc, const Tensor& vc, con
   check_cache(q_, kc, vc, table, positions, lens);
   CHECK_ARG(q_.is_cuda() && paged_attention_ok(q_, kc, vc), "the kernels take 16-bit types, heads of 64 or 128 numbers and caches of whole 16-byte packets");
   const int64_t ps = kc.size(1);
-  int64_t shared = 0;
+  int64_t shared = 0;                              // shared pages
   if (shared_pages.has_value()) {
     CHECK_ARG(shared_pages->dim() == 1, "shared_pages is a list of pages");
     check_ints(*shared_pages, "shared_pages", at::kInt, shared_pages->size(0), q_);
-    shared = shared_pages->size(0) * ps;
-    CHECK_ARG(shared_pages->size(0) <= table.size(1), "more shared pages than a sequence has: " + std::to_string(shared_pages->size(0)) + ", page_table of " + std::to_string(table.size(1)));
+    shared = shared_pages->size(0);
+    CHECK_ARG(shared_pages->size(0) <= table.size(1),
+              "more shared pages than a sequence has: " + std::to_string(shared_pages->size(0)) + ", page_table of " + std::to_string(table.size(1)));
   }
   CHECK_ARG(scale > 0 && scale < 1e30, "the scale of the scores is positive");
   c10::cuda::CUDAGuard guard(q_.device());
@@ -128,7 +131,7 @@ Tensor paged_attention(const Tensor& q_, const Tensor& kc, const Tensor& vc, con
   p.positions = positions.data_ptr<long>();
   p.lens = lens.has_value() ? lens->data_ptr<long>() : nullptr;
   p.B = (int)B; p.W = (int)W; p.G = (int)(H / Hkv); p.Hkv = (int)Hkv; p.cols = (int)table.size(1); p.ps = (int)ps; p.pages = (int)kc.size(0);
-  p.shared = (int)shared;
+  p.shared_cols = (int)shared;
   p.q_sb = q.stride(0); p.q_sw = q.stride(1); p.q_sh = q.stride(2);
   p.o_sb = out.stride(0); p.o_sw = out.stride(1); p.o_sh = out.stride(2);
   p.table_sb = table.stride(0);
@@ -156,8 +159,10 @@ std::vector<Tensor> verify_drafts(const Tensor& tokens, const Tensor& draft_, co
             list(target_.sizes()));
   CHECK_ARG(draft_.scalar_type() == target_.scalar_type() && (half_type(draft_) || draft_.scalar_type() == at::kFloat),
             "probabilities are float32, bfloat16 or float16, both of one type");
-  CHECK_ARG(accept.sizes() == tokens.sizes() && accept.scalar_type() == at::kFloat && accept.is_contiguous(), "accept_uniforms must be a contiguous float32 tensor [batch, drafts]");
-  CHECK_ARG(sample.dim() == 1 && sample.size(0) == B && sample.scalar_type() == at::kFloat && sample.is_contiguous(), "sample_uniforms must be a contiguous float32 tensor [batch]");
+  CHECK_ARG(accept.sizes() == tokens.sizes() && accept.scalar_type() == at::kFloat && accept.is_contiguous(),
+            "accept_uniforms must be a contiguous float32 tensor [batch, drafts]");
+  CHECK_ARG(sample.dim() == 1 && sample.size(0) == B && sample.scalar_type() == at::kFloat && sample.is_contiguous(),
+            "sample_uniforms must be a contiguous float32 tensor [batch]");
   for (const Tensor& t : {tokens, draft_, target_, accept, sample}) CHECK_ARG(t.is_cuda() && t.device() == target_.device(), "all tensors are on one device");
   CHECK_ARG(B < 65536 && K < (1 << 20), "too many sequences or drafts");
   c10::cuda::CUDAGuard guard(target_.device());

@@ -66,7 +66,7 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     if _ext.use_cuda(q) and _ext._load().paged_append_ok(q, k_cache, v_cache):
         _ext.count_launch()
         return _ext.ext().paged_append(q, k, v, positions, cos, sin, k_cache, v_cache, page_table, lens)
-    positions, page_table = _ints(positions, torch.long), _table(page_table)
+    positions, page_table = _ints(positions, torch.long).clamp(-1, 1 << 40), _table(page_table)
     lens = None if lens is None else _ints(lens, torch.long)
     _check(q, k_cache, v_cache, page_table, positions, lens)
     B, W, H, D = q.shape
@@ -103,14 +103,14 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pag
     memory): token ``w`` of row ``b`` sees keys ``0 … positions[b] + w``.  ``W`` = 1: token generation; a few: a drafted window; many: a portion
     of a prompt.  Tokens that do not count, or see no key, come back as zeros.  Keys and values that some token of a row sees have to be finite.
 
-    ``shared_pages [n]`` int32: the pages of the first ``n * page_size`` tokens of EVERY sequence, which then are read once for the whole batch; the
-    first ``n`` columns of ``page_table`` are not looked at."""
+    ``shared_pages [n]`` int32: the pages of the first ``n * page_size`` tokens of EVERY sequence; the first ``n`` columns of ``page_table`` are not
+    looked at.  Where a sequence has up to 128 query rows (tokens times heads of a group), they are read once for the whole batch."""
     _no_gradient("paged attention", q, k_cache, v_cache)
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
     if _ext.use_cuda(q) and _ext._load().paged_attention_ok(q, k_cache, v_cache):
         _ext.count_launch(2 if shared_pages is None else 3)
         return _ext.ext().paged_attention(q, k_cache, v_cache, page_table, positions, scale, lens, shared_pages)
-    positions, page_table = _ints(positions, torch.long), _table(page_table)
+    positions, page_table = _ints(positions, torch.long).clamp(-1, 1 << 40), _table(page_table)
     lens = None if lens is None else _ints(lens, torch.long)
     if shared_pages is not None:
         shared_pages = _ints(shared_pages, torch.int32)

@@ -86,6 +86,9 @@ def speculative_sample(target, draft, prompt_ids: torch.Tensor, max_new_tokens: 
     before = _make_room(target, draft, B, S, max_new_tokens, K)
 
     def probabilities(logits):
+        if logits.shape[-1] != target.cfg.vocab_size:
+            raise ValueError(f"logits of {logits.shape[-1]} tokens, a vocabulary of {target.cfg.vocab_size}: sampled speculation needs whole rows "
+                             "(tensor-parallel ranks have shards of them), and one vocabulary")
         return torch.softmax(logits.float() / temperature, -1)
 
     def uniforms(*shape):

@@ -191,6 +191,25 @@ def test_holes(W):
     assert not bool(got[2].any())
 
 
+@pytest.mark.parametrize("W", [1, 3, 24])
+def test_positions_beyond_everything(W):
+    """Positions and lengths that no table has: nothing is read or written outside; the row sees the whole table."""
+    far = make(11, "cuda", BF16, 3, W, 8, 2, 128, 16, [40, 17, 70])
+    far["positions"][0], far["positions"][1] = 2 ** 63 - 1, -2 ** 63
+    d = {**far, "lens": torch.tensor([2 ** 62, W, -5], device="cuda")}
+    d["k_cache"].nan_to_num_(0.0)
+    d["v_cache"].nan_to_num_(0.0)
+    cos, sin = ops.rope.rope_tables(64, 128, device="cuda")
+    before = d["k_cache"].clone()
+    q = ops.paged.rope_append(d["q"], d["k"], d["v"], d["positions"], cos, sin, d["k_cache"], d["v_cache"], d["table"], lens=d["lens"])
+    assert not bool(q.any()) and torch.equal(before, d["k_cache"])
+    got = attend(d)
+    end = {**d, "positions": torch.tensor([d["table"].shape[1] * 16 - 1, -1, 70], device="cuda"), "lens": torch.tensor([W, 0, 0], device="cuda")}
+    want, size = oracle.attention(end["q"], end["k_cache"], end["v_cache"], end["table"], end["positions"], lens=end["lens"])
+    assert bool(((got[0].double() - want[0]).abs() <= bound(BF16, want[0], size[0])).all())
+    assert not bool(got[1:].any())
+
+
 def test_positions_behind_the_table():
     d = make(11, "cuda", BF16, 2, 4, 8, 2, 128, 16, [30, 62], cols=6)
     d["table"] = d["table"][:, :3].contiguous()
@@ -255,6 +274,18 @@ def test_shared_is_what_the_tables_say():
     a = attend(d)
     d["table"][:, :2] = -1
     assert torch.equal(a, attend(d))
+
+
+@pytest.mark.parametrize("W", [1, 16, 17, 40, 100])
+def test_shared_windows_and_portions(W):
+    """Few rows, tiles of them, and portions of prompts, which read the shared pages as their own."""
+    d = make(19, "cuda", BF16, 3, W, 8, 1, 128, 32, [96, 150, 260], [W, 1, W], 3)
+    a = attend(d)
+    check(d, a)
+    d["table"][:, :3] = -1
+    assert torch.equal(a, attend(d))
+    none = {**d, "shared_pages": d["shared_pages"][:0], "table": torch.cat([d["shared_pages"].expand(3, 3), d["table"][:, 3:]], 1)}
+    check(none, attend(none))
 
 
 def test_long_shared_prefix():
