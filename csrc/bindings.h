@@ -27,5 +27,6 @@ void embedding_grad(const Tensor& ids, const Tensor& gy, Tensor out, bool zero_f
 c10::optional<Tensor> linear_swiglu(const Tensor& x, const Tensor& w, bool few, Tensor* keep);
 Tensor gemv(const Tensor& x, const Tensor& w, const c10::optional<Tensor>& residual);
 
+void count_launches(int64_t n);        // kernels of this package that a binding launched without Python's counting them
 void bind_native_autograd(pybind11::module_& m);
 void bind_paged(pybind11::module_& m);

@@ -230,7 +230,7 @@ struct PagedPlan {
   long slots, pre_slots;             // rows of parts that each leaves
 };
 PagedPlan paged_plan(PagedAttn& p);  // fills in p's cuts
-void paged_attention(const PagedAttn& p, const PagedPlan& plan, int D, int dt, cudaStream_t st);
+int paged_attention(const PagedAttn& p, const PagedPlan& plan, int D, int dt, cudaStream_t st);        // → launches
 void paged_tiles(const PagedAttn& p, int grid, bool over_shared, int D, int dt, cudaStream_t st);       // paged_attention_sm100.cu
 // strides s: (b, w, h) of q, k, v; cs: (page, row, head) of the caches; q_out: heads and columns contiguous
 void paged_append(const void* q, const void* k, const void* v, const long* positions, const long* lens, const float* cos_t, const float* sin_t,

@@ -527,7 +527,7 @@ void launch_rows(const PagedAttn& p, int grid, cudaStream_t st) {
   NXD_CUDA_CHECK(cudaLaunchKernelEx(&cfg, paged_rows_kernel<T, D, R, DEAL>, p));
 }
 template <typename T, int D>
-void launch(const PagedAttn& p, const PagedPlan& plan, int dt, cudaStream_t st) {
+int launch(const PagedAttn& p, const PagedPlan& plan, int dt, cudaStream_t st) {
   if (p.shared) {
     if (plan.pre_tiles) paged_tiles(p, plan.pre_grid, true, D, dt, st);
     else if (p.pre_tile_rows == 8) launch_rows<T, D, 1, kShared>(p, plan.pre_grid, st);
@@ -543,6 +543,7 @@ void launch(const PagedAttn& p, const PagedPlan& plan, int dt, cudaStream_t st) 
     launch_dependent(paged_join_kernel<T, D>, dim3(p.B * p.row_tiles, (rows * p.Hkv + kWarps - 1) / kWarps), kThreads, 0, st, p, plan.grid);
   else if (!p.cluster && plan.grid > 1)
     launch_dependent(paged_merge_kernel<T, D>, dim3(plan.grid - 1, (rows + kWarps - 1) / kWarps), kThreads, 0, st, p, plan.grid);
+  return p.shared ? 3 : !p.cluster && plan.grid > 1 ? 2 : 1;
 }
 
 }  // namespace
@@ -595,9 +596,9 @@ PagedPlan paged_plan(PagedAttn& p) {
   return plan;
 }
 
-void paged_attention(const PagedAttn& p, const PagedPlan& plan, int D, int dt, cudaStream_t st) {
-  if (dt == kBF16) { if (D == 128) launch<__nv_bfloat16, 128>(p, plan, dt, st); else launch<__nv_bfloat16, 64>(p, plan, dt, st); }
-  else { if (D == 128) launch<__half, 128>(p, plan, dt, st); else launch<__half, 64>(p, plan, dt, st); }
+int paged_attention(const PagedAttn& p, const PagedPlan& plan, int D, int dt, cudaStream_t st) {
+  if (dt == kBF16) return D == 128 ? launch<__nv_bfloat16, 128>(p, plan, dt, st) : launch<__nv_bfloat16, 64>(p, plan, dt, st);
+  return D == 128 ? launch<__half, 128>(p, plan, dt, st) : launch<__half, 64>(p, plan, dt, st);
 }
 
 void paged_append(const void* q, const void* k, const void* v, const long* positions, const long* lens, const float* cos_t, const float* sin_t,

@@ -3,6 +3,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <cmath>
 #include <string>
 
 #include "bindings.h"
@@ -77,11 +78,13 @@ Tensor rows_out(const Tensor& q) {
   return at::empty_strided({B, W, H, D}, {H * D, B * H * D, D, 1}, q.options());
 }
 
-Tensor paged_append(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& positions_, const Tensor& cos_t, const Tensor& sin_t, Tensor kc,
+// None: not for the kernel
+c10::optional<Tensor> paged_append(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& positions_, const Tensor& cos_t, const Tensor& sin_t, Tensor kc,
                     Tensor vc, const Tensor& table_, const c10::optional<Tensor>& lens_) {
   const Tensor positions = ints(positions_, at::kLong), table = as_table(table_);
   const c10::optional<Tensor> lens = ints(lens_, at::kLong);
   check_cache(q_, kc, vc, table, positions, lens);
+  if (!paged_append_ok(q_, kc, vc)) return c10::nullopt;
   CHECK_ARG(k_.sizes() == v_.sizes() && k_.dim() == 4 && k_.size(0) == q_.size(0) && k_.size(1) == q_.size(1) && k_.size(2) == kc.size(2) &&
             k_.size(3) == q_.size(3), "new keys and values must be " + list({q_.size(0), q_.size(1), kc.size(2), q_.size(3)}));
   CHECK_ARG(k_.scalar_type() == q_.scalar_type() && v_.scalar_type() == q_.scalar_type() && k_.device() == q_.device() && v_.device() == q_.device(),
@@ -89,7 +92,7 @@ Tensor paged_append(const Tensor& q_, const Tensor& k_, const Tensor& v_, const 
   CHECK_ARG(cos_t.dim() == 2 && cos_t.sizes() == sin_t.sizes() && cos_t.size(1) * 2 == q_.size(3) && cos_t.scalar_type() == at::kFloat &&
             sin_t.scalar_type() == at::kFloat && cos_t.is_contiguous() && sin_t.is_contiguous() && cos_t.device() == q_.device() && sin_t.device() == q_.device(),
             "cos and sin must be contiguous float32 tables [positions, " + std::to_string(q_.size(3) / 2) + "]");
-  CHECK_ARG(q_.is_cuda() && paged_append_ok(q_, kc, vc), "the kernel takes caches of whole 16-byte packets");
+  CHECK_ARG(q_.is_cuda(), "the kernel's tensors are on a GPU");
   c10::cuda::CUDAGuard guard(q_.device());
   const Tensor q = as_packets(q_), k = as_packets(k_), v = as_packets(v_), cos_p = as_packets(cos_t), sin_p = as_packets(sin_t);
   Tensor out = rows_out(q);
@@ -100,15 +103,18 @@ Tensor paged_append(const Tensor& q_, const Tensor& k_, const Tensor& v_, const 
                     cos_p.data_ptr<float>(), sin_p.data_ptr<float>(), out.data_ptr(), kc.data_ptr(), vc.data_ptr(), table.data_ptr<int>(), (int)q.size(0),
                     (int)q.size(1), (int)q.size(2), (int)kc.size(2), (int)q.size(3), (int)cos_t.size(0), (int)table.size(1), (int)kc.size(1),
                     (int)kc.size(0), table.stride(0), s, out.stride(0), out.stride(1), cs, dt_code(q), stream());
+  count_launches(1);
   return out;
 }
 
-Tensor paged_attention(const Tensor& q_, const Tensor& kc, const Tensor& vc, const Tensor& table_, const Tensor& positions_, double scale,
-                       const c10::optional<Tensor>& lens_, const c10::optional<Tensor>& shared_pages_) {
+// None: not for the kernels
+c10::optional<Tensor> paged_attention(const Tensor& q_, const Tensor& kc, const Tensor& vc, const Tensor& table_, const Tensor& positions_,
+                                      const c10::optional<double>& scale_, const c10::optional<Tensor>& lens_, const c10::optional<Tensor>& shared_pages_) {
   const Tensor positions = ints(positions_, at::kLong), table = as_table(table_);
   const c10::optional<Tensor> lens = ints(lens_, at::kLong), shared_pages = ints(shared_pages_, at::kInt);
   check_cache(q_, kc, vc, table, positions, lens);
-  CHECK_ARG(q_.is_cuda() && paged_attention_ok(q_, kc, vc), "the kernels take 16-bit types, heads of 64 or 128 numbers and caches of whole 16-byte packets");
+  if (!paged_attention_ok(q_, kc, vc)) return c10::nullopt;
+  CHECK_ARG(q_.is_cuda(), "the kernels' tensors are on a GPU");
   const int64_t ps = kc.size(1);
   int64_t shared = 0;                              // shared pages
   if (shared_pages.has_value()) {
@@ -118,6 +124,7 @@ Tensor paged_attention(const Tensor& q_, const Tensor& kc, const Tensor& vc, con
     CHECK_ARG(shared_pages->size(0) <= table.size(1),
               "more shared pages than a sequence has: " + std::to_string(shared_pages->size(0)) + ", page_table of " + std::to_string(table.size(1)));
   }
+  const double scale = scale_.has_value() ? *scale_ : 1 / std::sqrt((double)q_.size(3));
   CHECK_ARG(scale > 0 && scale < 1e30, "the scale of the scores is positive");
   c10::cuda::CUDAGuard guard(q_.device());
   const Tensor q = as_packets(q_);
@@ -146,7 +153,7 @@ Tensor paged_attention(const Tensor& q_, const Tensor& kc, const Tensor& vc, con
   p.part_ml = p.pre_o + plan.pre_slots * D;
   p.pre_ml = p.part_ml + plan.slots * 2;
   p.scale_log2 = (float)(scale * 1.4426950408889634);
-  nxd::paged_attention(p, plan, (int)D, dt_code(q), stream());
+  count_launches(nxd::paged_attention(p, plan, (int)D, dt_code(q), stream()));
   return out;
 }
 
@@ -171,6 +178,7 @@ std::vector<Tensor> verify_drafts(const Tensor& tokens, const Tensor& draft_, co
   const long ds[2] = {draft.stride(0), draft.stride(1)}, ts[2] = {target.stride(0), target.stride(1)};
   nxd::verify_drafts(tokens.data_ptr<long>(), draft.data_ptr(), target.data_ptr(), accept.data_ptr<float>(), sample.data_ptr<float>(),
                      out.data_ptr<long>(), accepted.data_ptr<long>(), (int)B, (int)K, (int)target.size(2), ds, ts, dt_code(target), stream());
+  count_launches(B > 0);
   return {out, accepted};
 }
 

@@ -32,6 +32,15 @@ def _no_gradient(name: str, *tensors: torch.Tensor) -> None:
         raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or with tensors that ask for none")
 
 
+def _kernels(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ok: str):
+    """The extension, whose entry points take what is for their kernels and return None for the rest; a recorded call has to be one that they take."""
+    if not _ext.use_cuda(q):
+        return None
+    if _ext._PLAN_PROXY is not None and not getattr(_ext._load(), ok)(q, k_cache, v_cache):
+        return None
+    return _ext.ext()
+
+
 def _check(q, k_cache, v_cache, page_table, positions, lens) -> None:
     """The refusals of ``csrc/paged_binding.cpp`` for tensors that the kernels do not take."""
     def need(ok, text):
@@ -63,9 +72,11 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     to the pages, in one launch.  ``cos`` / ``sin [positions, D / 2]`` fp32: :func:`ops.rope.rope_tables`.  Tokens that do not count, or that stand
     behind the tables' end, come back as zeros and are not written; tokens behind the page table's end are not written."""
     _no_gradient("rope_append", q, k, v, k_cache, v_cache)
-    if _ext.use_cuda(q) and _ext._load().paged_append_ok(q, k_cache, v_cache):
-        _ext.count_launch()
-        return _ext.ext().paged_append(q, k, v, positions, cos, sin, k_cache, v_cache, page_table, lens)
+    e = _kernels(q, k_cache, v_cache, "paged_append_ok")
+    if e is not None:
+        out = e.paged_append(q, k, v, positions, cos, sin, k_cache, v_cache, page_table, lens)
+        if out is not None:
+            return out
     positions, page_table = _ints(positions, torch.long).clamp(-1, 1 << 40), _table(page_table)
     lens = None if lens is None else _ints(lens, torch.long)
     _check(q, k_cache, v_cache, page_table, positions, lens)
@@ -106,10 +117,12 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pag
     ``shared_pages [n]`` int32: the pages of the first ``n * page_size`` tokens of EVERY sequence; the first ``n`` columns of ``page_table`` are not
     looked at.  Where a sequence has up to 128 query rows (tokens times heads of a group), they are read once for the whole batch."""
     _no_gradient("paged attention", q, k_cache, v_cache)
+    e = _kernels(q, k_cache, v_cache, "paged_attention_ok")
+    if e is not None:
+        out = e.paged_attention(q, k_cache, v_cache, page_table, positions, scale, lens, shared_pages)
+        if out is not None:
+            return out
     scale = 1.0 / math.sqrt(q.shape[-1]) if scale is None else float(scale)
-    if _ext.use_cuda(q) and _ext._load().paged_attention_ok(q, k_cache, v_cache):
-        _ext.count_launch(2 if shared_pages is None else 3)
-        return _ext.ext().paged_attention(q, k_cache, v_cache, page_table, positions, scale, lens, shared_pages)
     positions, page_table = _ints(positions, torch.long).clamp(-1, 1 << 40), _table(page_table)
     lens = None if lens is None else _ints(lens, torch.long)
     if shared_pages is not None:

@@ -56,8 +56,7 @@ def verify_drafts(draft_tokens: torch.Tensor, draft_probs: torch.Tensor, target_
     if torch.is_grad_enabled() and (draft_probs.requires_grad or target_probs.requires_grad):
         raise RuntimeError("verify_drafts has no gradient: call it under torch.no_grad(), or with tensors that ask for none")
     draft_tokens, accept_uniforms, sample_uniforms = draft_tokens.contiguous(), accept_uniforms.contiguous(), sample_uniforms.contiguous()
-    if _ext.use_cuda(draft_tokens, draft_probs, target_probs):
-        _ext.count_launch()
+    if _ext.use_cuda(target_probs):
         return tuple(_ext.ext().verify_drafts(draft_tokens, draft_probs, target_probs, accept_uniforms, sample_uniforms))
 
     def need(ok, text):
