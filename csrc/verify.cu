@@ -120,38 +120,34 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const long* tokens,
       if (lane == 0) block_sum = x;
     }
     cluster_sync_all();
-    double total = 0;
-    for (int r = 0; r < size; ++r) total += remote_double(&block_sum, r);
-    return total;
+    return lane < size ? remote_double(&block_sum, lane) : 0.;
   };
-  double total = add_up(q);
+  double of_block = add_up(q), total = warp_sum64(of_block);           // lane = block
   if (q && !(total > 0)) {                                 // nothing is left of p - q: from p itself
     cluster_sync_all();                                    // every block has read the sums
     q = nullptr;
-    total = add_up(q);
+    of_block = add_up(q);
+    total = warp_sum64(of_block);
   }
   if (warp == 0) {
     const double want = (double)sample[b] * total;
     // the block, then the part, in which the running sum passes `want`; if roundings leave none, the last that has anything
-    double before = 0, base = 0;
-    int mine = -1;
-    for (int r = 0; r < size; ++r) {
-      const double x = remote_double(&block_sum, r);
-      if (x > 0) { mine = r; base = before; }
-      before += x;
-      if (x > 0 && before > want) break;
-    }
-    if (mine == rank) {
-      const double x = sums[lane];
+    auto find = [&](double x, double before, double& start) {          // lane = place; start: the sum before the place found
       double scan = x;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const double y = __shfl_up_sync(0xffffffffu, scan, o);
         if (lane >= o) scan += y;
       }
-      const unsigned some = __ballot_sync(0xffffffffu, x > 0), past = __ballot_sync(0xffffffffu, x > 0 && base + scan > want);
+      const unsigned some = __ballot_sync(0xffffffffu, x > 0), past = __ballot_sync(0xffffffffu, x > 0 && before + scan > want);
       const int at = past ? __ffs(past) - 1 : 31 - __clz(some);
-      double start = base + __shfl_sync(0xffffffffu, scan - x, at);
+      if (at >= 0) start = before + __shfl_sync(0xffffffffu, scan - x, at);
+      return at;
+    };
+    double base = 0, start = 0;
+    const int mine = find(of_block, 0., base);
+    if (mine == rank) {
+      const int at = find(sums[lane], base, start);
       const int f0 = (int)first_step(at), f1 = (int)first_step(at + 1);
       long chosen = -1, last = -1;
       for (int s = f0; s < f1 && chosen < 0; s += kAhead) {
