@@ -449,8 +449,8 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn
   if (late) pdl_wait();
 }
 
-// Pairs that are cut: block (c − 1, ·) has the one that is cut first in front of block c's share, and a warp of it joins the parts of two rows.
-template <typename T, int D>
+// Pairs that are cut: block (c − 1, ·) has the one that is cut first in front of block c's share, and a warp of it joins the parts of ROWS rows at a time.
+template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const PagedAttn p, int grid) {
   const int block = blockIdx.x + 1;
   const Place at = find_place<kThreads, false>(p, grid, block);        // the kernel before this one waited for all that positions come from
@@ -461,10 +461,17 @@ __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const PagedAttn p
   const long off = at.tile % tiles, t0 = block * at.per - off;
   if (off == 0 || off > at.per) return;                    // not cut here, or before
   const int b = at.e / p.row_tiles, n = (int)((t0 + tiles - 1) / at.per) - (block - 1) + 1;
-  const int rs = blockIdx.y * kWarps + (threadIdx.x >> 5), row = at.e % p.row_tiles * p.tile_rows + rs, w = row / p.G;
-  if (rs >= p.tile_rows || row >= p.W * p.G) return;
-  join_parts<T, D>(p, w < new_tokens(p, b) ? n : 0, [&](int x) { return part_slot<false>(p, 0, block - 1 + x, x == 0) * p.tile_rows + rs; },
-                   reinterpret_cast<T*>(p.out) + b * p.o_sb + w * p.o_sw + (long)(head * p.G + row % p.G) * p.o_sh);
+  const int row0 = at.e % p.row_tiles * p.tile_rows, rows = min(p.tile_rows, p.W * p.G - row0), m = new_tokens(p, b);
+  for (int r0 = (blockIdx.y * kWarps + (threadIdx.x >> 5)) * ROWS; r0 < rows; r0 += gridDim.y * kWarps * ROWS) {
+    bool live[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) live[r] = r0 + r < rows && (row0 + r0 + r) / p.G < m;
+    join_parts<T, D, ROWS>(p, n, live, [&](int x, int r) { return part_slot<false>(p, 0, block - 1 + x, x == 0) * p.tile_rows + r0 + r; },
+                           [&](int r) {
+                             const int row = row0 + r0 + r, w = row / p.G;
+                             return r0 + r < rows ? reinterpret_cast<T*>(p.out) + b * p.o_sb + w * p.o_sw + (long)(head * p.G + row % p.G) * p.o_sh : nullptr;
+                           });
+  }
 }
 
 // With shared pages: every row's parts over the shared pages and over its own.  Block (entry, ·), a warp per row and key/value head.
@@ -501,12 +508,13 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const PagedAttn p,
   pdl_trigger();
   pdl_wait();
   if (item >= rows * p.Hkv) return;
-  join_parts<T, D>(p, live ? over + own : 0,
-                   [&](int x) {
-                     return x < over ? p.slots + part_slot<true>(p, pre, c0 + x, x == 0) * p.pre_tile_rows + at
-                                     : part_slot<false>(p, (long)e * p.Hkv + head, b0 + x - over, x == over) * p.tile_rows + rs;
-                   },
-                   reinterpret_cast<T*>(p.out) + b * p.o_sb + w * p.o_sw + (long)(head * p.G + row % p.G) * p.o_sh);
+  const bool counts[1] = {live};
+  join_parts<T, D, 1>(p, live ? over + own : 0, counts,
+                      [&](int x, int) {
+                        return x < over ? p.slots + part_slot<true>(p, pre, c0 + x, x == 0) * p.pre_tile_rows + at
+                                        : part_slot<false>(p, (long)e * p.Hkv + head, b0 + x - over, x == over) * p.tile_rows + rs;
+                      },
+                      [&](int) { return reinterpret_cast<T*>(p.out) + b * p.o_sb + w * p.o_sw + (long)(head * p.G + row % p.G) * p.o_sh; });
 }
 
 template <typename T, int D, int R, Deal DEAL>
@@ -541,8 +549,16 @@ int launch(const PagedAttn& p, const PagedPlan& plan, int dt, cudaStream_t st) {
   const int rows = std::min(p.tile_rows, p.W * p.G);
   if (p.shared)
     launch_dependent(paged_join_kernel<T, D>, dim3(p.B * p.row_tiles, (rows * p.Hkv + kWarps - 1) / kWarps), kThreads, 0, st, p, plan.grid);
-  else if (!p.cluster && plan.grid > 1)
-    launch_dependent(paged_merge_kernel<T, D>, dim3(plan.grid - 1, (rows + kWarps - 1) / kWarps), kThreads, 0, st, p, plan.grid);
+  else if (!p.cluster && plan.grid > 1) {
+    // a warp joins four rows at once where there are many, whose loads are in flight together; eight blocks of y, or what follows has waves (us, 2 x 1000
+    // tokens of 48 heads of 64 behind 6000 keys, a block for 8 rows each / this: 166 / 156; 2 x 1000 tokens, 32 heads, to 2000 keys 112 / 102; 463
+    // tokens, 64 heads, to 489 keys 54 / 45).  Few rows have more parts each, and warps enough.
+    auto merge = [&](auto kernel, int each) {
+      launch_dependent(kernel, dim3(plan.grid - 1, std::min((rows + each * kWarps - 1) / (each * kWarps), 8)), kThreads, 0, st, p, plan.grid);
+    };
+    if (rows > 64) merge(paged_merge_kernel<T, D, 4>, 4);
+    else merge(paged_merge_kernel<T, D, 1>, 1);
+  }
   return p.shared ? 3 : !p.cluster && plan.grid > 1 ? 2 : 1;
 }
 

@@ -119,46 +119,65 @@ NXD_DEVICE long part_slot(const PagedAttn& p, long pair, int block, bool begins)
   return begins ? pair : (long)p.Hkv * (SHARED ? p.pre_row_tiles : p.B * p.row_tiles) + block;
 }
 
-// Joins n parts of a row, D / 32 columns a lane; slot(x) is the row of part x among all parts' rows.  The first eight are asked for before their weights
-// are known.
-template <typename T, int D, typename F>
-NXD_DEVICE void join_parts(const PagedAttn& p, int n, F slot, T* row) {
-  constexpr int C = D / 32, AHEAD = 8;
+// Joins n parts of each of ROWS rows, D / 32 columns a lane; slot(x, r) is the row of part x of row r among all parts' rows, row(r) where it goes, null:
+// nowhere.  A row that is not live is zeros.  The first eight (parts times rows) are asked for before their weights are known.
+template <typename T, int D, int ROWS, typename F, typename G>
+NXD_DEVICE void join_parts(const PagedAttn& p, int n, const bool (&live)[ROWS], F slot, G row) {
+  constexpr int C = D / 32, AHEAD = 8 / ROWS;
   const int lane = threadIdx.x & 31;
   const float2* ml = reinterpret_cast<const float2*>(p.part_ml);
-  float m = -INFINITY, l = 0.f, acc[C] = {};
+  float m[ROWS], l[ROWS], acc[ROWS][C] = {};
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) { m[r] = -INFINITY; l[r] = 0.f; }
   for (int x0 = 0; x0 < n; x0 += 32) {
     const int here = min(32, n - x0);
-    float v[AHEAD][C];
+    float v[AHEAD][ROWS][C], f[ROWS];
     auto ask = [&](int x1) {
 #pragma unroll
       for (int x = 0; x < AHEAD; ++x)
-        if (x1 + x < here) {
-          const float* src = p.part_o + slot(x0 + x1 + x) * D + lane * C;
-          if constexpr (C == 4) *reinterpret_cast<float4*>(v[x]) = *reinterpret_cast<const float4*>(src);
-          else *reinterpret_cast<float2*>(v[x]) = *reinterpret_cast<const float2*>(src);
-        }
+#pragma unroll
+        for (int r = 0; r < ROWS; ++r)
+          if (x1 + x < here && live[r]) {
+            const float* src = p.part_o + slot(x0 + x1 + x, r) * D + lane * C;
+            if constexpr (C == 4) *reinterpret_cast<float4*>(v[x][r]) = *reinterpret_cast<const float4*>(src);
+            else *reinterpret_cast<float2*>(v[x][r]) = *reinterpret_cast<const float2*>(src);
+          }
     };
     ask(0);
-    const float2 a = lane < here ? ml[slot(x0 + lane)] : make_float2(-INFINITY, 0.f);
-    const float mn = fmaxf(m, warp_max(a.x)), old = m == -INFINITY ? 0.f : exp2f(m - mn), f = a.x == -INFINITY ? 0.f : exp2f(a.x - mn);
-    l = l * old + warp_sum(a.y * f);
-    m = mn;
+    float2 a[ROWS];
 #pragma unroll
-    for (int j = 0; j < C; ++j) acc[j] *= old;
+    for (int r = 0; r < ROWS; ++r) a[r] = lane < here && live[r] ? ml[slot(x0 + lane, r)] : make_float2(-INFINITY, 0.f);
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) {
+      const float mn = fmaxf(m[r], warp_max(a[r].x)), old = m[r] == -INFINITY ? 0.f : exp2f(m[r] - mn);
+      f[r] = a[r].x == -INFINITY ? 0.f : exp2f(a[r].x - mn);
+      l[r] = l[r] * old + warp_sum(a[r].y * f[r]);
+      m[r] = mn;
+#pragma unroll
+      for (int j = 0; j < C; ++j) acc[r][j] *= old;
+    }
     for (int x1 = 0; x1 < here; x1 += AHEAD) {
       if (x1) ask(x1);
 #pragma unroll
-      for (int x = 0; x < AHEAD; ++x) {
-        const float g = __shfl_sync(0xffffffffu, f, (x1 + x) & 31);
+      for (int x = 0; x < AHEAD; ++x)
 #pragma unroll
-        for (int j = 0; j < C; ++j) acc[j] += x1 + x >= here || g == 0.f ? 0.f : v[x][j] * g;        // a part without weights has no sums
-      }
+        for (int r = 0; r < ROWS; ++r) {
+          const float g = __shfl_sync(0xffffffffu, f[r], (x1 + x) & 31);
+#pragma unroll
+          for (int j = 0; j < C; ++j) acc[r][j] += x1 + x >= here || g == 0.f ? 0.f : v[x][r][j] * g;        // a part without weights has no sums
+        }
     }
   }
-  T* dst = row + lane * C;
 #pragma unroll
-  for (int j = 0; j < C; ++j) dst[j] = from_f32<T>(l == 0.f ? 0.f : acc[j] / l);
+  for (int r = 0; r < ROWS; ++r) {
+    T* const to = row(r);
+    if (!to) continue;
+    T o[C];
+#pragma unroll
+    for (int j = 0; j < C; ++j) o[j] = from_f32<T>(l[r] == 0.f ? 0.f : acc[r][j] / l[r]);
+    if constexpr (C == 4) *reinterpret_cast<uint2*>(to + lane * C) = *reinterpret_cast<const uint2*>(o);
+    else *reinterpret_cast<uint32_t*>(to + lane * C) = *reinterpret_cast<const uint32_t*>(o);
+  }
 }
 
 // Zeros for the rows of entries none of whose tokens sees a key, or counts, sixteen rows of an entry at a time, dealt out over the blocks.  (With shared
