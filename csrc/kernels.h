@@ -217,6 +217,7 @@ struct PagedAttn {
   int B, W, G, Hkv, cols, ps, pages, shared_cols;
   int shared;                        // keys in shared pages, if those are walked for the whole batch at once; otherwise 0
   int row_tiles, tile_rows, tile_keys, min_tiles; // how rows and keys are cut, and a block's least share of tiles
+  int whole_tiles;                   // pairs of at most this many tiles are not cut
   int cluster;                       // blocks that share a pair, none of them with others (0: dealt out)
   int pre_row_tiles, pre_tile_rows, pre_tiles, pre_per;      // the same over the shared pages: rows of the whole batch; key tiles of a pair and of a block
   long q_sb, q_sw, q_sh, o_sb, o_sw, o_sh, table_sb;

@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(kThreads) paged_merge_kernel(const PagedAttn p
   if (at.e >= p.B * p.row_tiles) return;
   const int tiles = entry_tiles(p, at.e), head = (int)(at.tile / tiles);
   const long off = at.tile % tiles, t0 = block * at.per - off;
-  if (off == 0 || off > at.per) return;                    // not cut here, or before
+  if (off == 0 || off > at.per || whole<false>(p, tiles)) return;      // not cut here, or before, or not at all
   const int b = at.e / p.row_tiles, n = (int)((t0 + tiles - 1) / at.per) - (block - 1) + 1;
   const int row0 = at.e % p.row_tiles * p.tile_rows, rows = min(p.tile_rows, p.W * p.G - row0), m = new_tokens(p, b);
   for (int r0 = (blockIdx.y * kWarps + (threadIdx.x >> 5)) * ROWS; r0 < rows; r0 += gridDim.y * kWarps * ROWS) {
@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(kThreads) paged_join_kernel(const PagedAttn p,
     const int tiles = entry_tiles(p, e);
     const long t0 = first * p.Hkv + (long)head * tiles;
     b0 = (int)(t0 / per);
-    own = tiles ? (int)((t0 + tiles - 1) / per) - b0 + 1 : 0;
+    own = tiles == 0 ? 0 : whole<false>(p, tiles) ? 1 : (int)((t0 + tiles - 1) / per) - b0 + 1;
   }
   const bool live = item < rows * p.Hkv && w < new_tokens(p, b);
   const long r = (long)b * p.W * p.G + row, pre = r / p.pre_tile_rows * p.Hkv + head, s0 = pre * p.pre_tiles;
@@ -581,10 +581,17 @@ PagedPlan paged_plan(PagedAttn& p) {
   // 11 / 18, 32 to 1000 33 / 43).
   const long pairs = (long)p.B * p.Hkv, cap = (long)p.cols * p.ps - p.shared;
   plan.tiles = cut(rows, cap > 2048 && pairs * cap > 131072 ? 8 : 16, p.tile_rows);
+  // Row tiles of 256 read keys half as often, but they have to fill the GPU (us, 256 / 128 rows: 33 tokens, 48 heads on 8, 21 / 17; 300, 8 on 8, 27 / 22;
+  // 4 x 64, 32 on 8, to 3000 keys 47 / 40; but 500, 32 on 8, to 6000 72 / 80, 1000 to 1000 46 / 83).
+  if (p.tile_rows == 256 && (rows + 255) / 256 * pairs * 5 < 2 * sms) p.tile_rows = 128;
   p.row_tiles = (int)((rows + p.tile_rows - 1) / p.tile_rows);
   auto tile_keys = [](int tile_rows) { return tile_rows == 256 ? 128 : kTileKeys; };
   p.tile_keys = tile_keys(p.tile_rows);
-  p.min_tiles = 256 / p.tile_keys;
+  p.min_tiles = plan.tiles ? 1 : 256 / p.tile_keys;
+  // A cut writes and reads the sums of all rows once more for each part, and a last launch has work: short pairs are not cut (us, cut / not: 463 tokens,
+  // 64 heads on 8, 45 / 37; 1000, 32 on 8, 56 / 46; 2 x 1000 to 2000 keys 104 / 90; 283, 8 on 8, 22 / 20).  Windows' sums are small: 16 x 6 tokens,
+  // 32 heads on 8, to 900 keys, 12 tiles at most not cut / 4: 32 / 28.
+  p.whole_tiles = !plan.tiles ? 0 : p.tile_rows == 64 ? 4 : 12;
   plan.grid = plan.tiles ? sms : 2 * sms;
   // A cluster per pair, as many blocks in it as the GPU takes at once, has neither a search for places nor a second launch (us, dealt out / cluster:
   // 1 sequence of 1000 keys, 8 heads, 19 / 9.8; 64 of 300 to 600, 8 heads, 36 / 28; 16 of 4096 to 8192, 8 heads, 72 / 68), but the longest

@@ -4,8 +4,9 @@
 // is a (sequence, row tile), a pair an (entry, key/value head); a pair's key tiles are those that its newest token sees.  All key tiles of a
 // launch, pair after pair, are dealt out evenly: block c takes `per` of them from c * per on, wherever that lies, so that long and short
 // sequences in one batch fill the GPU alike.  Each block finds its place from the positions alone: nothing about lengths has to be known on the
-// host.  A pair that lies within one block is finished there; of one that is cut every block leaves its part in a workspace (slot 2 c + 1 if the pair
-// begins in block c, 2 c if it began before), and a second launch joins them.  Where there are shared pages, their rows are those of the whole
+// host.  On the tensor memory a pair of few tiles is not cut: it belongs to the block in whose share it begins.  A pair that lies within one block is
+// finished there; of one that is cut every block leaves its part in a workspace (slot 2 c + 1 if the pair begins in block c, 2 c if it began before),
+// and a second launch joins them.  Where there are shared pages, their rows are those of the whole
 // batch, cut and dealt out in the same way by a launch of their own; then all results of either are parts (slot: the pair's number, or the
 // number of pairs + c), and the last launch joins both kinds.  The launch over the shared pages goes first.  Its blocks let the next launch start
 // when they have waited for everything before them, and that one, which reads nothing that they write, waits for them at its end alone: the two
@@ -111,6 +112,9 @@ NXD_DEVICE void next_pair(const PagedAttn& p, Walk& w) {
   if constexpr (!SHARED)
     while ((w.tiles = w.e < p.B * p.row_tiles ? entry_tiles(p, w.e) : 1) == 0) ++w.e;
 }
+
+// Whether a pair is not cut, so that it belongs to the block in whose share it begins, however far it reaches into the next one's
+template <bool SHARED> NXD_DEVICE bool whole(const PagedAttn& p, int tiles) { return !SHARED && tiles <= p.whole_tiles; }
 
 // Slot of the part that block `block` leaves of pair `pair`
 template <bool SHARED>

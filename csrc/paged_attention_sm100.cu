@@ -105,7 +105,7 @@ template <bool PAIR, bool SHARED>
 NXD_DEVICE Item make_item(const PagedAttn& p, const Walk& w, long left) {
   Item it;
   it.e = w.e; it.head = w.head; it.j0 = w.tile;
-  it.n = (int)min((long)(w.tiles - w.tile), left);
+  it.n = whole<SHARED>(p, w.tiles) ? w.tiles : (int)min((long)(w.tiles - w.tile), left);
   it.ends = (w.tile == 0) | (w.tile + it.n == w.tiles ? 2 : 0);
   it.keys = SHARED ? p.shared : all_keys(p, w.e / p.row_tiles);
   if constexpr (PAIR) {
@@ -353,6 +353,10 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         w.tiles = walk_tiles<SHARED>(p, at.e);
         w.head = (int)(at.tile / w.tiles);
         w.tile = (int)(at.tile % w.tiles);
+        if (w.tile > 0 && whole<SHARED>(p, w.tiles)) {       // the block in front has it
+          left -= w.tiles - w.tile;
+          if (left > 0) next_pair<SHARED>(p, w);
+        }
       }
       bool more = true;
       for (int i = 0; more; ++i) {

@@ -110,6 +110,19 @@ def test_windows_of_many_lengths(W, H, Hkv, shared):
         assert torch.equal(got, attend(d))
 
 
+@pytest.mark.parametrize("B, W, H, Hkv, shared", [(30, 5, 8, 1, 0), (30, 10, 8, 1, 0), (30, 10, 8, 1, 3), (24, 20, 16, 2, 0), (24, 40, 16, 2, 0), (2, 300, 8, 2, 0)])
+@pytest.mark.parametrize("D", [64, 128])
+def test_short_pairs_and_long_ones(B, W, H, Hkv, shared, D):
+    """Pairs that one block takes whole beside pairs that are cut, over all sizes of row tiles; rows that do not count and sequences without tokens."""
+    g = torch.Generator().manual_seed(W)
+    for most in (40, 500, 3000):
+        positions = (48 + torch.randint(0, most, (B,), generator=g)).tolist()
+        lens = torch.randint(0, W + 1, (B,), generator=g).tolist()
+        lens[0], positions[-1], lens[-1] = W, 2200, W
+        d = make(7, "cuda", BF16, B, W, H, Hkv, D, 16, positions, lens, shared)
+        check(d, attend(d))
+
+
 def oracle_size(d):
     """A bound of the weighted average of the values' magnitudes, without its softmax: the largest that a row sees."""
     v = d["v_cache"].double().nan_to_num(0.0)
