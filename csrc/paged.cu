@@ -608,11 +608,16 @@ PagedPlan paged_plan(PagedAttn& p) {
   p.slots = plan.slots;
   if (p.shared) {
     plan.pre_tiles = cut(all, 16, p.pre_tile_rows);
+    // Row tiles of 256 where there is work for all: fewer than two of their tiles for an SM are better cut finer (us, 256 / 128 rows: 57 rows of 48
+    // heads over 464 keys 33 / 29, 56 of 32 over 960 41 / 32, 32 x 4 over 2048 38 / 36; but 32 x 5 of 64 heads over 4096 73 / 90).
+    if (p.pre_tile_rows == 256 && (all + 255) / 256 * p.Hkv * ((p.shared + 127) / 128) <= 2 * sms) p.pre_tile_rows = 128;
     p.pre_row_tiles = (int)((all + p.pre_tile_rows - 1) / p.pre_tile_rows);
     const int keys = tile_keys(p.pre_tile_rows);
     p.pre_tiles = (p.shared + keys - 1) / keys;
+    // Small ones on three fifths of the GPU, so that the launch over the rows' own pages has the rest, but no more than 384 keys a block for that (8 rows
+    // of 32 heads over 4096 keys: 19 us with 86 blocks, 24 with 128; 43 of 64 heads over 368: 25 with 384 keys a block, 22 with 128).
     const long total = (long)p.pre_row_tiles * p.Hkv * p.pre_tiles, most = plan.pre_tiles ? sms : 2 * sms;
-    p.pre_per = (int)std::max((total + most - 1) / most, 384l / keys);
+    p.pre_per = (int)std::max((total + most - 1) / most, std::min(384l / keys, (5 * total + 3 * most - 1) / (3 * most)));
     plan.pre_grid = (int)((total + p.pre_per - 1) / p.pre_per);
     plan.pre_slots = ((long)p.pre_row_tiles * p.Hkv + plan.pre_grid) * p.pre_tile_rows;
   }
