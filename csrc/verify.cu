@@ -5,6 +5,7 @@
 // sums in 32 bits would make a per cent.
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -15,7 +16,6 @@ namespace nxd {
 namespace {
 
 constexpr int kThreads = 256, kWarps = kThreads / 32;
-constexpr int kAhead = 4;                                  // steps of a warp whose numbers are asked for at once
 constexpr int kParts = 32 / kWarps;                        // sums that a warp keeps: one for each lane of a block's search
 
 // N numbers of p and of q (0 where there is none, or behind the row's end)
@@ -62,7 +62,7 @@ NXD_DEVICE double remote_double(const double* at, int rank) {
 template <typename T>
 __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const long* tokens, const T* draft, const T* target, const float* accept, const float* sample,
                                                           long* out, long* accepted, int K, int V, long d_sb, long d_sk, long t_sb, long t_sk) {
-  constexpr int N = Pack16<T>::N, STEP = 32 * N;
+  constexpr int N = Pack16<T>::N, STEP = 32 * N, AHEAD = 16 / N;      // a warp's steps of 32 x 16 bytes, of which so many are asked for at once
   __shared__ double sums[32];
   __shared__ double block_sum;
   __shared__ int refused, bonus;
@@ -102,15 +102,21 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const long* tokens,
     for (int i = 0; i < kParts; ++i) {
       const int part = warp * kParts + i, s1 = (int)first_step(part + 1);
       double sum = 0;
-      for (int s = (int)first_step(part); s < s1; s += kAhead) {
-        Pair<T, N> x[kAhead];
+      auto walk = [&](int s, auto whole) {                 // AHEAD steps
+        constexpr bool all_there = decltype(whole)::value;
+        Pair<T, N> x[AHEAD];
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a) x[a].load(p, q, s + a < s1 ? (s + a) * STEP + lane * N : V, V, packets);
+        for (int a = 0; a < AHEAD; ++a) x[a].load(p, q, s + a < s1 ? (s + a) * STEP + lane * N : V, V, packets);
 #pragma unroll
-        for (int a = 0; a < kAhead; ++a)
+        for (int a = 0; a < AHEAD; ++a) {
+          if (!all_there && s + a >= s1) break;            // conversions to 64 bits are slow: none for what is not there
 #pragma unroll
           for (int j = 0; j < N; ++j) sum += x[a].weight(j);
-      }
+        }
+      };
+      int s = (int)first_step(part);
+      for (; s + AHEAD <= s1; s += AHEAD) walk(s, std::true_type{});
+      if (s < s1) walk(s, std::false_type{});
       sum = warp_sum64(sum);
       if (lane == 0) sums[part] = sum;
     }
@@ -150,12 +156,13 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const long* tokens,
       const int at = find(sums[lane], base, start);
       const int f0 = (int)first_step(at), f1 = (int)first_step(at + 1);
       long chosen = -1, last = -1;
-      for (int s = f0; s < f1 && chosen < 0; s += kAhead) {
-        Pair<T, N> x[kAhead];
+      for (int s = f0; s < f1 && chosen < 0; s += AHEAD) {
+        Pair<T, N> x[AHEAD];
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) x[i].load(p, q, s + i < f1 ? (s + i) * STEP + lane * N : V, V, packets);
+        for (int i = 0; i < AHEAD; ++i) x[i].load(p, q, s + i < f1 ? (s + i) * STEP + lane * N : V, V, packets);
 #pragma unroll
-        for (int i = 0; i < kAhead; ++i) {
+        for (int i = 0; i < AHEAD; ++i) {
+          if (s + i >= f1) break;
           double part = 0;
 #pragma unroll
           for (int j = 0; j < N; ++j) part += x[i].weight(j);
