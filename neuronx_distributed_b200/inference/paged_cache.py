@@ -44,7 +44,7 @@ class PagedKVCacheManager:
 
     def reserve(self, row: int, tokens: int) -> None:
         """Room for a sequence of ``tokens`` tokens in all, the shared ones among them.  Tokens without room are not kept."""
-        if tokens > self.columns * self.page_size:
+        if tokens > self.max_seq_len:                             # the last page may hold more, the rotation tables end there
             raise ValueError(f"a sequence of {tokens} tokens is longer than max_seq_len {self.max_seq_len}")
         held = len(self._shared) + len(self._rows[row])
         pages = self._take(max(0, (tokens + self.page_size - 1) // self.page_size - held))
@@ -56,7 +56,7 @@ class PagedKVCacheManager:
         """:meth:`reserve` for the first ``rows`` rows: all of them, or, where the pool has not as much, none."""
         want = max(0, (tokens + self.page_size - 1) // self.page_size - len(self._shared))
         need = sum(max(0, want - len(self._rows[r])) for r in range(rows))
-        if tokens <= self.columns * self.page_size and need > len(self._free):
+        if tokens <= self.max_seq_len and need > len(self._free):
             raise RuntimeError(f"the key/value pool has {len(self._free)} pages left, {need} are needed")
         for r in range(rows):
             self.reserve(r, tokens)
@@ -73,7 +73,7 @@ class PagedKVCacheManager:
         rows start anew."""
         if tokens % self.page_size:
             raise ValueError(f"a shared prefix fills whole pages of {self.page_size} tokens, got {tokens}")
-        if tokens > self.columns * self.page_size:
+        if tokens > self.max_seq_len:
             raise ValueError(f"a prefix of {tokens} tokens is longer than max_seq_len {self.max_seq_len}")
         n = tokens // self.page_size
         if n > self.num_pages:

@@ -21,7 +21,8 @@ def _make_room(target, draft, rows: int, prompt: int, new: int, window: int) -> 
         raise ValueError(f"the target's shared prefix has {before[0]} tokens, the draft's {before[1]}")
     for model in (target, draft):
         if getattr(model, "paged", False):
-            model.kv.reserve_rows(rows, min(before[0] + prompt + new + window, model.kv.columns * model.kv.page_size))
+            need = before[0] + prompt + new
+            model.kv.reserve_rows(rows, max(need, min(need + window, model.kv.max_seq_len)))
     return before[0]
 
 

@@ -1,0 +1,66 @@
+"""Rows of a paged cache as a model's callers use them: what has no page, or lies behind ``max_seq_len``, is refused and never left out quietly."""
+import pytest
+import torch
+
+from dist_utils import run_distributed
+
+
+def _model(pages=None, batch=2, length=128, logits=False, **kw):
+    from neuronx_distributed_b200.models.llama import LlamaConfig
+    from neuronx_distributed_b200.models.llama_inference import LlamaForInference
+
+    torch.manual_seed(1)
+    cfg = LlamaConfig(vocab_size=96, hidden_size=32, intermediate_size=64, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2,
+                      dtype=torch.float32, max_position_embeddings=128)
+    return LlamaForInference(cfg, batch_size=batch, max_seq_len=length, page_size=pages, on_device_sampling=not logits, **kw).eval()
+
+
+def _start(world=1):
+    from neuronx_distributed_b200.parallel_layers import parallel_state as ps
+
+    ps.initialize_model_parallel(tensor_model_parallel_size=world)
+
+
+def _ids(seed, *shape):
+    return torch.randint(0, 96, shape, generator=torch.Generator().manual_seed(seed))
+
+
+def _longest_sequence(rank, world):
+    from neuronx_distributed_b200.utils.speculative import speculative_generate
+
+    _start()
+    prompts = _ids(3, 2, 40)
+    rows, pages = _model(length=50), _model(48, length=50)       # two pages of 48 would hold 96 tokens, the rotation tables end at 50
+    assert torch.equal(rows.generate(prompts, 11), pages.generate(prompts, 11))          # the last token of the eleven has no place of its own
+    for call in (lambda: pages.generate(prompts, 12), lambda: pages.context_encoding(_ids(4, 2, 60)), lambda: pages.share_prefix(_ids(5, 96))):
+        with pytest.raises(ValueError, match="max_seq_len 50"):
+            call()
+    for tokens in (51, 96):
+        with pytest.raises(ValueError):
+            pages.kv.reserve(0, tokens)
+        with pytest.raises(ValueError):
+            pages.kv.reserve_rows(2, tokens)
+    one = _model(48, batch=1, length=50)
+    with pytest.raises(ValueError):
+        speculative_generate(one, _model(48, batch=1, length=50), prompts[:1], 24, 4)
+    want = _model(batch=1, length=50).generate(prompts[:1], 10)
+    assert torch.equal(speculative_generate(one, _model(48, batch=1, length=50), prompts[:1], 10, 4)[0], want)
+
+
+@pytest.mark.parametrize("part", [_longest_sequence])
+def test_rows(part):
+    run_distributed(part, 1, timeout=240)
+
+
+def test_manager_ends_at_max_seq_len():
+    from neuronx_distributed_b200.inference.paged_cache import PagedKVCacheManager
+
+    kv = PagedKVCacheManager(1, 2, 100, 1, 8, page_size=32, dtype=torch.float32)
+    kv.reserve(0, 100)
+    assert kv.free_pages == 4
+    for call in (lambda: kv.reserve(1, 101), lambda: kv.reserve_rows(2, 128), lambda: kv.take_shared(128)):
+        with pytest.raises(ValueError, match="max_seq_len 100"):
+            call()
+    assert kv.free_pages == 4 and kv.shared_pages is None and int((kv.page_table[0] >= 0).sum()) == 4
+    kv.take_shared(96)
+    assert kv.shared_tokens == 96
