@@ -4,9 +4,12 @@ and what they begin alike is there once.  The pages themselves are written and r
 whose they are.  Tables live on the device at fixed addresses (CUDA graphs read them as they are at the replay); pages are handed out on the host."""
 from __future__ import annotations
 
-from typing import List, Optional
+from contextlib import contextmanager
+from typing import Iterator, List, Optional
 
 import torch
+
+from ..utils.plan_registry import recording
 
 
 class PagedKVCacheManager:
@@ -28,6 +31,7 @@ class PagedKVCacheManager:
         self._shared: List[int] = []
         self._rows: List[List[int]] = [[] for _ in range(batch_size)]       # pages of a row behind the shared ones
         self._free: List[int] = list(range(self.num_pages))[::-1]
+        self._ahead = False                                   # inside reserved_ahead
 
     @property
     def shared_tokens(self) -> int:
@@ -43,7 +47,7 @@ class PagedKVCacheManager:
         return [self._free.pop() for _ in range(n)]
 
     def reserve(self, row: int, tokens: int) -> None:
-        """Room for a sequence of ``tokens`` tokens in all, the shared ones among them.  Tokens without room are not kept."""
+        """Room for a sequence of ``tokens`` tokens in all, the shared ones among them."""
         if tokens > self.max_seq_len:                             # the last page may hold more, the rotation tables end there
             raise ValueError(f"a sequence of {tokens} tokens is longer than max_seq_len {self.max_seq_len}")
         held = len(self._shared) + len(self._rows[row])
@@ -60,6 +64,25 @@ class PagedKVCacheManager:
             raise RuntimeError(f"the key/value pool has {len(self._free)} pages left, {need} are needed")
         for r in range(rows):
             self.reserve(r, tokens)
+
+    def cover(self, positions: torch.Tensor, tokens: int) -> None:
+        """Room for ``tokens`` new tokens of every row from ``positions [B]`` on (negative: an idle row).  The positions are read on the host, which
+        waits for them; inside :meth:`reserved_ahead`, and while a program is captured or recorded, nothing is looked at."""
+        if self._ahead or recording() or (positions.is_cuda and torch.cuda.is_current_stream_capturing()):
+            return
+        for row, first in enumerate(positions.tolist()):
+            if first >= 0:
+                self.reserve(row, first + tokens)
+
+    @contextmanager
+    def reserved_ahead(self, rows: int, tokens: int) -> Iterator[None]:
+        """:meth:`reserve_rows`, and the caller's word that no sequence gets longer than that inside: steps go on without waiting for positions."""
+        self.reserve_rows(rows, tokens)
+        before, self._ahead = self._ahead, True
+        try:
+            yield
+        finally:
+            self._ahead = before
 
     def release(self, row: int) -> None:
         """The row's own pages go back to the pool; the shared ones stay."""

@@ -5,6 +5,7 @@ No sequence parallelism at inference: Row-parallel outputs are all-reduced."""
 from __future__ import annotations
 
 import math
+from contextlib import nullcontext
 from typing import Optional
 
 import torch
@@ -257,8 +258,10 @@ class LlamaForInference(nn.Module):
 
     @torch.no_grad()
     def token_generation(self, input_ids: torch.Tensor, positions: torch.Tensor, kv_len: Optional[int] = None) -> torch.Tensor:
-        """``input_ids`` [B, 1], ``positions`` [B] → next token ids [B].  Positions count the shared prefix of a paged cache; its rows need
-        pages for them (``kv.reserve``), and one at -1 is idle."""
+        """``input_ids`` [B, 1], ``positions`` [B] → next token ids [B].  Positions count the shared prefix of a paged cache; its rows get
+        pages for them (a captured program takes none: ``kv.reserve`` them before), and one at -1 is idle."""
+        if self.paged:
+            self.kv.cover(positions, 1)
         h = self._body(input_ids, positions, False, kv_len)
         logits = self.lm.lm_head(h)[0].float()
         return self.sampler.sample(logits) if self.on_device_sampling else logits
@@ -272,6 +275,8 @@ class LlamaForInference(nn.Module):
         With ``tree_mask [W, W]`` (True = node row sees node column) and ``tree_depth [W]`` the window is a Medusa candidate
         tree instead of a chain.  ``return_hidden`` also returns the final hidden states ``[B, W, H]`` (Medusa heads input)."""
         tree = None if tree_mask is None else (tree_mask.bool(), tree_depth.long())
+        if self.paged and tree is None:
+            self.kv.cover(positions, input_ids.shape[1])
         h = self._body(input_ids, positions, False, kv_len, tree)                # [W, B, H]
         logits = self.lm.lm_head(h).float()                                       # [W, B, V/tp]
         W, B = logits.shape[:2]
@@ -282,16 +287,17 @@ class LlamaForInference(nn.Module):
     def generate(self, prompt_ids: torch.Tensor, max_new_tokens: int, prompt_lens: Optional[torch.Tensor] = None) -> torch.Tensor:
         B, S = prompt_ids.shape
         lens = prompt_lens if prompt_lens is not None else torch.full((B,), S, device=prompt_ids.device, dtype=torch.long)
-        pos = lens.clone()
+        pos, ahead = lens.clone(), nullcontext()
         if self.paged:
-            self.kv.reserve_rows(B, self.kv.shared_tokens + S + max(0, max_new_tokens - 1))
+            ahead = self.kv.reserved_ahead(B, self.kv.shared_tokens + S + max(0, max_new_tokens - 1))
             pos = pos + self.kv.shared_tokens
-        tok = self.context_encoding(prompt_ids, lens - 1)
-        out = [tok]
-        for _ in range(max_new_tokens - 1):
-            tok = self.token_generation(tok.view(B, 1), pos)
-            out.append(tok)
-            pos = pos + 1
+        with ahead:
+            tok = self.context_encoding(prompt_ids, lens - 1)
+            out = [tok]
+            for _ in range(max_new_tokens - 1):
+                tok = self.token_generation(tok.view(B, 1), pos)
+                out.append(tok)
+                pos = pos + 1
         return torch.stack(out, dim=1)
 
 

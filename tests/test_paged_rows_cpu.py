@@ -47,7 +47,50 @@ def _longest_sequence(rank, world):
     assert torch.equal(speculative_generate(one, _model(48, batch=1, length=50), prompts[:1], 10, 4)[0], want)
 
 
-@pytest.mark.parametrize("part", [_longest_sequence])
+def _steps_over_page_borders(rank, world):
+    """Prompt, then single tokens and windows, over several page borders, with nobody reserving: as contiguous rows."""
+    _start()
+    ids, lens = _ids(6, 2, 14), torch.tensor([14, 5])
+    rows, pages = _model(logits=True), _model(16, logits=True)
+    steps = []
+    for m in (rows, pages):
+        out, pos = [m.context_encoding(ids, lens - 1)], lens.clone()
+        for i in range(40):                                     # every fourth step a window of five, of which two stay
+            w = 5 if i % 4 == 3 else 1
+            step = m.speculation_forward if w > 1 else m.token_generation
+            out.append(step(_ids(50 + i, 2, w), pos).reshape(2, w, -1))
+            pos = pos + (2 if w > 1 else 1)
+        steps.append(out)
+    for a, b in zip(*steps):
+        torch.testing.assert_close(b, a, rtol=1e-5, atol=1e-5)
+    assert pages.kv.free_pages == 16 - 5 - 4                   # rows end at 14 + 50 (windows reach 3 further: 67) and 5 + 50 (58)
+    # a row that stands at -1 is idle and takes no pages, whatever its number of tokens before
+    pages.kv.release(1)
+    free = pages.kv.free_pages
+    a = rows.token_generation(ids[:, :1], torch.tensor([64, 0]))[0]
+    b = pages.token_generation(ids[:, :1], torch.tensor([64, -1]))[0]
+    torch.testing.assert_close(b, a, rtol=1e-5, atol=1e-5)
+    assert pages.kv.free_pages == free
+    # steps behind the longest sequence are refused, as contiguous rows refuse them; so are steps for which the pool has no page
+    for m in (rows, pages):
+        with pytest.raises((ValueError, IndexError)):
+            m.token_generation(ids[:, :1], torch.tensor([128, 3]))
+    with pytest.raises(ValueError):
+        pages.speculation_forward(_ids(7, 2, 5), torch.tensor([124, 3]))
+    small = _model(16, num_pages=3)
+    small.context_encoding(ids, lens - 1)
+    small.token_generation(ids[:, :1], torch.tensor([14, 5]))
+    small.token_generation(ids[:, :1], torch.tensor([15, 6]))
+    small.token_generation(ids[:, :1], torch.tensor([16, 7]))  # the third page
+    with pytest.raises(RuntimeError, match="pool"):
+        small.token_generation(ids[:, :1], torch.tensor([17, 16]))
+    # a row that starts over reserves anew
+    small.kv.release(0)
+    small.token_generation(ids[:, :1], torch.tensor([-1, 16]))
+    assert small.kv.free_pages == 1 and int((small.kv.page_table[0] >= 0).sum()) == 0
+
+
+@pytest.mark.parametrize("part", [_longest_sequence, _steps_over_page_borders])
 def test_rows(part):
     run_distributed(part, 1, timeout=240)
 
