@@ -5,10 +5,11 @@
 ``context_encoding`` / ``token_generation`` programs (bucketed CUDA graphs when wrapped by ``ModelBuilder``).
 
 Differences from running HF's own loop: the KV cache is the model's persistent on-device cache (no ``past_key_values``
-objects), prompts are re-packed right-padded for the prefill program, sampling runs on the vocab-parallel logits
-(distributed top-k) and the sampled ids are broadcast inside the TP group so every rank continues with the same token."""
+objects; in a paged one the rows start anew behind the shared prefix, which stays), prompts are re-packed right-padded for the
+prefill program, sampling runs on the vocab-parallel logits (distributed top-k) and the sampled ids are broadcast inside the TP group so every rank continues with the same token."""
 from __future__ import annotations
 
+from contextlib import nullcontext
 from typing import Callable, List, Optional, Sequence, Union
 
 import torch
@@ -83,7 +84,12 @@ class HuggingFaceGenerationAdapter:
         eos_ids = [] if eos is None else ([eos] if isinstance(eos, int) else list(eos))
         pad = pad_token_id if pad_token_id is not None else (self.pad_token_id if self.pad_token_id is not None else (eos_ids[0] if eos_ids else 0))
         packed, lens = self._pack_right(input_ids, attention_mask, pad)
-        room = m.max_seq_len - int(lens.max())
+        paged = getattr(m, "paged", False)
+        shared = m.kv.shared_tokens if paged else 0                                   # tokens that every sequence begins with
+        longest = shared + int(lens.max())
+        if paged:
+            packed = packed[:, :longest - shared]                                     # no pages for padding of all rows
+        room = m.max_seq_len - longest
         n_new = max_new_tokens if max_new_tokens is not None else ((max_length - S) if max_length is not None else room)
         n_new = max(0, min(n_new, room))
         if n_new == 0:
@@ -94,25 +100,31 @@ class HuggingFaceGenerationAdapter:
                           vocab_parallel=getattr(saved[0], "vocab_parallel", True)) if custom else saved[0]
         if custom:                                 # get logits back and sample here (per-call parameters, synchronised over TP)
             m.on_device_sampling = False
+        ahead = nullcontext()
         try:
-            if hasattr(m, "kv"):
+            if paged:                              # rows start anew behind the prefix, with pages for all that comes
+                for row in range(B):
+                    m.kv.release(row)
+                ahead = m.kv.reserved_ahead(B, longest + n_new - 1)
+            elif hasattr(m, "kv"):
                 m.kv.reset()
-            history = input_ids
-            tok = self._pick(self._ctx(packed, lens - 1), sampler, logits_processor, history, generator)
-            done = torch.zeros(B, dtype=torch.bool, device=input_ids.device)
-            eos_t = torch.tensor(eos_ids, device=input_ids.device) if eos_ids else None
-            out, pos = [], lens.clone()
-            for i in range(n_new):
-                tok = torch.where(done, torch.full_like(tok, pad), tok)
-                out.append(tok)
-                history = torch.cat([history, tok[:, None]], 1)
-                if eos_t is not None:
-                    done = done | torch.isin(tok, eos_t)
-                if i == n_new - 1 or (eos_t is not None and bool(done.all())) or \
-                        (stopping_criteria and any(bool(torch.as_tensor(c(history, None)).all()) for c in stopping_criteria)):
-                    break
-                tok = self._pick(self._tkg(tok.view(B, 1), pos), sampler, logits_processor, history, generator)
-                pos = pos + 1
+            with ahead:
+                history = input_ids
+                tok = self._pick(self._ctx(packed, lens - 1), sampler, logits_processor, history, generator)
+                done = torch.zeros(B, dtype=torch.bool, device=input_ids.device)
+                eos_t = torch.tensor(eos_ids, device=input_ids.device) if eos_ids else None
+                out, pos = [], lens + shared
+                for i in range(n_new):
+                    tok = torch.where(done, torch.full_like(tok, pad), tok)
+                    out.append(tok)
+                    history = torch.cat([history, tok[:, None]], 1)
+                    if eos_t is not None:
+                        done = done | torch.isin(tok, eos_t)
+                    if i == n_new - 1 or (eos_t is not None and bool(done.all())) or \
+                            (stopping_criteria and any(bool(torch.as_tensor(c(history, None)).all()) for c in stopping_criteria)):
+                        break
+                    tok = self._pick(self._tkg(tok.view(B, 1), pos), sampler, logits_processor, history, generator)
+                    pos = pos + 1
             return torch.cat([input_ids, torch.stack(out, 1)], 1)
         finally:
             m.sampler, m.on_device_sampling = saved

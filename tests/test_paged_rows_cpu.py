@@ -90,7 +90,51 @@ def _steps_over_page_borders(rank, world):
     assert small.kv.free_pages == 1 and int((small.kv.page_table[0] >= 0).sum()) == 0
 
 
-@pytest.mark.parametrize("part", [_longest_sequence, _steps_over_page_borders])
+def _adapter(rank, world):
+    """The transformers-like generate over pages: as over contiguous rows, behind a shared prefix too, which it keeps."""
+    from neuronx_distributed_b200.inference.hf_adapter import HuggingFaceGenerationAdapter
+
+    _start()
+    ids, mask = _ids(8, 2, 14), torch.ones(2, 14, dtype=torch.long)
+    mask[1, :6] = 0                                             # left-padded
+    rows, pages = HuggingFaceGenerationAdapter(_model()), HuggingFaceGenerationAdapter(_model(16))
+    want = rows.generate(ids, mask, max_new_tokens=40)
+    for _ in range(2):
+        assert torch.equal(pages.generate(ids, mask, max_new_tokens=40), want)
+    drawn = [a.generate(ids, mask, max_new_tokens=20, do_sample=True, top_k=5, generator=torch.Generator().manual_seed(2)) for a in (rows, pages)]
+    assert torch.equal(*drawn)
+    assert torch.equal(pages.generate(ids, mask), rows.generate(ids, mask))              # as far as max_seq_len goes
+    # steps that wait for nothing: the same when the model's steps may not reserve
+    m = _model(16)
+    m.kv.cover = lambda positions, tokens: (_ for _ in ()).throw(AssertionError()) if not m.kv._ahead else None
+    assert torch.equal(HuggingFaceGenerationAdapter(m).generate(ids, mask, max_new_tokens=40), want)
+    # behind a prefix
+    prefix = _ids(9, 32)
+    whole, lens = torch.zeros(2, 46, dtype=torch.long), [14, 8]
+    long_mask = torch.zeros(2, 46, dtype=torch.long)
+    for b, n in enumerate(lens):
+        whole[b, 46 - 32 - n:] = torch.cat([prefix, ids[b, 14 - n:]])
+        long_mask[b, 46 - 32 - n:] = 1
+    want = rows.generate(whole, long_mask, max_new_tokens=30)[:, 46:]
+    shared = _model(16)
+    shared.share_prefix(prefix)
+    adapter = HuggingFaceGenerationAdapter(shared)
+    for _ in range(2):
+        assert torch.equal(adapter.generate(ids, mask, max_new_tokens=30)[:, 14:], want)
+        assert shared.kv.shared_tokens == 32
+    full = adapter.generate(ids, mask)
+    assert full.shape[1] == 14 + 128 - 32 - 14 and torch.equal(full[:, 14:], rows.generate(whole, long_mask)[:, 46:])
+    # a pool with just enough pages for one call at a time
+    small = _model(16, num_pages=2 + 2 * 3)
+    small.share_prefix(prefix)
+    for _ in range(2):
+        assert torch.equal(HuggingFaceGenerationAdapter(small).generate(ids, mask, max_new_tokens=30)[:, 14:], want)
+    with pytest.raises(RuntimeError, match="pool"):
+        HuggingFaceGenerationAdapter(small).generate(ids, mask, max_new_tokens=40)
+    assert small.kv.shared_tokens == 32 and not small.kv._ahead
+
+
+@pytest.mark.parametrize("part", [_longest_sequence, _steps_over_page_borders, _adapter])
 def test_rows(part):
     run_distributed(part, 1, timeout=240)
 
