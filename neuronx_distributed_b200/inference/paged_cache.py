@@ -1,7 +1,8 @@
 """Key/value cache in pages: one pool per layer ``[pages, page_size, H_kv_local, D]``, a table of pages per batch row, and a prefix that all rows
 share.  Beside ``kv_cache.py``, whose rows are contiguous and as long as the longest sequence may get, rows here hold as many pages as they need,
 and what they begin alike is there once.  The pages themselves are written and read by ``ops.paged`` (``csrc/paged.cu``); this class says
-whose they are.  Tables live on the device at fixed addresses (CUDA graphs read them as they are at the replay); pages are handed out on the host."""
+whose they are.  Tables live on the device at fixed addresses (captured and recorded programs read them as they are when they run); pages are handed
+out on the host, so a program takes none: its rows have to be reserved before it runs, and the length of the shared prefix is part of it."""
 from __future__ import annotations
 
 from contextlib import contextmanager
@@ -27,11 +28,13 @@ class PagedKVCacheManager:
         self.k: List[torch.Tensor] = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(num_layers)]
         self.v: List[torch.Tensor] = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(num_layers)]
         self.page_table = torch.full((batch_size, self.columns), -1, dtype=torch.int32, device=device)
-        self.shared_pages: Optional[torch.Tensor] = None      # [n] int32: what every row begins with
+        self._shared_table = torch.full((self.columns,), -1, dtype=torch.int32, device=device)
+        self.shared_pages: Optional[torch.Tensor] = None      # [n] int32, the beginning of that table: what every row begins with
         self._shared: List[int] = []
         self._rows: List[List[int]] = [[] for _ in range(batch_size)]       # pages of a row behind the shared ones
         self._free: List[int] = list(range(self.num_pages))[::-1]
         self._ahead = False                                   # inside reserved_ahead
+        self._programs: Optional[int] = None                  # shared pages that captured and recorded programs count on
 
     @property
     def shared_tokens(self) -> int:
@@ -41,7 +44,22 @@ class PagedKVCacheManager:
     def free_pages(self) -> int:
         return len(self._free)
 
+    def in_program(self) -> bool:
+        """A program is being captured into a CUDA graph, or recorded into a launch plan."""
+        return recording() or (self.page_table.is_cuda and torch.cuda.is_current_stream_capturing())
+
+    def note_program(self) -> None:
+        """What is being captured or recorded counts on the length of the shared prefix from now on."""
+        if self.in_program():
+            self._programs = len(self._shared)
+
+    def forget_programs(self) -> None:
+        """The programs captured or recorded so far are not run any more."""
+        self._programs = None
+
     def _take(self, n: int) -> List[int]:
+        if n and self.in_program():
+            raise RuntimeError("pages are handed out on the host: reserve them before the call is captured or recorded")
         if n > len(self._free):
             raise RuntimeError(f"the key/value pool has {len(self._free)} pages left, {n} are needed")
         return [self._free.pop() for _ in range(n)]
@@ -68,7 +86,7 @@ class PagedKVCacheManager:
     def cover(self, positions: torch.Tensor, tokens: int) -> None:
         """Room for ``tokens`` new tokens of every row from ``positions [B]`` on (negative: an idle row).  The positions are read on the host, which
         waits for them; inside :meth:`reserved_ahead`, and while a program is captured or recorded, nothing is looked at."""
-        if self._ahead or recording() or (positions.is_cuda and torch.cuda.is_current_stream_capturing()):
+        if self._ahead or self.in_program():
             return
         for row, first in enumerate(positions.tolist()):
             if first >= 0:
@@ -93,7 +111,7 @@ class PagedKVCacheManager:
 
     def take_shared(self, tokens: int) -> torch.Tensor:
         """Pages for a prefix of ``tokens`` tokens that every row begins with, in place of the one before → ``[n]`` int32 (who asked fills them).  All
-        rows start anew."""
+        rows start anew.  Captured and recorded programs go on with another prefix of the same length; while there are any, another length is refused."""
         if tokens % self.page_size:
             raise ValueError(f"a shared prefix fills whole pages of {self.page_size} tokens, got {tokens}")
         if tokens > self.max_seq_len:
@@ -101,16 +119,23 @@ class PagedKVCacheManager:
         n = tokens // self.page_size
         if n > self.num_pages:
             raise RuntimeError(f"the key/value pool has {self.num_pages} pages, {n} are needed")
+        if self.in_program():
+            raise RuntimeError("a shared prefix cannot be taken by a call that is captured or recorded")
+        if self._programs not in (None, n):
+            raise RuntimeError(f"programs were captured or recorded behind a prefix of {self._programs * self.page_size} tokens and would go on with it, "
+                               f"{tokens} are asked for: kv.forget_programs() when none of them is run any more")
         for row in range(self.batch_size):
             self.release(row)
         self._free += self._shared[::-1]
         self._shared = self._take(n)
-        pages = torch.tensor(self._shared, dtype=torch.int32, device=self.page_table.device)
+        self._shared_table[:] = -1
+        pages = self._shared_table[:n]
+        pages.copy_(torch.tensor(self._shared, dtype=torch.int32, device=self.page_table.device))
         self.page_table[:] = -1
         self.page_table[:, :n] = pages
         self.shared_pages = pages if n else None
         return pages
 
     def reset(self) -> None:
-        """All pages go back to the pool, the shared ones too."""
+        """All pages go back to the pool, the shared ones too (:meth:`take_shared` of nothing)."""
         self.take_shared(0)

@@ -182,6 +182,8 @@ class LlamaForInference(nn.Module):
 
     def _body(self, input_ids: torch.Tensor, positions: Optional[torch.Tensor], prefill: bool, kv_len: Optional[int], tree=None):
         core = self._core
+        if self.paged:
+            self.kv.note_program()
         x = core.embed_tokens(input_ids).transpose(0, 1).contiguous()               # [S, B, H]
         if (prefill and x.shape[0] * x.shape[1] > 8 and type(self)._attn_block is LlamaForInference._attn_block
                 and "_attn_block" not in self.__dict__ and _plain_norms(core)):

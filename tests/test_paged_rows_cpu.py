@@ -134,7 +134,58 @@ def _adapter(rank, world):
     assert small.kv.shared_tokens == 32 and not small.kv._ahead
 
 
-@pytest.mark.parametrize("part", [_longest_sequence, _steps_over_page_borders, _adapter])
+def _record(call, *inputs):
+    from neuronx_distributed_b200.inference import launch_plan
+
+    return launch_plan.record(call, inputs)
+
+
+def _programs_and_prefixes(rank, world):
+    """A recorded program reads the pages of the prefix there is when it runs; a prefix of another length, which it cannot know, is refused."""
+    _start()
+    ids, lens = _ids(10, 2, 10), torch.tensor([10, 4])
+    x, pos = ids[:, :1].contiguous(), lens + 48
+    m = _model(16, logits=True, num_pages=12)
+    m.share_prefix(_ids(11, 48))
+    m.context_encoding(ids, lens - 1)
+    m.kv.reserve_rows(2, 64)
+    at = m.kv.shared_pages.data_ptr()
+    step = _record(m.token_generation, x, pos)
+    torch.testing.assert_close(step(x, pos), m.token_generation(x, pos), rtol=0, atol=0)
+    # another prefix, in other pages
+    m.kv.release(0)
+    m.share_prefix(_ids(12, 48))
+    m.context_encoding(ids, lens - 1)
+    m.kv.reserve_rows(2, 64)
+    assert m.kv.shared_pages.data_ptr() == at
+    fresh = _model(16, logits=True)
+    fresh.share_prefix(_ids(12, 48))
+    fresh.context_encoding(ids, lens - 1)
+    want = fresh.token_generation(x, pos)
+    torch.testing.assert_close(step(x, pos), want, rtol=0, atol=0)
+    torch.testing.assert_close(m.token_generation(x, pos), want, rtol=0, atol=0)
+    held, free = m.kv.shared_pages.tolist(), m.kv.free_pages
+    for n in (0, 32, 64):
+        with pytest.raises(RuntimeError, match="captured"):
+            m.share_prefix(_ids(13, n))
+    with pytest.raises(RuntimeError, match="captured"):
+        m.kv.reset()
+    assert m.kv.shared_pages.tolist() == held and m.kv.free_pages == free
+    torch.testing.assert_close(step(x, pos), want, rtol=0, atol=0)
+    m.kv.forget_programs()                                      # the step above is not run any more
+    m.share_prefix(_ids(13, 32))
+    assert m.kv.shared_tokens == 32
+    m.kv.reset()
+    assert m.kv.shared_pages is None and m.kv.free_pages == 12
+    # pages are handed out on the host: a program cannot take any, nor keep a prefix
+    with pytest.raises(RuntimeError, match="captured"):
+        _record(m.context_encoding, ids, lens - 1)
+    with pytest.raises(RuntimeError, match="captured"):
+        _record(m.share_prefix, _ids(13, 32))
+    assert m.kv.free_pages == 12 and not bool((m.kv.page_table >= 0).any())
+
+
+@pytest.mark.parametrize("part", [_longest_sequence, _steps_over_page_borders, _adapter, _programs_and_prefixes])
 def test_rows(part):
     run_distributed(part, 1, timeout=240)
 
