@@ -233,10 +233,11 @@ struct PagedPlan {
 PagedPlan paged_plan(PagedAttn& p);  // fills in p's cuts
 int paged_attention(const PagedAttn& p, const PagedPlan& plan, int D, int dt, cudaStream_t st);        // → launches
 void paged_tiles(const PagedAttn& p, int grid, bool over_shared, int D, int dt, cudaStream_t st);       // paged_attention_sm100.cu
-// strides s: (b, w, h) of q, k, v; cs: (page, row, head) of the caches; q_out: heads and columns contiguous
+// strides s: (b, w, h) of q, k, v; cs: (page, row, head) of the caches; q_out: heads and columns contiguous; lost: becomes 1 where a
+// token that counts was not written, or null
 void paged_append(const void* q, const void* k, const void* v, const long* positions, const long* lens, const float* cos_t, const float* sin_t,
-                  void* q_out, void* kc, void* vc, const int* table, int B, int W, int H, int Hkv, int D, int rows, int cols, int ps, int pages,
-                  long table_sb, const long (*s)[3], long o_sb, long o_sw, const long (*cs)[3], int dt, cudaStream_t st);
+                  void* q_out, void* kc, void* vc, const int* table, int* lost, int B, int W, int H, int Hkv, int D, int rows, int cols, int ps,
+                  int pages, long table_sb, const long (*s)[3], long o_sb, long o_sw, const long (*cs)[3], int dt, cudaStream_t st);
 
 // ---- drafted tokens against the target's probabilities (verify.cu); strides of rows in elements, dt of both sides
 void verify_drafts(const long* tokens, const void* draft, const void* target, const float* accept, const float* sample, long* out, long* accepted,

@@ -24,6 +24,7 @@ struct AppendArgs {
   const float *cos_t, *sin_t;
   void *q_out, *kc, *vc;
   const int* table;
+  int* lost;                                               // becomes 1 where a token that counts has no place; null: nobody asks
   int B, W, H, Hkv, half, rows, cols, ps, pages, parts;    // parts: blocks of a token
   long table_sb, q_sb, q_sw, q_sh, k_sb, k_sw, k_sh, v_sb, v_sw, v_sh, o_sb, o_sw, kc_sp, kc_sr, kc_sh, vc_sp, vc_sr, vc_sh;
 };
@@ -42,6 +43,7 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
   T* const q_out = (T*)p.q_out + b * p.o_sb + w * p.o_sw + (long)h * (2 * p.half) + c;
   Pack16<T> lo, hi;
   if (!live) {
+    if (p.lost && item == 0 && first >= 0 && w < m) *p.lost = 1;       // behind the rotation tables
     if (query) {
 #pragma unroll
       for (int e = 0; e < N; ++e) { lo.set(e, 0.f); hi.set(e, 0.f); }
@@ -59,7 +61,10 @@ __global__ void __launch_bounds__(kAppendThreads) paged_append_kernel(const Appe
   if (!query) {
     const int column = (int)pos / p.ps, row = (int)pos - column * p.ps;            // positions with a place in the tables fit
     const int page = column < p.cols ? p.table[b * p.table_sb + column] : -1;
-    if (page < 0 || page >= p.pages) return;
+    if (page < 0 || page >= p.pages) {
+      if (p.lost) *p.lost = 1;
+      return;
+    }
     dst = key ? (T*)p.kc + page * p.kc_sp + row * p.kc_sr + (h - p.H) * p.kc_sh + c
               : (T*)p.vc + page * p.vc_sp + row * p.vc_sr + (h - p.H - p.Hkv) * p.vc_sh + c;
   }
@@ -630,13 +635,13 @@ int paged_attention(const PagedAttn& p, const PagedPlan& plan, int D, int dt, cu
 }
 
 void paged_append(const void* q, const void* k, const void* v, const long* positions, const long* lens, const float* cos_t, const float* sin_t,
-                  void* q_out, void* kc, void* vc, const int* table, int B, int W, int H, int Hkv, int D, int rows, int cols, int ps, int pages,
-                  long table_sb, const long (*s)[3], long o_sb, long o_sw, const long (*cs)[3], int dt, cudaStream_t st) {
+                  void* q_out, void* kc, void* vc, const int* table, int* lost, int B, int W, int H, int Hkv, int D, int rows, int cols, int ps,
+                  int pages, long table_sb, const long (*s)[3], long o_sb, long o_sw, const long (*cs)[3], int dt, cudaStream_t st) {
   const int half = D / 2;
   const long tokens = (long)B * W, items = (long)(H + 2 * Hkv) * (half / (dt == kF32 ? 4 : 8)), parts = (items + kAppendThreads - 1) / kAppendThreads;
   if (tokens == 0) return;
   if (tokens * parts >= (1l << 31)) nxd_throw("paged_append: too many tokens", __FILE__, __LINE__);
-  const AppendArgs a{q, k, v, positions, lens, cos_t, sin_t, q_out, kc, vc, table, B, W, H, Hkv, half, rows, cols, ps, pages, (int)parts,
+  const AppendArgs a{q, k, v, positions, lens, cos_t, sin_t, q_out, kc, vc, table, lost, B, W, H, Hkv, half, rows, cols, ps, pages, (int)parts,
                      table_sb, s[0][0], s[0][1], s[0][2], s[1][0], s[1][1], s[1][2], s[2][0], s[2][1], s[2][2], o_sb, o_sw,
                      cs[0][0], cs[0][1], cs[0][2], cs[1][0], cs[1][1], cs[1][2]};
   const unsigned grid = (unsigned)(tokens * parts);

@@ -80,7 +80,7 @@ Tensor rows_out(const Tensor& q) {
 
 // None: not for the kernel
 c10::optional<Tensor> paged_append(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& positions_, const Tensor& cos_t, const Tensor& sin_t, Tensor kc,
-                    Tensor vc, const Tensor& table_, const c10::optional<Tensor>& lens_) {
+                    Tensor vc, const Tensor& table_, const c10::optional<Tensor>& lens_, const c10::optional<Tensor>& lost) {
   const Tensor positions = ints(positions_, at::kLong), table = as_table(table_);
   const c10::optional<Tensor> lens = ints(lens_, at::kLong);
   check_cache(q_, kc, vc, table, positions, lens);
@@ -92,6 +92,8 @@ c10::optional<Tensor> paged_append(const Tensor& q_, const Tensor& k_, const Ten
   CHECK_ARG(cos_t.dim() == 2 && cos_t.sizes() == sin_t.sizes() && cos_t.size(1) * 2 == q_.size(3) && cos_t.scalar_type() == at::kFloat &&
             sin_t.scalar_type() == at::kFloat && cos_t.is_contiguous() && sin_t.is_contiguous() && cos_t.device() == q_.device() && sin_t.device() == q_.device(),
             "cos and sin must be contiguous float32 tables [positions, " + std::to_string(q_.size(3) / 2) + "]");
+  CHECK_ARG(!lost.has_value() || (lost->scalar_type() == at::kInt && lost->dim() == 1 && lost->size(0) == 1 && lost->device() == q_.device()),
+            "lost must be an int32 tensor of one number on the queries' device");
   CHECK_ARG(q_.is_cuda(), "the kernel's tensors are on a GPU");
   c10::cuda::CUDAGuard guard(q_.device());
   const Tensor q = as_packets(q_), k = as_packets(k_), v = as_packets(v_), cos_p = as_packets(cos_t), sin_p = as_packets(sin_t);
@@ -100,7 +102,8 @@ c10::optional<Tensor> paged_append(const Tensor& q_, const Tensor& k_, const Ten
   const long s[3][3] = {{q.stride(0), q.stride(1), q.stride(2)}, {k.stride(0), k.stride(1), k.stride(2)}, {v.stride(0), v.stride(1), v.stride(2)}};
   const long cs[2][3] = {{kc.stride(0), kc.stride(1), kc.stride(2)}, {vc.stride(0), vc.stride(1), vc.stride(2)}};
   nxd::paged_append(q.data_ptr(), k.data_ptr(), v.data_ptr(), positions.data_ptr<long>(), lens.has_value() ? lens->data_ptr<long>() : nullptr,
-                    cos_p.data_ptr<float>(), sin_p.data_ptr<float>(), out.data_ptr(), kc.data_ptr(), vc.data_ptr(), table.data_ptr<int>(), (int)q.size(0),
+                    cos_p.data_ptr<float>(), sin_p.data_ptr<float>(), out.data_ptr(), kc.data_ptr(), vc.data_ptr(), table.data_ptr<int>(),
+                    lost.has_value() ? lost->data_ptr<int>() : nullptr, (int)q.size(0),
                     (int)q.size(1), (int)q.size(2), (int)kc.size(2), (int)q.size(3), (int)cos_t.size(0), (int)table.size(1), (int)kc.size(1),
                     (int)kc.size(0), table.stride(0), s, out.stride(0), out.stride(1), cs, dt_code(q), stream());
   count_launches(1);
@@ -185,7 +188,9 @@ std::vector<Tensor> verify_drafts(const Tensor& tokens, const Tensor& draft_, co
 }  // namespace
 
 void bind_paged(pybind11::module_& m) {
-  m.def("paged_append", &paged_append);
+  namespace py = pybind11;
+  m.def("paged_append", &paged_append, py::arg("q"), py::arg("k"), py::arg("v"), py::arg("positions"), py::arg("cos"), py::arg("sin"), py::arg("k_cache"),
+        py::arg("v_cache"), py::arg("page_table"), py::arg("lens"), py::arg("lost") = py::none());
   m.def("paged_append_ok", &paged_append_ok);
   m.def("paged_attention", &paged_attention);
   m.def("paged_attention_ok", &paged_attention_ok);

@@ -125,6 +125,8 @@ class HuggingFaceGenerationAdapter:
                         break
                     tok = self._pick(self._tkg(tok.view(B, 1), pos), sampler, logits_processor, history, generator)
                     pos = pos + 1
+            if paged:
+                m.kv.check()
             return torch.cat([input_ids, torch.stack(out, 1)], 1)
         finally:
             m.sampler, m.on_device_sampling = saved

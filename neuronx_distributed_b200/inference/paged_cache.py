@@ -2,7 +2,8 @@
 share.  Beside ``kv_cache.py``, whose rows are contiguous and as long as the longest sequence may get, rows here hold as many pages as they need,
 and what they begin alike is there once.  The pages themselves are written and read by ``ops.paged`` (``csrc/paged.cu``); this class says
 whose they are.  Tables live on the device at fixed addresses (captured and recorded programs read them as they are when they run); pages are handed
-out on the host, so a program takes none: its rows have to be reserved before it runs, and the length of the shared prefix is part of it."""
+out on the host, so a program takes none: its rows have to be reserved before it runs (:meth:`PagedKVCacheManager.check` says whether they were), and
+the length of the shared prefix is part of it."""
 from __future__ import annotations
 
 from contextlib import contextmanager
@@ -30,6 +31,7 @@ class PagedKVCacheManager:
         self.page_table = torch.full((batch_size, self.columns), -1, dtype=torch.int32, device=device)
         self._shared_table = torch.full((self.columns,), -1, dtype=torch.int32, device=device)
         self.shared_pages: Optional[torch.Tensor] = None      # [n] int32, the beginning of that table: what every row begins with
+        self.lost = torch.zeros(1, dtype=torch.int32, device=device)        # becomes 1 where a token had no page (ops.paged.rope_append)
         self._shared: List[int] = []
         self._rows: List[List[int]] = [[] for _ in range(batch_size)]       # pages of a row behind the shared ones
         self._free: List[int] = list(range(self.num_pages))[::-1]
@@ -56,6 +58,15 @@ class PagedKVCacheManager:
     def forget_programs(self) -> None:
         """The programs captured or recorded so far are not run any more."""
         self._programs = None
+        self.lost.zero_()
+
+    def check(self) -> None:
+        """Raises if a captured or recorded program has run for tokens without a page since the last look: their keys are missing from what came
+        after.  Waits for the device where there are such programs; sequences that end (:meth:`release`, :meth:`take_shared`) are a look, too."""
+        if self._programs is not None and bool(self.lost):
+            self.lost.zero_()
+            raise RuntimeError("a captured or recorded program ran for tokens without a page, whose keys are lost: rows have to be reserved before it runs, "
+                               f"and end at max_seq_len {self.max_seq_len}")
 
     def _take(self, n: int) -> List[int]:
         if n and self.in_program():
@@ -104,6 +115,7 @@ class PagedKVCacheManager:
 
     def release(self, row: int) -> None:
         """The row's own pages go back to the pool; the shared ones stay."""
+        self.check()
         if self._rows[row]:
             self._free += self._rows[row][::-1]
             self._rows[row] = []
@@ -124,6 +136,7 @@ class PagedKVCacheManager:
         if self._programs not in (None, n):
             raise RuntimeError(f"programs were captured or recorded behind a prefix of {self._programs * self.page_size} tokens and would go on with it, "
                                f"{tokens} are asked for: kv.forget_programs() when none of them is run any more")
+        self.check()
         for row in range(self.batch_size):
             self.release(row)
         self._free += self._shared[::-1]

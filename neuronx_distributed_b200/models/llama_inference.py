@@ -90,7 +90,7 @@ class LlamaForInference(nn.Module):
             # one launch: rotation of q and k and the new rows of the pages; prompts, windows and single tokens read them there
             first, lens, table, shared = self._rows if prefill else (positions.long(), None, self.kv.page_table[:B], self.kv.shared_pages)
             kc, vc = self.kv.k[layer_idx], self.kv.v[layer_idx]
-            q = ops.paged.rope_append(q, k, v, first, self.rope_cos, self.rope_sin, kc, vc, table, lens=lens)
+            q = ops.paged.rope_append(q, k, v, first, self.rope_cos, self.rope_sin, kc, vc, table, lens=lens, lost=self.kv.lost)
             o = ops.paged.attention(q, kc, vc, table, first, lens=lens, shared_pages=shared)
         elif self.flash_decoding and not prefill:
             v = v.contiguous()

@@ -67,19 +67,23 @@ def _new_tokens(positions, lens, W: int) -> torch.Tensor:
 
 
 def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.Tensor, cos: torch.Tensor, sin: torch.Tensor,
-                k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, lens: Optional[torch.Tensor] = None) -> torch.Tensor:
+                k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor, lens: Optional[torch.Tensor] = None,
+                lost: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Rotates ``q [B, W, H, D]`` (returned, ``[W, B, H, D]`` in memory) and ``k [B, W, Hkv, D]`` by their tokens' positions, and writes ``k`` and ``v``
     to the pages, in one launch.  ``cos`` / ``sin [positions, D / 2]`` fp32: :func:`ops.rope.rope_tables`.  Tokens that do not count, or that stand
-    behind the tables' end, come back as zeros and are not written; tokens behind the page table's end are not written."""
+    behind the tables' end, come back as zeros and are not written; tokens behind the page table's end are not written.  ``lost [1]`` int32 becomes 1
+    where a token that counts was not written (and stays as it is otherwise)."""
     _no_gradient("rope_append", q, k, v, k_cache, v_cache)
     e = _kernels(q, k_cache, v_cache, "paged_append_ok")
     if e is not None:
-        out = e.paged_append(q, k, v, positions, cos, sin, k_cache, v_cache, page_table, lens)
+        out = e.paged_append(q, k, v, positions, cos, sin, k_cache, v_cache, page_table, lens, lost)
         if out is not None:
             return out
     positions, page_table = _ints(positions, torch.long).clamp(-1, 1 << 40), _table(page_table)
     lens = None if lens is None else _ints(lens, torch.long)
     _check(q, k_cache, v_cache, page_table, positions, lens)
+    if lost is not None and (lost.dtype != torch.int32 or lost.shape != (1,) or lost.device != q.device):
+        raise ValueError("lost must be an int32 tensor of one number on the queries' device")
     B, W, H, D = q.shape
     if k.shape != v.shape or tuple(k.shape) != (B, W, k_cache.shape[2], D):
         raise ValueError(f"new keys and values must be [{B}, {W}, {k_cache.shape[2]}, {D}]")
@@ -90,7 +94,8 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
         raise ValueError(f"cos and sin must be contiguous float32 tables [positions, {D // 2}]")
     w = torch.arange(W, device=q.device)
     p = positions[:, None] + w
-    live = (w < _new_tokens(positions, lens, W)[:, None]) & (p < cos.shape[0])
+    counts = w < _new_tokens(positions, lens, W)[:, None]
+    live = counts & (p < cos.shape[0])
     at = p.clamp(0, max(cos.shape[0] - 1, 0))
     c, s = cos[at][:, :, None], sin[at][:, :, None]
 
@@ -103,6 +108,8 @@ def rope_append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: to
     held = live & (column < page_table.shape[1])
     page = page_table.long().gather(1, column.clamp(0, max(page_table.shape[1] - 1, 0))) if page_table.shape[1] else torch.full_like(p, -1)
     held &= (page >= 0) & (page < k_cache.shape[0])
+    if lost is not None:
+        lost.logical_or_((counts & ~held).any())
     k_cache[page[held], (p % ps)[held]] = rotate(k).to(k_cache.dtype)[held]
     v_cache[page[held], (p % ps)[held]] = v[held]
     return rotate(q).masked_fill(~live[:, :, None, None], 0.0).to(q.dtype).transpose(0, 1).contiguous().transpose(0, 1)

@@ -2,20 +2,21 @@
 import pytest
 import torch
 
+from test_paged_rows_cpu import LOST, append_notes
 from test_paged_serving_gpu import groups, model  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
 
 def capture(call, *inputs):
-    """One warm-up call, then the captured one, as a program that gives its results anew."""
+    """One warm-up call, then the captured one, as a program that gives its results anew and keeps its inputs."""
     call(*inputs)
     torch.cuda.synchronize()
     graph = torch.cuda.CUDAGraph()
     with torch.cuda.graph(graph):
         out = call(*inputs)
 
-    def run():
+    def run(held=inputs):
         graph.replay()
         return out.clone()
 
@@ -47,3 +48,49 @@ def test_another_prefix_of_the_same_length():
     with pytest.raises(RuntimeError, match="captured"):
         m.share_prefix(ids(5, 64))
     assert torch.equal(step(), want) and filler.numel()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("first, lens, noted", LOST)
+def test_append_notes_tokens_without_a_place(first, lens, noted, dtype):
+    append_notes("cuda", dtype, first, lens, noted)
+
+
+def test_captured_prompts_and_pages_that_come_and_go():
+    """A captured prompt and step go on with whatever pages the rows hold; tokens without a page are said at the next look."""
+    m, fresh = model(page_size=16, num_pages=3 * 16), model(page_size=16)
+    prompts, lens = ids(6, 3, 40), torch.tensor([40, 7, 21]).cuda()
+    x, pos = ids(7, 3, 1), lens.clone()
+    with pytest.raises(RuntimeError, match="captured"):          # no pages yet, and none are handed out inside
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            m.context_encoding(prompts, lens - 1)
+    torch.cuda.synchronize()
+    assert m.kv.free_pages == 48
+    prompt = capture(m.context_encoding, prompts, lens - 1)
+    m.kv.reserve_rows(3, 64)
+    step = capture(m.token_generation, x, pos)
+    for seed in (8, 9):
+        m.kv.reset()
+        m.kv.reserve(2, 64)
+        m.kv.reserve(1, 64)                                     # other pages than before
+        m.kv.reserve(0, 64)
+        prompts.copy_(ids(seed, 3, 40))
+        fresh.kv.reset()
+        want = [fresh.context_encoding(prompts, lens - 1), fresh.token_generation(x, pos)]
+        assert torch.equal(prompt(), want[0]) and torch.equal(step(), want[1])
+        m.kv.check()
+    m.kv.release(0)
+    prompt()
+    with pytest.raises(RuntimeError, match="without a page"):
+        m.kv.check()
+    m.kv.reserve(0, 64)
+    prompt()
+    step()
+    m.kv.check()
+    pos.fill_(64)
+    step()
+    with pytest.raises(RuntimeError, match="without a page"):
+        m.kv.reset()
+    m.kv.reset()
+    assert m.kv.free_pages == 48

@@ -185,9 +185,92 @@ def _programs_and_prefixes(rank, world):
     assert m.kv.free_pages == 12 and not bool((m.kv.page_table >= 0).any())
 
 
-@pytest.mark.parametrize("part", [_longest_sequence, _steps_over_page_borders, _adapter, _programs_and_prefixes])
+def _programs_without_pages(rank, world):
+    """A program that runs for tokens without a page says so at the next look: after a release, past the reserved pages, past max_seq_len."""
+    _start()
+    ids, lens = _ids(14, 2, 10), torch.tensor([10, 4])
+    x = ids[:, :1].contiguous()
+    m = _model(16, logits=True, length=50)
+    m.kv.reserve_rows(2, 16)
+    prompt, step = _record(m.context_encoding, ids, lens - 1), _record(m.token_generation, x, lens)
+    want = [m.context_encoding(ids, lens - 1), m.token_generation(x, lens)]
+
+    def run(at):
+        torch.testing.assert_close(prompt(ids, lens - 1), want[0], rtol=0, atol=0)
+        got = step(x, at)
+        if torch.equal(at, lens):
+            torch.testing.assert_close(got, want[1], rtol=0, atol=0)
+
+    run(lens)
+    m.kv.check()
+    run(torch.tensor([15, -1]))
+    m.kv.check()
+    m.kv.release(0)
+    m.kv.reserve(0, 16)
+    run(lens)
+    m.kv.check()
+    step(x, torch.tensor([16, 4]))                              # behind its one page
+    with pytest.raises(RuntimeError, match="without a page"):
+        m.kv.check()
+    m.kv.check()                                                # said once
+    m.kv.release(1)
+    step(x, torch.tensor([-1, 4]))
+    with pytest.raises(RuntimeError, match="without a page"):
+        m.kv.release(0)
+    prompt(ids, lens - 1)
+    with pytest.raises(RuntimeError, match="without a page"):
+        m.kv.reset()
+    m.kv.reserve_rows(2, 50)
+    run(torch.tensor([49, 49]))
+    m.kv.check()
+    step(x, torch.tensor([50, 3]))                              # its last page has room, the rotation tables end
+    with pytest.raises(RuntimeError, match="without a page"):
+        m.kv.reset()
+    run(lens)
+    m.kv.reset()
+    m.kv.reset()
+    prompt(ids, lens - 1)
+    m.kv.forget_programs()
+    m.kv.check()
+
+
+@pytest.mark.parametrize("part", [_longest_sequence, _steps_over_page_borders, _adapter, _programs_and_prefixes, _programs_without_pages])
 def test_rows(part):
     run_distributed(part, 1, timeout=240)
+
+
+# first positions, lens, whether a token that counts has no place: tables of three pages of 16 tokens (-1, 9: no page), rotation tables of 40 rows
+LOST = [([0, 14, 30], None, False), ([0, 14, 30], [2, 2, 3], False), ([31, 0, 0], None, True), ([31, 0, 0], [1, 2, 2], False),
+        ([0, 15, 0], None, True), ([0, 15, 0], [2, 1, 2], False), ([0, -1, 30], None, False), ([0, 0, 32], None, True), ([0, 0, 39], None, True),
+        ([0, 0, 38], [2, 2, 0], False), ([40, 0, 0], None, True), ([40, 0, 0], [0, 2, 2], False), ([1 << 40, 0, 0], None, True), ([-5, -1, -9], None, False)]
+
+
+def append_notes(device, dtype, first, lens, noted):
+    from neuronx_distributed_b200 import ops
+
+    B, W, H, D, ps = 3, 2, 2, 16, 16
+    g = torch.Generator().manual_seed(0)
+    q, k, v = (torch.randn(B, W, H, D, generator=g).to(device, dtype) for _ in range(3))
+    cos, sin = (t.to(device) for t in ops.rope.rope_tables(40, D))
+    table = torch.tensor([[0, 1, -1], [2, -1, -1], [3, 4, 9]], dtype=torch.int32, device=device)         # of six pages
+    lost = torch.zeros(1, dtype=torch.int32, device=device)
+    kc, vc = (torch.zeros(6, ps, H, D, device=device, dtype=dtype) for _ in range(2))
+    args = (q, k, v, torch.tensor(first, device=device), cos, sin, kc, vc, table)
+    lens = None if lens is None else torch.tensor(lens, device=device)
+    ops.paged.rope_append(*args, lens=lens, lost=lost)
+    assert int(lost) == noted
+    lost.fill_(1)
+    out = ops.paged.rope_append(*args, lens=lens, lost=lost)                     # it is never taken back
+    assert int(lost) == 1 and torch.equal(out, ops.paged.rope_append(*args, lens=lens))
+    for bad in (torch.zeros(1), torch.zeros(2, dtype=torch.int32), torch.zeros((), dtype=torch.int32)):
+        with pytest.raises(ValueError, match="lost"):
+            ops.paged.rope_append(*args, lost=bad.to(device))
+
+
+@pytest.mark.parametrize("first, lens, noted", LOST)
+def test_append_notes_tokens_without_a_place(first, lens, noted):
+    # the second row's second page is missing, the third row's third page lies outside the pool
+    append_notes("cpu", torch.float32, first, lens, noted)
 
 
 def test_manager_ends_at_max_seq_len():
