@@ -229,6 +229,7 @@ class ConstInfo:
     named: bool                     # a module parameter / buffer (survives under its own name) vs an anonymous capture
     device_type: str = ""           # where the recorded tensor lived ("" = the plan's device type)
     in_checkpoint: bool = True      # a key of the module's ``state_dict`` (non-persistent buffers and captures are not)
+    state: bool = False             # changes between calls although no node writes to it (a tensor with ``_plan_state``: tables that the host keeps)
 
 
 def _resolve_op(target: str) -> Callable:
@@ -413,10 +414,10 @@ class LaunchPlan:
         transposes, de-quantisation, input-independent masks / tables) and the remaining per-call plan, which consumes
         the transformer's results as new constants ``_derived_<id>``.  Returns ``(transformer, main, transform_map)``;
         ``transform_map`` names, per weight, the chain of hoisted ops that start from it.  Constants named in ``skip``
-        and everything written to in place (state) stay untouched."""
+        and everything written to in place (state), by the plan or by the host, stay untouched."""
         skip = set(skip)
         mut, root = self._mutated_roots(), self._roots()
-        frozen: Set[int] = {i for i, c in self.constants.items() if i not in mut and c.name not in skip}
+        frozen: Set[int] = {i for i, c in self.constants.items() if i not in mut and not c.state and c.name not in skip}
         hoisted: List[Node] = []
         rest: List[Node] = []
         origin: Dict[int, Set[int]] = {i: {i} for i in frozen}
@@ -495,7 +496,7 @@ class LaunchPlan:
     def to_json(self) -> Dict[str, Any]:
         return {"format": self.FORMAT, "device_type": self.device_type, "meta": self.meta,
                 "inputs": self.inputs, "outputs": self.outputs,
-                "constants": {str(i): [c.name, list(c.shape), c.dtype, c.named, c.device_type, c.in_checkpoint]
+                "constants": {str(i): [c.name, list(c.shape), c.dtype, c.named, c.device_type, c.in_checkpoint, c.state]
                               for i, c in self.constants.items()},
                 "nodes": [n.to_json() for n in self.nodes]}
 
@@ -504,7 +505,7 @@ class LaunchPlan:
         if d.get("format") != LaunchPlan.FORMAT:
             raise PlanError(f"launch plan format {d.get('format')} is not supported (expected {LaunchPlan.FORMAT})")
         consts = {int(i): ConstInfo(v[0], tuple(v[1]), v[2], bool(v[3]), v[4] if len(v) > 4 else "",
-                                   bool(v[5]) if len(v) > 5 else bool(v[3])) for i, v in d["constants"].items()}
+                                   bool(v[5]) if len(v) > 5 else bool(v[3]), len(v) > 6 and bool(v[6])) for i, v in d["constants"].items()}
         return LaunchPlan([Node.from_json(n) for n in d["nodes"]], d["inputs"], d["outputs"], consts, d["device_type"], d.get("meta"))
 
     def save(self, path: str) -> None:
@@ -593,7 +594,8 @@ class _Recorder(TorchDispatchMode):
         if name is None:
             name = f"_const_{vid}"
         in_ckpt = named and (self.checkpoint_keys is None or name in self.checkpoint_keys)
-        self.constants[vid] = (ConstInfo(name, tuple(t.shape), str(t.dtype).split(".", 1)[1], named, t.device.type, in_ckpt), t)
+        self.constants[vid] = (ConstInfo(name, tuple(t.shape), str(t.dtype).split(".", 1)[1], named, t.device.type, in_ckpt,
+                                          getattr(t, "_plan_state", False)), t)
         if key[0]:
             self.by_mem[key] = vid
         return vid

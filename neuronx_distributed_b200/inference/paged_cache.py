@@ -31,6 +31,7 @@ class PagedKVCacheManager:
         self.page_table = torch.full((batch_size, self.columns), -1, dtype=torch.int32, device=device)
         self._shared_table = torch.full((self.columns,), -1, dtype=torch.int32, device=device)
         self.shared_pages: Optional[torch.Tensor] = None      # [n] int32, the beginning of that table: what every row begins with
+        self.page_table._plan_state = True                    # a launch plan keeps nothing that follows from it (inference/launch_plan.py)
         self.lost = torch.zeros(1, dtype=torch.int32, device=device)        # becomes 1 where a token had no page (ops.paged.rope_append)
         self._shared: List[int] = []
         self._rows: List[List[int]] = [[] for _ in range(batch_size)]       # pages of a row behind the shared ones
@@ -143,6 +144,7 @@ class PagedKVCacheManager:
         self._shared = self._take(n)
         self._shared_table[:] = -1
         pages = self._shared_table[:n]
+        pages._plan_state = True
         pages.copy_(torch.tensor(self._shared, dtype=torch.int32, device=self.page_table.device))
         self.page_table[:] = -1
         self.page_table[:, :n] = pages

@@ -234,7 +234,39 @@ def _programs_without_pages(rank, world):
     m.kv.check()
 
 
-@pytest.mark.parametrize("part", [_longest_sequence, _steps_over_page_borders, _adapter, _programs_and_prefixes, _programs_without_pages])
+def _plans_without_their_weights_part(rank, world):
+    """A launch plan whose weight-only part has been taken out goes by the tables as they are, not as they were then."""
+    from neuronx_distributed_b200.inference.launch_plan import LaunchPlan
+
+    _start()
+    ids, lens = _ids(15, 2, 10), torch.tensor([10, 4])
+    x = ids[:, :1].contiguous()
+    for prefix in (0, 32):
+        m, pos = _model(16, logits=True), lens + prefix
+        m.share_prefix(_ids(16, prefix))
+        m.context_encoding(ids, lens - 1)
+        plan = _record(m.token_generation, x, pos)
+        transformer, main, _ = plan.hoist_weight_only()
+        assert transformer.nodes
+        main.apply_transformer(transformer)
+        stored = LaunchPlan.from_json(plan.to_json()).bind(plan.named_constants())
+        again, rest, _ = stored.hoist_weight_only()
+        rest.apply_transformer(again)
+        before = m.kv.page_table.clone()
+        for turn in range(2):
+            want = m.token_generation(x, pos)
+            for p in (plan, main, rest):
+                torch.testing.assert_close(p(x, pos), want, rtol=0, atol=0)
+            if turn == 0:                                       # rows change their pages, and the prefix its own
+                m.kv.release(0)
+                m.share_prefix(_ids(17, prefix))
+                m.kv.reserve(1, prefix + 30)
+                m.context_encoding(ids, lens - 1)
+                assert not torch.equal(m.kv.page_table, before)
+
+
+@pytest.mark.parametrize("part", [_longest_sequence, _steps_over_page_borders, _adapter, _programs_and_prefixes, _programs_without_pages,
+                                  _plans_without_their_weights_part])
 def test_rows(part):
     run_distributed(part, 1, timeout=240)
 
