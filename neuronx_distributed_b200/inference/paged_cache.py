@@ -116,7 +116,12 @@ class PagedKVCacheManager:
 
     def release(self, row: int) -> None:
         """The row's own pages go back to the pool; the shared ones stay."""
+        if self.in_program():
+            raise RuntimeError("pages are given back on the host: not by a call that is captured or recorded")
         self.check()
+        self._give_back(row)
+
+    def _give_back(self, row: int) -> None:
         if self._rows[row]:
             self._free += self._rows[row][::-1]
             self._rows[row] = []
@@ -138,8 +143,11 @@ class PagedKVCacheManager:
             raise RuntimeError(f"programs were captured or recorded behind a prefix of {self._programs * self.page_size} tokens and would go on with it, "
                                f"{tokens} are asked for: kv.forget_programs() when none of them is run any more")
         self.check()
+        return self._share(n)
+
+    def _share(self, n: int) -> torch.Tensor:
         for row in range(self.batch_size):
-            self.release(row)
+            self._give_back(row)
         self._free += self._shared[::-1]
         self._shared = self._take(n)
         self._shared_table[:] = -1
@@ -150,6 +158,11 @@ class PagedKVCacheManager:
         self.page_table[:, :n] = pages
         self.shared_pages = pages if n else None
         return pages
+
+    def drop_shared(self) -> None:
+        """The shared pages go back to the pool, and all rows start anew: what should have filled them failed.  Programs that count on them have to wait
+        for another prefix of their length."""
+        self._share(0)
 
     def reset(self) -> None:
         """All pages go back to the pool, the shared ones too (:meth:`take_shared` of nothing)."""

@@ -224,7 +224,8 @@ class LlamaForInference(nn.Module):
     @torch.no_grad()
     def share_prefix(self, prefix_ids: torch.Tensor) -> None:
         """A prefix ``[n]`` (whole pages) that every sequence begins with from now on: it is encoded once and kept once, prompts go on
-        behind it, and single tokens and windows of all rows read it together.  All rows start anew; ``n = 0`` ends it."""
+        behind it, and single tokens and windows of all rows read it together.  All rows start anew; ``n = 0`` ends it.  Programs that were
+        captured or recorded go on behind another prefix of the same length; another length is refused (``kv.forget_programs``)."""
         if not self.paged:
             raise ValueError("a shared prefix needs a cache in pages (page_size)")
         ids = prefix_ids.reshape(1, -1)
@@ -233,6 +234,9 @@ class LlamaForInference(nn.Module):
             self._rows = (torch.zeros(1, dtype=torch.long, device=ids.device), None, pages.view(1, -1), None)
             try:
                 self._body(ids, None, True, None)
+            except BaseException:
+                self.kv.drop_shared()
+                raise
             finally:
                 self._rows = None
 

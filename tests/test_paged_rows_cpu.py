@@ -182,6 +182,10 @@ def _programs_and_prefixes(rank, world):
         _record(m.context_encoding, ids, lens - 1)
     with pytest.raises(RuntimeError, match="captured"):
         _record(m.share_prefix, _ids(13, 32))
+    m.kv.reserve(0, 16)
+    with pytest.raises(RuntimeError, match="captured"):
+        _record(lambda t: m.kv.release(0) or t, ids)
+    m.kv.release(0)
     assert m.kv.free_pages == 12 and not bool((m.kv.page_table >= 0).any())
 
 
@@ -265,8 +269,41 @@ def _plans_without_their_weights_part(rank, world):
                 assert not torch.equal(m.kv.page_table, before)
 
 
+def _prefix_that_fails(rank, world):
+    """A prefix whose encoding fails is not kept: its pages hold nothing that a row may begin with."""
+    _start()
+    m, ids = _model(16, logits=True), _ids(18, 2, 10)
+    want = m.context_encoding(ids)
+    body = m._body
+    m._body = lambda *a: (_ for _ in ()).throw(MemoryError("no room"))
+    with pytest.raises(MemoryError):
+        m.share_prefix(_ids(19, 32))
+    m._body = body
+    assert m.kv.shared_tokens == 0 and m.kv.shared_pages is None and m.kv.free_pages == 16
+    torch.testing.assert_close(m.context_encoding(ids), want, rtol=0, atol=0)
+    # behind a prefix that programs count on: they are not run without one, and another of its length can be shared
+    m.kv.reset()
+    m.share_prefix(_ids(19, 32))
+    m.context_encoding(ids)
+    x = ids[:, :1].contiguous()
+    pos = torch.tensor([42, 42])
+    step = _record(m.token_generation, x, pos)
+    m._body = lambda *a: (_ for _ in ()).throw(MemoryError("no room"))
+    with pytest.raises(MemoryError):
+        m.share_prefix(_ids(20, 32))
+    m._body = body
+    assert m.kv.shared_tokens == 0 and m.kv.free_pages == 16
+    step(x, pos)
+    with pytest.raises(RuntimeError, match="without a page"):
+        m.kv.check()
+    m.share_prefix(_ids(20, 32))
+    m.context_encoding(ids)
+    torch.testing.assert_close(step(x, pos), m.token_generation(x, pos), rtol=0, atol=0)
+    m.kv.check()
+
+
 @pytest.mark.parametrize("part", [_longest_sequence, _steps_over_page_borders, _adapter, _programs_and_prefixes, _programs_without_pages,
-                                  _plans_without_their_weights_part])
+                                  _plans_without_their_weights_part, _prefix_that_fails])
 def test_rows(part):
     run_distributed(part, 1, timeout=240)
 
