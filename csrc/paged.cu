@@ -152,9 +152,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn
   __shared__ float sm_m[kWarps][8 * R], sm_l[kWarps][8 * R], sm_bm[8 * R], sm_bl[8 * R];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, hq = lane >> 2, quad = lane & 3;
   const int rows = SHARED ? p.B * p.W * p.G : p.W * p.G;
-  auto keys_of = [&](int e) { return SHARED ? p.shared : e < p.B ? all_keys(p, e) : 0; };
   const bool late = !SHARED && p.shared > 0;               // the launch over the shared pages is in front (paged.cuh)
   if (!late) pdl_wait();
+  int shared_keys = 0;
+  auto keys_of = [&](int e) { return SHARED ? shared_keys : e < p.B ? all_keys(p, e) : 0; };
   pdl_trigger();                                           // the last launch's blocks may take their places; they wait for this grid
   // Pages of this warp's keys in 32 tiles of a pair from tile t0 on, one a lane: -1 where there is none
   const int step = DEAL == kCluster ? p.cluster : 1;
@@ -181,8 +182,9 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn
       cur.w.tiles = walk_tiles<SHARED>(p, at.e);
       cur.w.head = (int)(at.tile / cur.w.tiles);
       cur.w.tile = (int)(at.tile % cur.w.tiles);
-      cur.n = keys_of(at.e);
       pages = fetch_pages(at.e, cur.w.tile);
+      if constexpr (SHARED) shared_keys = seen_of_shared(p, lane);       // beside the pages
+      cur.n = keys_of(at.e);
     }
   }
   const T* const kc = reinterpret_cast<const T*>(p.k);

@@ -32,6 +32,12 @@ NXD_DEVICE int all_keys(const PagedAttn& p, int b) {
   const int m = new_tokens(p, b);
   return m ? visible_keys(p, b, m - 1) : 0;
 }
+// Shared keys that some row of the batch sees (a whole warp asks): what lies behind them need not be finite
+NXD_DEVICE int seen_of_shared(const PagedAttn& p, int lane) {
+  int n = 0;
+  for (int b = lane; b < p.B; b += 32) n = max(n, all_keys(p, b));
+  return min(p.shared, __reduce_max_sync(0xffffffffu, n));
+}
 // Key tiles that rows [row0, row1) of a sequence see behind the shared pages
 NXD_DEVICE int row_key_tiles(const PagedAttn& p, int b, int row0, int row1) {
   const int m = new_tokens(p, b);

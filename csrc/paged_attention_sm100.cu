@@ -553,13 +553,14 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     // come.  Without it the first step took 3 to 5 us.
     const int part_of_step = warp;
     bool dry = true;
+    int shared_keys = 0;                           // SHARED: in place of the item's keys, which are loaded whether a row sees them or not
     Item it{};
     it.n0 = it.n1 = 1;
     while (true) {
       const int nt = t ? it.n1 : it.n0;
       if (nt > 0) {
         int b = 0, w = 0;
-        const int row = first_row(it) + (PAIR ? t * kRows : 0) + own, n = it.keys;
+        const int row = first_row(it) + (PAIR ? t * kRows : 0) + own, n = SHARED ? shared_keys : it.keys;
         const bool live = !dry && row_token(it, row, b, w);
         // keys that this row sees (one that does not count: all, whatever comes of it), and the fewest of the warp's rows
         const int sees = live ? min(visible_keys(p, b, w), n) : 0x7fffffff;
@@ -662,6 +663,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       if (dry) {
         if (!late) pdl_wait();
         pdl_trigger();
+        if constexpr (SHARED) shared_keys = seen_of_shared(p, lane);
       }
       dry = false;
       it = next_item();

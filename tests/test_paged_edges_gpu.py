@@ -1,0 +1,29 @@
+"""Calls of the paged operators that their documentation allows and ordinary programs seldom make."""
+import pytest
+import torch
+
+from paged_cases import make
+from test_paged_gpu import attend, check
+
+pytestmark = pytest.mark.gpu
+BF16, FP16 = torch.bfloat16, torch.float16
+
+
+@pytest.mark.parametrize("dtype, D", [(BF16, 128), (FP16, 64)])
+@pytest.mark.parametrize("B, W, H, Hkv", [(1, 1, 8, 8), (4, 2, 4, 2), (3, 5, 2, 2), (5, 1, 16, 2), (6, 6, 8, 2), (40, 2, 8, 1), (9, 14, 8, 1)])
+@pytest.mark.parametrize("last", [-1, 0, 37, 94, 95])
+def test_shared_pages_that_nobody_sees_to_the_end(dtype, D, B, W, H, Hkv, last):
+    """Every row stands inside the shared pages (or is idle): what lies there behind the last key that any of them sees may be anything."""
+    positions = [max(-1, last - W + 1 - 3 * b) for b in range(B)]
+    lens = [W if b % 3 else max(1, W - 1) for b in range(B)]
+    lens[0] = min(W, last + 1)
+    d = make(40, "cuda", dtype, B, W, H, Hkv, D, 16, positions, lens, 6)
+    end = max([p + n for p, n in zip(positions, lens) if p >= 0] + [0])
+    results = []
+    for x in (float("nan"), float("inf"), 0.0):
+        for i in range(end, 96):
+            for t in ("k_cache", "v_cache"):
+                d[t][d["shared_pages"][i // 16].long(), i % 16] = x
+        results.append(attend(d))
+    check(d, results[0])
+    assert torch.equal(results[0], results[1]) and torch.equal(results[0], results[2])
