@@ -38,8 +38,8 @@ struct Pair {
       for (int i = 0; i < N; ++i) b.v[i] = from_f32<T>(0.f);
   }
   NXD_DEVICE double weight(int i) const {
-    const double d = (double)a.f(i) - (double)b.f(i);
-    return d > 0 ? d : 0;                                  // NaN: 0
+    const double d = (double)a.f(i) - (double)fmaxf(b.f(i), 0.f);      // negative and NaN: 0, on the draft's side here
+    return d > 0 ? d : 0;                                              // and on the target's
   }
 };
 
@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(kThreads, 4) verify_kernel(const long* tokens,
       if (i < K) {
         const long x = tokens[(long)b * K + i];
         none = x < 0 || x >= V;                            // no token was drafted here
-        ok = !none && (double)accept[(long)b * K + i] * (double)to_f32<T>(draft[b * d_sb + i * d_sk + x]) < (double)to_f32<T>(target[b * t_sb + i * t_sk + x]);
+        ok = !none && (double)accept[(long)b * K + i] * (double)fmaxf(to_f32<T>(draft[b * d_sb + i * d_sk + x]), 0.f) < (double)to_f32<T>(target[b * t_sb + i * t_sk + x]);
       }
       const unsigned bad = __ballot_sync(0xffffffffu, !ok), ends = __ballot_sync(0xffffffffu, none);
       if (bad) {

@@ -79,15 +79,17 @@ def verify_drafts(draft_tokens: torch.Tensor, draft_probs: torch.Tensor, target_
     rows = torch.arange(B, device=target_probs.device)
     there = (draft_tokens >= 0) & (draft_tokens < V)
     at = draft_tokens.clamp(0, V - 1)[..., None]
-    ok = there & (accept_uniforms.double() * draft_probs.gather(2, at)[..., 0].double() < target_probs[:, :K].gather(2, at)[..., 0].double())
+    zero = lambda x: torch.where(x > 0, x, 0.0)               # negative numbers and NaN count as 0
+
+    ok = there & (accept_uniforms.double() * zero(draft_probs.gather(2, at)[..., 0].double()) < target_probs[:, :K].gather(2, at)[..., 0].double())
     n = ok.long().cumprod(1).sum(1)
     p = target_probs[rows, n].double()
     w = p
     if K:
         residual = (n < K) & there.gather(1, n.clamp(max=K - 1)[:, None])[:, 0]
-        w = p - torch.where(residual[:, None], draft_probs[rows, n.clamp(max=K - 1)].double(), 0.0)
-    w = torch.where(w > 0, w, 0.0)
-    w = torch.where((w.sum(1) > 0)[:, None], w, torch.where(p > 0, p, 0.0))
+        w = p - torch.where(residual[:, None], zero(draft_probs[rows, n.clamp(max=K - 1)].double()), 0.0)
+    w = zero(w)
+    w = torch.where((w.sum(1) > 0)[:, None], w, zero(p))
     cdf = w.cumsum(1)
     hit = (w > 0) & (cdf > sample_uniforms.double()[:, None] * cdf[:, -1:])
     index = torch.arange(V, device=w.device)

@@ -4,6 +4,9 @@ import torch
 
 from paged_cases import make
 from test_paged_gpu import attend, check
+from test_verify_edges_cpu import odd_rows
+
+from neuronx_distributed_b200 import ops
 
 pytestmark = pytest.mark.gpu
 BF16, FP16 = torch.bfloat16, torch.float16
@@ -27,3 +30,11 @@ def test_shared_pages_that_nobody_sees_to_the_end(dtype, D, B, W, H, Hkv, last):
         results.append(attend(d))
     check(d, results[0])
     assert torch.equal(results[0], results[1]) and torch.equal(results[0], results[2])
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF16, FP16])
+@pytest.mark.parametrize("V", [9, 1000, 32016])
+def test_verify_counts_negative_numbers_and_nan_as_zero(dtype, V):
+    args, want = odd_rows(V, dtype)
+    got = ops.select.verify_drafts(*[t.cuda() for t in args])
+    assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
