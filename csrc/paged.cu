@@ -582,7 +582,8 @@ PagedPlan paged_plan(PagedAttn& p) {
   };
   const long rows = (long)p.W * p.G, all = rows * p.B;
   // Portions of prompts, whose own rows fill the row tiles, gain nothing from the batch's: the shared pages are the first of their own
-  p.shared = rows <= 128 ? p.shared_cols * p.ps : 0;
+  // (nor is there room for them where the join, a warp for each row and head, would have more than 65535 blocks of one sequence).
+  p.shared = rows <= 128 && rows * p.Hkv <= 65535l * kWarps ? p.shared_cols * p.ps : 0;
   // Nine to sixteen rows of long sequences, enough of them to fill the GPU, are the tensor memory's, too: there the few-row kernel is bound by its
   // instructions (us, few rows / tiles: 16 sequences to 3000 keys, 16 rows, 8 heads, 50 / 45; 4 to 8000 50 / 34; 8 to 4000 38 / 35; but 1 to 2000
   // 11 / 18, 32 to 1000 33 / 43).

@@ -38,3 +38,16 @@ def test_verify_counts_negative_numbers_and_nan_as_zero(dtype, V):
     args, want = odd_rows(V, dtype)
     got = ops.select.verify_drafts(*[t.cuda() for t in args])
     assert torch.equal(got[0].cpu(), want[0]) and torch.equal(got[1].cpu(), want[1])
+
+
+def test_shared_pages_under_very_many_heads():
+    """The join of parts has a warp for every row and key/value head: 128 rows of 2048 heads are more than a launch takes; the shared pages are then the
+    first of every sequence's own."""
+    d = make(41, "cuda", BF16, 1, 128, 2048, 2048, 64, 16, [20], [128], 1, spare=1)
+    got = attend(d)
+    # the same heads 512 at a time (8 of them against the definition)
+    for h in range(0, 2048, 512):
+        part = {**d, "q": d["q"][:, :, h:h + 512], "k_cache": d["k_cache"][:, :, h:h + 512], "v_cache": d["v_cache"][:, :, h:h + 512]}
+        few = {**d, "q": d["q"][:, :, h:h + 2], "k_cache": d["k_cache"][:, :, h:h + 2], "v_cache": d["v_cache"][:, :, h:h + 2]}
+        check(few, got[:, :, h:h + 2])
+        check(few, attend(part)[:, :, :2])
