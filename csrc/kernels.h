@@ -223,6 +223,7 @@ struct PagedAttn {
   long q_sb, q_sw, q_sh, o_sb, o_sw, o_sh, table_sb;
   long k_sp, k_sr, k_sh, v_sp, v_sr, v_sh;        // strides of pages, rows in a page, heads
   float scale_log2;
+  int wait_ns;                       // after which a wait in the tile kernel gives up; negative: after so many, and no keys are loaded (tests)
 };
 // How a launch is dealt out (rows: few, the kernel of paged.cu, or tiles of 128, paged_attention_sm100.cu); workspaces follow from it
 struct PagedPlan {

@@ -12,7 +12,9 @@
 //                              outside the map, which arrives as zeros
 //   warp 13     products     : S = Q Kᵀ and O += P V, issued by one elected lane
 //   warp 14     pieces       : the block's share cut into pieces of pairs, handed to the others two at a time
-// Every wait gives up after two seconds (a wait that long is an error in here): the block then runs to its end without waiting, and its rows are NaN.
+//   warp 15     failures     : rows of NaN where a wait ran out
+// The row warps, which wait for all that the others do, give a wait up after two seconds (one that long is an error in here), and so do the others then.
+// What a thread hands on from there is worth nothing; at the end copies and products in flight are waited for, and the block's rows become NaN.
 #include <cuda.h>
 
 #include <algorithm>
@@ -49,7 +51,10 @@ struct Cut {
   static constexpr uint32_t SMEM = FIXED + SLOTS * TILE;
 };
 
-NXD_DEVICE void give_up_wait(uint32_t bar, uint32_t parity, uint32_t gave_up) {
+constexpr uint32_t kLimit = 4;                   // behind the word that says that a block has given up: after how many ns
+// → whether the phase has ended.  CLOCK: at most that long, and the word (WORD) says so to the others; otherwise until the word says so.
+template <bool CLOCK, bool WORD>
+NXD_DEVICE bool bounded_wait(uint32_t bar, uint32_t parity, uint32_t gave_up) {
   uint32_t done, tries = 0;
   uint64_t t0 = 0;
   while (true) {
@@ -60,17 +65,23 @@ NXD_DEVICE void give_up_wait(uint32_t bar, uint32_t parity, uint32_t gave_up) {
         : "=r"(done)
         : "r"(bar), "r"(parity)
         : "memory");
-    if (done) return;
+    if (done) return true;
     if ((++tries & 63u) == 0) {
-      uint32_t over;
-      uint64_t t;
-      asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(over) : "r"(gave_up) : "memory");
-      if (over) return;
-      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-      if (t0 == 0) t0 = t;
-      else if (t - t0 > 2000000000ull) {
-        asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(gave_up), "r"(1u) : "memory");
-        return;
+      if constexpr (WORD) {
+        uint32_t over;
+        asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(over) : "r"(gave_up) : "memory");
+        if (over) return false;
+      }
+      if constexpr (CLOCK) {
+        uint32_t limit;
+        uint64_t t;
+        asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(limit) : "r"(gave_up + kLimit) : "memory");
+        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+        if (t0 == 0) t0 = t;
+        else if (t - t0 > limit) {
+          if constexpr (WORD) asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(gave_up), "r"(1u) : "memory");
+          return false;
+        }
       }
     }
   }
@@ -128,6 +139,23 @@ NXD_DEVICE Item make_item(const PagedAttn& p, const Walk& w, long left) {
   return it;
 }
 
+// Where block's share begins, and how many tiles it has
+template <bool SHARED>
+NXD_DEVICE long begin_share(const PagedAttn& p, const Place& at, Walk& w) {
+  long left = min(at.per, at.total - blockIdx.x * at.per);
+  w = Walk{at.e, 0, 0, 1};
+  if (left > 0) {
+    w.tiles = walk_tiles<SHARED>(p, at.e);
+    w.head = (int)(at.tile / w.tiles);
+    w.tile = (int)(at.tile % w.tiles);
+    if (w.tile > 0 && whole<SHARED>(p, w.tiles)) {         // the block in front has it
+      left -= w.tiles - w.tile;
+      if (left > 0) next_pair<SHARED>(p, w);
+    }
+  }
+  return left;
+}
+
 // PAIR: a step of two row tiles and 128 keys takes 2.2 us: exponentials 1.05, products 1.05 (heads of 128 numbers), which overlap little.  2 x 1000 tokens (a
 // quarter padding) behind 6000 keys, 48 heads of 64 on 8: 158 us, 470 TFLOP/s.  Otherwise: two tiles of 64 keys in 1.7 us, 5 TB/s over the GPU; windows of 5
 // tokens of 8 sequences to 6000 keys, 64 heads on 8: 43 us, of which 7 are the start and 5 the launch that joins parts.
@@ -141,14 +169,21 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
   const uint32_t sQ = smem_base, sKV = smem_base + 2 * C::Q_TILE, sO = sKV + SLOTS * TILE, sStat = sO + C::STAGE;
   const uint32_t bars = sStat + 2048;
-  // per stream or row tile: qf[2] qe[2] s[2] p[2] of[2] oe[2] lf[2] le[2] | pieces: full[2] empty[2] | ring: kvf[] kve[] | tmem slot, gave up | pieces[2] |
-  // holes[]
+  // per stream or row tile: qf[2] qe[2] s[2] p[2] of[2] oe[2] lf[2] le[2] | pieces: full[2] empty[2] | ring: kvf[] kve[] | tmem slot, products done |
+  // gave up, limit, ring's end (slot, lap) | pieces[2] | holes[]
   const uint32_t bar_qf = bars, bar_qe = bars + 16, bar_s = bars + 32, bar_p = bars + 48, bar_of = bars + 64, bar_oe = bars + 80, bar_lf = bars + 96,
                  bar_le = bars + 112, bar_nf = bars + 128, bar_ne = bars + 144, bar_kvf = bars + 160, bar_kve = bar_kvf + 8 * SLOTS,
-                 tmem_slot = bar_kve + 8 * SLOTS, gave_up = tmem_slot + 4, pieces = tmem_slot + 16, holes = pieces + 64;
-  static_assert(160 + 16 * SLOTS + 16 + 64 + 4 * kHoles <= 1024, "barriers");
+                 tmem_slot = bar_kve + 8 * SLOTS, bar_end = tmem_slot + 8, gave_up = tmem_slot + 16, last_key = tmem_slot + 24, pieces = tmem_slot + 32, holes = pieces + 64;
+  static_assert(160 + 16 * SLOTS + 32 + 64 + 4 * kHoles <= 1024, "barriers");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  auto wait = [&](uint32_t bar, uint32_t parity) { give_up_wait(bar, parity, gave_up); };
+  auto wait = [&](uint32_t bar, uint32_t parity) { return bounded_wait<false, true>(bar, parity, gave_up); };
+  auto clocked_wait = [&](uint32_t bar, uint32_t parity) { bounded_wait<true, true>(bar, parity, gave_up); };
+  // Whoever is told of something by a thread that gave up before sees this, too: the word is written first
+  auto failed = [&] {
+    uint32_t over;
+    asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(over) : "r"(gave_up) : "memory");
+    return over;
+  };
 
   if (warp == 12 && lane == 0) {
     for (int i = 0; i < 2; ++i) {
@@ -158,7 +193,8 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       mbar_init(bar_nf + 8 * i, 1); mbar_init(bar_ne + 8 * i, 14);       // readers: softmax, row, key and product warps
     }
     for (int i = 0; i < SLOTS; ++i) { mbar_init(bar_kvf + 8 * i, 1); mbar_init(bar_kve + 8 * i, 1); }
-    asm volatile("st.shared.u32 [%0], %1;" ::"r"(gave_up), "r"(0u) : "memory");
+    mbar_init(bar_end, 1);
+    asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(gave_up), "r"(0u), "r"(abs(p.wait_ns)) : "memory");
     fence_barrier_init();
     prefetch_tmap(&tk);
     prefetch_tmap(&tv);
@@ -179,16 +215,15 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
   auto key_at = [&](int j) { return (SHARED ? 0 : p.shared) + j * KEYS; };
   // a warp's next piece; n = 0: no more
   int piece = 0;
-  auto next_item = [&]() {
+  auto next_item = [&](auto... clock) {
     const int st = piece & 1;
-    wait(bar_nf + 8 * st, (uint32_t)((piece >> 1) & 1));
+    bounded_wait<sizeof...(clock) != 0, true>(bar_nf + 8 * st, (uint32_t)((piece >> 1) & 1), gave_up);
     ++piece;
     Item it;
     const uint32_t at = pieces + st * 32;
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(it.e), "=r"(it.head), "=r"(it.j0), "=r"(it.n) : "r"(at) : "memory");
     asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(it.n0), "=r"(it.n1), "=r"(it.keys), "=r"(it.ends) : "r"(at + 16) : "memory");
-    uint32_t over;
-    asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(over) : "r"(gave_up) : "memory");
+    const uint32_t over = failed();
     __syncwarp();
     if (lane == 0) mbar_arrive(bar_ne + 8 * st);
     if (over) it.n = it.n0 = it.n1 = 0;            // pieces may not be what they should
@@ -238,8 +273,9 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       // lane = box of a tile; pages are looked up for 32 boxes at a time, one round ahead of those that are asked for
       int slot = 0, tile = 0;
       uint32_t ph = 0;
+      bool ok = true;
       const int boxes = KEYS / box, round = 32 / boxes;
-      for (Item it = next_item(); it.n > 0; it = next_item()) {
+      for (Item it = p.wait_ns < 0 ? Item{} : next_item(); it.n > 0; it = next_item()) {
         const int n = it.keys;
         const int* table = p.table + (SHARED ? 0 : it.e / row_tiles * p.table_sb);
         auto look_up = [&](int j) {
@@ -258,13 +294,13 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
           const int row = key % p.ps;
 #pragma unroll
           for (int kv = 0; kv < 2; ++kv) {
-            wait(bar_kve + 8 * slot, ph ^ 1);
-            if (lane == 0) {
+            ok &= wait(bar_kve + 8 * slot, ph ^ 1);
+            if (lane == 0 && ok) {
               if (kv == 0) asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(holes + (tile % kHoles) * 4), "r"(hole) : "memory");
               mbar_expect_tx(bar_kvf + 8 * slot, TILE);
             }
             __syncwarp();
-            if (lane < boxes) {
+            if (lane < boxes && ok) {
               // x, row in the page, head, page; a page of -1 is outside the map
               const uint32_t dst = sKV + slot * TILE + lane * box * 128;
 #pragma unroll
@@ -274,13 +310,8 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
           }
         }
       }
-      uint32_t over;
-      asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(over) : "r"(gave_up) : "memory");
-      if (over) {                                  // nothing of this block is on its way when it ends
-        asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(gave_up), "r"(0u) : "memory");
-        for (int i = 0; i < SLOTS; ++i) wait(bar_kvf + 8 * ((slot + i) % SLOTS), (slot + i) / SLOTS ? ph : ph ^ 1);
-        asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(gave_up), "r"(1u) : "memory");
-      }
+      if (lane == 0) asm volatile("st.shared.v2.u32 [%0], {%1, %2};" ::"r"(last_key), "r"(slot), "r"(ph) : "memory");
+      asm volatile("bar.arrive 2, 224;" ::: "memory");     // warp 15 waits for this
     } else if (warp == 13) {
       // all 32 lanes run this loop; the helpers elect one lane
       constexpr uint32_t kTypes = sizeof(T) == 2 && std::is_same<T, __half>::value ? (1u << 7) | (1u << 10) : 0u;
@@ -345,19 +376,12 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         it = nx;
         pos0 = pos1;
       }
+      tcgen05_commit_e(bar_end);
+      asm volatile("bar.arrive 2, 224;" ::: "memory");     // warp 15 waits for this
     }
     if (warp == 14) {
-      long left = min(at.per, at.total - blockIdx.x * at.per);
-      Walk w{at.e, 0, 0, 1};
-      if (left > 0) {
-        w.tiles = walk_tiles<SHARED>(p, at.e);
-        w.head = (int)(at.tile / w.tiles);
-        w.tile = (int)(at.tile % w.tiles);
-        if (w.tile > 0 && whole<SHARED>(p, w.tiles)) {       // the block in front has it
-          left -= w.tiles - w.tile;
-          if (left > 0) next_pair<SHARED>(p, w);
-        }
-      }
+      Walk w;
+      long left = begin_share<SHARED>(p, at, w);
       bool more = true;
       for (int i = 0; more; ++i) {
         more = left > 0;
@@ -376,22 +400,55 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         }
       }
     }
+    if (warp == 15) {
+      asm volatile("bar.sync 2, 224;" ::: "memory");       // keys have been asked for, products issued, rows have left
+      Walk w;
+      long left = 0;
+      if (failed()) {                              // nothing of this block is on its way when it ends
+        int slot;
+        uint32_t ph;
+        asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(slot), "=r"(ph) : "r"(last_key) : "memory");
+        for (int i = 0; i < SLOTS; ++i) bounded_wait<true, false>(bar_kvf + 8 * ((slot + i) % SLOTS), (slot + i) / SLOTS ? ph : ph ^ 1, gave_up);
+        bounded_wait<true, false>(bar_end, 0, gave_up);
+        left = begin_share<SHARED>(p, at, w);
+      }
+      while (left > 0) {                           // and its rows are NaN, or parts that make them NaN
+        const Item it = make_item<PAIR, SHARED>(p, w, left);
+        left -= it.n;
+        if (left > 0) next_pair<SHARED>(p, w);
+        const long slot = part_slot<SHARED>(p, (long)it.e * p.Hkv + it.head, blockIdx.x, it.ends & 1) * tile_rows;
+#pragma unroll 1
+        for (int r = lane; r < tile_rows; r += 32) {
+          const int row = first_row(it) + r;
+          int b, t;
+          const bool live = row_token(it, row, b, t);
+          if (!SHARED && p.shared == 0 && it.ends == 3) {
+            const uint32_t x = live ? 0x7fff7fffu : 0u;
+            T* const to = reinterpret_cast<T*>(p.out) + b * p.o_sb + t * p.o_sw + (long)(it.head * p.G + row % p.G) * p.o_sh;
+            if (row < all_rows)
+              for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(to + c) = make_uint4(x, x, x, x);
+          } else if (live) {
+            *reinterpret_cast<float2*>((SHARED ? p.pre_ml : p.part_ml) + (slot + r) * 2) = make_float2(0.f, __int_as_float(0x7fffffff));
+          }
+        }
+      }
+    }
     __syncwarp();
   } else if (warp >= 8) {
     const int quarter = warp & 3, own = quarter * 32 + lane;
     const uint32_t tO = tmem_O + ((uint32_t)(quarter * 32) << 16), stage = sO + quarter * kOutStage;
     uint32_t ph = 0, q_loads = 0;                  // bit t: parity of stream t's items, of row tile t's loads
     auto load_rows = [&](const Item& it, int q, int tile) {
-      wait(bar_qe + 8 * q, ((q_loads >> q) & 1) ^ 1);
+      clocked_wait(bar_qe + 8 * q, ((q_loads >> q) & 1) ^ 1);
       q_loads ^= 1u << q;
       load_q(it, q, tile, own);
     };
-    Item it = next_item();
+    Item it = next_item(true);
     if (it.n > 0)
       for (int t = 0; t < (PAIR ? 2 : 1); ++t)
         if (!PAIR || (t ? it.n1 : it.n0) > 0) load_rows(it, t, t);
     for (int il = 0; it.n > 0; ++il) {
-      const Item nx = next_item();
+      const Item nx = next_item(true);
       // the next item's rows before this one's sums: the products wait for those rows before they have issued the last of this item's
       if (nx.n > 0) {
         if (!PAIR) load_rows(nx, (il + 1) & 1, 0);
@@ -410,14 +467,14 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         const bool none = (t ? it.n1 : it.n0) == 0;
         float m = -INFINITY, l = 0.f, f0 = 1.f, f1 = 0.f;
         if (!none) {
-          wait(bar_of + 8 * t, (ph >> t) & 1);
-          wait(bar_lf + 8 * t, (ph >> t) & 1);
+          clocked_wait(bar_of + 8 * t, (ph >> t) & 1);
+          clocked_wait(bar_lf + 8 * t, (ph >> t) & 1);
           ph ^= 1u << t;
           asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(m), "=f"(l) : "r"(sStat + t * 1024 + own * 8) : "memory");
           mbar_arrive(bar_le + 8 * t);
           if (merge) {
-            wait(bar_of + 8, (ph >> 1) & 1);
-            wait(bar_lf + 8, (ph >> 1) & 1);
+            clocked_wait(bar_of + 8, (ph >> 1) & 1);
+            clocked_wait(bar_lf + 8, (ph >> 1) & 1);
             ph ^= 2u;
             float m1, l1;
             asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(m1), "=f"(l1) : "r"(sStat + 1024 + own * 8) : "memory");
@@ -429,9 +486,6 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             m = mm;
           }
           tcgen05_fence_after();
-          uint32_t over;
-          asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(over) : "r"(gave_up) : "memory");
-          if (over) l = __int_as_float(0x7fffffff);
         }
         if (!direct && live) {
           float* const ml = (SHARED ? p.pre_ml : p.part_ml) + (slot + r0 + lane) * 2;
@@ -537,6 +591,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
       it = nx;
     }
     if (!SHARED && p.shared == 0) finish_idle<T, D, 128>(p, threadIdx.x - 256);
+    asm volatile("bar.arrive 2, 224;" ::: "memory");       // warp 15 waits for this
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
     const int t = warp >= 4;                       // stream of this warpgroup

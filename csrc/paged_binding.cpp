@@ -3,6 +3,7 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
+#include <atomic>
 #include <cmath>
 #include <string>
 
@@ -110,6 +111,9 @@ c10::optional<Tensor> paged_append(const Tensor& q_, const Tensor& k_, const Ten
   return out;
 }
 
+// Nanoseconds after which the tile kernel gives a wait up, so that its rows are NaN; negative: its keys are not loaded, so that waits do run out
+std::atomic<int> wait_ns{2000000000};
+
 // None: not for the kernels
 c10::optional<Tensor> paged_attention(const Tensor& q_, const Tensor& kc, const Tensor& vc, const Tensor& table_, const Tensor& positions_,
                                       const c10::optional<double>& scale_, const c10::optional<Tensor>& lens_, const c10::optional<Tensor>& shared_pages_) {
@@ -155,6 +159,7 @@ c10::optional<Tensor> paged_attention(const Tensor& q_, const Tensor& kc, const 
   p.pre_o = p.part_o + plan.slots * D;             // join_parts counts on this order
   p.part_ml = p.pre_o + plan.pre_slots * D;
   p.pre_ml = p.part_ml + plan.slots * 2;
+  p.wait_ns = wait_ns.load();
   p.scale_log2 = (float)(scale * 1.4426950408889634);
   count_launches(nxd::paged_attention(p, plan, (int)D, dt_code(q), stream()));
   return out;
@@ -193,6 +198,7 @@ void bind_paged(pybind11::module_& m) {
         py::arg("v_cache"), py::arg("page_table"), py::arg("lens"), py::arg("lost") = py::none());
   m.def("paged_append_ok", &paged_append_ok);
   m.def("paged_attention", &paged_attention);
+  m.def("paged_wait_ns", [](int ns) { return wait_ns.exchange(ns); });      // → what it was
   m.def("paged_attention_ok", &paged_attention_ok);
   m.def("verify_drafts", &verify_drafts);
 }

@@ -51,3 +51,47 @@ def test_shared_pages_under_very_many_heads():
         few = {**d, "q": d["q"][:, :, h:h + 2], "k_cache": d["k_cache"][:, :, h:h + 2], "v_cache": d["v_cache"][:, :, h:h + 2]}
         check(few, got[:, :, h:h + 2])
         check(few, attend(part)[:, :, :2])
+
+
+@pytest.fixture
+def waits():
+    """→ a function that sets after how many ns the tile kernel's waits give up; negative: with keys that never come."""
+    call = ops._ext.ext().paged_wait_ns
+    before = call(2_000_000_000)
+    yield call
+    call(before)
+
+
+def live_rows(d):
+    w = torch.arange(d["q"].shape[1], device="cuda")
+    n = torch.full_like(d["positions"], len(w)) if d["lens"] is None else d["lens"]
+    return (w < n[:, None]) & (d["positions"] >= 0)[:, None]
+
+
+@pytest.mark.parametrize("dtype, D", [(BF16, 128), (FP16, 64)])
+@pytest.mark.parametrize("B, W, H, Hkv, shared, most", [
+    (3, 300, 8, 2, 0, 500), (2, 100, 8, 2, 0, 5000), (30, 10, 8, 1, 0, 3000), (3, 40, 2, 2, 0, 40), (40, 5, 8, 1, 0, 30), (1, 700, 4, 1, 0, 1),
+    (20, 1, 16, 2, 5, 600), (9, 9, 8, 2, 33, 300), (24, 20, 16, 2, 5, 2000), (2, 9, 8, 2, 5, 50),
+])
+def test_waits_that_run_out(waits, dtype, D, B, W, H, Hkv, shared, most):
+    """Keys that never come: every row that counts is NaN, whatever was left of the output and the workspace before; the next call is as ever."""
+    g = torch.Generator().manual_seed(W)
+    positions = (shared * 16 + torch.randint(0, most, (B,), generator=g)).tolist()
+    lens = torch.randint(1, W + 1, (B,), generator=g).tolist()
+    if B > 2:
+        positions[1] = -1
+    lens[0] = W
+    d = make(42, "cuda", dtype, B, W, H, Hkv, D, 16, positions, lens, shared)
+    want = attend(d)
+    torch.cuda.synchronize()
+    live = live_rows(d)
+    for left in (0.0, 1.0):
+        spare = torch.full((want.numel() * 8 + 300 * 256 * (D + 2) * 4,), left, device="cuda")         # what the allocator hands out next
+        del spare
+        waits(-1_000_000)
+        bad = attend(d)
+        torch.cuda.synchronize()
+        waits(2_000_000_000)
+        assert bool(bad[live].isnan().all()) and not bool(bad[~live].any())
+        assert torch.equal(attend(d), want)
+    check(d, want)
