@@ -37,6 +37,8 @@ def main():
     p.add_argument("--temperature", type=float, default=0.0, help="above 0: sampled tokens, accepted against the target's probabilities")
     p.add_argument("--batch_size", type=int, default=1, help="rows of the batch (sampling only)")
     a = p.parse_args()
+    if a.temperature > 0 and a.tp_degree > 1:
+        p.error("--temperature needs --tp_degree 1: sampled speculation goes by whole rows of logits, and tensor-parallel ranks have shards of them")
     dev = init_distributed()
     ps.initialize_model_parallel(tensor_model_parallel_size=a.tp_degree)
     dtype = torch.bfloat16 if dev.type == "cuda" else torch.float32

@@ -71,8 +71,8 @@ def speculative_generate(target, draft, prompt_ids: torch.Tensor, max_new_tokens
 @torch.no_grad()
 def speculative_sample(target, draft, prompt_ids: torch.Tensor, max_new_tokens: int, speculation_length: int = 4, temperature: float = 1.0,
                        generator: Optional[torch.Generator] = None, prompt_lens: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, float]:
-    """``target`` / ``draft``: :class:`models.llama_inference.LlamaForInference` with ``on_device_sampling=False`` (they return logits of the
-    whole vocabulary), contiguous or paged caches, a shared prefix of the same length in both or none.  ``prompt_ids [B, S]`` (right-padded,
+    """``target`` / ``draft``: :class:`models.llama_inference.LlamaForInference` on one rank, with ``on_device_sampling=False`` (they return logits of
+    the whole vocabulary; tensor-parallel ranks have shards of them and are refused), contiguous or paged caches, a shared prefix of the same length in both or none.  ``prompt_ids [B, S]`` (right-padded,
     ``prompt_lens [B]``) → (generated ids ``[B, max_new_tokens]``, mean accepted draft tokens per target forward)."""
     if temperature <= 0:
         raise ValueError(f"temperature must be positive, got {temperature} (greedy decoding: speculative_generate)")

@@ -354,3 +354,15 @@ def test_manager_ends_at_max_seq_len():
     assert kv.free_pages == 4 and kv.shared_pages is None and int((kv.page_table[0] >= 0).sum()) == 4
     kv.take_shared(96)
     assert kv.shared_tokens == 96
+
+
+def test_example_refuses_sampling_on_tensor_parallel_ranks():
+    """Before any model is built: the whole rows of logits that sampled speculation goes by are not there."""
+    import os
+    import subprocess
+    import sys
+
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, os.path.join(root, "examples", "inference", "run_llama_speculative.py"), "--temperature", "0.8", "--tp_degree", "2"],
+                       capture_output=True, text=True, timeout=240)
+    assert r.returncode == 2 and "--tp_degree 1" in r.stderr, r.stderr[-500:]
