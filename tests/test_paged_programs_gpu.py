@@ -94,3 +94,62 @@ def test_captured_prompts_and_pages_that_come_and_go():
         m.kv.reset()
     m.kv.reset()
     assert m.kv.free_pages == 48
+
+
+@pytest.mark.parametrize("prefix", [0, 64])
+def test_recorded_plans(prefix):
+    """Append, attention over own and shared pages, and verification as nodes of a launch plan: run at other positions and over other pages than it was
+    recorded with, with and without its weight-only part, and captured."""
+    from neuronx_distributed_b200 import ops
+    from neuronx_distributed_b200.inference.launch_plan import record
+
+    m = model(page_size=32)
+    prompts, lens = ids(10, 3, 40), torch.tensor([40, 7, 21]).cuda()
+
+    def begin(seed):
+        m.share_prefix(ids(seed, prefix))
+        m.context_encoding(prompts, lens - 1)
+        m.kv.reserve_rows(3, prefix + 100)
+
+    def step(window, pos, drafted, draft, accept, sample):
+        judged = torch.softmax(m.speculation_forward(window, pos), -1)
+        new, n = ops.select.verify_drafts(drafted, draft, judged, accept, sample)
+        return judged, new, n
+
+    def inputs(seed, shift):
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        draft = torch.softmax(torch.randn(3, 4, 512, generator=g, device="cuda"), -1)
+        drafted = ids(seed, 3, 4)
+        return [torch.cat([ids(seed + 1, 3, 1), drafted], 1), lens + prefix + shift, drafted, draft, torch.rand(3, 4, generator=g, device="cuda"),
+                torch.rand(3, generator=g, device="cuda")]
+
+    begin(11)
+    plan = record(step, inputs(20, 0))
+    targets = plan.summary()["top_targets"] and {n.target for n in plan.nodes}
+    assert {"paged_append", "paged_attention", "verify_drafts"} <= targets, targets
+    transformer, main, _ = plan.hoist_weight_only()
+    main.apply_transformer(transformer)
+    live = [t.clone() for t in inputs(20, 0)]
+    captured = capture(lambda *a: torch.cat([main(*a)[0].flatten(), main(*a)[1].flatten().float()]), *live)
+    for turn in range(2):
+        for shift in (0, 9, 30):
+            x = inputs(21 + shift, shift)
+            want = step(*x)
+            for p in (plan, main):
+                for a, b in zip(p(*x), want):
+                    assert torch.equal(a, b)
+            for a, b in zip(live, x):
+                a.copy_(b)
+            assert torch.equal(captured(), torch.cat([want[0].flatten(), want[1].flatten().float()]))
+        m.kv.check()
+        if turn == 0:
+            before = m.kv.page_table.clone()
+            m.kv.release(0)
+            m.kv.reserve(2, prefix + 100)
+            begin(12)
+            m.kv.release(0)
+            m.kv.release(1)
+            m.kv.reserve(1, prefix + 100)
+            m.context_encoding(prompts, lens - 1)
+            m.kv.reserve_rows(3, prefix + 100)
+            assert not torch.equal(before, m.kv.page_table)

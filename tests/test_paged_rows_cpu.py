@@ -302,8 +302,36 @@ def _prefix_that_fails(rank, world):
     m.kv.check()
 
 
+def _kv_len_and_experts(rank, world):
+    """kv_len, which contiguous rows read no further than, changes nothing over pages; a model of routed experts goes by them as well."""
+    from neuronx_distributed_b200.models.llama_inference import LlamaForInference
+    from neuronx_distributed_b200.models.mixtral import MixtralConfig, MixtralForCausalLM
+
+    _start()
+    ids, lens = _ids(21, 2, 14), torch.tensor([14, 5])
+    rows, pages = _model(logits=True), _model(16, logits=True)
+    for m in (rows, pages):
+        m.context_encoding(ids, lens - 1)
+    pos = lens                                                  # no position is left out: keys that nobody wrote are whatever a cache held before
+    for i in range(6):
+        w = 1 + 3 * (i % 2)
+        call = "speculation_forward" if w > 1 else "token_generation"
+        a, b, c = (getattr(m, call)(_ids(30 + i, 2, w), pos, **kw) for m, kw in ((rows, {"kv_len": 48}), (pages, {"kv_len": 48}), (pages, {})))
+        torch.testing.assert_close(b.reshape(a.shape), a, rtol=1e-5, atol=1e-5)
+        torch.testing.assert_close(b, c, rtol=0, atol=0)
+        pos = pos + w
+    out = []
+    for page in (None, 16):
+        torch.manual_seed(3)
+        cfg = MixtralConfig(vocab_size=64, hidden_size=32, intermediate_size=48, num_hidden_layers=2, num_attention_heads=4, num_key_value_heads=2,
+                            num_local_experts=4, num_experts_per_tok=2, dtype=torch.float32, max_position_embeddings=64)
+        m = LlamaForInference(cfg, batch_size=2, max_seq_len=64, lm_cls=MixtralForCausalLM, page_size=page).eval()
+        out.append(m.generate(_ids(22, 2, 9) % 64, 30, torch.tensor([9, 4])))
+    assert torch.equal(*out)
+
+
 @pytest.mark.parametrize("part", [_longest_sequence, _steps_over_page_borders, _adapter, _programs_and_prefixes, _programs_without_pages,
-                                  _plans_without_their_weights_part, _prefix_that_fails])
+                                  _plans_without_their_weights_part, _prefix_that_fails, _kv_len_and_experts])
 def test_rows(part):
     run_distributed(part, 1, timeout=240)
 
