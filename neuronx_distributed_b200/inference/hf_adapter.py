@@ -87,8 +87,6 @@ class HuggingFaceGenerationAdapter:
         paged = getattr(m, "paged", False)
         shared = m.kv.shared_tokens if paged else 0                                   # tokens that every sequence begins with
         longest = shared + int(lens.max())
-        if paged:
-            packed = packed[:, :longest - shared]                                     # no pages for padding of all rows
         room = m.max_seq_len - longest
         n_new = max_new_tokens if max_new_tokens is not None else ((max_length - S) if max_length is not None else room)
         n_new = max(0, min(n_new, room))

@@ -124,6 +124,11 @@ def _adapter(rank, world):
         assert shared.kv.shared_tokens == 32
     full = adapter.generate(ids, mask)
     assert full.shape[1] == 14 + 128 - 32 - 14 and torch.equal(full[:, 14:], rows.generate(whole, long_mask)[:, 46:])
+    # prompts as wide as they come go to the programs, which were captured for that width
+    seen = []
+    adapter.use_programs(lambda i, last: seen.append(tuple(i.shape)) or shared.context_encoding(i, last), shared.token_generation)
+    wide, wide_mask = torch.cat([ids, ids[:, :4]], 1), torch.cat([mask, torch.zeros(2, 4, dtype=torch.long)], 1)
+    assert torch.equal(adapter.generate(wide, wide_mask, max_new_tokens=30)[:, 18:], want) and seen == [(2, 18)]
     # a pool with just enough pages for one call at a time
     small = _model(16, num_pages=2 + 2 * 3)
     small.share_prefix(prefix)
