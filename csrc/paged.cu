@@ -140,9 +140,10 @@ enum Deal { kDealt, kCluster, kShared };
 // Bound by HBM: 4 D bytes per key and key/value head.  A warp walks 16-key tiles of its own through its own ring of cp.async stages, which runs
 // ahead over the ends of pairs.  Scores Sᵀ = K Qᵀ and sums Oᵀ += Vᵀ Pᵀ by mma.sync with the keys, then the head's columns, as the 16 rows of the
 // instruction and 8 R query rows as its columns, so that a group of up to 8 heads wastes nothing; the accumulator of Sᵀ becomes the operand Pᵀ by an
-// 8 x 8 transposition in registers.  Probabilities are rounded to the cache's type for the second product: half a step of 2^-8 (2^-11) each, which average out over
-// the keys; row sums are those of the unrounded ones.  One token of 16 sequences to 8192 keys, 32 heads on 8: 66 us, 6.0 TB/s; of 6 to 2500, 40 single
-// heads: 40 us; of one to 300: 6.7.
+// 8 x 8 transposition in registers.  The second product takes probabilities as two numbers of the cache's type, the rounded one and what that left, 2^-16
+// (2^-22) of them at most: memory is what bounds this kernel, and a product more costs nothing where it does (us, one / two: one token of 16 sequences
+// to 8192 keys, 32 heads on 8, 72 / 73, the call; of 6 to 2500, 40 single heads, 43 / 43; 16 rows to 1000 keys, 32 pairs of 4, 31 / 31; one sequence to
+// 4000 keys, 16 rows of 8 heads, 20.5 / 21.3).  The first of these alone: 66 us, 6.0 TB/s; the second 40; one sequence to 300: 6.7.
 template <typename T, int D, int R, Deal DEAL>
 __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn p) {
   constexpr bool SHARED = DEAL == kShared;
@@ -353,7 +354,7 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn
         for (int i = 0; i < R; ++i) mma16816<T>(k & 1 ? s1[i] : s[i], a, qf[i][k][0], qf[i][k][1]);
       }
       const bool masked = key + kKeys > lim_all;
-      uint32_t pf[R][2];
+      uint32_t pf[R][2], pl[R][2];                         // weights to the type, and what that left of them
 #pragma unroll
       for (int i = 0; i < R; ++i) {
 #pragma unroll
@@ -390,8 +391,14 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn
           pr[e] = exp2f(x[e]);
           l[i][e & 1] += pr[e];
         }
-        pf[i][0] = transpose8x8(pack16<T>(pr[0], pr[1]));
-        pf[i][1] = transpose8x8(pack16<T>(pr[2], pr[3]));
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t hi = pack16<T>(pr[2 * e], pr[2 * e + 1]);
+          float h0, h1;
+          unpack16<T>(hi, h0, h1);
+          pf[i][e] = transpose8x8(hi);
+          pl[i][e] = transpose8x8(pack16<T>(pr[2 * e] - h0, pr[2 * e + 1] - h1));
+        }
       }
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
@@ -400,7 +407,10 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn
         uint32_t a[4];
         ldmatrix_x4t(a, vs + r * (D * 2) + ((c ^ (r & 7)) << 4));
 #pragma unroll
-        for (int i = 0; i < R; ++i) mma16816<T>(o[i][k], a, pf[i][0], pf[i][1]);
+        for (int i = 0; i < R; ++i) {
+          mma16816<T>(o[i][k], a, pf[i][0], pf[i][1]);
+          mma16816<T>(o[i][k], a, pl[i][0], pl[i][1]);
+        }
       }
     }
     const bool end = cur.w.tile + 1 == cur.w.tiles;

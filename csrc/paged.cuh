@@ -220,5 +220,13 @@ template <> NXD_DEVICE uint32_t pack16<__half>(float lo, float hi) {
   return r;
 }
 
+template <typename T> NXD_DEVICE void unpack16(uint32_t v, float& lo, float& hi);
+template <> NXD_DEVICE void unpack16<__nv_bfloat16>(uint32_t v, float& lo, float& hi) { lo = __uint_as_float(v << 16); hi = __uint_as_float(v & 0xffff0000u); }
+template <> NXD_DEVICE void unpack16<__half>(uint32_t v, float& lo, float& hi) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&v));
+  lo = f.x;
+  hi = f.y;
+}
+
 }  // namespace paged
 }  // namespace nxd

@@ -79,6 +79,23 @@ def test_windows_of_many_lengths(dtype, D, W, H, Hkv, shared):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dtype, D", [(FP16, 64), (BF16, 128), (BF16, 64)])
+@pytest.mark.parametrize("B, W, H, Hkv, shared, most", [(5, 1, 8, 8, 0, 700), (5, 1, 8, 1, 0, 3000), (3, 4, 8, 2, 0, 500), (7, 2, 16, 2, 0, 1500),
+                                                        (2, 2, 8, 2, 3, 300), (1, 1, 8, 1, 33, 200)])
+def test_weights_of_few_rows_are_not_rounded(dtype, D, B, W, H, Hkv, shared, most):
+    """Up to 16 query rows of a sequence and key/value head (and of the batch, over shared pages): the bound of `bound` without the rounding of the weights
+    to the type; what is left of it, a half step of a half step (2^-17 in bf16; 2^-25 of a weight of 1 in fp16, of up to 4000 of them), lies within the
+    2^-13 of products and exponentials with which it is added."""
+    from test_paged_gpu import attend
+
+    d = case("cuda", dtype, W, H, Hkv, shared, most, B=B, D=D)
+    want, size = definition(d)
+    u = torch.finfo(dtype).eps / 2
+    off = (attend(d).double() - want).abs() - (u * want.abs() + (2.0 ** -13 + 4000 * 2.0 ** -25) * size + 1e-7)
+    assert bool((off <= 0).all()), (float(off.max()), off.argmax())
+
+
+@pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [FP16, BF16])
 def test_dealt_out_many(dtype):
     """More sequences than threads that look for places, in tables that few-row launches are dealt out for."""
