@@ -225,7 +225,7 @@ struct PagedAttn {
   float scale_log2;
   int wait_ns;                       // after which a wait in the tile kernel gives up; negative: after so many, and no keys are loaded (tests)
 };
-// How a launch is dealt out (rows: few, the kernel of paged.cu, or tiles of 128, paged_attention_sm100.cu); workspaces follow from it
+// How a launch is dealt out (rows: few, the kernel of paged.cu, or tiles of 64, 128 or 256, paged_attention_sm100.cu); workspaces follow from it
 struct PagedPlan {
   bool tiles, pre_tiles;             // whether the tile kernel has the rows, and those over the shared pages
   int grid, pre_grid;                // blocks of each walk

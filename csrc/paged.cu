@@ -581,7 +581,8 @@ int launch(const PagedAttn& p, const PagedPlan& plan, int dt, cudaStream_t st) {
 
 }  // namespace
 
-// Up to 16 query rows of a sequence and key/value head go to the kernel above, more to tiles of 128 or 256 rows on the tensor memory.
+// Up to 16 query rows of a sequence and key/value head (8 where there are many long tables, below) go to the kernel above, more to tiles of 64, 128 or 256
+// rows on the tensor memory.  Lengths are the tables': nothing about positions is known here.
 PagedPlan paged_plan(PagedAttn& p) {
   PagedPlan plan{};
   const int sms = device_sm_count();

@@ -119,7 +119,12 @@ def attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, pag
               scale: Optional[float] = None, lens: Optional[torch.Tensor] = None, shared_pages: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal attention of new tokens ``q [B, W, H, D]`` (their keys are in the pages already) over the cache → ``[B, W, H, D]`` (``[W, B, H, D]`` in
     memory): token ``w`` of row ``b`` sees keys ``0 … positions[b] + w``.  ``W`` = 1: token generation; a few: a drafted window; many: a portion
-    of a prompt.  Tokens that do not count, or see no key, come back as zeros.  Keys and values that some token of a row sees have to be finite.
+    of a prompt.  Tokens that do not count, or see no key, come back as zeros.  Keys and values that some token of a row sees have to be finite, and
+    scores, held in 32 bits, below 2^30 in magnitude.
+
+    Sums and statistics are in 32 bits.  Weights are rounded to the cache's type before they meet the values where a sequence has more than 16 query rows
+    for a key/value head (tokens times heads of a group; more than 8 of long sequences), and over pages that all share where the batch has; fewer rows
+    keep them.  The sizes of tables, not positions, say which kernel it is: one sequence in a table for many tokens takes longer than in a narrow one.
 
     ``shared_pages [n]`` int32: the pages of the first ``n * page_size`` tokens of EVERY sequence; the first ``n`` columns of ``page_table`` are not
     looked at.  Where a sequence has up to 128 query rows (tokens times heads of a group), they are read once for the whole batch."""
