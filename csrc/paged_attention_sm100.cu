@@ -402,14 +402,14 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     }
     if (warp == 15) {
       asm volatile("bar.sync 2, 224;" ::: "memory");       // keys have been asked for, products issued, rows have left
+      bounded_wait<true, false>(bar_end, 0, gave_up);      // nothing of this block is being multiplied, or told of that, when it ends
       Walk w;
       long left = 0;
-      if (failed()) {                              // nothing of this block is on its way when it ends
+      if (failed()) {                              // nor is anything on its way
         int slot;
         uint32_t ph;
         asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(slot), "=r"(ph) : "r"(last_key) : "memory");
         for (int i = 0; i < SLOTS; ++i) bounded_wait<true, false>(bar_kvf + 8 * ((slot + i) % SLOTS), (slot + i) / SLOTS ? ph : ph ^ 1, gave_up);
-        bounded_wait<true, false>(bar_end, 0, gave_up);
         left = begin_share<SHARED>(p, at, w);
       }
       while (left > 0) {                           // and its rows are NaN, or parts that make them NaN
