@@ -100,7 +100,10 @@ class PagedKVCacheManager:
         waits for them; inside :meth:`reserved_ahead`, and while a program is captured or recorded, nothing is looked at."""
         if self._ahead or self.in_program():
             return
-        for row, first in enumerate(positions.tolist()):
+        starts = positions.tolist()
+        if any(0 <= first < self.shared_tokens for first in starts):            # its keys would be everybody's
+            raise ValueError(f"positions {starts}: some lie inside the shared prefix of {self.shared_tokens} tokens, which rows do not write to")
+        for row, first in enumerate(starts):
             if first >= 0:
                 self.reserve(row, first + tokens)
 

@@ -307,6 +307,22 @@ def _prefix_that_fails(rank, world):
     m.kv.check()
 
 
+def _rows_keep_out_of_the_prefix(rank, world):
+    """A token of one row inside the shared prefix would change it for all rows: refused, and the prefix is as it was."""
+    _start()
+    m, ids, lens = _model(16, logits=True), _ids(23, 2, 10), torch.tensor([10, 4])
+    m.share_prefix(_ids(24, 32))
+    m.context_encoding(ids, lens - 1)
+    pool = [t.clone() for t in m.kv.k + m.kv.v]
+    for pos in ([10, 4], [42, 31], [0, -1]):                    # positions that do not count the prefix, or all of it
+        with pytest.raises(ValueError, match="shared prefix"):
+            m.token_generation(ids[:, :1], torch.tensor(pos))
+        with pytest.raises(ValueError, match="shared prefix"):
+            m.speculation_forward(ids[:, :3], torch.tensor(pos))
+    assert all(torch.equal(a, b) for a, b in zip(pool, m.kv.k + m.kv.v))
+    m.token_generation(ids[:, :1], torch.tensor([32, -1]))      # the first token behind it
+
+
 def _kv_len_and_experts(rank, world):
     """kv_len, which contiguous rows read no further than, changes nothing over pages; a model of routed experts goes by them as well."""
     from neuronx_distributed_b200.models.llama_inference import LlamaForInference
@@ -336,7 +352,7 @@ def _kv_len_and_experts(rank, world):
 
 
 @pytest.mark.parametrize("part", [_longest_sequence, _steps_over_page_borders, _adapter, _programs_and_prefixes, _programs_without_pages,
-                                  _plans_without_their_weights_part, _prefix_that_fails, _kv_len_and_experts])
+                                  _plans_without_their_weights_part, _prefix_that_fails, _kv_len_and_experts, _rows_keep_out_of_the_prefix])
 def test_rows(part):
     run_distributed(part, 1, timeout=240)
 
