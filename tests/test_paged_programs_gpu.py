@@ -153,3 +153,35 @@ def test_recorded_plans(prefix):
             m.context_encoding(prompts, lens - 1)
             m.kv.reserve_rows(3, prefix + 100)
             assert not torch.equal(before, m.kv.page_table)
+
+
+@pytest.mark.parametrize("prefix", [0, 64])
+def test_adapter_over_captured_programs(prefix):
+    """Prompt and step of a paged model captured by the builder, called by the generation adapter, over several calls: the tokens of eager steps."""
+    from neuronx_distributed_b200.inference.hf_adapter import HuggingFaceGenerationAdapter
+    from neuronx_distributed_b200.trace.model_builder import ModelBuilder
+
+    def served():
+        m = model(page_size=16, num_pages=prefix // 16 + 3 * 8)
+        m.on_device_sampling = True
+        m.share_prefix(ids(30, prefix))
+        return m
+
+    eager, m = served(), served()
+    prompts, mask = ids(31, 3, 40), torch.ones(3, 40, dtype=torch.long, device="cuda")
+    mask[1, :33], mask[2, :19] = 0, 0
+    builder = ModelBuilder(use_cuda_graphs=True)
+    builder.add("prompt", m, [(torch.zeros(3, 40, dtype=torch.long, device="cuda"), torch.full((3,), 39, device="cuda"))],
+                step_fn=lambda m, i, last: m.context_encoding(i, last))
+    builder.add("step", m, [(torch.zeros(3, 1, dtype=torch.long, device="cuda"), torch.full((3,), prefix + 40, device="cuda"))],
+                step_fn=lambda m, i, pos: m.token_generation(i, pos))
+    programs = builder.trace()
+    by_steps = HuggingFaceGenerationAdapter(eager)
+    captured = HuggingFaceGenerationAdapter(m).use_programs(programs, programs)
+    for seed in (31, 32):
+        for new in (60, 20, 88):
+            prompts = ids(seed, 3, 40)
+            assert torch.equal(captured.generate(prompts, mask, max_new_tokens=new), by_steps.generate(prompts, mask, max_new_tokens=new))
+            assert m.kv.shared_tokens == prefix
+    with pytest.raises(RuntimeError, match="pool"):
+        captured.generate(prompts, mask, max_new_tokens=100)
