@@ -1040,6 +1040,7 @@ static Tensor nvls_reduce_scatter(const Tensor& x, const Tensor& peer_bases, int
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   bind_native_autograd(m);
   bind_paged(m);
+  bind_paged_int4(m);
   m.def("rmsnorm_fwd", &rmsnorm_fwd);
   m.def("rmsnorm_bwd", &rmsnorm_bwd);
   m.def("add_rmsnorm_fwd", &add_rmsnorm_fwd);

@@ -30,3 +30,4 @@ Tensor gemv(const Tensor& x, const Tensor& w, const c10::optional<Tensor>& resid
 void count_launches(int64_t n);        // kernels of this package that a binding launched without Python's counting them
 void bind_native_autograd(pybind11::module_& m);
 void bind_paged(pybind11::module_& m);
+void bind_paged_int4(pybind11::module_& m);

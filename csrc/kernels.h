@@ -240,6 +240,47 @@ void paged_append(const void* q, const void* k, const void* v, const long* posit
                   void* q_out, void* kc, void* vc, const int* table, int* lost, int B, int W, int H, int Hkv, int D, int rows, int cols, int ps,
                   int pages, long table_sb, const long (*s)[3], long o_sb, long o_sw, const long (*cs)[3], int dt, cudaStream_t st);
 
+// ---- page tables and slots from the lengths of requests (page_tables.cu)
+constexpr int kMaxPageRows = 32768;                         // fewer rows than these
+struct PageTables {
+  const int *table, *held, *free;
+  const long *span, *positions, *lens, *lengths;           // lens, lengths: or null
+  int *table_out, *held_out, *free_out, *slots, *few;      // outputs may be the inputs where the call is in place; few: or null
+  long* span_out;
+  int B, W, cols, ps, P, shared, rows;                     // rows: of a block
+  bool trim;
+  long table_sb, out_sb;
+};
+void page_tables(PageTables p, bool in_place, cudaStream_t st);
+
+// ---- key/value cache in pages of 4 bits (paged_int4.cu); steps of pages, rows and heads in bytes (codes) and halves (steps)
+struct Int4Pages {
+  uint8_t* codes;
+  uint16_t* steps;
+  long c_sp, c_sr, c_sh, s_sp, s_sr, s_sh;
+};
+struct Int4Append {
+  const void *q, *k, *v;
+  const long* positions;
+  const int* slots;
+  const float *cos_t, *sin_t;
+  void* q_out;
+  int* lost;
+  Int4Pages kp, vp;
+  int B, W, H, Hkv, D, half, rows, ps, parts;              // half: pairs that turn; rows: of the rotation tables; parts: blocks of a token
+  long tokens;                                             // of the pool
+  bool pairs;
+  long q_sb, q_sw, q_sh, k_sb, k_sw, k_sh, v_sb, v_sw, v_sh, o_sb, o_sw;
+};
+void int4_append(Int4Append p, int dt, cudaStream_t st);
+void int4_gather(const Int4Pages& kp, const Int4Pages& vp, const int* slots, void* k, void* v, long n, int Hkv, int D, int ps, long tokens, int dt, cudaStream_t st);
+struct Int4Attn : PagedAttn {        // k, v: codes, their strides in bytes
+  const void *ks, *vs;               // steps, strides in halves
+  long ks_sp, ks_sr, ks_sh, vs_sp, vs_sr, vs_sh;
+};
+PagedPlan int4_plan(Int4Attn& p);    // fills in p's cuts
+int int4_attention(const Int4Attn& p, const PagedPlan& plan, int D, int dt, cudaStream_t st);          // → launches
+
 // ---- drafted tokens against the target's probabilities (verify.cu); strides of rows in elements, dt of both sides
 void verify_drafts(const long* tokens, const void* draft, const void* target, const float* accept, const float* sample, long* out, long* accepted,
                    int B, int K, int V, const long* draft_s, const long* target_s, int dt, cudaStream_t st);

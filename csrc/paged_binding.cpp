@@ -1,43 +1,10 @@
 // Bindings of the paged key/value cache and of the verification of drafted tokens: checks of arguments, workspaces, launches.
-#include <ATen/cuda/CUDAContext.h>
-#include <c10/cuda/CUDAGuard.h>
-#include <torch/extension.h>
-
 #include <atomic>
 #include <cmath>
-#include <string>
 
-#include "bindings.h"
-#include "kernels.h"
+#include "paged_checks.h"
 
 namespace {
-
-// Messages are put together as plain strings: c10's own, which goes by a stream as soon as it has more than one part, ends the process here.
-#define CHECK_ARG(cond, msg) TORCH_CHECK_VALUE(cond, std::string(msg))
-
-std::string list(at::IntArrayRef sizes) {
-  std::string s = "[";
-  for (size_t i = 0; i < sizes.size(); ++i) s += (i ? ", " : "") + std::to_string(sizes[i]);
-  return s + "]";
-}
-
-int dt_code(const Tensor& t) { return t.scalar_type() == at::kFloat ? nxd::kF32 : t.scalar_type() == at::kBFloat16 ? nxd::kBF16 : nxd::kF16; }
-bool half_type(const Tensor& t) { return t.scalar_type() == at::kBFloat16 || t.scalar_type() == at::kHalf; }
-cudaStream_t stream() { return at::cuda::getCurrentCUDAStream().stream(); }
-
-// Last dimension contiguous, everything else whole 16-byte packets apart, and so the address
-bool packets(const Tensor& t) {
-  const int64_t per = 16 / t.element_size();
-  bool ok = t.stride(-1) == 1 && (uintptr_t)t.data_ptr() % 16 == 0 && t.size(-1) % per == 0;
-  for (int64_t d = 0; d + 1 < t.dim(); ++d) ok = ok && (t.size(d) <= 1 || t.stride(d) % per == 0);
-  return ok;
-}
-Tensor as_packets(const Tensor& t) { return packets(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
-
-void check_ints(const Tensor& t, const char* name, at::ScalarType type, int64_t n, const Tensor& like) {
-  CHECK_ARG(t.scalar_type() == type && t.dim() == 1 && t.size(0) == n && t.is_contiguous() && t.device() == like.device(),
-            std::string(name) + " must be a contiguous " + c10::toString(type) + " tensor of " + std::to_string(n) + " numbers on the queries' device");
-}
 
 // q [B, W, H, D], caches [pages, page_size, Hkv, D], table [B, cols], positions [B], lens [B] or none
 void check_cache(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tensor& table, const Tensor& positions, const c10::optional<Tensor>& lens) {
@@ -56,13 +23,6 @@ void check_cache(const Tensor& q, const Tensor& kc, const Tensor& vc, const Tens
   CHECK_ARG(q.size(0) < (1 << 20) && q.size(1) < (1 << 24) && q.size(0) * q.size(1) * q.size(2) < (1ll << 30), "too many query rows: " + list(q.sizes()));
 }
 
-// Numbers of another type, or not one after the other, are converted
-Tensor ints(const Tensor& t, at::ScalarType type) { return t.scalar_type() == type && t.is_contiguous() ? t : t.to(type).contiguous(); }
-c10::optional<Tensor> ints(const c10::optional<Tensor>& t, at::ScalarType type) { return t.has_value() ? c10::optional<Tensor>(ints(*t, type)) : t; }
-Tensor as_table(const Tensor& t) {
-  return t.scalar_type() == at::kInt && (t.dim() != 2 || t.size(1) <= 1 || t.stride(1) == 1) ? t : t.to(at::kInt).contiguous();
-}
-
 // Whether the append kernel takes these: 32- or 16-bit types, halves of heads and cache rows of whole 16-byte packets
 bool paged_append_ok(const Tensor& q, const Tensor& kc, const Tensor& vc) {
   return q.dim() == 4 && kc.dim() == 4 && vc.dim() == 4 && (half_type(q) || q.scalar_type() == at::kFloat) &&
@@ -71,12 +31,6 @@ bool paged_append_ok(const Tensor& q, const Tensor& kc, const Tensor& vc) {
 // Whether the attention kernels take these: 16-bit types, heads of 64 or 128 numbers, cache rows of whole 16-byte packets
 bool paged_attention_ok(const Tensor& q, const Tensor& kc, const Tensor& vc) {
   return q.dim() == 4 && kc.dim() == 4 && vc.dim() == 4 && half_type(q) && (q.size(3) == 64 || q.size(3) == 128) && packets(kc) && packets(vc);
-}
-
-// [B, W, H, D] with tokens first in memory, as the layers around take and leave it
-Tensor rows_out(const Tensor& q) {
-  const int64_t B = q.size(0), W = q.size(1), H = q.size(2), D = q.size(3);
-  return at::empty_strided({B, W, H, D}, {H * D, B * H * D, D, 1}, q.options());
 }
 
 // None: not for the kernel
