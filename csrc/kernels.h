@@ -274,8 +274,8 @@ struct Int4Append {
 };
 void int4_append(Int4Append p, int dt, cudaStream_t st);
 void int4_gather(const Int4Pages& kp, const Int4Pages& vp, const int* slots, void* k, void* v, long n, int Hkv, int D, int ps, long tokens, int dt, cudaStream_t st);
-struct Int4Attn : PagedAttn {        // k, v: codes, their strides in bytes
-  const void *ks, *vs;               // steps, strides in halves
+struct Int4Attn : PagedAttn {        // k, v: codes, their strides in units of 16 bytes, those of a pool's pages and rows together below 2^32
+  const void *ks, *vs;               // steps, strides in rows of them (D / 8 bytes), below 2^32 alike
   long ks_sp, ks_sr, ks_sh, vs_sp, vs_sr, vs_sh;
 };
 PagedPlan int4_plan(Int4Attn& p);    // fills in p's cuts

@@ -465,6 +465,31 @@ __global__ void __launch_bounds__(kThreads, 2) paged_rows_kernel(const PagedAttn
   if (late) pdl_wait();
 }
 
+// Pairs that are cut: block (c − 1, ·) has the one that is cut first in front of block c's share, and a warp of it joins the parts of ROWS rows at a time.
+template <typename T, int D, int ROWS>
+__global__ void __launch_bounds__(kThreads) paged_merge_kernel(const PagedAttn p, int grid) {
+  const int block = blockIdx.x + 1;
+  const Place at = find_place<kThreads, false>(p, grid, block);        // the kernel before this one waited for all that positions come from
+  pdl_trigger();
+  pdl_wait();
+  if (at.e >= p.B * p.row_tiles) return;
+  const int tiles = entry_tiles(p, at.e), head = (int)(at.tile / tiles);
+  const long off = at.tile % tiles, t0 = block * at.per - off;
+  if (off == 0 || off > at.per || whole<false>(p, tiles)) return;      // not cut here, or before, or not at all
+  const int b = at.e / p.row_tiles, n = (int)((t0 + tiles - 1) / at.per) - (block - 1) + 1;
+  const int row0 = at.e % p.row_tiles * p.tile_rows, rows = min(p.tile_rows, p.W * p.G - row0), m = new_tokens(p, b);
+  for (int r0 = (blockIdx.y * kWarps + (threadIdx.x >> 5)) * ROWS; r0 < rows; r0 += gridDim.y * kWarps * ROWS) {
+    bool live[ROWS];
+#pragma unroll
+    for (int r = 0; r < ROWS; ++r) live[r] = r0 + r < rows && (row0 + r0 + r) / p.G < m;
+    join_parts<T, D, ROWS>(p, n, live, [&](int x, int r) { return part_slot<false>(p, 0, block - 1 + x, x == 0) * p.tile_rows + r0 + r; },
+                           [&](int r) {
+                             const int row = row0 + r0 + r, w = row / p.G;
+                             return r0 + r < rows ? reinterpret_cast<T*>(p.out) + b * p.o_sb + w * p.o_sw + (long)(head * p.G + row % p.G) * p.o_sh : nullptr;
+                           });
+  }
+}
+
 // With shared pages: every row's parts over the shared pages and over its own.  Block (entry, ·), a warp per row and key/value head.
 template <typename T, int D>
 __global__ void __launch_bounds__(kThreads) paged_join_kernel(const PagedAttn p, int grid) {

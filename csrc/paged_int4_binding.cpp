@@ -1,4 +1,5 @@
 // Bindings of the paged key/value cache in 4 bits and of the page tables: checks of arguments, workspaces, launches.
+#include <array>
 #include <cmath>
 #include <limits>
 
@@ -162,10 +163,13 @@ c10::optional<Tensor> int4_attention(const Tensor& q_, const Tensor& kc, const T
   p.q_sb = q.stride(0); p.q_sw = q.stride(1); p.q_sh = q.stride(2);
   p.o_sb = out.stride(0); p.o_sw = out.stride(1); p.o_sh = out.stride(2);
   p.table_sb = table.stride(0);
-  p.k_sp = kc.stride(0); p.k_sr = kc.stride(1); p.k_sh = kc.stride(2);
-  p.v_sp = vc.stride(0); p.v_sr = vc.stride(1); p.v_sh = vc.stride(2);
-  p.ks_sp = ks.stride(0); p.ks_sr = ks.stride(1); p.ks_sh = ks.stride(2);
-  p.vs_sp = vs.stride(0); p.vs_sr = vs.stride(1); p.vs_sh = vs.stride(2);
+  const int64_t row = D / 16;                       // halves of a token's steps
+  p.k_sp = kc.stride(0) / 16; p.k_sr = kc.stride(1) / 16; p.k_sh = kc.stride(2) / 16;
+  p.v_sp = vc.stride(0) / 16; p.v_sr = vc.stride(1) / 16; p.v_sh = vc.stride(2) / 16;
+  p.ks_sp = ks.stride(0) / row; p.ks_sr = ks.stride(1) / row; p.ks_sh = ks.stride(2) / row;
+  p.vs_sp = vs.stride(0) / row; p.vs_sr = vs.stride(1) / row; p.vs_sh = vs.stride(2) / row;
+  for (const auto& s : {std::array<long, 2>{p.k_sp, p.k_sr}, {p.v_sp, p.v_sr}, {p.ks_sp, p.ks_sr}, {p.vs_sp, p.vs_sr}})
+    CHECK_ARG(s[0] >= 0 && s[1] >= 0 && (kc.size(0) - 1) * s[0] + (ps - 1) * s[1] < (1ll << 32) - 1, "pages that span more than 64 GB");
   const nxd::PagedPlan plan = nxd::int4_plan(p);
   Tensor work;                                     // parts of pairs that are cut: sums and statistics
   if (plan.slots > 0) work = at::empty({plan.slots * (D + 2)}, q.options().dtype(at::kFloat));

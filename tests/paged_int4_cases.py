@@ -76,12 +76,11 @@ def attention(d, scale=None):
 
 
 def bound(dtype, out, size):
-    """A half step of the result's own rounding; with 16-bit floats of 8 bits, a half step of half precision (2^-11) for each weight and one for its product
-    with s, with half precision what two halves leave of either (2^-22 each); and what sums, products and exponentials in 32 bits leave: scores are sums of up to
-    128 products, in parts of magnitude 64 at most, off by 128 * 2^-24 * 64 < 2^-11 of them, of which the tests' random signs leave less than a quarter."""
+    """A half step of the result's own rounding; with 16-bit floats a half step of half precision (2^-11) for each weight and one for each value, which are made
+    halves before their product; and what sums, products and exponentials in 32 bits leave: scores are sums of up to 128 products, in parts of magnitude 64 at
+    most, off by 128 * 2^-24 * 64 < 2^-11 of them, of which the tests' random signs leave less than a quarter."""
     u = torch.finfo(dtype).eps / 2
-    weights = {torch.bfloat16: 2 * 2.0 ** -11, torch.float16: 2 * 2.0 ** -22}.get(dtype, 0.0)
-    return u * out.abs() + (weights + 2.0 ** -13) * size + 1e-7
+    return u * out.abs() + ((2 * 2.0 ** -11 if dtype.itemsize == 2 else 0.0) + 2.0 ** -13) * size + 1e-7
 
 
 def rotate(x, position, cos, sin, interleaved):
