@@ -224,6 +224,8 @@ struct PagedAttn {
   long k_sp, k_sr, k_sh, v_sp, v_sr, v_sh;        // strides of pages, rows in a page, heads
   float scale_log2;
   int wait_ns;                       // after which a wait in the tile kernel gives up; negative: after so many, and no keys are loaded (tests)
+  const float* units;                // tiles: what the scores of a query row are multiplied by, beside the scale, or null: 1
+  long u_sb, u_sw;                   // their strides of sequences and tokens
 };
 // How a launch is dealt out (rows: few, the kernel of paged.cu, or tiles of 64, 128 or 256, paged_attention_sm100.cu); workspaces follow from it
 struct PagedPlan {
@@ -233,7 +235,9 @@ struct PagedPlan {
 };
 PagedPlan paged_plan(PagedAttn& p);  // fills in p's cuts
 int paged_attention(const PagedAttn& p, const PagedPlan& plan, int D, int dt, cudaStream_t st);        // → launches
-void paged_tiles(const PagedAttn& p, int grid, bool over_shared, int D, int dt, cudaStream_t st);       // paged_attention_sm100.cu
+// dt: of queries and caches; out_dt: of what comes out, another one (bf16 of half) only without shared pages (paged_attention_sm100.cu)
+void paged_tiles(const PagedAttn& p, int grid, bool over_shared, int D, int dt, int out_dt, cudaStream_t st);
+int paged_attention_half(const PagedAttn& p, const PagedPlan& plan, int D, int out_dt, cudaStream_t st);      // tiles of half precision, no shared pages
 // strides s: (b, w, h) of q, k, v; cs: (page, row, head) of the caches; q_out: heads and columns contiguous; lost: becomes 1 where a
 // token that counts was not written, or null
 void paged_append(const void* q, const void* k, const void* v, const long* positions, const long* lens, const float* cos_t, const float* sin_t,
@@ -278,8 +282,11 @@ struct Int4Attn : PagedAttn {        // k, v: codes, their strides in units of 1
   const void *ks, *vs;               // steps, strides in rows of them (D / 8 bytes), below 2^32 alike
   long ks_sp, ks_sr, ks_sh, vs_sp, vs_sr, vs_sh;
 };
-PagedPlan int4_plan(Int4Attn& p);    // fills in p's cuts
+PagedPlan int4_plan(Int4Attn& p);    // fills in p's cuts; tiles: the pages are better unpacked
 int int4_attention(const Int4Attn& p, const PagedPlan& plan, int D, int dt, cudaStream_t st);          // → launches
+// The pages of p's sequences as half-precision numbers that `to` reads: k, v [p.B * p.cols][Hkv][ps][D], a table of them, and queries of halves with their units
+void int4_unpack(const Int4Attn& p, void* k, void* v, int* table, int D, cudaStream_t st);
+void int4_queries(const void* q, void* out, float* units, int B, int W, int H, int D, long q_sb, long q_sw, long q_sh, cudaStream_t st);
 
 // ---- drafted tokens against the target's probabilities (verify.cu); strides of rows in elements, dt of both sides
 void verify_drafts(const long* tokens, const void* draft, const void* target, const float* accept, const float* sample, long* out, long* accepted,

@@ -550,16 +550,17 @@ void launch_rows(const PagedAttn& p, int grid, cudaStream_t st) {
   cfg.attrs = attr; cfg.numAttrs = 2;
   NXD_CUDA_CHECK(cudaLaunchKernelEx(&cfg, paged_rows_kernel<T, D, R, DEAL>, p));
 }
+// T: of what comes out; dt: of queries and caches
 template <typename T, int D>
-int launch(const PagedAttn& p, const PagedPlan& plan, int dt, cudaStream_t st) {
+int launch(const PagedAttn& p, const PagedPlan& plan, int dt, int out_dt, cudaStream_t st) {
   if (p.shared) {
-    if (plan.pre_tiles) paged_tiles(p, plan.pre_grid, true, D, dt, st);
+    if (plan.pre_tiles) paged_tiles(p, plan.pre_grid, true, D, dt, out_dt, st);
     else if (p.pre_tile_rows == 8) launch_rows<T, D, 1, kShared>(p, plan.pre_grid, st);
     else launch_rows<T, D, 2, kShared>(p, plan.pre_grid, st);
   }
   if (p.cluster && p.tile_rows == 8) launch_rows<T, D, 1, kCluster>(p, plan.grid, st);
   else if (p.cluster) launch_rows<T, D, 2, kCluster>(p, plan.grid, st);
-  else if (plan.tiles) paged_tiles(p, plan.grid, false, D, dt, st);
+  else if (plan.tiles) paged_tiles(p, plan.grid, false, D, dt, out_dt, st);
   else if (p.tile_rows == 8) launch_rows<T, D, 1, kDealt>(p, plan.grid, st);
   else launch_rows<T, D, 2, kDealt>(p, plan.grid, st);
   const int rows = std::min(p.tile_rows, p.W * p.G);
@@ -643,8 +644,14 @@ PagedPlan paged_plan(PagedAttn& p) {
 }
 
 int paged_attention(const PagedAttn& p, const PagedPlan& plan, int D, int dt, cudaStream_t st) {
-  if (dt == kBF16) return D == 128 ? launch<__nv_bfloat16, 128>(p, plan, dt, st) : launch<__nv_bfloat16, 64>(p, plan, dt, st);
-  return D == 128 ? launch<__half, 128>(p, plan, dt, st) : launch<__half, 64>(p, plan, dt, st);
+  if (dt == kBF16) return D == 128 ? launch<__nv_bfloat16, 128>(p, plan, dt, dt, st) : launch<__nv_bfloat16, 64>(p, plan, dt, dt, st);
+  return D == 128 ? launch<__half, 128>(p, plan, dt, dt, st) : launch<__half, 64>(p, plan, dt, dt, st);
+}
+
+int paged_attention_half(const PagedAttn& p, const PagedPlan& plan, int D, int out_dt, cudaStream_t st) {
+  if (!plan.tiles || p.shared) nxd_throw("paged_attention_half: not for tiles", __FILE__, __LINE__);
+  if (out_dt == kBF16) return D == 128 ? launch<__nv_bfloat16, 128>(p, plan, kF16, out_dt, st) : launch<__nv_bfloat16, 64>(p, plan, kF16, out_dt, st);
+  return D == 128 ? launch<__half, 128>(p, plan, kF16, out_dt, st) : launch<__half, 64>(p, plan, kF16, out_dt, st);
 }
 
 void paged_append(const void* q, const void* k, const void* v, const long* positions, const long* lens, const float* cos_t, const float* sin_t,

@@ -159,7 +159,8 @@ NXD_DEVICE long begin_share(const PagedAttn& p, const Place& at, Walk& w) {
 // PAIR: a step of two row tiles and 128 keys takes 2.2 us: exponentials 1.05, products 1.05 (heads of 128 numbers), which overlap little.  2 x 1000 tokens (a
 // quarter padding) behind 6000 keys, 48 heads of 64 on 8: 158 us, 470 TFLOP/s.  Otherwise: two tiles of 64 keys in 1.7 us, 5 TB/s over the GPU; windows of 5
 // tokens of 8 sequences to 6000 keys, 64 heads on 8: 43 us, of which 7 are the start and 5 the launch that joins parts.
-template <typename T, int D, bool PAIR, int ROWS, bool SHARED>
+// O: of what comes out, T or another 16-bit type.
+template <typename T, int D, bool PAIR, int ROWS, bool SHARED, typename O>
 __global__ void __launch_bounds__(kRowsThreads, 1)
 paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const PagedAttn p, int box) {
   using C = Cut<D, PAIR, ROWS>;
@@ -424,7 +425,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
           const bool live = row_token(it, row, b, t);
           if (!SHARED && p.shared == 0 && it.ends == 3) {
             const uint32_t x = live ? 0x7fff7fffu : 0u;
-            T* const to = reinterpret_cast<T*>(p.out) + b * p.o_sb + t * p.o_sw + (long)(it.head * p.G + row % p.G) * p.o_sh;
+            O* const to = reinterpret_cast<O*>(p.out) + b * p.o_sb + t * p.o_sw + (long)(it.head * p.G + row % p.G) * p.o_sh;
             if (row < all_rows)
               for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(to + c) = make_uint4(x, x, x, x);
           } else if (live) {
@@ -537,8 +538,8 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                 for (int v = 0; v < 4; ++v) {
                   uint32_t o[4];
 #pragma unroll
-                  for (int i = 0; i < 4; ++i) o[i] = pack16<T>(__uint_as_float(r[v * 8 + 2 * i]), __uint_as_float(r[v * 8 + 2 * i + 1]));
-                  *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + to + c * COLS + v * 8) = make_uint4(o[0], o[1], o[2], o[3]);
+                  for (int i = 0; i < 4; ++i) o[i] = pack16<O>(__uint_as_float(r[v * 8 + 2 * i]), __uint_as_float(r[v * 8 + 2 * i + 1]));
+                  *reinterpret_cast<uint4*>(reinterpret_cast<O*>(p.out) + to + c * COLS + v * 8) = make_uint4(o[0], o[1], o[2], o[3]);
                 }
               } else if (to >= 0) {
                 uint4* dst = reinterpret_cast<uint4*>((SHARED ? p.pre_o : p.part_o) + to + c * COLS);
@@ -553,7 +554,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
               for (int v = 0; v < 4; ++v) {
                 uint32_t o[4];
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[i] = pack16<T>(__uint_as_float(r[v * 8 + 2 * i]), __uint_as_float(r[v * 8 + 2 * i + 1]));
+                for (int i = 0; i < 4; ++i) o[i] = pack16<O>(__uint_as_float(r[v * 8 + 2 * i]), __uint_as_float(r[v * 8 + 2 * i + 1]));
                 asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(stage + lane * 64 + ((v ^ ((lane >> 1) & 3)) << 4)), "r"(o[0]), "r"(o[1]), "r"(o[2]),
                              "r"(o[3]) : "memory");
               }
@@ -565,7 +566,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
                 asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(o.x), "=r"(o.y), "=r"(o.z), "=r"(o.w)
                              : "r"(stage + rr * 64 + (((lane & 3) ^ ((rr >> 1) & 3)) << 4)) : "memory");
                 const long dst = __shfl_sync(0xffffffffu, to, rr);
-                if (dst >= 0) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + dst + c * COLS + (lane & 3) * 8) = o;
+                if (dst >= 0) *reinterpret_cast<uint4*>(reinterpret_cast<O*>(p.out) + dst + c * COLS + (lane & 3) * 8) = o;
               }
             } else {
 #pragma unroll
@@ -585,12 +586,12 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
             }
           }
         } else if (direct && to >= 0) {                      // rows that do not count
-          for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + to + c) = make_uint4(0, 0, 0, 0);
+          for (int c = 0; c < D; c += 8) *reinterpret_cast<uint4*>(reinterpret_cast<O*>(p.out) + to + c) = make_uint4(0, 0, 0, 0);
         }
       }
       it = nx;
     }
-    if (!SHARED && p.shared == 0) finish_idle<T, D, 128>(p, threadIdx.x - 256);
+    if (!SHARED && p.shared == 0) finish_idle<O, D, 128>(p, threadIdx.x - 256);
     asm volatile("bar.arrive 2, 224;" ::: "memory");       // warp 15 waits for this
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 168;");
@@ -600,8 +601,6 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     const uint32_t tS = tmem_S + t * 128 + lane_base, tO = tmem_O + t * 128 + lane_base;
     const uint32_t my_s = bar_s + 8 * t, my_p = bar_p + 8 * t;
     constexpr int Q = KEYS / 32;
-    const float sl2 = p.scale_log2;
-    const uint64_t sl2_2 = pack2(sl2, sl2);
     int g = 0, items = 0, pos0 = 0, tile0 = 0;
     // A piece of one step in front of the first works on whatever there is and leaves nothing behind (its weights go over the sums, which the first
     // product does not add to): a step's 10 KB of instructions come from memory, a part by each warp, while the place is found and the first keys
@@ -617,6 +616,8 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         int b = 0, w = 0;
         const int row = first_row(it) + (PAIR ? t * kRows : 0) + own, n = SHARED ? shared_keys : it.keys;
         const bool live = !dry && row_token(it, row, b, w);
+        const float sl2 = live && p.units ? p.scale_log2 * p.units[b * p.u_sb + w * p.u_sw + it.head * p.G + row % p.G] : p.scale_log2;
+        const uint64_t sl2_2 = pack2(sl2, sl2);
         // keys that this row sees (one that does not count: all, whatever comes of it), and the fewest of the warp's rows
         const int sees = live ? min(visible_keys(p, b, w), n) : 0x7fffffff;
         const int sees_lo = __reduce_min_sync(0xffffffffu, sees);
@@ -731,7 +732,7 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
   if (warp == 13) tcgen05_dealloc(tmem_base, 512);
 }
 
-template <typename T, int D, bool PAIR, int ROWS, bool SHARED>
+template <typename T, int D, bool PAIR, int ROWS, bool SHARED, typename O>
 void launch_tiles(const PagedAttn& p, int grid, cudaStream_t st) {
   using C = Cut<D, PAIR, ROWS>;
   // boxes of the largest power of two that divides a page
@@ -742,22 +743,23 @@ void launch_tiles(const PagedAttn& p, int grid, cudaStream_t st) {
   const uint64_t ks[3] = {step(p.k_sr, p.ps), step(p.k_sh, p.Hkv), step(p.k_sp, p.pages)}, vs[3] = {step(p.v_sr, p.ps), step(p.v_sh, p.Hkv), step(p.v_sp, p.pages)};
   const CUtensorMap tk = make_tmap_bf16_heads(p.k, dims, ks, 64, box), tv = make_tmap_bf16_heads(p.v, dims, vs, 64, box);
   constexpr uint32_t smem = C::SMEM;
-  NXD_ALLOW_SMEM((paged_tiles_kernel<T, D, PAIR, ROWS, SHARED>), smem);
-  launch_dependent(paged_tiles_kernel<T, D, PAIR, ROWS, SHARED>, grid, kRowsThreads, smem, st, tk, tv, p, box);
+  NXD_ALLOW_SMEM((paged_tiles_kernel<T, D, PAIR, ROWS, SHARED, O>), smem);
+  launch_dependent(paged_tiles_kernel<T, D, PAIR, ROWS, SHARED, O>, grid, kRowsThreads, smem, st, tk, tv, p, box);
 }
-template <typename T, int D, bool SHARED>
+template <typename T, int D, bool SHARED, typename O>
 void launch_rows(const PagedAttn& p, int rows, int grid, cudaStream_t st) {
-  if (rows == 64) launch_tiles<T, D, false, 64, SHARED>(p, grid, st);
-  else if (rows == kRows) launch_tiles<T, D, false, kRows, SHARED>(p, grid, st);
-  else launch_tiles<T, D, true, kRows, SHARED>(p, grid, st);
+  if (rows == 64) launch_tiles<T, D, false, 64, SHARED, O>(p, grid, st);
+  else if (rows == kRows) launch_tiles<T, D, false, kRows, SHARED, O>(p, grid, st);
+  else launch_tiles<T, D, true, kRows, SHARED, O>(p, grid, st);
 }
 
 }  // namespace
 
-void paged_tiles(const PagedAttn& p, int grid, bool over_shared, int D, int dt, cudaStream_t st) {
+void paged_tiles(const PagedAttn& p, int grid, bool over_shared, int D, int dt, int out_dt, cudaStream_t st) {
   const int rows = over_shared ? p.pre_tile_rows : p.tile_rows;
-#define NXD_TILES(T, Dv) do { if (over_shared) launch_rows<T, Dv, true>(p, rows, grid, st); else launch_rows<T, Dv, false>(p, rows, grid, st); } while (0)
-  if (dt == kBF16) { if (D == 128) NXD_TILES(__nv_bfloat16, 128); else NXD_TILES(__nv_bfloat16, 64); }
+#define NXD_TILES(T, Dv) do { if (over_shared) launch_rows<T, Dv, true, T>(p, rows, grid, st); else launch_rows<T, Dv, false, T>(p, rows, grid, st); } while (0)
+  if (dt != out_dt) { if (D == 128) launch_rows<__half, 128, false, __nv_bfloat16>(p, rows, grid, st); else launch_rows<__half, 64, false, __nv_bfloat16>(p, rows, grid, st); }
+  else if (dt == kBF16) { if (D == 128) NXD_TILES(__nv_bfloat16, 128); else NXD_TILES(__nv_bfloat16, 64); }
   else { if (D == 128) NXD_TILES(__half, 128); else NXD_TILES(__half, 64); }
 #undef NXD_TILES
 }

@@ -171,6 +171,81 @@ __global__ void __launch_bounds__(kGatherThreads) int4_gather_kernel(const Int4P
   out.store((key ? k : v) + i * 8);
 }
 
+// ----------------------------------------------------------------------------------------------- numbers for portions of prompts
+constexpr int kUnpackThreads = 128, kUnpackEach = 4;       // packets of a thread at a time
+// Pages of all sequences as halves, for the attention of many rows (paged_attention_sm100.cu), which the unpacked numbers serve many times: m + s c rounded
+// once.  Block (column of a sequence, head, keys or values), a thread 16 bytes at a time.  Keys that nobody sees are left as they are.  Bound by the start of its many
+// small blocks: 2 sequences of 6000 keys, 8 heads of 64, 10 us, 25 MB written (16 numbers a thread: 12).
+template <int D>
+__global__ void __launch_bounds__(kUnpackThreads) int4_unpack_kernel(const Int4Attn p, __half* k, __half* v, int* table) {
+  constexpr int C = D / 8;
+  pdl_trigger();
+  pdl_wait();
+  const int b = blockIdx.x / p.cols, col = blockIdx.x % p.cols, head = blockIdx.y;
+  const bool key = blockIdx.z == 0;
+  int page = col < p.shared_cols ? p.shared_pages[col] : p.table[b * p.table_sb + col];
+  if ((unsigned)page >= (unsigned)p.pages) page = -1;
+  if (head == 0 && key && threadIdx.x == 0) table[blockIdx.x] = page < 0 ? -1 : blockIdx.x;
+  const int items = page < 0 ? 0 : min(p.ps, all_keys(p, b) - col * p.ps) * C;
+  const uint8_t* const codes = key ? reinterpret_cast<const uint8_t*>(p.k) + (page * p.k_sp + head * p.k_sh) * 16 : reinterpret_cast<const uint8_t*>(p.v) + (page * p.v_sp + head * p.v_sh) * 16;
+  const __half* const steps = key ? reinterpret_cast<const __half*>(p.ks) + (page * p.ks_sp + head * p.ks_sh) * (D / 16) : reinterpret_cast<const __half*>(p.vs) + (page * p.vs_sp + head * p.vs_sh) * (D / 16);
+  const long c_sr = (key ? p.k_sr : p.v_sr) * 16, s_sr = (key ? p.ks_sr : p.vs_sr) * (D / 16);
+  __half* const to = (key ? k : v) + ((long)blockIdx.x * p.Hkv + head) * p.ps * D;
+  for (int i0 = threadIdx.x; i0 < items; i0 += kUnpackThreads * kUnpackEach) {
+    uint32_t word[kUnpackEach];
+    __half s[kUnpackEach], m[kUnpackEach];
+#pragma unroll
+    for (int y = 0; y < kUnpackEach; ++y) {
+      const int i = i0 + y * kUnpackThreads, row = i / C, c = i % C;
+      if (i < items) {
+        word[y] = *reinterpret_cast<const uint32_t*>(codes + row * c_sr + c * 4);
+        s[y] = steps[row * s_sr + c / 4];
+        m[y] = steps[row * s_sr + D / 32 + c / 4];
+      }
+    }
+#pragma unroll
+    for (int y = 0; y < kUnpackEach; ++y) {
+      const int i = i0 + y * kUnpackThreads;
+      if (i >= items) break;
+      const __half2 s2 = __half2half2(s[y]), m2 = __half2half2(m[y]);
+      uint32_t o[4];
+#pragma unroll
+      for (int x = 0; x < 4; ++x) {
+        const uint32_t two = word[y] >> (8 * x);           // numbers 2 x and 2 x + 1
+        o[x] = as_u32(__hfma2(__hsub2(as_half2((two & 0xfu) | (two & 0xf0u) << 12 | 0x64006400u), __float2half2_rn(1024.f)), s2, m2));
+      }
+      *reinterpret_cast<uint4*>(to + (long)i * 8) = make_uint4(o[0], o[1], o[2], o[3]);
+    }
+  }
+}
+
+// Queries as halves: a row is multiplied by a power of two that brings its largest number to 2^14; the row's unit takes that back.  A thread has eight numbers.
+template <int D>
+__global__ void __launch_bounds__(128) int4_queries_kernel(const __nv_bfloat16* q, __half* out, float* units, unsigned rows, unsigned W, unsigned H, long q_sb, long q_sw,
+                                                           long q_sh) {
+  constexpr unsigned C = D / 8;
+  pdl_trigger();
+  pdl_wait();
+  const unsigned r = (blockIdx.x * 128 + threadIdx.x) / C, c = threadIdx.x % C;
+  const unsigned mask = (C == 16 ? 0xffffu : 0xffu) << (threadIdx.x % 32 / C * C);       // a row's threads
+  if (r >= rows) return;
+  const unsigned h = r % H, t = r / H, w = t % W, b = t / W;
+  Eight<__nv_bfloat16> x;
+  x.load(q + b * q_sb + w * q_sw + h * q_sh + c * 8);
+  float most = 0.f;
+#pragma unroll
+  for (int k = 0; k < 8; ++k) most = fmaxf(most, fabsf(x.f(k)));
+#pragma unroll
+  for (int k = 1; k < (int)C; k <<= 1) most = fmaxf(most, __shfl_xor_sync(mask, most, k));
+  const int e = min(max((int)(__float_as_uint(most) >> 23), 20), 244);
+  const float up = __uint_as_float((uint32_t)(268 - e) << 23);
+  uint32_t o[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) o[k] = pack_half(x.f(2 * k) * up, x.f(2 * k + 1) * up);
+  reinterpret_cast<uint4*>(out)[(size_t)r * C + c] = make_uint4(o[0], o[1], o[2], o[3]);
+  if (c == 0) units[r] = __uint_as_float((uint32_t)(e - 14) << 23);
+}
+
 // ------------------------------------------------------------------------------------------------------- attention, up to eight rows
 constexpr int kRowWarps = 8;                               // two blocks an SM; the warps have a pair's keys in turn
 template <int D> constexpr int kRing = kRowWarps * kStages * kStage<D>;
@@ -647,16 +722,24 @@ PagedPlan int4_plan(Int4Attn& p) {
   p.row_tiles = rows <= 8 ? 1 : (int)((rows + 39) / 40);
   p.tile_rows = rows <= 8 ? 8 : std::max(16, (int)((rows + 8l * p.row_tiles - 1) / (8l * p.row_tiles)) * 8);
   p.row_tiles = (int)((rows + p.tile_rows - 1) / p.tile_rows);
-  const int each = 2;                                      // blocks of an SM
   p.tile_keys = 128;
   p.min_tiles = 1;
   p.whole_tiles = 0;
   p.shared = 0;
-  const long pairs = (long)p.B * p.row_tiles * p.Hkv, cap = (long)p.cols * p.ps;
+  const int each = 2;                                      // blocks of an SM
+  const long heads = (long)p.B * p.Hkv, pairs = heads * p.row_tiles, cap = (long)p.cols * p.ps;
+  // Every row tile reads and unpacks the keys for itself, 0.115 us for 1000 keys of a head over the GPU; unpacking them once to half precision for the tensor memory
+  // takes 0.19 us for 1000 and 18 us in all (us, row tiles / unpacked: 8 sequences to 6000 keys, 8 heads, 64 rows 81 / 93, 96 rows 134 / 96; 2 to 3000, 8
+  // heads, 128 rows 30 / 36, 256 rows 54 / 40; 1 to 1000, 40 heads, 200 rows 26 / 31; 2 x 1000 tokens to 6000, 48 heads of 64 on 8, 504 / 169).
+  plan.tiles = (23l * p.row_tiles - 38) * heads * cap > 3600000;
+  if (plan.tiles) return plan;
   plan.grid = each * sms;
+  // A cluster per pair, as many blocks in it as the GPU takes at once, has neither a search for places nor a second launch, but the longest sequence lasts as long as
+  // its own blocks take (us, dealt out / cluster: 1 sequence of 300 keys, 8 heads, 11.1 / 6.2; 16 to 8192 keys, 8 heads, 41.7 / 38.2; 6 to 2500, 40
+  // heads, 30.5 / 25.1; but 1 of 100000, 8 heads, 36.5 / 49.6): 4096 keys a block at most.
   int size = 1;
-  while (size < kCluster8 && ((cap > p.tile_keys * size && pairs * size * 2 <= (long)each * sms) || cap > 8192l * size)) size *= 2;
-  if (cap <= 8192l * size && pairs * size < (1l << 30)) {
+  while (size < kCluster8 && ((cap > 512l * size && pairs * size * 2 <= (long)each * sms) || cap > 4096l * size)) size *= 2;
+  if (cap <= 4096l * size && pairs * size < (1l << 30)) {
     p.cluster = size;
     plan.grid = (int)(pairs * size);
   }
@@ -668,6 +751,23 @@ PagedPlan int4_plan(Int4Attn& p) {
 int int4_attention(const Int4Attn& p, const PagedPlan& plan, int D, int dt, cudaStream_t st) {
   if (dt == kBF16) return D == 128 ? launch<__nv_bfloat16, 128>(p, plan, dt, st) : launch<__nv_bfloat16, 64>(p, plan, dt, st);
   return D == 128 ? launch<__half, 128>(p, plan, dt, st) : launch<__half, 64>(p, plan, dt, st);
+}
+
+void int4_unpack(const Int4Attn& p, void* k, void* v, int* table, int D, cudaStream_t st) {
+  const long blocks = (long)p.B * p.cols;
+  if (blocks == 0) return;
+  if (blocks >= (1l << 31) || p.Hkv > 65535) nxd_throw("int4_unpack: too many keys", __FILE__, __LINE__);
+  const dim3 grid((unsigned)blocks, p.Hkv, 2);
+  if (D == 128) launch_dependent(int4_unpack_kernel<128>, grid, kUnpackThreads, 0, st, p, (__half*)k, (__half*)v, table);
+  else launch_dependent(int4_unpack_kernel<64>, grid, kUnpackThreads, 0, st, p, (__half*)k, (__half*)v, table);
+}
+void int4_queries(const void* q, void* out, float* units, int B, int W, int H, int D, long q_sb, long q_sw, long q_sh, cudaStream_t st) {
+  const long rows = (long)B * W * H;
+  if (rows == 0) return;
+  if (rows * (D / 8) >= (1l << 31)) nxd_throw("int4_queries: too many rows", __FILE__, __LINE__);
+  const unsigned grid = (unsigned)((rows * (D / 8) + 127) / 128);
+  if (D == 128) launch_dependent(int4_queries_kernel<128>, grid, 128, 0, st, (const __nv_bfloat16*)q, (__half*)out, units, (unsigned)rows, W, H, q_sb, q_sw, q_sh);
+  else launch_dependent(int4_queries_kernel<64>, grid, 128, 0, st, (const __nv_bfloat16*)q, (__half*)out, units, (unsigned)rows, W, H, q_sb, q_sw, q_sh);
 }
 
 void int4_append(Int4Append p, int dt, cudaStream_t st) {

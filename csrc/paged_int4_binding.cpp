@@ -129,6 +129,56 @@ c10::optional<std::vector<Tensor>> int4_gather(const Tensor& kc, const Tensor& k
   return std::vector<Tensor>{k, v};
 }
 
+// Bytes of unpacked keys and values at a time: sequences, then key/value heads, in turns where there are more
+constexpr int64_t kUnpacked = 256ll << 20;
+
+// Many rows: their sequences' pages are unpacked to halves, which the attention on the tensor memory reads
+void attend_portion(const nxd::Int4Attn& p, const Tensor& q, const Tensor& out, int64_t D, const at::TensorOptions& on) {
+  const int64_t head = (int64_t)p.cols * p.ps * D * 4, each = std::max<int64_t>(head, 1) * p.Hkv;                   // bytes of a head, of a sequence
+  const int64_t seqs = std::min<int64_t>(p.B, std::max<int64_t>(1, kUnpacked / each));
+  const int64_t heads = std::min<int64_t>(p.Hkv, std::max<int64_t>(1, kUnpacked / std::max<int64_t>(head, 1)));
+  const bool bf16 = q.scalar_type() == at::kBFloat16;
+  Tensor q16 = q, units;
+  if (bf16) {
+    q16 = at::empty({p.B, p.W, (int64_t)p.G * p.Hkv, D}, q.options().dtype(at::kHalf));
+    units = at::empty({p.B, p.W, (int64_t)p.G * p.Hkv}, q.options().dtype(at::kFloat));
+    nxd::int4_queries(q.data_ptr(), q16.data_ptr(), units.data_ptr<float>(), p.B, p.W, p.G * p.Hkv, (int)D, p.q_sb, p.q_sw, p.q_sh, stream());
+    count_launches(1);
+  }
+  const int64_t pages = seqs * p.cols;
+  const Tensor k16 = at::empty({pages, heads, p.ps, D}, on.dtype(at::kHalf)), v16 = at::empty_like(k16), table = at::empty({seqs, p.cols}, on.dtype(at::kInt));
+  for (int64_t b = 0; b < p.B; b += seqs)
+    for (int64_t h = 0; h < p.Hkv; h += heads) {
+      nxd::Int4Attn from = p;
+      from.B = (int)std::min<int64_t>(seqs, p.B - b);
+      from.Hkv = (int)std::min<int64_t>(heads, p.Hkv - h);
+      from.positions = p.positions + b;
+      from.lens = p.lens ? p.lens + b : nullptr;
+      from.table = p.table + b * p.table_sb;
+      from.k = (const uint8_t*)p.k + h * p.k_sh * 16; from.v = (const uint8_t*)p.v + h * p.v_sh * 16;
+      from.ks = (const uint16_t*)p.ks + h * p.ks_sh * (D / 16); from.vs = (const uint16_t*)p.vs + h * p.vs_sh * (D / 16);
+      nxd::int4_unpack(from, k16.data_ptr(), v16.data_ptr(), table.data_ptr<int>(), (int)D, stream());
+      nxd::PagedAttn to = from;
+      to.q = (const uint16_t*)q16.data_ptr() + b * q16.stride(0) + h * p.G * q16.stride(2);
+      to.q_sb = q16.stride(0); to.q_sw = q16.stride(1); to.q_sh = q16.stride(2);
+      to.k = k16.data_ptr(); to.v = v16.data_ptr();
+      to.out = (uint16_t*)p.out + b * p.o_sb + h * p.G * p.o_sh;
+      to.table = table.data_ptr<int>(); to.table_sb = p.cols;
+      to.shared_pages = nullptr; to.shared_cols = 0;
+      to.pages = (int)pages;
+      to.k_sp = to.v_sp = heads * p.ps * D; to.k_sh = to.v_sh = p.ps * D; to.k_sr = to.v_sr = D;
+      to.units = bf16 ? units.data_ptr<float>() + b * units.stride(0) + h * p.G : nullptr;
+      to.u_sb = bf16 ? units.stride(0) : 0; to.u_sw = bf16 ? units.stride(1) : 0;
+      to.wait_ns = 2000000000;
+      const nxd::PagedPlan plan = nxd::paged_plan(to);
+      Tensor work;
+      if (plan.slots > 0) work = at::empty({plan.slots * (D + 2)}, on.dtype(at::kFloat));
+      to.part_o = to.pre_o = work.defined() ? work.data_ptr<float>() : nullptr;
+      to.part_ml = to.pre_ml = to.part_o + plan.slots * D;
+      count_launches(1 + nxd::paged_attention_half(to, plan, (int)D, bf16 ? nxd::kBF16 : nxd::kF16, stream()));
+    }
+}
+
 c10::optional<Tensor> int4_attention(const Tensor& q_, const Tensor& kc, const Tensor& ks, const Tensor& vc, const Tensor& vs, const Tensor& table_,
                                      const Tensor& positions_, const c10::optional<double>& scale_, const c10::optional<Tensor>& lens_,
                                      const c10::optional<Tensor>& shared_) {
@@ -170,12 +220,17 @@ c10::optional<Tensor> int4_attention(const Tensor& q_, const Tensor& kc, const T
   p.vs_sp = vs.stride(0) / row; p.vs_sr = vs.stride(1) / row; p.vs_sh = vs.stride(2) / row;
   for (const auto& s : {std::array<long, 2>{p.k_sp, p.k_sr}, {p.v_sp, p.v_sr}, {p.ks_sp, p.ks_sr}, {p.vs_sp, p.vs_sr}})
     CHECK_ARG(s[0] >= 0 && s[1] >= 0 && (kc.size(0) - 1) * s[0] + (ps - 1) * s[1] < (1ll << 32) - 1, "pages that span more than 64 GB");
+  p.scale_log2 = (float)(scale * 1.4426950408889634);
+  if (p.cols == 0) return out.zero_();               // nobody sees a key
   const nxd::PagedPlan plan = nxd::int4_plan(p);
+  if (plan.tiles) {
+    attend_portion(p, q, out, D, kc.options());
+    return out;
+  }
   Tensor work;                                     // parts of pairs that are cut: sums and statistics
   if (plan.slots > 0) work = at::empty({plan.slots * (D + 2)}, q.options().dtype(at::kFloat));
   p.part_o = work.defined() ? work.data_ptr<float>() : nullptr;
   p.part_ml = p.part_o + plan.slots * D;
-  p.scale_log2 = (float)(scale * 1.4426950408889634);
   count_launches(nxd::int4_attention(p, plan, (int)D, dt_code(q), stream()));
   return out;
 }

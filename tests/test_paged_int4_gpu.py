@@ -157,6 +157,7 @@ def test_append_outside_the_rotation_tables():
     (2, 3, 6, 2, 128, [600, 100], None),
     (3, 33, 4, 2, 64, [0, 17, 400], [33, 0, 20]),
     (2, 90, 3, 1, 16, [-1, 37], None),
+    (2, 300, 8, 2, 64, [500, 30], [300, 111]),             # enough for the tensor memory
     (1, 4, 4, 4, 16, [700], None),
 ])
 @pytest.mark.parametrize("layout", ["heads", "rows", "slice"])
