@@ -271,7 +271,7 @@ struct Int4Append {
   void* q_out;
   int* lost;
   Int4Pages kp, vp;
-  int B, W, H, Hkv, D, half, rows, ps, parts;              // half: pairs that turn; rows: of the rotation tables; parts: blocks of a token
+  int B, W, H, Hkv, D, half, rows, ps;                     // half: pairs that turn; rows: of the rotation tables
   long tokens;                                             // of the pool
   bool pairs;
   long q_sb, q_sw, q_sh, k_sb, k_sw, k_sh, v_sb, v_sw, v_sh, o_sb, o_sw;

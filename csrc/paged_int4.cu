@@ -17,6 +17,7 @@ using namespace int4;
 
 // ---------------------------------------------------------------------------------------------------------------- append
 constexpr int kAppendThreads = 128;
+constexpr long kSplitTokens = 2000;
 
 NXD_DEVICE float min_nan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
 NXD_DEVICE float max_nan(float a, float b) { float r; asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
@@ -36,139 +37,201 @@ template <typename T> struct Eight {                       // eight numbers besi
   NXD_DEVICE void set(int i, float x) { p[i / Pack16<T>::N].set(i % Pack16<T>::N, x); }
 };
 
-// A thread has eight numbers of one head, which lie beside one another, and reads the eight that turn with them where those lie elsewhere; four threads
-// have the 32 numbers that share m and s.  Bound by HBM.  Keys turn as a c - b s with what the rounding of b s left put back, one rounding in
-// all; a code whose quotient is nearer than 2^-15 to a border is found again from the products in 64 bits, so that codes are those of exact numbers.
-template <typename T>
-__global__ void __launch_bounds__(kAppendThreads) int4_append_kernel(const Int4Append p) {
+// How the numbers of a head turn: halves of the whole head, neighbours, or halves of a part of it
+enum Turn { kHalves, kPairs, kPart };
+
+// m and s of 32 numbers that four threads have, from the least and the largest of them, which are off by `off` at most; from exact ones where that leaves two halves
+template <typename F>
+NXD_DEVICE void steps_of(float lo, float hi, float off, unsigned four, F exact, __half& m16, __half& s16) {
+  constexpr float k15 = 1.f / 15.f;
+  m16 = __float2half_rn(lo + off);
+  const float range = hi - __half2float(m16);
+  s16 = __float2half_rn((range + off) * k15);
+  const bool doubt = __half_as_ushort(m16) != __half_as_ushort(__float2half_rn(lo - off)) || __half_as_ushort(s16) != __half_as_ushort(__float2half_rn((range - off) * k15));
+  if (doubt) {                                             // never where a NaN is: its halves are alike
+    double a = exact(0), b = a;
+#pragma unroll
+    for (int i = 1; i < 8; ++i) { const double x = exact(i); a = fmin(a, x); b = fmax(b, x); }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      a = fmin(a, __shfl_xor_sync(four, a, o));
+      b = fmax(b, __shfl_xor_sync(four, b, o));
+    }
+    m16 = __double2half(a);
+    s16 = __double2half((b - (double)__half2float(m16)) / 15.);
+  }
+}
+
+// A thread has CH times eight numbers of one head, half a head apart, so that with kHalves all that turns together is its own (kPart reads the eight that turn with
+// its own once more); four threads have the 32 numbers that share m and s.  Bound by HBM: 4 x 2000 tokens, 64 heads on 8, … .  Keys turn as a c - b s with what the
+// rounding of b s left put back, one rounding in all; a code whose quotient is near a border, and steps that are, are found again from the products in
+// 64 bits, so that codes are those of exact numbers.
+enum Role { kAll, kQueries0, kCache };                     // whose numbers a launch has: everybody's, queries', or keys' and values'
+template <typename T, int D0, Turn TURN, int CH, Role ROLE>
+__global__ void __launch_bounds__(kAppendThreads, ROLE == kQueries0 ? 12 : 8) int4_append_kernel(const Int4Append p) {
+  const int D = D0 ? D0 : p.D;
   pdl_trigger();
-  const unsigned t = blockIdx.x / p.parts, item = blockIdx.x % p.parts * kAppendThreads + threadIdx.x, chunks = p.D / 8;
-  const int h = (int)(item / chunks), c = (int)(item % chunks) * 8;
-  const int w = (int)(t / p.B), b = (int)(t % p.B);        // tokens of all sequences beside one another, as projections leave them
+  const unsigned t = blockIdx.x, item = blockIdx.y * kAppendThreads + threadIdx.x, chunks = D / (8 * CH);
+  const int h = (int)(item / chunks) + (ROLE == kCache ? p.H : 0), c0 = (int)(item % chunks) * 8;
+  const int w = (int)(t / (unsigned)p.B), b = (int)(t - (unsigned)w * p.B);        // tokens of all sequences beside one another, as projections leave them
   pdl_wait();
-  if (h >= p.H + 2 * p.Hkv) return;
+  if (h >= (ROLE == kQueries0 ? p.H : p.H + 2 * p.Hkv)) return;
+  const bool query = ROLE == kQueries0 || (ROLE == kAll && h < p.H), key = !query && h < p.H + p.Hkv;
+  const T* const src = query ? (const T*)p.q + b * p.q_sb + w * p.q_sw + h * p.q_sh
+                       : key ? (const T*)p.k + b * p.k_sb + w * p.k_sw + (h - p.H) * p.k_sh
+                             : (const T*)p.v + b * p.v_sb + w * p.v_sw + (h - p.H - p.Hkv) * p.v_sh;
+  Eight<T> x[CH], other[CH];                               // the numbers, and with kPart those that turn with them
+#pragma unroll
+  for (int j = 0; j < CH; ++j) x[j].load(src + c0 + j * (D / 2));       // whether the token counts or not: beside its slot and position
   const long slot = p.slots[(long)b * p.W + w], first = p.positions[b], pos = first + w;
   const bool has = slot >= 0 && slot < p.tokens, inside = first > -(1l << 40) && first < p.rows && pos >= 0 && pos < p.rows;
-  const bool live = has && inside, query = h < p.H, key = !query && h < p.H + p.Hkv;
+  const bool live = has && inside;
   if (!live) {
-    if (p.lost && item == 0 && has) *p.lost = 1;
+    if (ROLE != kCache && p.lost && item == 0 && has) *p.lost = 1;
     if (query) {
       Eight<T> zero;
 #pragma unroll
       for (int i = 0; i < 8; ++i) zero.set(i, 0.f);
-      zero.store((T*)p.q_out + b * p.o_sb + w * p.o_sw + (long)h * p.D + c);
+#pragma unroll
+      for (int j = 0; j < CH; ++j) zero.store((T*)p.q_out + b * p.o_sb + w * p.o_sw + (long)h * D + c0 + j * (D / 2));
     }
     return;
   }
-  const T* const src = query ? (const T*)p.q + b * p.q_sb + w * p.q_sw + h * p.q_sh
-                       : key ? (const T*)p.k + b * p.k_sb + w * p.k_sw + (h - p.H) * p.k_sh
-                             : (const T*)p.v + b * p.v_sb + w * p.v_sw + (h - p.H - p.Hkv) * p.v_sh;
-  Eight<T> mine, other;
-  mine.load(src + c);
-  // x = a co + b si, for each of the eight numbers: what turns with it, with the sine's sign
-  float x[8], co[8], si[8], turned[8];
-  const bool turns = (query || key) && c < 2 * p.half;
+  // y = x co + (what turns with it) si, the sine's sign taken where it is used: with kHalves both halves have the same angles
+  constexpr int ANGLES = TURN == kHalves ? 1 : CH;
+  float co[ANGLES][8], si[ANGLES][8];
+  bool turns[CH];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) { co[i] = 1.f; si[i] = 0.f; x[i] = mine.f(i); turned[i] = 0.f; }
-  if (turns && p.pairs) {
-    const float4 cv = *reinterpret_cast<const float4*>(p.cos_t + pos * p.half + c / 2), sv = *reinterpret_cast<const float4*>(p.sin_t + pos * p.half + c / 2);
-    const float cf[4] = {cv.x, cv.y, cv.z, cv.w}, sf[4] = {sv.x, sv.y, sv.z, sv.w};
+  for (int j = 0; j < CH; ++j) {
+    const int c = c0 + j * (D / 2);
+    turns[j] = (query || key) && (TURN == kHalves || c < 2 * p.half);
+    if (!turns[j] || j >= ANGLES) continue;
+    const int at = TURN == kPairs ? c / 2 : TURN == kHalves || c < p.half ? c : c - p.half;
+    if constexpr (TURN == kPart) other[j].load(src + (c < p.half ? c + p.half : at));
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      turned[i] = x[i ^ 1];
-      co[i] = cf[i / 2];
-      si[i] = i & 1 ? sf[i / 2] : -sf[i / 2];
-    }
-  } else if (turns) {
-    const bool low = c < p.half;
-    const int at = low ? c : c - p.half;
-    other.load(src + (low ? c + p.half : at));
-#pragma unroll
-    for (int i = 0; i < 8; i += 4) {
+    for (int i = 0; i < (TURN == kPairs ? 4 : 8); i += 4) {
       const float4 cv = *reinterpret_cast<const float4*>(p.cos_t + pos * p.half + at + i), sv = *reinterpret_cast<const float4*>(p.sin_t + pos * p.half + at + i);
-      const float cf[4] = {cv.x, cv.y, cv.z, cv.w}, sf[4] = {sv.x, sv.y, sv.z, sv.w};
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        turned[i + j] = other.f(i + j);
-        co[i + j] = cf[j];
-        si[i + j] = low ? -sf[j] : sf[j];
-      }
+      co[j][i] = cv.x; co[j][i + 1] = cv.y; co[j][i + 2] = cv.z; co[j][i + 3] = cv.w;
+      si[j][i] = sv.x; si[j][i + 1] = sv.y; si[j][i + 2] = sv.z; si[j][i + 3] = sv.w;
     }
   }
+  auto turned = [&](int j, int i) { return TURN == kPairs ? x[j].f(i ^ 1) : TURN == kHalves ? x[CH - 1 - j].f(i) : other[j].f(i); };
+  auto cosine = [&](int j, int i) { return co[j % ANGLES][TURN == kPairs ? i / 2 : i]; };
+  auto sine = [&](int j, int i) {
+    const float f = si[j % ANGLES][TURN == kPairs ? i / 2 : i];
+    const bool low = TURN == kPairs ? !(i & 1) : TURN == kHalves ? j == 0 : c0 + j * (D / 2) < p.half;
+    return low ? -f : f;
+  };
   if (query) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) mine.set(i, turns ? x[i] * co[i] + turned[i] * si[i] : x[i]);
-    mine.store((T*)p.q_out + b * p.o_sb + w * p.o_sw + (long)h * p.D + c);
-    return;
-  }
-  float y[8];
+    for (int j = 0; j < CH; ++j) {
+      Eight<T> y = x[j];
+      if (turns[j])
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float e = __fmul_rn(turned[i], si[i]);
-    y[i] = turns ? __fadd_rn(__fmaf_rn(x[i], co[i], e), __fmaf_rn(turned[i], si[i], -e)) : x[i];
-  }
-  float lo = y[0], hi = y[0];
-#pragma unroll
-  for (int i = 1; i < 8; ++i) { lo = min_nan(lo, y[i]); hi = max_nan(hi, y[i]); }
-  const unsigned four = 0xfu << (threadIdx.x & 28);        // the threads of the 32 numbers: all of one head
-#pragma unroll
-  for (int o = 1; o < 4; o <<= 1) {
-    lo = min_nan(lo, __shfl_xor_sync(four, lo, o));
-    hi = max_nan(hi, __shfl_xor_sync(four, hi, o));
-  }
-  const __half m16 = __float2half_rn(lo);
-  const float m = __half2float(m16);
-  const __half s16 = __float2half_rn(__fdiv_rn(__fsub_rn(hi, m), 15.f));
-  const float s = __half2float(s16), inv = s > 0.f && s <= 65504.f ? 1.f / s : 0.f;
-  uint32_t codes = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float q = inv == 0.f ? 0.f : (y[i] - m) * inv;
-    float r = rintf(q);
-    if (fabsf(q - r) > 0.5f - 0x1p-15f) {                  // a border, from numbers that are exact
-      const double exact = turns ? (double)x[i] * co[i] + (double)turned[i] * si[i] : (double)x[i], at = floorf(q);
-      const double above = (exact - m) - (at + 0.5) * s;
-      r = (float)(above > 0 || (above == 0 && ((int)at & 1)) ? at + 1 : at);
+        for (int i = 0; i < 8; ++i) y.set(i, x[j].f(i) * cosine(j, i) + turned(j, i) * sine(j, i));
+      y.store((T*)p.q_out + b * p.o_sb + w * p.o_sw + (long)h * D + c0 + j * (D / 2));
     }
-    codes |= (uint32_t)fminf(fmaxf(r, 0.f), 15.f) << (4 * i);
+    return;
   }
   const Int4Pages& to = key ? p.kp : p.vp;
   const int head = h - p.H - (key ? 0 : p.Hkv), page = (int)slot / p.ps, row = (int)slot - page * p.ps;
-  *reinterpret_cast<uint32_t*>(to.codes + page * to.c_sp + row * to.c_sr + head * to.c_sh + c / 2) = codes;
-  uint16_t* const steps = to.steps + page * to.s_sp + row * to.s_sr + head * to.s_sh + c / 32;
-  if (c % 32 == 0) *steps = __half_as_ushort(s16);
-  if (c % 32 == 8) steps[p.D / 32] = __half_as_ushort(m16);
+  uint8_t* const codes_to = to.codes + page * to.c_sp + row * to.c_sr + head * to.c_sh;
+  uint16_t* const steps_to = to.steps + page * to.s_sp + row * to.s_sr + head * to.s_sh;
+  const unsigned four = 0xfu << (threadIdx.x & 28);        // the threads of the 32 numbers: all of one head
+#pragma unroll
+  for (int j = 0; j < CH; ++j) {
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      y[i] = x[j].f(i);
+      if (turns[j]) {
+        const float z = turned(j, i), f = sine(j, i), e = __fmul_rn(z, f);
+        y[i] = __fadd_rn(__fmaf_rn(y[i], cosine(j, i), e), __fmaf_rn(z, f, -e));
+      }
+    }
+    const int c = c0 + j * (D / 2);
+    auto exact = [&](int i) {                              // seldom: from memory once more
+      const int at = c + i;
+      const double own = to_f32<T>(src[at]);
+      if (!turns[j]) return own;
+      const bool low = TURN == kPairs ? !(i & 1) : at < p.half;
+      const int with = TURN == kPairs ? at ^ 1 : low ? at + p.half : at - p.half, angle = TURN == kPairs ? at / 2 : low ? at : at - p.half;
+      const double turn = (double)to_f32<T>(src[with]) * p.sin_t[pos * p.half + angle], keep = own * p.cos_t[pos * p.half + angle];
+      return low ? keep - turn : keep + turn;
+    };
+    float lo = y[0], hi = y[0];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) { lo = min_nan(lo, y[i]); hi = max_nan(hi, y[i]); }
+#pragma unroll
+    for (int o = 1; o < 4; o <<= 1) {
+      lo = min_nan(lo, __shfl_xor_sync(four, lo, o));
+      hi = max_nan(hi, __shfl_xor_sync(four, hi, o));
+    }
+    __half m16, s16;
+    const float size = fmaxf(fabsf(lo), fabsf(hi));
+    steps_of(lo, hi, fminf(size, 0x1p17f) * (key ? 0x1.8p-23f : 0x1p-24f), four, exact, m16, s16);       // one bound for all four threads: they meet in there
+    const float m = __half2float(m16), s = __half2float(s16), inv = s > 0.f && s <= 65504.f ? (1.f / 15.f) / s : 0.f;
+    // quotients as shares of 15, held between 0 and 1 (NaN: 0); with 2^23 and a half of that added their last bits are the codes
+    constexpr float kBits = 0x1.8p23f;
+    uint32_t codes = 0;
+    float worst = 0.f;
+#pragma unroll
+    for (int i = 7; i >= 0; --i) {
+      const float q = __saturatef((y[i] - m) * inv), r = fmaf(q, 15.f, kBits);
+      worst = fmaxf(worst, fabsf(fmaf(q, 15.f, kBits - r)));
+      codes = codes * 16 + __float_as_uint(r);
+    }
+    codes -= 0x4b400000u * 0x11111111u;
+    // quotients are off by 15 * 2^-22, what the numbers are off by aside
+    const float border = 0.5f - 0x1p-17f - 0x1p-18f * size * inv;
+    if (worst > border) {                                  // those near a border from numbers that are exact
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const float q = __saturatef((y[i] - m) * inv), r = fmaf(q, 15.f, kBits);
+        if (!(fabsf(fmaf(q, 15.f, kBits - r)) > border)) continue;
+        const double d = exact(i) - m;
+        const int at = min(14, max(0, (int)floor(d / s))); // the border is at + 1 / 2, whichever way the quotient was rounded
+        const double above = d - (at + 0.5) * s;
+        codes = (codes & ~(15u << (4 * i))) | (uint32_t)(above > 0 || (above == 0 && (at & 1)) ? at + 1 : at) << (4 * i);
+      }
+    }
+    *reinterpret_cast<uint32_t*>(codes_to + c / 2) = codes;
+    if (c % 32 == 0) steps_to[c / 32] = __half_as_ushort(s16);
+    if (c % 32 == 8) steps_to[D / 32 + c / 32] = __half_as_ushort(m16);
+  }
 }
 
 // ---------------------------------------------------------------------------------------------------------------- gather
-constexpr int kGatherThreads = 256;
-// Tokens at slots as numbers of T: a thread has eight of them.  Bound by HBM.
-template <typename T>
-__global__ void __launch_bounds__(kGatherThreads) int4_gather_kernel(const Int4Pages kp, const Int4Pages vp, const int* slots, T* k, T* v, long items, int Hkv, int D,
-                                                                    int ps, long tokens) {
+constexpr int kGatherThreads = 128;
+// Tokens at slots as numbers of T: a block has a token's keys or values (or, with many heads, a part of them), a thread eight numbers at a time.  Bound by HBM.
+template <typename T, int D0>
+__global__ void __launch_bounds__(kGatherThreads) int4_gather_kernel(const Int4Pages kp, const Int4Pages vp, const int* slots, T* k, T* v, int Hkv, int D1, int ps, long tokens) {
+  const int D = D0 ? D0 : D1, items = Hkv * (D / 8);
   pdl_trigger();
   pdl_wait();
-  const long i = (long)blockIdx.x * kGatherThreads + threadIdx.x;
-  if (i >= items) return;
-  const bool key = blockIdx.y == 0;
-  const unsigned chunks = D / 8, per = Hkv * chunks;
-  const long t = i / per;
-  const unsigned x = (unsigned)(i - t * per), head = x / chunks, c = x % chunks * 8;
-  const long slot = slots[t];
-  Eight<T> out;
-  if (slot >= 0 && slot < tokens) {
-    const Int4Pages& from = key ? kp : vp;
-    const int page = (int)slot / ps, row = (int)slot - page * ps;
-    const uint32_t codes = *reinterpret_cast<const uint32_t*>(from.codes + page * from.c_sp + row * from.c_sr + head * from.c_sh + c / 2);
-    const uint16_t* const steps = from.steps + page * from.s_sp + row * from.s_sr + head * from.s_sh + c / 32;
-    const float s = __half2float(__ushort_as_half(steps[0])), m = __half2float(__ushort_as_half(steps[D / 32]));
+  const bool key = blockIdx.z == 0;
+  const Int4Pages& from = key ? kp : vp;
+  const int slot = slots[blockIdx.x];
+  const bool there = slot >= 0 && slot < tokens;
+  const int page = there ? slot / ps : 0, row = there ? slot - page * ps : 0;
+  const uint8_t* const codes = from.codes + page * from.c_sp + row * from.c_sr;
+  const uint16_t* const steps = from.steps + page * from.s_sp + row * from.s_sr;
+  T* const to = (key ? k : v) + (long)blockIdx.x * Hkv * D;
+  for (int i = blockIdx.y * kGatherThreads + threadIdx.x; i < items; i += gridDim.y * kGatherThreads) {
+    const int head = i / (D / 8), c = (i - head * (D / 8)) * 8;
+    Eight<T> out;
+    if (there) {
+      const uint32_t word = *reinterpret_cast<const uint32_t*>(codes + head * from.c_sh + c / 2);
+      const uint16_t* const st = steps + head * from.s_sh + c / 32;
+      const float s = __half2float(__ushort_as_half(st[0])), m = __half2float(__ushort_as_half(st[D / 32]));
 #pragma unroll
-    for (int j = 0; j < 8; ++j) out.set(j, fmaf((float)(codes >> (4 * j) & 15), s, m));
-  } else {
+      for (int j = 0; j < 8; ++j) out.set(j, fmaf(__uint_as_float(0x4b000000u | (word >> (4 * j) & 15)) - 0x1p23f, s, m));
+    } else {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) out.set(j, 0.f);
+      for (int j = 0; j < 8; ++j) out.set(j, 0.f);
+    }
+    out.store(to + (long)i * 8);
   }
-  out.store((key ? k : v) + i * 8);
 }
 
 // ----------------------------------------------------------------------------------------------- numbers for portions of prompts
@@ -771,25 +834,47 @@ void int4_queries(const void* q, void* out, float* units, int B, int W, int H, i
 }
 
 void int4_append(Int4Append p, int dt, cudaStream_t st) {
-  const long tokens = (long)p.B * p.W, items = (long)(p.H + 2 * p.Hkv) * (p.D / 8);
-  p.parts = (int)((items + kAppendThreads - 1) / kAppendThreads);
+  const bool two = p.D % 64 == 0;                          // eight numbers of each half: four threads have the same 32 in either
+  const long tokens = (long)p.B * p.W;
   if (tokens == 0) return;
-  if (tokens * p.parts >= (1l << 31)) nxd_throw("int4_append: too many tokens", __FILE__, __LINE__);
-  const unsigned grid = (unsigned)(tokens * p.parts);
-  if (dt == kBF16) launch_dependent(int4_append_kernel<__nv_bfloat16>, grid, kAppendThreads, 0, st, p);
-  else if (dt == kF16) launch_dependent(int4_append_kernel<__half>, grid, kAppendThreads, 0, st, p);
-  else launch_dependent(int4_append_kernel<float>, grid, kAppendThreads, 0, st, p);
+  auto go = [&](auto kernel, int heads) {
+    const long parts = ((long)heads * (p.D / (two ? 16 : 8)) + kAppendThreads - 1) / kAppendThreads;
+    if (tokens >= (1l << 31) || parts > 65535) nxd_throw("int4_append: too many tokens or heads", __FILE__, __LINE__);
+    launch_dependent(kernel, dim3((unsigned)tokens, (unsigned)parts), kAppendThreads, 0, st, p);
+  };
+  // Queries alone take fewer registers, so that more of their threads wait for memory at a time; few tokens go by one launch.
+  auto split = [&](auto all, auto queries, auto cache) {
+    if (tokens < kSplitTokens) return go(all, p.H + 2 * p.Hkv);
+    go(queries, p.H);
+    go(cache, 2 * p.Hkv);
+  };
+#define NXD_TURN(Dv, turn) split(int4_append_kernel<T, Dv, turn, 2, kAll>, int4_append_kernel<T, Dv, turn, 2, kQueries0>, int4_append_kernel<T, Dv, turn, 2, kCache>)
+  auto typed = [&](auto zero) {
+    using T = decltype(zero);
+    if (!two) return p.pairs ? go(int4_append_kernel<T, 0, kPairs, 1, kAll>, p.H + 2 * p.Hkv) : go(int4_append_kernel<T, 0, kPart, 1, kAll>, p.H + 2 * p.Hkv);
+    if (p.pairs) return p.D == 128 ? NXD_TURN(128, kPairs) : NXD_TURN(0, kPairs);
+    if (2 * p.half == p.D) return p.D == 128 ? NXD_TURN(128, kHalves) : NXD_TURN(0, kHalves);
+    return p.D == 128 ? NXD_TURN(128, kPart) : NXD_TURN(0, kPart);
+  };
+#undef NXD_TURN
+  if (dt == kBF16) typed(__nv_bfloat16());
+  else if (dt == kF16) typed(__half());
+  else typed(float());
 }
 
 void int4_gather(const Int4Pages& kp, const Int4Pages& vp, const int* slots, void* k, void* v, long n, int Hkv, int D, int ps, long tokens, int dt, cudaStream_t st) {
-  const long items = n * Hkv * (D / 8), blocks = (items + kGatherThreads - 1) / kGatherThreads;
-  if (items == 0) return;
-  if (blocks >= (1l << 31)) nxd_throw("int4_gather: too many tokens", __FILE__, __LINE__);
-  const dim3 grid((unsigned)blocks, 2);
-  auto go = [&](auto* k, auto* v, auto kernel) { launch_dependent(kernel, grid, kGatherThreads, 0, st, kp, vp, slots, k, v, items, Hkv, D, ps, tokens); };
-  if (dt == kBF16) go((__nv_bfloat16*)k, (__nv_bfloat16*)v, int4_gather_kernel<__nv_bfloat16>);
-  else if (dt == kF16) go((__half*)k, (__half*)v, int4_gather_kernel<__half>);
-  else go((float*)k, (float*)v, int4_gather_kernel<float>);
+  if (n == 0) return;
+  if (n >= (1l << 31)) nxd_throw("int4_gather: too many tokens", __FILE__, __LINE__);
+  const dim3 grid((unsigned)n, std::min(64, (Hkv * (D / 8) + kGatherThreads - 1) / kGatherThreads), 2);
+  auto go = [&](auto* k, auto* v, auto kernel) { launch_dependent(kernel, grid, kGatherThreads, 0, st, kp, vp, slots, k, v, Hkv, D, ps, tokens); };
+  auto typed = [&](auto zero) {
+    using T = decltype(zero);
+    if (D == 128) go((T*)k, (T*)v, int4_gather_kernel<T, 128>);
+    else go((T*)k, (T*)v, int4_gather_kernel<T, 0>);
+  };
+  if (dt == kBF16) typed(__nv_bfloat16());
+  else if (dt == kF16) typed(__half());
+  else typed(float());
 }
 
 }  // namespace nxd
