@@ -96,14 +96,15 @@ __global__ void __launch_bounds__(kThreads) page_tables_kernel(const PageTables 
   }
   if (few && p.few) *p.few = 1;
   const long P = p.P;
+  auto place = [&](long i) { return (unsigned)((unsigned long)i % (unsigned long)P); };       // in the ring, whatever the counts are
   const int n = b1 - b0, part = blockIdx.y * kThreads + threadIdx.x, stride = gridDim.y * kThreads;
   if (blockIdx.y == 0)
     for (int i = threadIdx.x; i < n; i += kThreads) p.held_out[b0 + i] = rows[i].had + rows[i].take - rows[i].give;
   auto column = [&](const Row& r, int b, int c) {          // what a column holds from now on, and to the ring what it gives back
     const int old = p.table[b * p.table_sb + c];
-    if (c >= r.had && c < r.had + r.take) return p.free[(r.at + c - r.had) % P];
+    if (c >= r.had && c < r.had + r.take) return p.free[place(r.at + c - r.had)];
     if (c < r.had && c >= r.had - r.give) {
-      p.free_out[(r.back + c - (r.had - r.give)) % P] = old;
+      p.free_out[place(r.back + c - (r.had - r.give))] = old;
       return -1;
     }
     return old;
@@ -114,28 +115,67 @@ __global__ void __launch_bounds__(kThreads) page_tables_kernel(const PageTables 
       for (int c = r.had - r.give + lane; c < r.had + r.take; c += 32) p.table_out[(b0 + i) * p.out_sb + c] = column(r, b0 + i, c);
     }
   } else {
-    for (long x = part; x < (long)n * p.cols; x += stride) {
-      const int i = (int)(x / p.cols), c = (int)(x % p.cols);
-      p.table_out[(b0 + i) * p.out_sb + c] = column(rows[i], b0 + i, c);
+    // four columns at a time where nothing changes; a row's threads beside one another
+    const bool fours = p.cols % 4 == 0 && p.table_sb % 4 == 0 && ((uintptr_t)p.table | (uintptr_t)p.table_out) % 16 == 0;
+    if (fours) {
+      constexpr int ROWS = 4;                              // of which a thread asks for its columns at a time
+      for (int i0 = 0; i0 < n; i0 += ROWS)
+        for (int c = part * 4; c < p.cols; c += stride * 4) {
+          int4 x[ROWS];
+#pragma unroll
+          for (int y = 0; y < ROWS; ++y)
+            if (i0 + y < n) x[y] = *reinterpret_cast<const int4*>(p.table + (b0 + i0 + y) * p.table_sb + c);
+#pragma unroll
+          for (int y = 0; y < ROWS; ++y) {
+            if (i0 + y >= n) break;
+            const Row& r = rows[i0 + y];
+            int* const to = p.table_out + (b0 + i0 + y) * p.out_sb + c;
+            if (c + 4 <= r.had - r.give || c >= r.had + r.take) *reinterpret_cast<int4*>(to) = x[y];
+            else
+              for (int k = 0; k < 4; ++k) to[k] = column(r, b0 + i0 + y, c + k);
+          }
+        }
+    } else {
+      for (int i = 0; i < n; ++i)
+        for (int c = part; c < p.cols; c += stride) p.table_out[(b0 + i) * p.out_sb + c] = column(rows[i], b0 + i, c);
     }
     // the rest of the ring, as it was: all places but those that pages were given back to
-    const long given = totals[1], block = (long)blockIdx.y * gridDim.x + blockIdx.x, all = (long)gridDim.x * gridDim.y * kThreads;
-    const long from = tail % P;
-    for (long i = block * kThreads + threadIdx.x; i < P; i += all) {
-      const long off = i >= from ? i - from : i - from + P;
-      if (off >= given) p.free_out[i] = p.free[i];
+    const unsigned given = (unsigned)min((long)totals[1], P), tail_at = place(tail), all = gridDim.x * gridDim.y * kThreads;
+    auto kept = [&](unsigned i) { return (i >= tail_at ? i - tail_at : i - tail_at + (unsigned)P) >= given; };
+    const unsigned me = (blockIdx.y * gridDim.x + blockIdx.x) * kThreads + threadIdx.x, whole = (((uintptr_t)p.free | (uintptr_t)p.free_out) % 16 == 0) ? (unsigned)P / 4 : 0;
+    constexpr int PACKS = 4;
+    for (unsigned i0 = me; i0 < whole; i0 += all * PACKS) {
+      int4 x[PACKS];
+#pragma unroll
+      for (int y = 0; y < PACKS; ++y)
+        if (i0 + y * all < whole) x[y] = reinterpret_cast<const int4*>(p.free)[i0 + y * all];
+#pragma unroll
+      for (int y = 0; y < PACKS; ++y) {
+        const unsigned i = i0 + y * all;
+        if (i >= whole) break;
+        if (given == 0 || (kept(4 * i) && kept(4 * i + 1) && kept(4 * i + 2) && kept(4 * i + 3))) reinterpret_cast<int4*>(p.free_out)[i] = x[y];
+        else {
+          if (kept(4 * i)) p.free_out[4 * i] = x[y].x;
+          if (kept(4 * i + 1)) p.free_out[4 * i + 1] = x[y].y;
+          if (kept(4 * i + 2)) p.free_out[4 * i + 2] = x[y].z;
+          if (kept(4 * i + 3)) p.free_out[4 * i + 3] = x[y].w;
+        }
+      }
     }
+    for (unsigned i = whole * 4 + me; i < (unsigned)P; i += all)
+      if (kept(i)) p.free_out[i] = p.free[i];
   }
   bool lost = false;
-  for (long x = part; x < (long)n * p.W; x += stride) {
-    const int i = (int)(x / p.W), w = (int)(x % p.W);
+  for (unsigned x = part; x < (unsigned)n * p.W; x += stride) {          // fewer than 2^31
+    const int i = (int)(x / p.W), w = (int)(x - (unsigned)i * p.W);
     const Row r = rows[i];
     int slot = -1;
     if (w < r.count) {
-      const long pos = r.first + w, c = pos / p.ps;
+      const long pos = r.first + w;
+      const int c = pos < (long)p.cols * p.ps ? (int)((unsigned)pos / (unsigned)p.ps) : p.cols;
       if (c >= p.shared && c < r.had + r.take - r.give) {
-        const int page = c < r.had ? p.table[(b0 + i) * p.table_sb + c] : p.free[(r.at + c - r.had) % P];
-        if (page >= 0 && page < P) slot = page * p.ps + (int)(pos - c * p.ps);
+        const int page = c < r.had ? p.table[(b0 + i) * p.table_sb + c] : p.free[place(r.at + c - r.had)];
+        if (page >= 0 && page < P) slot = page * p.ps + (int)((unsigned)pos - (unsigned)c * p.ps);
       }
       lost |= slot < 0;
     }
