@@ -5,6 +5,7 @@ forward — counterpart of the reference's ``examples/inference/run_llama_specul
   python examples/inference/run_llama_speculative.py --model tiny --speculation_length 4
   torchrun --nproc-per-node 8 examples/inference/run_llama_speculative.py --model 13b --draft_layers 4 --tp_degree 8
   python examples/inference/run_llama_speculative.py --model tiny --page_size 32 --temperature 0.8 --batch_size 4
+  python examples/inference/run_llama_speculative.py --model tiny --page_size 32 --kv_bits 4 --device_tables
 """
 import argparse
 import os
@@ -34,6 +35,8 @@ def main():
     p.add_argument("--max_new_tokens", type=int, default=32)
     p.add_argument("--speculation_length", type=int, default=4)
     p.add_argument("--page_size", type=int, default=0, help="keep keys and values in pages of that many tokens (0: contiguous rows)")
+    p.add_argument("--kv_bits", type=int, default=None, choices=[4], help="with --page_size: keys and values in that many bits")
+    p.add_argument("--device_tables", action="store_true", help="with --page_size: pages are handed out on the device")
     p.add_argument("--temperature", type=float, default=0.0, help="above 0: sampled tokens, accepted against the target's probabilities")
     p.add_argument("--batch_size", type=int, default=1, help="rows of the batch (sampling only)")
     a = p.parse_args()
@@ -48,7 +51,8 @@ def main():
         vocab_size=4096, hidden_size=256, intermediate_size=704, num_hidden_layers=4, num_attention_heads=8, **k))
     torch.manual_seed(0)
     sampled = a.temperature > 0
-    how = dict(batch_size=a.batch_size if sampled else 1, max_seq_len=L, page_size=a.page_size or None, on_device_sampling=not sampled)
+    how = dict(batch_size=a.batch_size if sampled else 1, max_seq_len=L, page_size=a.page_size or None, kv_bits=a.kv_bits,
+               device_tables=a.device_tables, on_device_sampling=not sampled)
     target = LlamaForInference(mk(**kw), **how).eval()
     dcfg = mk(**kw)
     dcfg.num_hidden_layers = a.draft_layers

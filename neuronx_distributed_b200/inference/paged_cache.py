@@ -3,7 +3,8 @@ share.  Beside ``kv_cache.py``, whose rows are contiguous and as long as the lon
 and what they begin alike is there once.  The pages themselves are written and read by ``ops.paged`` (``csrc/paged.cu``); this class says
 whose they are.  Tables live on the device at fixed addresses (captured and recorded programs read them as they are when they run); pages are handed
 out on the host, so a program takes none: its rows have to be reserved before it runs (:meth:`PagedKVCacheManager.check` says whether they were), and
-the length of the shared prefix is part of it."""
+the length of the shared prefix is part of it.  :class:`DevicePagedKVCacheManager` hands pages out on the device instead, so that programs take what they
+need and nothing waits for positions.  Either keeps numbers of the model's type or, with ``bits=4``, codes (``ops.paged_int4``)."""
 from __future__ import annotations
 
 from contextlib import contextmanager
@@ -11,13 +12,17 @@ from typing import Iterator, List, Optional
 
 import torch
 
+from ..ops import page_tables, paged_int4
 from ..utils.plan_registry import recording
 
 
 class PagedKVCacheManager:
     def __init__(self, num_layers: int, batch_size: int, max_seq_len: int, num_kv_heads_local: int, head_dim: int, page_size: int = 32,
-                 num_pages: Optional[int] = None, dtype: torch.dtype = torch.bfloat16, device=None):
-        """``num_pages``: of the pool (default: enough for every row to be ``max_seq_len`` long)."""
+                 num_pages: Optional[int] = None, dtype: torch.dtype = torch.bfloat16, device=None, bits: Optional[int] = None):
+        """``num_pages``: of the pool (default: enough for every row to be ``max_seq_len`` long).  ``bits``: 4: keys and values as codes, ``k`` and ``v``
+        hold :class:`ops.paged_int4.Pages`."""
+        if bits not in (None, 4):
+            raise ValueError(f"keys and values are held in the model's type or in 4 bits, got {bits}")
         if page_size < 16 or page_size % 16:
             raise ValueError(f"a page holds a multiple of 16 tokens, got {page_size}")
         self.num_layers, self.batch_size, self.max_seq_len, self.page_size = num_layers, batch_size, max_seq_len, page_size
@@ -26,8 +31,13 @@ class PagedKVCacheManager:
         if self.num_pages < 1:
             raise ValueError("a pool without pages")
         shape = (self.num_pages, page_size, num_kv_heads_local, head_dim)
-        self.k: List[torch.Tensor] = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(num_layers)]
-        self.v: List[torch.Tensor] = [torch.zeros(shape, dtype=dtype, device=device) for _ in range(num_layers)]
+        self.bits = bits
+
+        def pool():
+            return torch.zeros(shape, dtype=dtype, device=device) if bits is None else paged_int4.new_pages(*shape, device=device)
+
+        self.k: List = [pool() for _ in range(num_layers)]
+        self.v: List = [pool() for _ in range(num_layers)]
         self.page_table = torch.full((batch_size, self.columns), -1, dtype=torch.int32, device=device)
         self._shared_table = torch.full((self.columns,), -1, dtype=torch.int32, device=device)
         self.shared_pages: Optional[torch.Tensor] = None      # [n] int32, the beginning of that table: what every row begins with
@@ -36,6 +46,9 @@ class PagedKVCacheManager:
         self._shared: List[int] = []
         self._rows: List[List[int]] = [[] for _ in range(batch_size)]       # pages of a row behind the shared ones
         self._free: List[int] = list(range(self.num_pages))[::-1]
+        # what slots() gives ops.page_tables.assign for rows that stay as they are: no free pages, all columns to be looked at
+        self._no_ring = torch.zeros(self.num_pages, dtype=torch.int32, device=device)
+        self._no_span = torch.zeros(2, dtype=torch.long, device=device)
         self._ahead = False                                   # inside reserved_ahead
         self._programs: Optional[int] = None                  # shared pages that captured and recorded programs count on
 
@@ -75,6 +88,15 @@ class PagedKVCacheManager:
         if n > len(self._free):
             raise RuntimeError(f"the key/value pool has {len(self._free)} pages left, {n} are needed")
         return [self._free.pop() for _ in range(n)]
+
+    def slots(self, positions: torch.Tensor, new: int, lens: Optional[torch.Tensor] = None, table: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Slots ``[B, new]`` of new tokens of the first ``B`` rows from ``positions [B]`` on, or of the rows of ``table``; where there is no page, -1, and
+        ``lost`` is noted (:meth:`check`).  Without waiting for the device, in programs too."""
+        rows, shared = positions.shape[0], 0 if table is not None else len(self._shared)
+        table = self.page_table[:rows] if table is None else table
+        held = torch.full((rows,), table.shape[1], dtype=torch.int32, device=table.device)
+        return page_tables.assign(table, held, self._no_ring, self._no_span, positions, new, self.page_size, lens=lens,
+                                  lengths=torch.full((rows,), -1, dtype=torch.long, device=table.device), shared=shared, short=self.lost, in_place=True).slots
 
     def reserve(self, row: int, tokens: int) -> None:
         """Room for a sequence of ``tokens`` tokens in all, the shared ones among them."""
@@ -170,3 +192,82 @@ class PagedKVCacheManager:
     def reset(self) -> None:
         """All pages go back to the pool, the shared ones too (:meth:`take_shared` of nothing)."""
         self.take_shared(0)
+
+
+class DevicePagedKVCacheManager(PagedKVCacheManager):
+    """Pages handed out on the device, by ``ops.page_tables.assign``: :meth:`slots` gives the rows of a step what pages they are short of, from positions
+    that the host does not look at, in captured and recorded programs as outside.  A pool that runs short, and positions without a page, are noted in ``lost``
+    and said by :meth:`check` (which the end of a sequence does not wait for).  Rows of a prompt get pages for the tokens that count."""
+
+    def __init__(self, *args, **kwargs):
+        super().__init__(*args, **kwargs)
+        device = self.page_table.device
+        self.held = torch.zeros(self.batch_size, dtype=torch.int32, device=device)
+        self.free = torch.arange(self.num_pages, dtype=torch.int32, device=device)
+        self.span = torch.tensor([0, self.num_pages], device=device)
+        self._row = torch.arange(self.batch_size, device=device)
+        for t in (self.held, self.free, self.span):
+            t._plan_state = True
+
+    @property
+    def free_pages(self) -> int:
+        """Waits for the device."""
+        taken, put = self.span.tolist()
+        return put - taken
+
+    def _assign(self, rows: int, positions: torch.Tensor, new: int = 0, lens=None, lengths=None) -> torch.Tensor:
+        return page_tables.assign(self.page_table[:rows], self.held[:rows], self.free, self.span, positions, new, self.page_size, lens=lens, lengths=lengths,
+                                  shared=len(self._shared), short=self.lost, in_place=True).slots
+
+    def slots(self, positions, new, lens=None, table=None):
+        """As in the class above, and pages for the tokens that have none."""
+        return self._assign(positions.shape[0], positions, new, lens) if table is None else super().slots(positions, new, lens, table)
+
+    def check(self) -> None:
+        """Raises if tokens were left without a page since the last look, whose keys are missing from what came after: the pool was too small for its rows, or
+        they are longer than ``max_seq_len``.  Waits for the device."""
+        if bool(self.lost):
+            self.lost.zero_()
+            raise RuntimeError(f"tokens were left without a page, and their keys are lost: a pool of {self.num_pages} pages of {self.page_size} tokens ran short, or "
+                               f"rows went on behind max_seq_len {self.max_seq_len}")
+
+    def reserve(self, row: int, tokens: int) -> None:
+        if tokens > self.max_seq_len:
+            raise ValueError(f"a sequence of {tokens} tokens is longer than max_seq_len {self.max_seq_len}")
+        if tokens > 0:
+            self._assign(self.batch_size, self._row, lengths=torch.where(self._row == row, tokens, -1))
+
+    def reserve_rows(self, rows: int, tokens: int) -> None:
+        """:meth:`reserve` for the first ``rows`` rows, in their order, as far as the pool goes."""
+        if tokens > self.max_seq_len:
+            raise ValueError(f"a sequence of {tokens} tokens is longer than max_seq_len {self.max_seq_len}")
+        if tokens > 0:
+            self._assign(self.batch_size, self._row, lengths=torch.where(self._row < rows, tokens, -1))
+
+    def cover(self, positions: torch.Tensor, tokens: int) -> None:
+        """:meth:`slots` does that."""
+
+    @contextmanager
+    def reserved_ahead(self, rows: int, tokens: int) -> Iterator[None]:
+        """Rows get their pages when they need them, and nothing ahead."""
+        if tokens > self.max_seq_len:
+            raise ValueError(f"a sequence of {tokens} tokens is longer than max_seq_len {self.max_seq_len}")
+        yield
+
+    def release(self, row: int) -> None:
+        self._assign(self.batch_size, self._row, lengths=torch.where(self._row == row, 0, -1))
+
+    def _share(self, n: int) -> torch.Tensor:
+        # all rows start anew: the first pages of the pool are everybody's, the others free
+        self._shared = list(range(n))
+        self._shared_table[:] = -1
+        pages = self._shared_table[:n]
+        pages._plan_state = True
+        pages.copy_(torch.arange(n, dtype=torch.int32, device=pages.device))
+        self.page_table[:] = -1
+        self.page_table[:, :n] = pages
+        self.held.fill_(n)
+        self.free.copy_(torch.arange(self.num_pages, dtype=torch.int32, device=pages.device).roll(-n))
+        self.span.copy_(torch.tensor([0, self.num_pages - n], device=pages.device))
+        self.shared_pages = pages if n else None
+        return pages

@@ -14,7 +14,7 @@ from torch.nn.modules.module import _global_forward_hooks, _global_forward_pre_h
 
 from .. import ops
 from ..inference.kv_cache import KVCacheManager
-from ..inference.paged_cache import PagedKVCacheManager
+from ..inference.paged_cache import DevicePagedKVCacheManager, PagedKVCacheManager
 from ..utils.sampling import Sampler
 from ..modules.rms_norm import RMSNorm
 from ..parallel_layers.layers import column_swiglu
@@ -24,10 +24,12 @@ from .llama import LlamaConfig, LlamaForCausalLM
 class LlamaForInference(nn.Module):
     def __init__(self, cfg: LlamaConfig, batch_size: int = 1, max_seq_len: int = 2048, on_device_sampling: bool = True,
                  sampler: Optional[Sampler] = None, lm_cls=None, flash_decoding: bool = False, page_size: Optional[int] = None,
-                 num_pages: Optional[int] = None):
+                 num_pages: Optional[int] = None, kv_bits: Optional[int] = None, device_tables: bool = False):
         """``lm_cls``: any decoder built from Llama attention blocks (``LlamaForCausalLM`` default; ``MixtralForCausalLM`` for
         the MoE families — its layers' ``mlp`` returns ``(y, router_logits)``, handled in ``_body``).  ``page_size``: the cache
-        lies in pages of that many tokens (``inference/paged_cache.py``), ``num_pages`` of them; without it, in contiguous rows."""
+        lies in pages of that many tokens (``inference/paged_cache.py``), ``num_pages`` of them; without it, in contiguous rows.  ``kv_bits``: 4:
+        pages hold codes of 4 bits (``ops.paged_int4``).  ``device_tables``: pages are handed out on the device, so that steps wait for no positions and captured
+        programs take what pages they need."""
         super().__init__()
         cfg.sequence_parallel_enabled = False
         cfg.activation_checkpointing = "none"
@@ -48,11 +50,15 @@ class LlamaForInference(nn.Module):
             assert max_seq_len % shards == 0, f"max_seq_len {max_seq_len} must divide by the KV replication factor {shards}"
         self.paged = page_size is not None
         self._rows = None                                # rows of a prompt in a paged cache: first position, lengths, tables, shared pages
+        self._slots = None                               # where the new tokens of a step go
+        if not self.paged and (kv_bits is not None or device_tables):
+            raise ValueError("kv_bits and device_tables are of a cache in pages (page_size)")
         if self.paged:
             if flash_decoding:
                 raise ValueError("flash decoding shards contiguous cache rows; it does not go with pages")
-            self.kv = PagedKVCacheManager(cfg.num_hidden_layers, batch_size, max_seq_len, attn0.num_kv_heads_local, cfg.head_dim,
-                                          page_size=page_size, num_pages=num_pages, dtype=cfg.dtype, device=cfg.device)
+            manager = DevicePagedKVCacheManager if device_tables else PagedKVCacheManager
+            self.kv = manager(cfg.num_hidden_layers, batch_size, max_seq_len, attn0.num_kv_heads_local, cfg.head_dim, page_size=page_size,
+                              num_pages=num_pages, dtype=cfg.dtype, device=cfg.device, bits=kv_bits)
         else:
             self.kv = KVCacheManager(cfg.num_hidden_layers, batch_size, max_seq_len, attn0.num_kv_heads_local, cfg.head_dim,
                                      dtype=cfg.dtype, device=cfg.device, num_cores_per_group=shards)
@@ -90,8 +96,12 @@ class LlamaForInference(nn.Module):
             # one launch: rotation of q and k and the new rows of the pages; prompts, windows and single tokens read them there
             first, lens, table, shared = self._rows if prefill else (positions.long(), None, self.kv.page_table[:B], self.kv.shared_pages)
             kc, vc = self.kv.k[layer_idx], self.kv.v[layer_idx]
-            q = ops.paged.rope_append(q, k, v, first, self.rope_cos, self.rope_sin, kc, vc, table, lens=lens, lost=self.kv.lost)
-            o = ops.paged.attention(q, kc, vc, table, first, lens=lens, shared_pages=shared)
+            if self.kv.bits is None:
+                q = ops.paged.rope_append(q, k, v, first, self.rope_cos, self.rope_sin, kc, vc, table, lens=lens, lost=self.kv.lost)
+                o = ops.paged.attention(q, kc, vc, table, first, lens=lens, shared_pages=shared)
+            else:
+                q = ops.paged_int4.append(q, k, v, first, self.rope_cos, self.rope_sin, kc, vc, self._slots, lost=self.kv.lost)
+                o = ops.paged_int4.attention(q, kc, vc, table, first, lens=lens, shared_pages=shared)
         elif self.flash_decoding and not prefill:
             v = v.contiguous()
             assert S == 1 and tree is None, "flash decoding serves plain token generation (no speculation window)"
@@ -220,6 +230,20 @@ class LlamaForInference(nn.Module):
             x = x + (y[0] if isinstance(y, tuple) else y)                           # MoE blocks also return router logits
         return core.norm(x)
 
+    def _take_slots(self, positions: torch.Tensor, new: int, lens: Optional[torch.Tensor] = None, prompt: int = 0) -> None:
+        """Pages for the step's new tokens, and where those go (a cache in pages).  ``prompt``: tokens of every row, the padding among them."""
+        if isinstance(self.kv, DevicePagedKVCacheManager):
+            if prompt > self.max_seq_len:
+                raise ValueError(f"a sequence of {prompt} tokens is longer than max_seq_len {self.max_seq_len}")
+            self._slots = self.kv.slots(positions, new, lens)
+            return
+        if prompt:
+            self.kv.reserve_rows(positions.shape[0], prompt)
+        else:
+            self.kv.cover(positions, new)
+        if self.kv.bits is not None:
+            self._slots = self.kv.slots(positions, new, lens)
+
     # ------------------------------------------------------------------ entry points
     @torch.no_grad()
     def share_prefix(self, prefix_ids: torch.Tensor) -> None:
@@ -231,14 +255,17 @@ class LlamaForInference(nn.Module):
         ids = prefix_ids.reshape(1, -1)
         pages = self.kv.take_shared(ids.shape[1])
         if ids.shape[1]:
-            self._rows = (torch.zeros(1, dtype=torch.long, device=ids.device), None, pages.view(1, -1), None)
+            first, table = torch.zeros(1, dtype=torch.long, device=ids.device), pages.view(1, -1)
+            self._rows = (first, None, table, None)
             try:
+                if self.kv.bits is not None:
+                    self._slots = self.kv.slots(first, ids.shape[1], table=table)
                 self._body(ids, None, True, None)
             except BaseException:
                 self.kv.drop_shared()
                 raise
             finally:
-                self._rows = None
+                self._rows = self._slots = None
 
     @torch.no_grad()
     def context_encoding(self, input_ids: torch.Tensor, last_token_index: Optional[torch.Tensor] = None) -> torch.Tensor:
@@ -247,14 +274,14 @@ class LlamaForInference(nn.Module):
         B = input_ids.shape[0]
         if self.paged:
             shared = self.kv.shared_tokens
-            self.kv.reserve_rows(B, shared + input_ids.shape[1])
             first = torch.full((B,), shared, dtype=torch.long, device=input_ids.device)
             lens = None if last_token_index is None else last_token_index.long() + 1
+            self._take_slots(first, input_ids.shape[1], lens, prompt=shared + input_ids.shape[1])
             self._rows = (first, lens, self.kv.page_table[:B], self.kv.shared_pages)
         try:
             h = self._body(input_ids, None, True, None)                          # [S, B, H]
         finally:
-            self._rows = None
+            self._rows = self._slots = None
         if last_token_index is None:
             last = h[-1]
         else:
@@ -267,8 +294,11 @@ class LlamaForInference(nn.Module):
         """``input_ids`` [B, 1], ``positions`` [B] → next token ids [B].  Positions count the shared prefix of a paged cache; its rows get
         pages for them (a captured program takes none: ``kv.reserve`` them before), and one at -1 is idle."""
         if self.paged:
-            self.kv.cover(positions, 1)
-        h = self._body(input_ids, positions, False, kv_len)
+            self._take_slots(positions, 1)
+        try:
+            h = self._body(input_ids, positions, False, kv_len)
+        finally:
+            self._slots = None
         logits = self.lm.lm_head(h)[0].float()
         return self.sampler.sample(logits) if self.on_device_sampling else logits
 
@@ -282,8 +312,11 @@ class LlamaForInference(nn.Module):
         tree instead of a chain.  ``return_hidden`` also returns the final hidden states ``[B, W, H]`` (Medusa heads input)."""
         tree = None if tree_mask is None else (tree_mask.bool(), tree_depth.long())
         if self.paged and tree is None:
-            self.kv.cover(positions, input_ids.shape[1])
-        h = self._body(input_ids, positions, False, kv_len, tree)                # [W, B, H]
+            self._take_slots(positions, input_ids.shape[1])
+        try:
+            h = self._body(input_ids, positions, False, kv_len, tree)            # [W, B, H]
+        finally:
+            self._slots = None
         logits = self.lm.lm_head(h).float()                                       # [W, B, V/tp]
         W, B = logits.shape[:2]
         out = self.sampler.sample(logits.reshape(W * B, -1)).view(W, B).t() if self.on_device_sampling else logits.transpose(0, 1)
