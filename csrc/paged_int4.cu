@@ -45,9 +45,9 @@ template <typename F>
 NXD_DEVICE void steps_of(float lo, float hi, float off, unsigned four, F exact, __half& m16, __half& s16) {
   constexpr float k15 = 1.f / 15.f;
   m16 = __float2half_rn(lo + off);
-  const float range = hi - __half2float(m16);
-  s16 = __float2half_rn((range + off) * k15);
-  const bool doubt = __half_as_ushort(m16) != __half_as_ushort(__float2half_rn(lo - off)) || __half_as_ushort(s16) != __half_as_ushort(__float2half_rn((range - off) * k15));
+  const float range = hi - __half2float(m16), more = off + fminf(range, 0x1p17f) * 0x1p-22f;          // its own roundings and the product's
+  s16 = __float2half_rn((range + more) * k15);
+  const bool doubt = __half_as_ushort(m16) != __half_as_ushort(__float2half_rn(lo - off)) || __half_as_ushort(s16) != __half_as_ushort(__float2half_rn((range - more) * k15));
   if (doubt) {                                             // never where a NaN is: its halves are alike
     double a = exact(0), b = a;
 #pragma unroll
@@ -169,7 +169,7 @@ __global__ void __launch_bounds__(kAppendThreads, ROLE == kQueries0 ? 12 : 8) in
     }
     __half m16, s16;
     const float size = fmaxf(fabsf(lo), fabsf(hi));
-    steps_of(lo, hi, fminf(size, 0x1p17f) * (key ? 0x1.8p-23f : 0x1p-24f), four, exact, m16, s16);       // one bound for all four threads: they meet in there
+    steps_of(lo, hi, fminf(size, 0x1p17f) * (key ? 0x1.8p-23f : 0.f), four, exact, m16, s16);       // one bound for all four threads: they meet in there
     const float m = __half2float(m16), s = __half2float(s16), inv = s > 0.f && s <= 65504.f ? (1.f / 15.f) / s : 0.f;
     // quotients as shares of 15, held between 0 and 1 (NaN: 0); with 2^23 and a half of that added their last bits are the codes
     constexpr float kBits = 0x1.8p23f;

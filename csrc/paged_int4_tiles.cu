@@ -1,5 +1,6 @@
 // Attention of nine and more query rows of a (sequence, key/value head) over a cache in pages of 4 bits.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "kernels.h"
@@ -14,12 +15,15 @@ constexpr int kTileWarps = 8, kTileThreads = kTileWarps * 32;
 constexpr int kTileKeys = kTileWarps * kKeys;
 constexpr float kRoom = 15.f;                              // weights are at most 2^15: halves
 constexpr int kWeightPitch = kTileKeys * 2 + 16;           // bytes of a row of weights: ldmatrix and stmatrix meet no bank twice
-template <int D> constexpr int kRing = kTileWarps * kStages * kStage<D>;
+// Where the output is in half precision too, weights are two halves, the rounded one and what that left; with 40 rows there is room for two stages then
+template <typename T> constexpr int kHalves = std::is_same<T, __half>::value ? 2 : 1;
+template <typename T, int R> constexpr int kTileStages = kHalves<T> == 2 && R == 5 ? 2 : 3;
+template <typename T, int D, int R> constexpr int kRing = kTileWarps * kTileStages<T, R> * kStage<D>;
 template <int D> constexpr int kParts = kTileWarps / (D / 32);                         // warps that have the same 32 columns of the sums, for other keys
 // two tiles' weights; at a pair's end the sums of all parts but the first lie over them
-template <int D, int R> constexpr int kWeights = 8 * R * std::max(2 * kWeightPitch, (kParts<D> - 1) * kPitch<D> * 4);
+template <typename T, int D, int R> constexpr int kWeights = 8 * R * std::max(2 * kHalves<T> * kWeightPitch, (kParts<D> - 1) * kPitch<D> * 4);
 // a cluster's sums lie over the ring, which has been read by then
-template <int D, int R> constexpr int tiles_smem = kQueries<D, R> + kWeights<D, R> + std::max(kRing<D>, 8 * R * D * 4);
+template <typename T, int D, int R> constexpr int tiles_smem = kQueries<D, R> + kWeights<T, D, R> + std::max(kRing<T, D, R>, 8 * R * D * 4);
 
 // Scores Sᵀ = K Qᵀ and sums Oᵀ += Vᵀ Pᵀ by mma.sync of half precision, with the keys, then the head's numbers, as the 16 rows of the instruction and query rows
 // as its columns, 8 R of them in a row tile.  A block walks tiles of 128 keys: in the first product each of its eight warps has 16 keys, in the second 32 columns of the
@@ -34,7 +38,7 @@ template <int D, int R> constexpr int tiles_smem = kQueries<D, R> + kWeights<D, 
 // below which they have all their bits down to 2^-29 of it.
 template <typename T, int D, int R, bool CLUSTER>
 __global__ void __launch_bounds__(kTileThreads, 2) int4_tiles_kernel(const Int4Attn p) {
-  constexpr int NG = D / 32, PITCH = kPitch<D>, STAGES = kStages, STAGE = kStage<D>, PARTS = kParts<D>;
+  constexpr int NG = D / 32, PITCH = kPitch<D>, STAGES = kTileStages<T, R>, HALVES = kHalves<T>, STAGE = kStage<D>, PARTS = kParts<D>;
   constexpr int V_AT = kKeys * (D / 2), KS_AT = 2 * V_AT, VS_AT = KS_AT + kKeys * 16;
   constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -70,8 +74,8 @@ __global__ void __launch_bounds__(kTileThreads, 2) int4_tiles_kernel(const Int4A
   float* const sm_unit = reinterpret_cast<float*>(smem + 8 * R * (kQPitch<D> + 16));
   int* const sm_lim = reinterpret_cast<int*>(sm_unit + 8 * R);
   float* const sm_o = reinterpret_cast<float*>(smem + kQueries<D, R>);          // sums of all parts but the first [part - 1][8 R][PITCH]
-  float* const sm_b = reinterpret_cast<float*>(smem + kQueries<D, R> + kWeights<D, R>);        // a cluster's: the block's sums [8 R][D]
-  const uint32_t ring0 = sm_p + kWeights<D, R>;
+  float* const sm_b = reinterpret_cast<float*>(smem + kQueries<D, R> + kWeights<T, D, R>);        // a cluster's: the block's sums [8 R][D]
+  const uint32_t ring0 = sm_p + kWeights<T, D, R>;
   Ring<D, kTileWarps, CLUSTER> ring(p, sm_ahead + warp, cur, tiles_left, step, ring0 + warp * (STAGES * STAGE), warp, lane);
 #pragma unroll
   for (int s = 0; s < STAGES - 1; ++s) ring.ask(s);
@@ -166,7 +170,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) int4_tiles_kernel(const Int4A
   for (int t = 0; t < tiles_left; ++t) {
     cp_async_wait<STAGES - 2>();
     __syncwarp();                                          // tile t of all lanes is there
-    const uint32_t at = ring.ring + stage * STAGE, weights = sm_p + (t & 1) * (8 * R * kWeightPitch);
+    const uint32_t at = ring.ring + stage * STAGE, weights = sm_p + (t & 1) * (8 * R * HALVES * kWeightPitch);
     // scores: keys hq and hq + 8, rows 2 quad and 2 quad + 1
     float s[R][4];
     {
@@ -226,7 +230,12 @@ __global__ void __launch_bounds__(kTileThreads, 2) int4_tiles_kernel(const Int4A
         const float p0 = exp2f(s[i][0]), p1 = exp2f(s[i][1]), p2 = exp2f(s[i][2]), p3 = exp2f(s[i][3]);
         more[i][0] = p0 + p2;
         more[i][1] = p1 + p3;
-        stmatrix_x2t(to + i * 8 * kWeightPitch, pack_half(p0, p1), pack_half(p2, p3));
+        const uint32_t h0 = pack_half(p0, p1), h1 = pack_half(p2, p3);
+        stmatrix_x2t(to + i * 8 * kWeightPitch, h0, h1);
+        if constexpr (HALVES == 2) {
+          const float2 f0 = __half22float2(as_half2(h0)), f1 = __half22float2(as_half2(h1));
+          stmatrix_x2t(to + (R + i) * 8 * kWeightPitch, pack_half(p0 - f0.x, p1 - f0.y), pack_half(p2 - f1.x, p3 - f1.y));
+        }
       }
     };
 #pragma unroll
@@ -304,14 +313,16 @@ __global__ void __launch_bounds__(kTileThreads, 2) int4_tiles_kernel(const Int4A
         }
       }
 #pragma unroll
-      for (int i = 0; i < R; ++i) {
-        uint32_t q[4];
-        ldmatrix_x4(q, weights + (i * 8 + (lane & 7)) * kWeightPitch + ((part * NG + j) * kKeys + (lane >> 3) * 8) * 2);
+      for (int i = 0; i < R; ++i)
 #pragma unroll
-        for (int x = 0; x < 2; ++x)
+        for (int h = 0; h < HALVES; ++h) {
+          uint32_t q[4];
+          ldmatrix_x4(q, weights + ((h * R + i) * 8 + (lane & 7)) * kWeightPitch + ((part * NG + j) * kKeys + (lane >> 3) * 8) * 2);
 #pragma unroll
-          for (int k = 0; k < 2; ++k) mma16816(o[i][k], v[x][0][2 * k], v[x][0][2 * k + 1], v[x][1][2 * k], v[x][1][2 * k + 1], q[2 * x], q[2 * x + 1]);
-      }
+          for (int x = 0; x < 2; ++x)
+#pragma unroll
+            for (int k = 0; k < 2; ++k) mma16816(o[i][k], v[x][0][2 * k], v[x][0][2 * k + 1], v[x][1][2 * k], v[x][1][2 * k + 1], q[2 * x], q[2 * x + 1]);
+        }
     }
     stage = stage + 1 == STAGES ? 0 : stage + 1;
     cur.tile += step;
@@ -333,7 +344,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) int4_tiles_kernel(const Int4A
 
 template <typename T, int D, int R>
 void launch_tiles(const Int4Attn& p, int grid, cudaStream_t st) {
-  constexpr int smem = tiles_smem<D, R>;
+  constexpr int smem = tiles_smem<T, D, R>;
   if (p.cluster) {
     NXD_ALLOW_SMEM((int4_tiles_kernel<T, D, R, true>), smem);
     launch_cluster(int4_tiles_kernel<T, D, R, true>, p, grid, kTileThreads, smem, p.cluster, st);
