@@ -57,8 +57,9 @@ NXD_DEVICE void steps_of(float lo, float hi, float off, unsigned four, F exact, 
       a = fmin(a, __shfl_xor_sync(four, a, o));
       b = fmax(b, __shfl_xor_sync(four, b, o));
     }
-    m16 = __double2half(a);
-    s16 = __double2half((b - (double)__half2float(m16)) / 15.);
+    // by way of 32 bits, as torch rounds numbers of 64 to halves (a value that the first rounding puts on a border differs)
+    m16 = __float2half_rn((float)a);
+    s16 = __float2half_rn((float)((b - (double)__half2float(m16)) / 15.));
   }
 }
 

@@ -24,33 +24,19 @@ def check(d, got, scale=None):
 
 # ------------------------------------------------------------------------------------------------------------------ append
 def check_append(q, k, v, positions, cos, sin, slots, pages, got, before, interleaved):
-    """Queries within a half step of their type and three roundings in 32 bits of numbers below 6; steps within a half step of half precision of the
-    exact ones, codes those of exact numbers between them; everything else as it was."""
+    """Queries within a half step of their type and three roundings in 32 bits of numbers below 6; steps and codes those of exact numbers, everything else
+    as it was."""
     dtype, ps = q.dtype, pages[0].codes.shape[1]
     tokens = pages[0].codes.shape[0] * ps
     want_q, written = append(q.cpu(), k.cpu(), v.cpu(), positions.cpu(), cos.cpu(), sin.cpu(), slots.cpu(), tokens, interleaved)
     assert got.dtype == dtype and got.transpose(0, 1).is_contiguous()
     assert bool(((got.double().cpu() - want_q).abs() <= torch.finfo(dtype).eps / 2 * want_q.abs() + 6 * 3 * 2.0 ** -24).all())
-    same = groups = 0
     for i, p in enumerate(pages):
         codes, steps = p.codes.cpu(), p.steps.cpu()
         for slot in range(tokens):
-            c, s = codes[slot // ps, slot % ps], steps[slot // ps, slot % ps]
-            if slot not in written:
-                assert torch.equal(c, before[i].codes[slot // ps, slot % ps].cpu()) and torch.equal(s.view(torch.int16), before[i].steps[slot // ps, slot % ps].cpu().view(torch.int16))
-                continue
-            want = packed(written[slot][i])
-            d = (s.double() - want.steps.double()).abs()
-            assert bool((d <= 2.0 ** -10 * want.steps.double().abs() + 2.0 ** -24).all())
-            equal = (d == 0).all(-2)                         # [heads, groups]
-            code_equal = (c == want.codes).unflatten(-1, (-1, 16)).all(-1)
-            assert bool((code_equal | ~equal).all())
-            # with other steps: the nearest of 16 values all the same
-            x, off = written[slot][i], (values(Pages(c, s)) - written[slot][i]).abs()
-            step, least = s.double()[..., 0, :].repeat_interleave(32, -1), s.double()[..., 1, :].repeat_interleave(32, -1)
-            assert bool((off <= step / 2 + 2.0 ** -11 * (15 * step + least.abs()) + 2.0 ** -20 * x.abs() + 16 * 2.0 ** -25).all())
-            same, groups = same + int(equal.sum()), groups + equal.numel()
-    assert same >= groups - max(2, groups // 500)            # 32 bits next to a border of half precision: about one group in 2^12
+            at = slot // ps, slot % ps
+            want = packed(written[slot][i]) if slot in written else Pages(before[i].codes[at].cpu(), before[i].steps[at].cpu())
+            assert torch.equal(codes[at], want.codes) and torch.equal(steps[at].view(torch.int16), want.steps.view(torch.int16)), (i, slot)
 
 
 @pytest.mark.parametrize("dtype, D", [(BF16, 128), (BF16, 64), (FP16, 96), (F32, 128), (F32, 32)])
