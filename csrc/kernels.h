@@ -276,9 +276,9 @@ struct Int4Append {
   bool pairs;
   long q_sb, q_sw, q_sh, k_sb, k_sw, k_sh, v_sb, v_sw, v_sh, o_sb, o_sw;
 };
-void int4_append(Int4Append p, int dt, cudaStream_t st);
+int int4_append(const Int4Append& p, int dt, cudaStream_t st);      // → launches
 void int4_gather(const Int4Pages& kp, const Int4Pages& vp, const int* slots, void* k, void* v, long n, int Hkv, int D, int ps, long tokens, int dt, cudaStream_t st);
-struct Int4Attn : PagedAttn {        // k, v: codes, their strides in units of 16 bytes, those of a pool's pages and rows together below 2^32
+struct Int4Attn : PagedAttn {        // k, v: codes, their strides in units of 16 bytes, places in a pool below 2^32
   const void *ks, *vs;               // steps, strides in rows of them (D / 8 bytes), below 2^32 alike
   long ks_sp, ks_sr, ks_sh, vs_sp, vs_sr, vs_sh;
 };

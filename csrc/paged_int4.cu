@@ -67,17 +67,17 @@ NXD_DEVICE void steps_of(float lo, float hi, float off, unsigned four, F exact, 
 // its own once more); four threads have the 32 numbers that share m and s.  Bound by HBM: 4 x 2000 tokens, 64 heads on 8, … .  Keys turn as a c - b s with what the
 // rounding of b s left put back, one rounding in all; a code whose quotient is near a border, and steps that are, are found again from the products in
 // 64 bits, so that codes are those of exact numbers.
-enum Role { kAll, kQueries0, kCache };                     // whose numbers a launch has: everybody's, queries', or keys' and values'
+enum Role { kAll, kQuery, kCache };                     // whose numbers a launch has: everybody's, queries', or keys' and values'
 template <typename T, int D0, Turn TURN, int CH, Role ROLE>
-__global__ void __launch_bounds__(kAppendThreads, ROLE == kQueries0 ? 12 : 8) int4_append_kernel(const Int4Append p) {
+__global__ void __launch_bounds__(kAppendThreads, ROLE == kQuery ? 12 : 8) int4_append_kernel(const Int4Append p) {
   const int D = D0 ? D0 : p.D;
   pdl_trigger();
   const unsigned t = blockIdx.x, item = blockIdx.y * kAppendThreads + threadIdx.x, chunks = D / (8 * CH);
   const int h = (int)(item / chunks) + (ROLE == kCache ? p.H : 0), c0 = (int)(item % chunks) * 8;
   const int w = (int)(t / (unsigned)p.B), b = (int)(t - (unsigned)w * p.B);        // tokens of all sequences beside one another, as projections leave them
   pdl_wait();
-  if (h >= (ROLE == kQueries0 ? p.H : p.H + 2 * p.Hkv)) return;
-  const bool query = ROLE == kQueries0 || (ROLE == kAll && h < p.H), key = !query && h < p.H + p.Hkv;
+  if (h >= (ROLE == kQuery ? p.H : p.H + 2 * p.Hkv)) return;
+  const bool query = ROLE == kQuery || (ROLE == kAll && h < p.H), key = !query && h < p.H + p.Hkv;
   const T* const src = query ? (const T*)p.q + b * p.q_sb + w * p.q_sw + h * p.q_sh
                        : key ? (const T*)p.k + b * p.k_sb + w * p.k_sw + (h - p.H) * p.k_sh
                              : (const T*)p.v + b * p.v_sb + w * p.v_sw + (h - p.H - p.Hkv) * p.v_sh;
@@ -249,7 +249,7 @@ __global__ void __launch_bounds__(kUnpackThreads) int4_unpack_kernel(const Int4A
   const bool key = blockIdx.z == 0;
   int page = col < p.shared_cols ? p.shared_pages[col] : p.table[b * p.table_sb + col];
   if ((unsigned)page >= (unsigned)p.pages) page = -1;
-  if (head == 0 && key && threadIdx.x == 0) table[blockIdx.x] = page < 0 ? -1 : blockIdx.x;
+  if (head == 0 && key && threadIdx.x == 0) table[blockIdx.x] = page < 0 ? -1 : (int)blockIdx.x;
   const int items = page < 0 ? 0 : min(p.ps, all_keys(p, b) - col * p.ps) * C;
   const uint8_t* const codes = key ? reinterpret_cast<const uint8_t*>(p.k) + (page * p.k_sp + head * p.k_sh) * 16 : reinterpret_cast<const uint8_t*>(p.v) + (page * p.v_sp + head * p.v_sh) * 16;
   const __half* const steps = key ? reinterpret_cast<const __half*>(p.ks) + (page * p.ks_sp + head * p.ks_sh) * (D / 16) : reinterpret_cast<const __half*>(p.vs) + (page * p.vs_sp + head * p.vs_sh) * (D / 16);
@@ -327,11 +327,10 @@ template <int D, bool CLUSTER> constexpr int rows_smem = kQueries<D, 1> + (CLUST
 // Queries are multiplied by a power of two that brings the row's largest to 2^14.  Weights p are relative to a reference M, at most 2^15 and with s at
 // most 2^15 (`room` below), so that they are halves of all their bits: 11 of each product's.  Where the output is in half precision too, weights
 // are two halves, the rounded one and what that left (22 bits).
-// TWO: so for T = half.
 template <typename T, int D, bool CLUSTER>
 __global__ void __launch_bounds__(kRowWarps * 32, 2) int4_rows_kernel(const Int4Attn p) {
-  constexpr bool TWO = std::is_same<T, __half>::value;
-  constexpr int R = 1, NG = D / 32, PITCH = kPitch<D>, WARPS = kRowWarps, THREADS = WARPS * 32, STAGE = kStage<D>, TILE = WARPS * kKeys;
+  constexpr bool TWO = std::is_same<T, __half>::value;     // weights as two halves
+  constexpr int NG = D / 32, PITCH = kPitch<D>, WARPS = kRowWarps, THREADS = WARPS * 32, STAGE = kStage<D>, TILE = WARPS * kKeys;
   constexpr int V_AT = kKeys * (D / 2), KS_AT = 2 * V_AT, VS_AT = KS_AT + kKeys * 16;
   constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u;
   extern __shared__ __align__(128) uint8_t smem[];
@@ -373,9 +372,9 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) int4_rows_kernel(const Int4
 #pragma unroll
   for (int s = 0; s < kStages - 1; ++s) ring.ask(s);
 
-  uint32_t qf[R][NG][4], qs[R];                            // queries of group g: two steps of 16 numbers; sums of queries
-  float m[R][2], l[R][2], o[R][2 * NG][4], om[R][4], unit[R][2];
-  int lim[R][2], lim_all = 0;                              // first key that a row does not see; that none of the live rows has before it
+  uint32_t qf[NG][4], qs;                                  // queries of group g: two steps of 16 numbers; sums of queries
+  float m[2], l[2], o[2 * NG][4], om[4], unit[2];          // of rows 2 quad and 2 quad + 1
+  int lim[2], lim_all = 0;                                 // first key that a row does not see; that none of the live rows has before it
   float room = 15.f;                                       // weights relative to M may be at most 2^room: 15 less what the largest s needs
   __half2 s_most2 = __half2half2(__ushort_as_half(0x3c00));                              // 2^(15 - room), twice
   bool whole = false;                                      // the pair begins in this block
@@ -386,7 +385,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) int4_rows_kernel(const Int4
     rows = min(8, p.W * p.G - row0);
     whole = CLUSTER || cur.tile == 0;
     lim_all = min(visible_keys(p, b, row0 / p.G), n);
-    if (warp < 8) {
+    {                                                      // a row a warp
       const int w = (row0 + warp) / p.G;
       const bool live = warp < rows && w < count;
       ready_query<T, D>(reinterpret_cast<const T*>(p.q) + (live ? b * p.q_sb + w * p.q_sw + (long)(cur.head * p.G + (row0 + warp) % p.G) * p.q_sh : 0), live,
@@ -395,23 +394,20 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) int4_rows_kernel(const Int4
     }
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
+    for (int g = 0; g < NG; ++g) ldmatrix_x4(qf[g], sm_q + (lane & 7) * kQPitch<D> + g * 64 + (lane >> 3) * 16);
+    qs = lds32(sm_qs + hq * 16 + quad * 4);
 #pragma unroll
-      for (int g = 0; g < NG; ++g) ldmatrix_x4(qf[i][g], sm_q + (i * 8 + (lane & 7)) * kQPitch<D> + g * 64 + (lane >> 3) * 16);
-      qs[i] = lds32(sm_qs + (i * 8 + hq) * 16 + quad * 4);
+    for (int k = 0; k < 2 * NG; ++k)
 #pragma unroll
-      for (int k = 0; k < 2 * NG; ++k)
+      for (int x = 0; x < 4; ++x) o[k][x] = 0.f;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) o[i][k][x] = 0.f;
+    for (int x = 0; x < 4; ++x) om[x] = 0.f;
 #pragma unroll
-      for (int x = 0; x < 4; ++x) om[i][x] = 0.f;
-#pragma unroll
-      for (int x = 0; x < 2; ++x) {
-        unit[i][x] = sm_unit[i * 8 + quad * 2 + x];
-        lim[i][x] = sm_lim[i * 8 + quad * 2 + x];
-        m[i][x] = kNone;
-        l[i][x] = 0.f;
-      }
+    for (int x = 0; x < 2; ++x) {
+      unit[x] = sm_unit[quad * 2 + x];
+      lim[x] = sm_lim[quad * 2 + x];
+      m[x] = kNone;
+      l[x] = 0.f;
     }
   };
 
@@ -420,64 +416,169 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) int4_rows_kernel(const Int4
     const int kvh = cur.head, b = cur.e / p.row_tiles, count = new_tokens(p, b);
     const bool direct = whole && last;
 #pragma unroll
-    for (int i = 0; i < R; ++i)
+    for (int e = 0; e < 2; ++e) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-#pragma unroll
-        for (int s = 4; s < 32; s <<= 1) l[i][e] += __shfl_xor_sync(0xffffffffu, l[i][e], s);
-        if (hq == 0) sm_m[warp][i * 8 + quad * 2 + e] = m[i][e] == kNone ? -INFINITY : m[i][e];
-      }
+      for (int s = 4; s < 32; s <<= 1) l[e] += __shfl_xor_sync(0xffffffffu, l[e], s);
+      if (hq == 0) sm_m[warp][quad * 2 + e] = m[e] == kNone ? -INFINITY : m[e];
+    }
     __syncthreads();                                       // all of the ring has been read (a cluster's), and what was read of the last pair's sums
+    // every warp's sums relative to the block's maximum
+    float f[2];
 #pragma unroll
-    for (int i = 0; i < R; ++i) {
-      if (i) __syncthreads();
-      // every warp's sums relative to the block's maximum
-      float f[2];
+    for (int e = 0; e < 2; ++e) {
+      const int row = quad * 2 + e;
+      float mn = sm_m[hq][row];
+#pragma unroll
+      for (int s = 4; s < 32; s <<= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, s));
+      f[e] = mn == -INFINITY || m[e] == kNone ? 0.f : exp2f(m[e] - mn);
+      if (hq == 0) {
+        sm_l[warp][row] = l[e] * f[e];
+        if (warp == 0) sm_bm[row] = mn;
+      }
+    }
+#pragma unroll
+    for (int g = 0; g < NG; ++g)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const int row = i * 8 + quad * 2 + e;
-        float mn = sm_m[hq][row];
-        if constexpr (WARPS == 16) mn = fmaxf(mn, sm_m[hq + 8][row]);
+        // what m adds to group g stands in row NG + g of its product
+        const float m0 = __shfl_sync(0xffffffffu, om[e], (NG + g) * 4 + quad) * f[e], f24 = f[e] * 0x1p24f, f20 = f[e] * 0x1p20f;
+        *reinterpret_cast<float4*>(sm_o + (warp * 8 + quad * 2 + e) * PITCH + g * 32 + hq * 4) =
+            make_float4(fmaf(o[2 * g][e], f24, m0), fmaf(o[2 * g][e + 2], f20, m0), fmaf(o[2 * g + 1][e], f24, m0), fmaf(o[2 * g + 1][e + 2], f20, m0));
+      }
+    __syncthreads();
+    constexpr int PER = THREADS / D;                       // rows at a time
 #pragma unroll
-        for (int s = 4; s < 32; s <<= 1) mn = fmaxf(mn, __shfl_xor_sync(0xffffffffu, mn, s));
-        f[e] = mn == -INFINITY || m[i][e] == kNone ? 0.f : exp2f(m[i][e] - mn);
-        if (hq == 0) {
-          sm_l[warp][row] = l[i][e] * f[e];
-          if (warp == 0) sm_bm[row] = mn;
-        }
+    for (int x = 0; x < 8 / PER; ++x) {
+      const int row = x * PER + (int)threadIdx.x / D, col = threadIdx.x % D;
+      if (row >= rows) break;
+      float acc = 0.f, ls = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) {
+        acc += sm_o[(w * 8 + row) * PITCH + col];
+        ls += sm_l[w][row];
+      }
+      if (CLUSTER && p.cluster > 1) {
+        sm_b[row * D + col] = acc;
+        if (col == 0) sm_bl[row] = ls;
+      } else if (direct) {
+        const int w = (row0 + row) / p.G;
+        const bool live = w < count && !(ls == 0.f);
+        reinterpret_cast<T*>(p.out)[b * p.o_sb + w * p.o_sw + (long)(kvh * p.G + (row0 + row) % p.G) * p.o_sh + col] = from_f32<T>(live ? acc / ls : 0.f);
+      } else {
+        const long slot = part_slot<false>(p, (long)cur.e * p.Hkv + kvh, blockIdx.x, whole) * p.tile_rows + row;
+        p.part_o[slot * D + col] = acc;
+        if (col == 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(sm_bm[row], ls);
+      }
+    }
+  };
+
+  // 16 keys from `key` on, which lie in shared memory at `at`
+  auto tile = [&](const uint32_t at, const int key) {
+    const int rr = lane & 15, rc = lane >> 4;              // whose 16 bytes of codes this lane has ldmatrix read: row, group
+    // scores: keys hq and hq + 8, rows 2 quad and 2 quad + 1
+    float s[4] = {0.f, 0.f, 0.f, 0.f};
+    const uint32_t km = at + KS_AT + hq * 16 + NG * 2 + (NG == 4 ? (quad & 1) * 4 : 0);
+    mma1688(s, lds32(km), lds32(km + 8 * 16), qs);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s[e] *= 0x1p-19f;          // sums of q were divided by 2^5, codes by 2^24
+    const uint2 a0 = lds64(at + KS_AT + hq * 16), b0 = lds64(at + KS_AT + (hq + 8) * 16);
+    const uint32_t ua[2] = {a0.x, a0.y}, ub[2] = {b0.x, b0.y};
+#pragma unroll
+    for (int g = 0; g < NG; g += 2) {
+      const float2 s0 = __half22float2(as_half2(ua[g / 2])), s1 = __half22float2(as_half2(ub[g / 2]));
+      uint32_t a[4];                                       // keys hq, hq + 8 of group g, of group g + 1: eight codes each
+      ldmatrix_x4(a, at + chunk_at<D>(rr, g + rc));
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        const uint32_t k0 = a[2 * x], k1 = a[2 * x + 1], k2 = k0 >> 8, k3 = k1 >> 8;
+        const float f0 = x ? s0.y : s0.x, f1 = x ? s1.y : s1.x;
+        float d[4] = {0.f, 0.f, 0.f, 0.f};
+        mma16816(d, k0 & LOW, k1 & LOW, k0 & HIGH, k1 & HIGH, qf[g + x][0], qf[g + x][1]);
+        mma16816(d, k2 & LOW, k3 & LOW, k2 & HIGH, k3 & HIGH, qf[g + x][2], qf[g + x][3]);
+        s[0] = fmaf(d[0], f0, s[0]);
+        s[1] = fmaf(d[1], f0, s[1]);
+        s[2] = fmaf(d[2], f1, s[2]);
+        s[3] = fmaf(d[3], f1, s[3]);
+      }
+    }
+    // steps of the values: row x of the operand is the x-th number of the steps (s of all groups, then m) of keys 2 quad, 2 quad + 1, and of those + 8
+    uint32_t va[2];
+    const uint32_t vs_at = at + VS_AT + rr * 16;
+    ldmatrix_x2t(va, vs_at);
+    const uint32_t mine = lds32(vs_at + (NG == 4 ? rc * 4 : 0));        // two s of one key
+    bool passed = !__hble2(as_half2(mine), s_most2);
+    if (key + kKeys > lim_all) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (key + hq + (e >> 1) * 8 >= lim[e & 1]) s[e] = -INFINITY;
+    }
+    float x[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      x[e] = fmaf(s[e], unit[e & 1], -m[e & 1]);
+      passed = passed || x[e] > room;
+    }
+    // a weight, or a weight times s, would pass 2^15: another reference, 2^3 away from that
+    if (__any_sync(0xffffffffu, passed)) {
+      // the largest s, as a half's bits (NaN: as it comes), and the power of two above it
+      const uint32_t most = __reduce_max_sync(0xffffffffu, max(mine & 0xffffu, mine >> 16));
+      if (most > (as_u32(s_most2) & 0xffffu)) {
+        const int e = min((int)(most >> 10) - 15 + 1, 16);
+        s_most2 = e < 16 ? __half2half2(__ushort_as_half((unsigned short)((e + 15) << 10))) : __half2half2(__ushort_as_half(0x7bff));
+        room = 15.f - e;
       }
 #pragma unroll
-      for (int g = 0; g < NG; ++g)
+      for (int e = 0; e < 2; ++e) {
+        float mx = fmaxf(s[e], s[e + 2]) * unit[e];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          // what m adds to group g stands in row NG + g of its product
-          const float m0 = __shfl_sync(0xffffffffu, om[i][e], (NG + g) * 4 + quad) * f[e], f24 = f[e] * 0x1p24f, f20 = f[e] * 0x1p20f;
-          const float4 x = make_float4(fmaf(o[i][2 * g][e], f24, m0), fmaf(o[i][2 * g][e + 2], f20, m0), fmaf(o[i][2 * g + 1][e], f24, m0), fmaf(o[i][2 * g + 1][e + 2], f20, m0));
-          *reinterpret_cast<float4*>(sm_o + (warp * 8 + quad * 2 + e) * PITCH + g * 32 + hq * 4) = x;
+        for (int y = 4; y < 32; y <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, y));
+        const float mn = fmaxf(m[e], mx - (room - 3.f)), f = exp2f(m[e] - mn);      // none before: 0
+        m[e] = mn;
+        l[e] *= f;
+        om[e] *= f;
+        om[e + 2] *= f;
+#pragma unroll
+        for (int k = 0; k < 2 * NG; ++k) { o[k][e] *= f; o[k][e + 2] *= f; }
+        x[e] = fmaf(s[e], unit[e], -mn);
+        x[e + 2] = fmaf(s[e + 2], unit[e], -mn);
+      }
+    }
+    uint32_t ph[2], pl[2];                                 // weights as the second product's operand: rounded, and what that left
+    {
+      float pr[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        pr[e] = exp2f(x[e]);
+        l[e & 1] += pr[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t hi = pack_half(pr[2 * e], pr[2 * e + 1]);
+        ph[e] = transpose8x8(hi);
+        if constexpr (TWO) {
+          const float2 f = __half22float2(as_half2(hi));
+          pl[e] = transpose8x8(pack_half(pr[2 * e] - f.x, pr[2 * e + 1] - f.y));
         }
-      __syncthreads();
-      constexpr int PER = THREADS / D;                     // rows at a time
+      }
+    }
+    mma16816(om, va[0], 0u, va[1], 0u, ph[0], ph[1]);
+    if constexpr (TWO) mma16816(om, va[0], 0u, va[1], 0u, pl[0], pl[1]);
 #pragma unroll
-      for (int x = 0; x < 8 / PER; ++x) {
-        const int rr = x * PER + (int)threadIdx.x / D, col = threadIdx.x % D, row = i * 8 + rr;
-        if (row >= rows) break;
-        float acc = 0.f, ls = 0.f;
+    for (int g = 0; g < NG; g += 2) {
+      uint32_t a[4];                                       // keys 2 quad.. and 8 + 2 quad.. of group g, of group g + 1: four codes of either key
+      ldmatrix_x4t(a, at + V_AT + chunk_at<D>(rr, g + rc));
 #pragma unroll
-        for (int w = 0; w < WARPS; ++w) {
-          acc += sm_o[(w * 8 + rr) * PITCH + col];
-          ls += sm_l[w][row];
-        }
-        if (CLUSTER && p.cluster > 1) {
-          sm_b[row * D + col] = acc;
-          if (col == 0) sm_bl[row] = ls;
-        } else if (direct) {
-          const int w = (row0 + row) / p.G;
-          const bool live = w < count && !(ls == 0.f);
-          reinterpret_cast<T*>(p.out)[b * p.o_sb + w * p.o_sw + (long)(kvh * p.G + (row0 + row) % p.G) * p.o_sh + col] = from_f32<T>(live ? acc / ls : 0.f);
-        } else {
-          const long slot = part_slot<false>(p, (long)cur.e * p.Hkv + kvh, blockIdx.x, whole) * p.tile_rows + row;
-          p.part_o[slot * D + col] = acc;
-          if (col == 0) *reinterpret_cast<float2*>(p.part_ml + slot * 2) = make_float2(sm_bm[row], ls);
+      for (int y = 0; y < 2; ++y) {
+        const uint32_t v0 = a[2 * y], v1 = a[2 * y + 1], v2 = v0 >> 8, v3 = v1 >> 8;
+        const __half2 s0 = as_half2(__shfl_sync(0xffffffffu, va[0], (g + y) * 4 + quad)), s1 = as_half2(__shfl_sync(0xffffffffu, va[1], (g + y) * 4 + quad));
+        const __half2 w0 = __hmul2(as_half2(ph[0]), s0), w1 = __hmul2(as_half2(ph[1]), s1);
+        mma16816(o[2 * (g + y)], v0 & LOW, v0 & HIGH, v1 & LOW, v1 & HIGH, as_u32(w0), as_u32(w1));
+        mma16816(o[2 * (g + y) + 1], v2 & LOW, v2 & HIGH, v3 & LOW, v3 & HIGH, as_u32(w0), as_u32(w1));
+        if constexpr (TWO) {                               // what the roundings of the weights and of their products with s left
+          const __half2 y0 = __hfma2(as_half2(pl[0]), s0, __hfma2(as_half2(ph[0]), s0, __hneg2(w0)));
+          const __half2 y1 = __hfma2(as_half2(pl[1]), s1, __hfma2(as_half2(ph[1]), s1, __hneg2(w1)));
+          mma16816(o[2 * (g + y)], v0 & LOW, v0 & HIGH, v1 & LOW, v1 & HIGH, as_u32(y0), as_u32(y1));
+          mma16816(o[2 * (g + y) + 1], v2 & LOW, v2 & HIGH, v3 & LOW, v3 & HIGH, as_u32(y0), as_u32(y1));
         }
       }
     }
@@ -491,152 +592,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) int4_rows_kernel(const Int4
     const bool hole = ring.holes >> stage & 1;
     ring.ask(ask_stage);
     ask_stage = ask_stage + 1 == kStages ? 0 : ask_stage + 1;
-    const int key = cur.tile * TILE + warp * kKeys;
-    if (!hole) {
-      const uint32_t at = ring.ring + stage * STAGE;
-      // scores: keys hq and hq + 8 of each 16, rows 2 quad and 2 quad + 1
-      float s[R][4];
-      const int rr = (((lane >> 3) & 1) << 3) + (lane & 7), rc = lane >> 4;
-      {
-        const uint32_t km = at + KS_AT + hq * 16 + NG * 2 + (NG == 4 ? (quad & 1) * 4 : 0);
-        const uint32_t m0 = lds32(km), m1 = lds32(km + 8 * 16);
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
-          mma1688(s[i], m0, m1, qs[i]);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) s[i][e] *= 0x1p-19f;        // sums of q were divided by 2^5, codes by 2^24
-        }
-        float ks0[NG], ks1[NG];
-        const uint2 a0 = lds64(at + KS_AT + hq * 16), b0 = lds64(at + KS_AT + (hq + 8) * 16);
-        const uint32_t ua[2] = {a0.x, a0.y}, ub[2] = {b0.x, b0.y};
-#pragma unroll
-        for (int g = 0; g < NG; g += 2) {
-          const float2 x = __half22float2(as_half2(ua[g / 2])), y = __half22float2(as_half2(ub[g / 2]));
-          ks0[g] = x.x; ks0[g + 1] = x.y;
-          ks1[g] = y.x; ks1[g + 1] = y.y;
-        }
-#pragma unroll
-        for (int g = 0; g < NG; g += 2) {
-          uint32_t a[4];                                   // keys hq, hq + 8 of group g, of group g + 1: eight codes each
-          ldmatrix_x4(a, at + chunk_at<D>(rr, g + rc));
-#pragma unroll
-          for (int x = 0; x < 2; ++x) {
-            const uint32_t k0 = a[2 * x], k1 = a[2 * x + 1], k2 = k0 >> 8, k3 = k1 >> 8;
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-              float d[4] = {0.f, 0.f, 0.f, 0.f};
-              mma16816(d, k0 & LOW, k1 & LOW, k0 & HIGH, k1 & HIGH, qf[i][g + x][0], qf[i][g + x][1]);
-              mma16816(d, k2 & LOW, k3 & LOW, k2 & HIGH, k3 & HIGH, qf[i][g + x][2], qf[i][g + x][3]);
-              s[i][0] = fmaf(d[0], ks0[g + x], s[i][0]);
-              s[i][1] = fmaf(d[1], ks0[g + x], s[i][1]);
-              s[i][2] = fmaf(d[2], ks1[g + x], s[i][2]);
-              s[i][3] = fmaf(d[3], ks1[g + x], s[i][3]);
-            }
-          }
-        }
-      }
-      // steps of the values: row x of the operand is the x-th number of the steps (s of all groups, then m) of keys 2 quad, 2 quad + 1, and of those + 8
-      uint32_t va[2], mine;
-      bool passed = false;
-      {
-        const uint32_t vs_at = at + VS_AT + (lane & 15) * 16;
-        ldmatrix_x2t(va, vs_at);
-        mine = lds32(vs_at + (NG == 4 ? (lane >> 4) * 4 : 0));    // two s of one key
-        passed = passed || !__hble2(as_half2(mine), s_most2);
-      }
-      if (key + kKeys > lim_all) {
-#pragma unroll
-          for (int i = 0; i < R; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (key + hq + (e >> 1) * 8 >= lim[i][e & 1]) s[i][e] = -INFINITY;
-      }
-      float x[R][4];
-#pragma unroll
-        for (int i = 0; i < R; ++i)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            x[i][e] = fmaf(s[i][e], unit[i][e & 1], -m[i][e & 1]);
-            passed = passed || x[i][e] > room;
-          }
-      // a weight, or a weight times s, would pass 2^15: another reference, 2^3 away from that
-      if (__any_sync(0xffffffffu, passed)) {
-        // the largest s, as a half's bits (NaN: as it comes), and the power of two above it
-        const uint32_t most = __reduce_max_sync(0xffffffffu, max(mine & 0xffffu, mine >> 16));
-        if (most > (as_u32(s_most2) & 0xffffu)) {
-          const int e = min((int)(most >> 10) - 15 + 1, 16);
-          s_most2 = e < 16 ? __half2half2(__ushort_as_half((unsigned short)((e + 15) << 10))) : __half2half2(__ushort_as_half(0x7bff));
-          room = 15.f - e;
-        }
-#pragma unroll
-        for (int i = 0; i < R; ++i)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            float mx = fmaxf(s[i][e], s[i][e + 2]) * unit[i][e];
-#pragma unroll
-            for (int y = 4; y < 32; y <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, y));
-            const float mn = fmaxf(m[i][e], mx - (room - 3.f)), f = exp2f(m[i][e] - mn);      // none before: 0
-            m[i][e] = mn;
-            l[i][e] *= f;
-            om[i][e] *= f;
-            om[i][e + 2] *= f;
-#pragma unroll
-            for (int k = 0; k < 2 * NG; ++k) { o[i][k][e] *= f; o[i][k][e + 2] *= f; }
-            x[i][e] = fmaf(s[i][e], unit[i][e], -mn);
-            x[i][e + 2] = fmaf(s[i][e + 2], unit[i][e], -mn);
-          }
-      }
-      uint32_t ph[R][2], pl[R][2];
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-          float pr[4];
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            pr[e] = exp2f(x[i][e]);
-            l[i][e & 1] += pr[e];
-          }
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint32_t hi = pack_half(pr[2 * e], pr[2 * e + 1]);
-            ph[i][e] = transpose8x8(hi);
-            if constexpr (TWO) {
-              const float2 f = __half22float2(as_half2(hi));
-              pl[i][e] = transpose8x8(pack_half(pr[2 * e] - f.x, pr[2 * e + 1] - f.y));
-            }
-          }
-        }
-      {
-#pragma unroll
-        for (int i = 0; i < R; ++i) {
-          mma16816(om[i], va[0], 0u, va[1], 0u, ph[i][0], ph[i][1]);
-          if constexpr (TWO) mma16816(om[i], va[0], 0u, va[1], 0u, pl[i][0], pl[i][1]);
-        }
-#pragma unroll
-        for (int g = 0; g < NG; g += 2) {
-          uint32_t a[4];                                   // keys 2 quad.. and 8 + 2 quad.. of group g, of group g + 1: four codes of either key
-          ldmatrix_x4t(a, at + V_AT + chunk_at<D>(rr, g + rc));
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const uint32_t v0 = a[2 * y], v1 = a[2 * y + 1], v2 = v0 >> 8, v3 = v1 >> 8;
-            const __half2 s0 = as_half2(__shfl_sync(0xffffffffu, va[0], (g + y) * 4 + quad)), s1 = as_half2(__shfl_sync(0xffffffffu, va[1], (g + y) * 4 + quad));
-#pragma unroll
-            for (int i = 0; i < R; ++i) {
-              const __half2 w0 = __hmul2(as_half2(ph[i][0]), s0), w1 = __hmul2(as_half2(ph[i][1]), s1);
-              mma16816(o[i][2 * (g + y)], v0 & LOW, v0 & HIGH, v1 & LOW, v1 & HIGH, as_u32(w0), as_u32(w1));
-              mma16816(o[i][2 * (g + y) + 1], v2 & LOW, v2 & HIGH, v3 & LOW, v3 & HIGH, as_u32(w0), as_u32(w1));
-              if constexpr (TWO) {
-                const __half2 y0 = __hfma2(as_half2(pl[i][0]), s0, __hfma2(as_half2(ph[i][0]), s0, __hneg2(w0)));
-                const __half2 y1 = __hfma2(as_half2(pl[i][1]), s1, __hfma2(as_half2(ph[i][1]), s1, __hneg2(w1)));
-                mma16816(o[i][2 * (g + y)], v0 & LOW, v0 & HIGH, v1 & LOW, v1 & HIGH, as_u32(y0), as_u32(y1));
-                mma16816(o[i][2 * (g + y) + 1], v2 & LOW, v2 & HIGH, v3 & LOW, v3 & HIGH, as_u32(y0), as_u32(y1));
-              }
-            }
-          }
-        }
-      }
-    }
+    if (!hole) tile(ring.ring + stage * STAGE, cur.tile * TILE + warp * kKeys);
     stage = stage + 1 == kStages ? 0 : stage + 1;
     cur.tile += step;
     if (!CLUSTER && (cur.tile == cur.tiles || t + 1 == tiles_left)) {
@@ -834,14 +790,16 @@ void int4_queries(const void* q, void* out, float* units, int B, int W, int H, i
   else launch_dependent(int4_queries_kernel<64>, grid, 128, 0, st, (const __nv_bfloat16*)q, (__half*)out, units, (unsigned)rows, W, H, q_sb, q_sw, q_sh);
 }
 
-void int4_append(Int4Append p, int dt, cudaStream_t st) {
+int int4_append(const Int4Append& p, int dt, cudaStream_t st) {
   const bool two = p.D % 64 == 0;                          // eight numbers of each half: four threads have the same 32 in either
   const long tokens = (long)p.B * p.W;
-  if (tokens == 0) return;
+  if (tokens == 0) return 0;
+  int launches = 0;
   auto go = [&](auto kernel, int heads) {
     const long parts = ((long)heads * (p.D / (two ? 16 : 8)) + kAppendThreads - 1) / kAppendThreads;
     if (tokens >= (1l << 31) || parts > 65535) nxd_throw("int4_append: too many tokens or heads", __FILE__, __LINE__);
     launch_dependent(kernel, dim3((unsigned)tokens, (unsigned)parts), kAppendThreads, 0, st, p);
+    ++launches;
   };
   // Queries alone take fewer registers, so that more of their threads wait for memory at a time; few tokens go by one launch.
   auto split = [&](auto all, auto queries, auto cache) {
@@ -849,7 +807,7 @@ void int4_append(Int4Append p, int dt, cudaStream_t st) {
     go(queries, p.H);
     go(cache, 2 * p.Hkv);
   };
-#define NXD_TURN(Dv, turn) split(int4_append_kernel<T, Dv, turn, 2, kAll>, int4_append_kernel<T, Dv, turn, 2, kQueries0>, int4_append_kernel<T, Dv, turn, 2, kCache>)
+#define NXD_TURN(Dv, turn) split(int4_append_kernel<T, Dv, turn, 2, kAll>, int4_append_kernel<T, Dv, turn, 2, kQuery>, int4_append_kernel<T, Dv, turn, 2, kCache>)
   auto typed = [&](auto zero) {
     using T = decltype(zero);
     if (!two) return p.pairs ? go(int4_append_kernel<T, 0, kPairs, 1, kAll>, p.H + 2 * p.Hkv) : go(int4_append_kernel<T, 0, kPart, 1, kAll>, p.H + 2 * p.Hkv);
@@ -861,6 +819,7 @@ void int4_append(Int4Append p, int dt, cudaStream_t st) {
   if (dt == kBF16) typed(__nv_bfloat16());
   else if (dt == kF16) typed(__half());
   else typed(float());
+  return launches;
 }
 
 void int4_gather(const Int4Pages& kp, const Int4Pages& vp, const int* slots, void* k, void* v, long n, int Hkv, int D, int ps, long tokens, int dt, cudaStream_t st) {

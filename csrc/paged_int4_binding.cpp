@@ -1,5 +1,4 @@
 // Bindings of the paged key/value cache in 4 bits and of the page tables: checks of arguments, workspaces, launches.
-#include <array>
 #include <cmath>
 #include <limits>
 
@@ -31,6 +30,16 @@ void check_queries(const Tensor& q, const Pool& p) {
   CHECK_ARG(q.size(0) < (1 << 20) && q.size(1) < (1 << 24) && q.size(0) * q.size(1) * q.size(2) < (1ll << 30), "too many query rows: " + list(q.sizes()));
 }
 bool float_type(const Tensor& t) { return half_type(t) || t.scalar_type() == at::kFloat; }
+// Places within a pool are counted in 32 bits: packets of 16 bytes of codes, rows of steps
+bool places_ok(const Tensor& t, int64_t unit, int64_t behind) {
+  int64_t last = behind;
+  for (int64_t d = 0; d < 3; ++d) {
+    if (t.size(d) <= 1) continue;
+    if (t.stride(d) < 0 || t.stride(d) / unit > (1ll << 32) / (t.size(d) - 1)) return false;
+    last += (t.size(d) - 1) * (t.stride(d) / unit);
+  }
+  return last < (1ll << 32) - 1;
+}
 // Codes in whole 16-byte packets, a row's steps beside one another and aligned to all of them where they are 8 or 16 bytes
 bool pages_ok(const Tensor& codes, const Tensor& steps) {
   if (codes.dim() != 4 || steps.dim() != 5 || !packets(codes)) return false;
@@ -107,8 +116,7 @@ c10::optional<Tensor> int4_append(const Tensor& q_, const Tensor& k_, const Tens
   p.k_sb = k.stride(0); p.k_sw = k.stride(1); p.k_sh = k.stride(2);
   p.v_sb = v.stride(0); p.v_sw = v.stride(1); p.v_sh = v.stride(2);
   p.o_sb = out.stride(0); p.o_sw = out.stride(1);
-  nxd::int4_append(p, dt_code(q), stream());
-  count_launches(1);
+  count_launches(nxd::int4_append(p, dt_code(q), stream()));
   return out;
 }
 
@@ -187,8 +195,8 @@ c10::optional<Tensor> int4_attention(const Tensor& q_, const Tensor& kc, const T
   check_queries(q_, pool);
   const int64_t B = q_.size(0), W = q_.size(1), H = q_.size(2), D = q_.size(3), Hkv = kc.size(2), ps = kc.size(1);
   const std::string rows = std::to_string(B);
-  CHECK_ARG(table_.dim() == 2 && table_.size(0) == B && table_.device() == q_.device() && table_.size(1) * ps < (1ll << 31),
-            "page_table must be [" + rows + ", pages of a sequence] on the queries' device");
+  CHECK_ARG(table_.dim() == 2 && table_.size(0) == B && table_.device() == q_.device() && table_.size(1) * ps < (1ll << 31) &&
+            table_.size(1) * ps * Hkv < (1ll << 38), "page_table must be [" + rows + ", pages of a sequence] on the queries' device, of fewer than 2^31 tokens");
   CHECK_ARG(positions_.dim() == 1 && positions_.size(0) == B && positions_.device() == q_.device(), "positions must be [" + rows + "] on the queries' device");
   CHECK_ARG(!lens_.has_value() || (lens_->dim() == 1 && lens_->size(0) == B && lens_->device() == q_.device()), "lens must be [" + rows + "] on the queries' device");
   CHECK_ARG(!shared_.has_value() || (shared_->dim() == 1 && shared_->device() == q_.device() && shared_->size(0) <= table_.size(1)),
@@ -196,6 +204,8 @@ c10::optional<Tensor> int4_attention(const Tensor& q_, const Tensor& kc, const T
   const double scale = scale_.has_value() ? *scale_ : 1 / std::sqrt((double)D);
   CHECK_ARG(scale > 0 && scale < 1e30, "the scale of the scores is positive");
   if (!int4_attention_ok(q_, kc, ks, vc, vs)) return c10::nullopt;
+  for (const Tensor* t : {&kc, &vc}) CHECK_ARG(places_ok(*t, 16, D / 32 - 1), "pages whose codes span 64 GB and more");
+  for (const Tensor* t : {&ks, &vs}) CHECK_ARG(places_ok(*t, D / 16, 0), "pages whose steps span 2^32 rows and more");
   CHECK_ARG(q_.is_cuda(), "the kernels' tensors are on a GPU");
   c10::cuda::CUDAGuard guard(q_.device());
   const Tensor positions = ints(positions_, at::kLong), table = as_table(table_), q = as_packets(q_);
@@ -218,8 +228,6 @@ c10::optional<Tensor> int4_attention(const Tensor& q_, const Tensor& kc, const T
   p.v_sp = vc.stride(0) / 16; p.v_sr = vc.stride(1) / 16; p.v_sh = vc.stride(2) / 16;
   p.ks_sp = ks.stride(0) / row; p.ks_sr = ks.stride(1) / row; p.ks_sh = ks.stride(2) / row;
   p.vs_sp = vs.stride(0) / row; p.vs_sr = vs.stride(1) / row; p.vs_sh = vs.stride(2) / row;
-  for (const auto& s : {std::array<long, 2>{p.k_sp, p.k_sr}, {p.v_sp, p.v_sr}, {p.ks_sp, p.ks_sr}, {p.vs_sp, p.vs_sr}})
-    CHECK_ARG(s[0] >= 0 && s[1] >= 0 && (kc.size(0) - 1) * s[0] + (ps - 1) * s[1] < (1ll << 32) - 1, "pages that span more than 64 GB");
   p.scale_log2 = (float)(scale * 1.4426950408889634);
   if (p.cols == 0) return out.zero_();               // nobody sees a key
   const nxd::PagedPlan plan = nxd::int4_plan(p);
@@ -255,6 +263,7 @@ std::vector<Tensor> assign_pages(const Tensor& table, const Tensor& held, const 
   rows(positions_, "positions");
   if (lens_.has_value()) rows(*lens_, "lens");
   if (lengths_.has_value()) rows(*lengths_, "lengths");
+  CHECK_ARG(!in_place || B <= 1 || table.stride(0) >= n, "rows of a page_table that is changed in place lie apart");
   const int64_t P = free.size(0);
   CHECK_ARG(W >= 0 && W < (1ll << 31) && ps > 0 && ps < (1ll << 31) && P < (1ll << 31) && n < (1ll << 31) && P * ps < (1ll << 31) && n * ps < (1ll << 31) &&
             B * std::max<int64_t>(W, 1) < (1ll << 31) && B < nxd::kMaxPageRows,

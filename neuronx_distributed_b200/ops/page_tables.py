@@ -44,7 +44,7 @@ def assign(page_table: torch.Tensor, held: torch.Tensor, free: torch.Tensor, spa
     return _assign_plain(page_table, held, free, span, positions, new, page_size, lens, lengths, shared, trim, short, in_place)
 
 
-def _check(page_table, held, free, span, positions, new, page_size, lens, lengths, shared, short) -> None:
+def _check(page_table, held, free, span, positions, new, page_size, lens, lengths, shared, short, in_place) -> None:
     """The refusals of ``csrc/paged_int4_binding.cpp``."""
     def need(ok, text):
         if not ok:
@@ -63,13 +63,14 @@ def _check(page_table, held, free, span, positions, new, page_size, lens, length
         need(t is None and name != "positions" or t is not None and t.shape == (B,) and t.device == dev, f"{name} must be [{B}] on the tables' device")
     need(new >= 0 and page_size > 0 and free.shape[0] * page_size < 1 << 31 and n * page_size < 1 << 31 and B * max(new, 1) < 1 << 31 and B < 1 << 15,
          f"too many tokens: {free.shape[0]} pages of {page_size}, {B} rows of {new} new tokens")
+    need(not in_place or B <= 1 or page_table.stride(0) >= n, "rows of a page_table that is changed in place lie apart")
     need(0 <= shared <= n, f"shared columns: {shared} of {n}")
     need(short is None or (short.dtype == torch.int32 and short.shape == (1,) and short.device == dev),
          "short must be an int32 tensor of one number on the tables' device")
 
 
 def _assign_plain(page_table, held, free, span, positions, new, page_size, lens, lengths, shared, trim, short, in_place) -> Tables:
-    _check(page_table, held, free, span, positions, new, page_size, lens, lengths, shared, short)
+    _check(page_table, held, free, span, positions, new, page_size, lens, lengths, shared, short, in_place)
     (B, n), P, dev = page_table.shape, free.shape[0], page_table.device
     positions = _ints(positions, torch.long).clamp(-1, 1 << 40)
     counts = torch.full_like(positions, new) if lens is None else _ints(lens, torch.long).clamp(0, new)

@@ -67,6 +67,16 @@ def refusals(device):
 
 def test_refusals():
     refusals("cpu")
+    with pytest.raises(ValueError):
+        one_row_for_all("cpu")
+
+
+def one_row_for_all(device):
+    """Rows that are one another's memory are not changed in place."""
+    z = lambda *s, dtype=torch.int32: torch.zeros(*s, dtype=dtype, device=device)  # noqa: E731
+    state = z(1, 3).expand(2, 3), z(2), z(4), z(2, dtype=torch.long), z(2, dtype=torch.long)
+    ops.page_tables.assign(*state, 1, 16)
+    ops.page_tables.assign(*state, 1, 16, in_place=True)
 
 
 def test_no_rows():

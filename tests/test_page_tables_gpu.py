@@ -4,7 +4,7 @@ import torch
 
 from page_tables_cases import CASES, seeded, state, step
 from paged_int4_cases import assign
-from test_page_tables_cpu import refusals
+from test_page_tables_cpu import one_row_for_all, refusals
 
 from neuronx_distributed_b200 import ops
 
@@ -80,6 +80,8 @@ def test_captured_on_another_stream():
 
 def test_refusals():
     refusals("cuda")
+    with pytest.raises(ValueError):
+        one_row_for_all("cuda")
     with pytest.raises(ValueError):
         ops.page_tables.assign(torch.zeros(2, 3, dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int32), torch.zeros(4, dtype=torch.int32, device="cuda"),
                                torch.zeros(2, dtype=torch.long, device="cuda"), torch.zeros(2, dtype=torch.long, device="cuda"), 1, 16)

@@ -135,3 +135,27 @@ def test_empty_calls():
     assert k.shape == v.shape == (2, 0, 2, 64)
     q = ops.paged_int4.append(d["q"][:, :0], d["k"][:, :0], d["v"][:, :0], d["positions"], torch.ones(9, 32), torch.zeros(9, 32), d["k_pages"], d["v_pages"], none)
     assert q.shape == (2, 0, 4, 64)
+
+
+@pytest.mark.skipif(ops._ext._load() is None, reason="extension not built")
+@pytest.mark.parametrize("heads_outside", [False, True])
+def test_pools_whose_places_pass_32_bits(heads_outside):
+    """The kernels count packets of 16 bytes and rows of steps in 32 bits, heads among them: a pool of 2^32 packets is refused, one of a page less is not."""
+    q, table, positions = torch.empty(1, 1, 8, 128, dtype=BF16, device="meta"), torch.empty(1, 4, dtype=torch.int32, device="meta"), torch.empty(1, dtype=torch.long, device="meta")
+
+    def pages(n):
+        shape = (8, n, 16) if heads_outside else (n, 8, 16)
+        to = (1, 2, 0, 3) if heads_outside else (0, 2, 1, 3)
+        codes = torch.empty(*shape, 64, dtype=torch.uint8, device="meta").permute(*to)
+        return codes, torch.empty(*shape, 2, 4, dtype=torch.float16, device="meta").permute(*to, 4)
+
+    small, large = pages(2 ** 23 - 1), pages(2 ** 23)
+    one = tuple(t[:1].expand(2 ** 23, *t.shape[1:]) for t in small)
+    apart = one[0], torch.empty_strided(one[1].shape, (8 * 513, 0, 0, 4, 1), dtype=torch.float16, device="meta")
+    for k, v in ((large, one), (one, large), (apart, one), (one, apart)):
+        with pytest.raises(ValueError, match="span"):
+            ops._ext._load().int4_attention(q, *k, *v, table, positions, None, None, None)
+    with pytest.raises(ValueError, match="on a GPU"):
+        ops._ext._load().int4_attention(q, *small, *small, table, positions, None, None, None)
+    with pytest.raises(ValueError, match="2.31 tokens"):
+        ops._ext._load().int4_attention(q, *small, *small, table[:, :1].expand(1, 2 ** 28), positions, None, None, None)
