@@ -265,7 +265,7 @@ std::vector<Tensor> assign_pages(const Tensor& table, const Tensor& held, const 
   if (lengths_.has_value()) rows(*lengths_, "lengths");
   CHECK_ARG(!in_place || B <= 1 || table.stride(0) >= n, "rows of a page_table that is changed in place lie apart");
   const int64_t P = free.size(0);
-  CHECK_ARG(W >= 0 && W < (1ll << 31) && ps > 0 && ps < (1ll << 31) && P < (1ll << 31) && n < (1ll << 31) && P * ps < (1ll << 31) && n * ps < (1ll << 31) &&
+  CHECK_ARG(W >= 0 && W < (1ll << 31) && ps > 0 && ps < (1ll << 31) && P < (1ll << 31) && n < (1ll << 30) && P * ps < (1ll << 31) && n * ps < (1ll << 31) &&
             B * std::max<int64_t>(W, 1) < (1ll << 31) && B < nxd::kMaxPageRows,
             "too many tokens: " + std::to_string(P) + " pages of " + std::to_string(ps) + ", " + std::to_string(B) + " rows of " + std::to_string(W) + " new tokens");
   CHECK_ARG(0 <= shared && shared <= n, "shared columns: " + std::to_string(shared) + " of " + std::to_string(n));

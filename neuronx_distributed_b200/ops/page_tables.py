@@ -61,7 +61,7 @@ def _check(page_table, held, free, span, positions, new, page_size, lens, length
          "free must be a contiguous int32 tensor with a place for every page of the pool")
     for t, name in ((positions, "positions"), (lens, "lens"), (lengths, "lengths")):
         need(t is None and name != "positions" or t is not None and t.shape == (B,) and t.device == dev, f"{name} must be [{B}] on the tables' device")
-    need(new >= 0 and page_size > 0 and free.shape[0] * page_size < 1 << 31 and n * page_size < 1 << 31 and B * max(new, 1) < 1 << 31 and B < 1 << 15,
+    need(new >= 0 and page_size > 0 and free.shape[0] * page_size < 1 << 31 and n < 1 << 30 and n * page_size < 1 << 31 and B * max(new, 1) < 1 << 31 and B < 1 << 15,
          f"too many tokens: {free.shape[0]} pages of {page_size}, {B} rows of {new} new tokens")
     need(not in_place or B <= 1 or page_table.stride(0) >= n, "rows of a page_table that is changed in place lie apart")
     need(0 <= shared <= n, f"shared columns: {shared} of {n}")
