@@ -332,7 +332,6 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) int4_rows_kernel(const Int4
   constexpr bool TWO = std::is_same<T, __half>::value;     // weights as two halves
   constexpr int NG = D / 32, PITCH = kPitch<D>, WARPS = kRowWarps, THREADS = WARPS * 32, STAGE = kStage<D>, TILE = WARPS * kKeys;
   constexpr int V_AT = kKeys * (D / 2), KS_AT = 2 * V_AT, VS_AT = KS_AT + kKeys * 16;
-  constexpr uint32_t LOW = 0x000f000fu, HIGH = 0x00f000f0u;
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ float sm_m[WARPS][8], sm_l[WARPS][8], sm_bm[8], sm_bl[8];
   __shared__ Walk sm_ahead[WARPS];
@@ -490,11 +489,11 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) int4_rows_kernel(const Int4
       ldmatrix_x4(a, at + chunk_at<D>(rr, g + rc));
 #pragma unroll
       for (int x = 0; x < 2; ++x) {
-        const uint32_t k0 = a[2 * x], k1 = a[2 * x + 1], k2 = k0 >> 8, k3 = k1 >> 8;
+        const Codes k0 = codes_of(a[2 * x]), k1 = codes_of(a[2 * x + 1]);
         const float f0 = x ? s0.y : s0.x, f1 = x ? s1.y : s1.x;
         float d[4] = {0.f, 0.f, 0.f, 0.f};
-        mma16816(d, k0 & LOW, k1 & LOW, k0 & HIGH, k1 & HIGH, qf[g + x][0], qf[g + x][1]);
-        mma16816(d, k2 & LOW, k3 & LOW, k2 & HIGH, k3 & HIGH, qf[g + x][2], qf[g + x][3]);
+        mma16816(d, k0.c0, k1.c0, k0.c1, k1.c1, qf[g + x][0], qf[g + x][1]);
+        mma16816(d, k0.c2, k1.c2, k0.c3, k1.c3, qf[g + x][2], qf[g + x][3]);
         s[0] = fmaf(d[0], f0, s[0]);
         s[1] = fmaf(d[1], f0, s[1]);
         s[2] = fmaf(d[2], f1, s[2]);
@@ -514,10 +513,8 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) int4_rows_kernel(const Int4
     }
     float x[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      x[e] = fmaf(s[e], unit[e & 1], -m[e & 1]);
-      passed = passed || x[e] > room;
-    }
+    for (int e = 0; e < 4; ++e) x[e] = fmaf(s[e], unit[e & 1], -m[e & 1]);
+    passed = passed || fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3])) > room;
     // a weight, or a weight times s, would pass 2^15: another reference, 2^3 away from that
     if (__any_sync(0xffffffffu, passed)) {
       // the largest s, as a half's bits (NaN: as it comes), and the power of two above it
@@ -569,16 +566,16 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) int4_rows_kernel(const Int4
       ldmatrix_x4t(a, at + V_AT + chunk_at<D>(rr, g + rc));
 #pragma unroll
       for (int y = 0; y < 2; ++y) {
-        const uint32_t v0 = a[2 * y], v1 = a[2 * y + 1], v2 = v0 >> 8, v3 = v1 >> 8;
+        const Codes v0 = codes_of(a[2 * y]), v1 = codes_of(a[2 * y + 1]);
         const __half2 s0 = as_half2(__shfl_sync(0xffffffffu, va[0], (g + y) * 4 + quad)), s1 = as_half2(__shfl_sync(0xffffffffu, va[1], (g + y) * 4 + quad));
         const __half2 w0 = __hmul2(as_half2(ph[0]), s0), w1 = __hmul2(as_half2(ph[1]), s1);
-        mma16816(o[2 * (g + y)], v0 & LOW, v0 & HIGH, v1 & LOW, v1 & HIGH, as_u32(w0), as_u32(w1));
-        mma16816(o[2 * (g + y) + 1], v2 & LOW, v2 & HIGH, v3 & LOW, v3 & HIGH, as_u32(w0), as_u32(w1));
+        mma16816(o[2 * (g + y)], v0.c0, v0.c1, v1.c0, v1.c1, as_u32(w0), as_u32(w1));
+        mma16816(o[2 * (g + y) + 1], v0.c2, v0.c3, v1.c2, v1.c3, as_u32(w0), as_u32(w1));
         if constexpr (TWO) {                               // what the roundings of the weights and of their products with s left
           const __half2 y0 = __hfma2(as_half2(pl[0]), s0, __hfma2(as_half2(ph[0]), s0, __hneg2(w0)));
           const __half2 y1 = __hfma2(as_half2(pl[1]), s1, __hfma2(as_half2(ph[1]), s1, __hneg2(w1)));
-          mma16816(o[2 * (g + y)], v0 & LOW, v0 & HIGH, v1 & LOW, v1 & HIGH, as_u32(y0), as_u32(y1));
-          mma16816(o[2 * (g + y) + 1], v2 & LOW, v2 & HIGH, v3 & LOW, v3 & HIGH, as_u32(y0), as_u32(y1));
+          mma16816(o[2 * (g + y)], v0.c0, v0.c1, v1.c0, v1.c1, as_u32(y0), as_u32(y1));
+          mma16816(o[2 * (g + y) + 1], v0.c2, v0.c3, v1.c2, v1.c3, as_u32(y0), as_u32(y1));
         }
       }
     }
@@ -589,7 +586,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) int4_rows_kernel(const Int4
   for (int t = 0; t < tiles_left; ++t) {
     cp_async_wait<kStages - 2>();
     __syncwarp();                                          // tile t of all lanes is there; all lanes are done with tile t - 1
-    const bool hole = ring.holes >> stage & 1;
+    const bool hole = ring.template hole<kStages>();
     ring.ask(ask_stage);
     ask_stage = ask_stage + 1 == kStages ? 0 : ask_stage + 1;
     if (!hole) tile(ring.ring + stage * STAGE, cur.tile * TILE + warp * kKeys);

@@ -25,6 +25,10 @@ template <int BYTES> NXD_DEVICE void cp_async(uint32_t dst, const void* src, boo
   if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(live ? 16 : 0) : "memory");
   else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(dst), "l"(src), "r"(live ? BYTES : 0), "n"(BYTES) : "memory");
 }
+template <int BYTES> NXD_DEVICE void cp_async(uint32_t dst, const void* src) {
+  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+  else asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
 NXD_DEVICE void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> NXD_DEVICE void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 NXD_DEVICE void ldmatrix_x4(uint32_t (&r)[4], uint32_t addr) {
@@ -72,6 +76,13 @@ NXD_DEVICE float remote(const float* at, int rank) {       // the same place in 
 NXD_DEVICE __half2 as_half2(uint32_t v) { return *reinterpret_cast<__half2*>(&v); }
 NXD_DEVICE uint32_t as_u32(__half2 v) { return *reinterpret_cast<uint32_t*>(&v); }
 NXD_DEVICE uint32_t pack_half(float lo, float hi) { return as_u32(__floats2half2_rn(lo, hi)); }
+// Codes 0 to 3 of either half of a word as halves: the denormals c 2^-24, those of 1 and 3 times 16.  The last by a difference, which is exact and leaves the pipe of
+// logic, the one that these kernels fill, one of five instructions less.
+struct Codes { uint32_t c0, c1, c2, c3; };
+NXD_DEVICE Codes codes_of(uint32_t w) {
+  const uint32_t up = __byte_perm(w, 0, 0x4341), c2 = up & 0x000f000fu;
+  return {w & 0x000f000fu, w & 0x00f000f0u, c2, as_u32(__hsub2(as_half2(up), as_half2(c2)))};
+}
 // 16-byte chunk c of row r of a tile of codes lies at chunk c ^ (…): ldmatrix meets no bank twice
 template <int D> NXD_DEVICE uint32_t chunk_at(int r, int c) { return r * (D / 2) + ((c ^ (D == 128 ? (r >> 1) & 3 : (r >> 2) & 1)) << 4); }
 
@@ -148,7 +159,7 @@ struct Ring {
   uint32_t kc = kHole, vc = 0, ks = 0, vs = 0;             // where the warp's keys in 32 tiles lie, a tile a lane; no page there: kHole
   int asked = 0, next_page = 32, tile, last, n;            // tiles that have been asked for, the next one's lane; the pair's next tile, tiles, keys
   const int tiles, step;                                   // of the block
-  uint32_t holes = 0;                                      // bit s: none of the warp's keys in stage s is there
+  uint32_t holes = 0;                                      // bit i: there is no page for the warp's keys of the tile that was asked for i before the last one
 
   NXD_DEVICE Ring(const Int4Attn& p_, Walk* pair_, const Walk& first, int tiles_, int step_, uint32_t ring_, int warp_, int lane_)
       : p(p_), pair(pair_), warp(warp_), lane(lane_), ring(ring_), dst0(ring_ + chunk_at<D>(lane_ / CH, lane_ % CH)),
@@ -192,23 +203,38 @@ struct Ring {
       ++next_page;
       const bool there = k != kHole;
       const int row = lane / CH, seen = there ? n - (tile * TILE + warp * kKeys) : 0;          // keys that anybody sees
-      const uint8_t* const kb = reinterpret_cast<const uint8_t*>(p.k) + (uint64_t)(there ? k + k_mine : 0u) * 16;
-      const uint8_t* const vb = reinterpret_cast<const uint8_t*>(p.v) + (uint64_t)(v + (there ? v_mine : 0u)) * 16;
-      const uint8_t* const sb = reinterpret_cast<const uint8_t*>(lane < 16 ? p.ks : p.vs) + (uint64_t)((lane < 16 ? sk : sv) + (there ? s_mine : 0u)) * (NG * 4);
-      const uint32_t to = stage * STAGE;
-      cp_async<16>(dst0 + to, kb, row < seen);
-      cp_async<16>(dst0 + to + V_AT, vb, row < seen);
-      if constexpr (PASS < 16) {
-        cp_async<16>(dst1 + to, kb + (there ? PASS * p.k_sr * 16 : 0), PASS + row < seen);
-        cp_async<16>(dst1 + to + V_AT, vb + (there ? PASS * p.v_sr * 16 : 0), PASS + row < seen);
+      const uint8_t* const kp = reinterpret_cast<const uint8_t*>(p.k);
+      const uint8_t* const vp = reinterpret_cast<const uint8_t*>(p.v);
+      const uint8_t* const sp = reinterpret_cast<const uint8_t*>(lane < 16 ? p.ks : p.vs);
+      const uint32_t to = stage * STAGE, ka = k + k_mine, va = v + v_mine, sa = (lane < 16 ? sk : sv) + s_mine;
+      const uint32_t kb = ka + PASS * (uint32_t)p.k_sr, vb = va + PASS * (uint32_t)p.v_sr;
+      if (seen >= kKeys) {                                 // all of them
+        cp_async<16>(dst0 + to, kp + (uint64_t)ka * 16);
+        cp_async<16>(dst0 + to + V_AT, vp + (uint64_t)va * 16);
+        if constexpr (PASS < 16) {
+          cp_async<16>(dst1 + to, kp + (uint64_t)kb * 16);
+          cp_async<16>(dst1 + to + V_AT, vp + (uint64_t)vb * 16);
+        }
+        cp_async<NG * 4>(ring + to + KS_AT + lane * 16, sp + (uint64_t)sa * (NG * 4));
+      } else {                                             // the others are zeros; addresses of what is not read stay inside all the same
+        cp_async<16>(dst0 + to, kp + (uint64_t)(row < seen ? ka : 0u) * 16, row < seen);
+        cp_async<16>(dst0 + to + V_AT, vp + (uint64_t)(row < seen ? va : 0u) * 16, row < seen);
+        if constexpr (PASS < 16) {
+          cp_async<16>(dst1 + to, kp + (uint64_t)(PASS + row < seen ? kb : 0u) * 16, PASS + row < seen);
+          cp_async<16>(dst1 + to + V_AT, vp + (uint64_t)(PASS + row < seen ? vb : 0u) * 16, PASS + row < seen);
+        }
+        cp_async<NG * 4>(ring + to + KS_AT + lane * 16, sp + (uint64_t)((lane & 15) < seen ? sa : 0u) * (NG * 4), (lane & 15) < seen);
       }
-      cp_async<NG * 4>(ring + to + KS_AT + lane * 16, sb, (lane & 15) < seen);
-      holes = (holes & ~(1u << stage)) | (there ? 0u : 1u << stage);
+      holes = holes * 2 + !there;
       ++asked;
       tile += step;
+    } else {
+      holes *= 2;
     }
     cp_async_commit();
   }
+  template <int STAGES> NXD_DEVICE bool hole() const { return holes >> (STAGES - 2) & 1; }         // of the tile that comes next, before another one is asked for
+
 };
 
 // A warp makes a row of queries ready: number d of a group at (d % 4) 8 + d / 4, so that four 8 x 8 matrices of a group are the operands of its two products; odd

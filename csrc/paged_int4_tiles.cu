@@ -193,15 +193,15 @@ __global__ void __launch_bounds__(kTileThreads, 2) int4_tiles_kernel(const Int4A
         ldmatrix_x4(a, at + chunk_at<D>((((lane >> 3) & 1) << 3) + (lane & 7), g + (lane >> 4)));
 #pragma unroll
         for (int x = 0; x < 2; ++x) {
-          const uint32_t k0 = a[2 * x], k1 = a[2 * x + 1], k2 = k0 >> 8, k3 = k1 >> 8;
+          const Codes k0 = codes_of(a[2 * x]), k1 = codes_of(a[2 * x + 1]);
           const float f0 = x ? k0s.y : k0s.x, f1 = x ? k1s.y : k1s.x;
 #pragma unroll
           for (int i = 0; i < R; ++i) {
             uint32_t q[4];
             ldmatrix_x4(q, sm_q + (i * 8 + (lane & 7)) * kQPitch<D> + (g + x) * 64 + (lane >> 3) * 16);
             float d[4] = {0.f, 0.f, 0.f, 0.f};
-            mma16816(d, k0 & LOW, k1 & LOW, k0 & HIGH, k1 & HIGH, q[0], q[1]);
-            mma16816(d, k2 & LOW, k3 & LOW, k2 & HIGH, k3 & HIGH, q[2], q[3]);
+            mma16816(d, k0.c0, k1.c0, k0.c1, k1.c1, q[0], q[1]);
+            mma16816(d, k0.c2, k1.c2, k0.c3, k1.c3, q[2], q[3]);
             s[i][0] = fmaf(d[0], f0, s[i][0]);
             s[i][1] = fmaf(d[1], f0, s[i][1]);
             s[i][2] = fmaf(d[2], f1, s[i][2]);
@@ -211,7 +211,7 @@ __global__ void __launch_bounds__(kTileThreads, 2) int4_tiles_kernel(const Int4A
       }
     }
     const int key = cur.tile * kTileKeys + warp * kKeys;
-    const bool hole = ring.holes >> stage & 1;
+    const bool hole = ring.template hole<STAGES>();
     if (hole || key + kKeys > lim_all) {
 #pragma unroll
       for (int i = 0; i < R; ++i)
