@@ -17,6 +17,8 @@ using namespace int4;
 
 // ---------------------------------------------------------------------------------------------------------------- append
 constexpr int kAppendThreads = 128;
+// From here on queries go by a launch of their own, which takes fewer registers, so that more of its threads wait for memory at a time (us, one launch / two: 1 token of 32
+// heads 4.1 / 5.4, 4 x 500 tokens of 64 heads on 8 alike, 4 x 2000 100 / 95).
 constexpr long kSplitTokens = 2000;
 
 NXD_DEVICE float min_nan(float a, float b) { float r; asm("min.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b)); return r; }
@@ -64,9 +66,10 @@ NXD_DEVICE void steps_of(float lo, float hi, float off, unsigned four, F exact, 
 }
 
 // A thread has CH times eight numbers of one head, half a head apart, so that with kHalves all that turns together is its own (kPart reads the eight that turn with
-// its own once more); four threads have the 32 numbers that share m and s.  Bound by HBM: 4 x 2000 tokens, 64 heads on 8, … .  Keys turn as a c - b s with what the
-// rounding of b s left put back, one rounding in all; a code whose quotient is near a border, and steps that are, are found again from the products in
-// 64 bits, so that codes are those of exact numbers.
+// its own once more); four threads have the 32 numbers that share m and s.  Keys turn as a c - b s with what the rounding of b s left put back, one rounding in all; a
+// code whose quotient is near a border, and steps that are, are found again from the products in 64 bits, so that codes are those of exact numbers.  Queries
+// are bound by HBM (4 x 2000 tokens of 64 heads, a quarter padding: 40 us, 0.75 of the copy rate), keys and values by their arithmetic: 8 heads of those tokens 25 us,
+// where memory would take 7; a call for single tokens by its launch, 4 us.
 enum Role { kAll, kQuery, kCache };                     // whose numbers a launch has: everybody's, queries', or keys' and values'
 template <typename T, int D0, Turn TURN, int CH, Role ROLE>
 __global__ void __launch_bounds__(kAppendThreads, ROLE == kQuery ? 12 : 8) int4_append_kernel(const Int4Append p) {
@@ -204,7 +207,8 @@ __global__ void __launch_bounds__(kAppendThreads, ROLE == kQuery ? 12 : 8) int4_
 
 // ---------------------------------------------------------------------------------------------------------------- gather
 constexpr int kGatherThreads = 128;
-// Tokens at slots as numbers of T: a block has a token's keys or values (or, with many heads, a part of them), a thread eight numbers at a time.  Bound by HBM.
+// Tokens at slots as numbers of T: a block has a token's keys or values (or, with many heads, a part of them), a thread eight numbers at a time.  Bound by the start of many
+// small blocks: 4 x 2000 tokens of 8 heads 17 us, where the 43 MB that move would take 7.
 template <typename T, int D0>
 __global__ void __launch_bounds__(kGatherThreads) int4_gather_kernel(const Int4Pages kp, const Int4Pages vp, const int* slots, T* k, T* v, int Hkv, int D1, int ps, long tokens) {
   const int D = D0 ? D0 : D1, items = Hkv * (D / 8);
@@ -283,7 +287,8 @@ __global__ void __launch_bounds__(kUnpackThreads) int4_unpack_kernel(const Int4A
   }
 }
 
-// Queries as halves: a row is multiplied by a power of two that brings its largest number to 2^14; the row's unit takes that back.  A thread has eight numbers.
+// Queries as halves: a row is multiplied by a power of two that brings its largest number to 2^14; the row's unit takes that back.  A thread has
+// eight numbers.  2 x 1000 tokens of 48 heads of 64: 6 us, 25 MB.
 template <int D>
 __global__ void __launch_bounds__(128) int4_queries_kernel(const __nv_bfloat16* q, __half* out, float* units, unsigned rows, unsigned W, unsigned H, long q_sb, long q_sw,
                                                            long q_sh) {
@@ -327,6 +332,9 @@ template <int D, bool CLUSTER> constexpr int rows_smem = kQueries<D, 1> + (CLUST
 // Queries are multiplied by a power of two that brings the row's largest to 2^14.  Weights p are relative to a reference M, at most 2^15 and with s at
 // most 2^15 (`room` below), so that they are halves of all their bits: 11 of each product's.  Where the output is in half precision too, weights
 // are two halves, the rounded one and what that left (22 bits).
+//
+// Bound by instructions: some 220 of a warp for 16 keys, 18 of them products of 8 cycles each, 1030 cycles an SM for 128 keys where memory would take 650 (16 sequences of 8192
+// keys, 8 heads: 37 us, 3.4 TB/s; copies alone take 26).
 template <typename T, int D, bool CLUSTER>
 __global__ void __launch_bounds__(kRowWarps * 32, 2) int4_rows_kernel(const Int4Attn p) {
   constexpr bool TWO = std::is_same<T, __half>::value;     // weights as two halves
@@ -609,7 +617,7 @@ __global__ void __launch_bounds__(kRowWarps * 32, 2) int4_rows_kernel(const Int4
 }
 
 // Joins the parts of pairs that are cut: block (x, r) row r of pair x, or, where there are fewer blocks than pairs (CUTS), of the pair that is cut first in front
-// of block x + 1's share; each warp has a quarter of the parts.
+// of block x + 1's share; each warp has a quarter of the parts.  Bound by its start and two dependent loads, 5 us.
 template <typename T, int D, bool CUTS>
 __global__ void __launch_bounds__(kThreads) int4_merge_kernel(const Int4Attn p, int grid, float factor) {
   constexpr int C = D / 32, AHEAD = 8;
@@ -798,7 +806,6 @@ int int4_append(const Int4Append& p, int dt, cudaStream_t st) {
     launch_dependent(kernel, dim3((unsigned)tokens, (unsigned)parts), kAppendThreads, 0, st, p);
     ++launches;
   };
-  // Queries alone take fewer registers, so that more of their threads wait for memory at a time; few tokens go by one launch.
   auto split = [&](auto all, auto queries, auto cache) {
     if (tokens < kSplitTokens) return go(all, p.H + 2 * p.Hkv);
     go(queries, p.H);
