@@ -1,6 +1,7 @@
 // What the bindings of the paged caches check and convert alike.
 #pragma once
 #include <ATen/cuda/CUDAContext.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/extension.h>
 
@@ -45,10 +46,13 @@ Tensor as_table(const Tensor& t) {
   return t.scalar_type() == at::kInt && (t.dim() != 2 || t.size(1) <= 1 || t.stride(1) == 1) ? t : t.to(at::kInt).contiguous();
 }
 
+// Memory of a GPU without a walk through the dispatcher, which costs these calls 0.5 us of 7 for each tensor that they return
+Tensor empty_on(at::IntArrayRef sizes, at::ScalarType type, const at::Device& device) { return Tensor(at::detail::empty_cuda(sizes, type, device, c10::nullopt)); }
+
 // [B, W, H, D] with tokens first in memory, as the layers around take and leave it
 Tensor rows_out(const Tensor& q) {
   const int64_t B = q.size(0), W = q.size(1), H = q.size(2), D = q.size(3);
-  return at::empty_strided({B, W, H, D}, {H * D, B * H * D, D, 1}, q.options());
+  return Tensor(at::detail::empty_strided_cuda({B, W, H, D}, {H * D, B * H * D, D, 1}, q.scalar_type(), q.device()));
 }
 
 }  // namespace

@@ -130,7 +130,7 @@ c10::optional<std::vector<Tensor>> int4_gather(const Tensor& kc, const Tensor& k
   c10::cuda::CUDAGuard guard(kc.device());
   const Tensor slots = as_slots(slots_, slots_.size(0), slots_.size(1), kc);
   const int64_t B = slots.size(0), W = slots.size(1), Hkv = kc.size(2), D = 2 * kc.size(3);
-  Tensor k = at::empty({B, W, Hkv, D}, kc.options().dtype(type)), v = at::empty_like(k);
+  Tensor k = empty_on({B, W, Hkv, D}, type, kc.device()), v = empty_on({B, W, Hkv, D}, type, kc.device());
   nxd::int4_gather(pages_of(kc, ks), pages_of(vc, vs), slots.data_ptr<int>(), k.data_ptr(), v.data_ptr(), B * W, (int)Hkv, (int)D, (int)kc.size(1),
                    kc.size(0) * kc.size(1), dt_code(k), stream());
   count_launches(k.numel() > 0);
@@ -141,20 +141,21 @@ c10::optional<std::vector<Tensor>> int4_gather(const Tensor& kc, const Tensor& k
 constexpr int64_t kUnpacked = 256ll << 20;
 
 // Many rows: their sequences' pages are unpacked to halves, which the attention on the tensor memory reads
-void attend_portion(const nxd::Int4Attn& p, const Tensor& q, const Tensor& out, int64_t D, const at::TensorOptions& on) {
+void attend_portion(const nxd::Int4Attn& p, const Tensor& q, int64_t D) {
   const int64_t head = (int64_t)p.cols * p.ps * D * 4, each = std::max<int64_t>(head, 1) * p.Hkv;                   // bytes of a head, of a sequence
   const int64_t seqs = std::min<int64_t>(p.B, std::max<int64_t>(1, kUnpacked / each));
   const int64_t heads = std::min<int64_t>(p.Hkv, std::max<int64_t>(1, kUnpacked / std::max<int64_t>(head, 1)));
   const bool bf16 = q.scalar_type() == at::kBFloat16;
   Tensor q16 = q, units;
   if (bf16) {
-    q16 = at::empty({p.B, p.W, (int64_t)p.G * p.Hkv, D}, q.options().dtype(at::kHalf));
-    units = at::empty({p.B, p.W, (int64_t)p.G * p.Hkv}, q.options().dtype(at::kFloat));
+    q16 = empty_on({p.B, p.W, (int64_t)p.G * p.Hkv, D}, at::kHalf, q.device());
+    units = empty_on({p.B, p.W, (int64_t)p.G * p.Hkv}, at::kFloat, q.device());
     nxd::int4_queries(q.data_ptr(), q16.data_ptr(), units.data_ptr<float>(), p.B, p.W, p.G * p.Hkv, (int)D, p.q_sb, p.q_sw, p.q_sh, stream());
     count_launches(1);
   }
   const int64_t pages = seqs * p.cols;
-  const Tensor k16 = at::empty({pages, heads, p.ps, D}, on.dtype(at::kHalf)), v16 = at::empty_like(k16), table = at::empty({seqs, p.cols}, on.dtype(at::kInt));
+  const Tensor k16 = empty_on({pages, heads, p.ps, D}, at::kHalf, q.device()), v16 = empty_on({pages, heads, p.ps, D}, at::kHalf, q.device());
+  const Tensor table = empty_on({seqs, p.cols}, at::kInt, q.device());
   for (int64_t b = 0; b < p.B; b += seqs)
     for (int64_t h = 0; h < p.Hkv; h += heads) {
       nxd::Int4Attn from = p;
@@ -180,7 +181,7 @@ void attend_portion(const nxd::Int4Attn& p, const Tensor& q, const Tensor& out, 
       to.wait_ns = 2000000000;
       const nxd::PagedPlan plan = nxd::paged_plan(to);
       Tensor work;
-      if (plan.slots > 0) work = at::empty({plan.slots * (D + 2)}, on.dtype(at::kFloat));
+      if (plan.slots > 0) work = empty_on({plan.slots * (D + 2)}, at::kFloat, q.device());
       to.part_o = to.pre_o = work.defined() ? work.data_ptr<float>() : nullptr;
       to.part_ml = to.pre_ml = to.part_o + plan.slots * D;
       count_launches(1 + nxd::paged_attention_half(to, plan, (int)D, bf16 ? nxd::kBF16 : nxd::kF16, stream()));
@@ -232,11 +233,11 @@ c10::optional<Tensor> int4_attention(const Tensor& q_, const Tensor& kc, const T
   if (p.cols == 0) return out.zero_();               // nobody sees a key
   const nxd::PagedPlan plan = nxd::int4_plan(p);
   if (plan.tiles) {
-    attend_portion(p, q, out, D, kc.options());
+    attend_portion(p, q, D);
     return out;
   }
   Tensor work;                                     // parts of pairs that are cut: sums and statistics
-  if (plan.slots > 0) work = at::empty({plan.slots * (D + 2)}, q.options().dtype(at::kFloat));
+  if (plan.slots > 0) work = empty_on({plan.slots * (D + 2)}, at::kFloat, q.device());
   p.part_o = work.defined() ? work.data_ptr<float>() : nullptr;
   p.part_ml = p.part_o + plan.slots * D;
   count_launches(nxd::int4_attention(p, plan, (int)D, dt_code(q), stream()));
@@ -274,9 +275,10 @@ std::vector<Tensor> assign_pages(const Tensor& table, const Tensor& held, const 
   c10::cuda::CUDAGuard guard(table.device());
   const Tensor positions = ints(positions_, at::kLong);
   const c10::optional<Tensor> lens = ints(lens_, at::kLong), lengths = ints(lengths_, at::kLong);
-  const Tensor table_out = in_place ? table : at::empty({B, n}, table.options()), held_out = in_place ? held : at::empty_like(held);
-  const Tensor free_out = in_place ? free : at::empty_like(free), span_out = in_place ? span : at::empty_like(span);
-  Tensor slots = at::empty({B, W}, table.options());
+  const at::Device on = table.device();
+  const Tensor table_out = in_place ? table : empty_on({B, n}, at::kInt, on), held_out = in_place ? held : empty_on({B}, at::kInt, on);
+  const Tensor free_out = in_place ? free : empty_on({P}, at::kInt, on), span_out = in_place ? span : empty_on({2}, at::kLong, on);
+  const Tensor slots = empty_on({B, W}, at::kInt, on);
   nxd::PageTables p{};
   p.table = table.data_ptr<int>(); p.held = held.data_ptr<int>(); p.free = free.data_ptr<int>(); p.span = span.data_ptr<long>();
   p.positions = positions.data_ptr<long>();

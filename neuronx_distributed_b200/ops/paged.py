@@ -28,8 +28,9 @@ def _table(t: torch.Tensor) -> torch.Tensor:
 
 
 def _no_gradient(name: str, *tensors: torch.Tensor) -> None:
-    if torch.is_grad_enabled() and any(t.requires_grad for t in tensors):
-        raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or with tensors that ask for none")
+    for t in tensors:
+        if t.requires_grad and torch.is_grad_enabled():
+            raise RuntimeError(f"{name} has no gradient: call it under torch.no_grad(), or with tensors that ask for none")
 
 
 def _kernels(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, ok: str):
