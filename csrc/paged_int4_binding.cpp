@@ -140,19 +140,15 @@ c10::optional<std::vector<Tensor>> int4_gather(const Tensor& kc, const Tensor& k
 // Bytes of unpacked keys and values at a time: sequences, then key/value heads, in turns where there are more
 constexpr int64_t kUnpacked = 256ll << 20;
 
-// Many rows: their sequences' pages are unpacked to halves, which the attention on the tensor memory reads
+// Many rows of bf16: their sequences' pages are unpacked to halves, which the attention on the tensor memory reads
 void attend_portion(const nxd::Int4Attn& p, const Tensor& q, int64_t D) {
   const int64_t head = (int64_t)p.cols * p.ps * D * 4, each = std::max<int64_t>(head, 1) * p.Hkv;                   // bytes of a head, of a sequence
   const int64_t seqs = std::min<int64_t>(p.B, std::max<int64_t>(1, kUnpacked / each));
   const int64_t heads = std::min<int64_t>(p.Hkv, std::max<int64_t>(1, kUnpacked / std::max<int64_t>(head, 1)));
-  const bool bf16 = q.scalar_type() == at::kBFloat16;
-  Tensor q16 = q, units;
-  if (bf16) {
-    q16 = empty_on({p.B, p.W, (int64_t)p.G * p.Hkv, D}, at::kHalf, q.device());
-    units = empty_on({p.B, p.W, (int64_t)p.G * p.Hkv}, at::kFloat, q.device());
-    nxd::int4_queries(q.data_ptr(), q16.data_ptr(), units.data_ptr<float>(), p.B, p.W, p.G * p.Hkv, (int)D, p.q_sb, p.q_sw, p.q_sh, stream());
-    count_launches(1);
-  }
+  const int H = p.G * p.Hkv;
+  const Tensor q16 = empty_on({p.B, p.W, H, D}, at::kHalf, q.device()), units = empty_on({p.B, p.W, H}, at::kFloat, q.device());
+  nxd::int4_queries(q.data_ptr(), q16.data_ptr(), units.data_ptr<float>(), p.B, p.W, H, (int)D, p.q_sb, p.q_sw, p.q_sh, stream());
+  count_launches(1);
   const int64_t pages = seqs * p.cols;
   const Tensor k16 = empty_on({pages, heads, p.ps, D}, at::kHalf, q.device()), v16 = empty_on({pages, heads, p.ps, D}, at::kHalf, q.device());
   const Tensor table = empty_on({seqs, p.cols}, at::kInt, q.device());
@@ -175,16 +171,16 @@ void attend_portion(const nxd::Int4Attn& p, const Tensor& q, int64_t D) {
       to.table = table.data_ptr<int>(); to.table_sb = p.cols;
       to.shared_pages = nullptr; to.shared_cols = 0;
       to.pages = (int)pages;
-      to.k_sp = to.v_sp = heads * p.ps * D; to.k_sh = to.v_sh = p.ps * D; to.k_sr = to.v_sr = D;
-      to.units = bf16 ? units.data_ptr<float>() + b * units.stride(0) + h * p.G : nullptr;
-      to.u_sb = bf16 ? units.stride(0) : 0; to.u_sw = bf16 ? units.stride(1) : 0;
+      to.k_sp = to.v_sp = (int64_t)from.Hkv * p.ps * D; to.k_sh = to.v_sh = p.ps * D; to.k_sr = to.v_sr = D;
+      to.units = units.data_ptr<float>() + b * units.stride(0) + h * p.G;
+      to.u_sb = units.stride(0); to.u_sw = units.stride(1);
       to.wait_ns = 2000000000;
       const nxd::PagedPlan plan = nxd::paged_plan(to);
       Tensor work;
       if (plan.slots > 0) work = empty_on({plan.slots * (D + 2)}, at::kFloat, q.device());
       to.part_o = to.pre_o = work.defined() ? work.data_ptr<float>() : nullptr;
       to.part_ml = to.pre_ml = to.part_o + plan.slots * D;
-      count_launches(1 + nxd::paged_attention_half(to, plan, (int)D, bf16 ? nxd::kBF16 : nxd::kF16, stream()));
+      count_launches(1 + nxd::paged_attention_half(to, plan, (int)D, nxd::kBF16, stream()));
     }
 }
 
@@ -231,7 +227,7 @@ c10::optional<Tensor> int4_attention(const Tensor& q_, const Tensor& kc, const T
   p.vs_sp = vs.stride(0) / row; p.vs_sr = vs.stride(1) / row; p.vs_sh = vs.stride(2) / row;
   p.scale_log2 = (float)(scale * 1.4426950408889634);
   if (p.cols == 0) return out.zero_();               // nobody sees a key
-  const nxd::PagedPlan plan = nxd::int4_plan(p);
+  const nxd::PagedPlan plan = nxd::int4_plan(p, dt_code(q));
   if (plan.tiles) {
     attend_portion(p, q, D);
     return out;

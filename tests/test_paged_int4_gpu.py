@@ -327,6 +327,17 @@ def test_on_another_stream_and_captured_twice():
     torch.cuda.current_stream().wait_stream(side)
 
 
+@pytest.mark.parametrize("B, H, shared", [(1, 3, 0), (3, 1, 0), (3, 1, 1)])
+def test_portions_whose_pages_are_unpacked_in_unlike_turns(B, H, shared):
+    """Tables of 200,000 tokens, of which a few hundred are there: two heads, or two sequences, are unpacked in the first turn, and one in the second."""
+    d = make(5, "cuda", BF16, B, 48, H, H, 128, 128, [300, 17, 411][:B])
+    d["table"] = torch.cat([d["table"], torch.full((B, 200000 // 128 - d["table"].shape[1]), -1, dtype=torch.int32, device="cuda")], 1)
+    if shared:
+        d["shared_pages"] = d["table"][0, :1].contiguous()
+        d["table"][1:, 0] = -1
+    check(d, attend(d))
+
+
 def test_refusals():
     refusals("cuda")
     d = make(1, "cuda", BF16, 2, 3, 4, 2, 64, 16, [3, 20])
