@@ -338,6 +338,15 @@ def test_portions_whose_pages_are_unpacked_in_unlike_turns(B, H, shared):
     check(d, attend(d))
 
 
+@pytest.mark.parametrize("B, W, H, Hkv, D, positions", [(2, 1, 8, 8, 128, [26930, 20000]), (1, 1, 8, 2, 64, [60000]), (1, 2, 8, 1, 128, [30000]), (1, 8, 4, 4, 128, [9000])])
+def test_half_precision_over_many_keys(B, W, H, Hkv, D, positions):
+    """Averages of thousands of values are a hundredth of them.  What rounding the result leaves is at most 2^-11 of each number, evenly spread, in the 2-norm 2^-11 / sqrt(3)
+    of all at most (and 0.75 of that, because numbers lie all over between two powers of two): with everything else the error stays below that."""
+    d = make(3, "cuda", FP16, B, W, H, Hkv, D, 64, positions)
+    got, want = attend(d), attention(d)[0]
+    assert float((got.double() - want).norm() / want.norm()) < 2.0 ** -11 / 3 ** 0.5
+
+
 def test_refusals():
     refusals("cuda")
     d = make(1, "cuda", BF16, 2, 3, 4, 2, 64, 16, [3, 20])
