@@ -37,8 +37,8 @@ template <typename T, int D, int R> constexpr int tiles_smem = kQueries<D, R> + 
 // to half precision (2^-11 of them; half, so that none is too large), and meet weights rounded to halves: relative to a reference of the row, at most 2^15
 // below which they have all their bits down to 2^-29 of it.
 //
-// Bound by the products and by what feeds them from shared memory: with 40 rows 5000 cycles an SM for 128 keys, 6300 with weights in two halves (windows of 5 tokens, 64 heads on 8,
-// 8 sequences to 6000 keys: 58 us in bf16, 67 in half precision).
+// Bound by the products, which hold the tensor pipe for 8 cycles each, and by what feeds them from shared memory: with 40 rows 3600 cycles an SM for 128 keys, 4350 with weights in two
+// halves (windows of 5 tokens, 64 heads on 8, 8 sequences to 6000 keys: 58 us in bf16, 67 in half precision).
 template <typename T, int D, int R, bool CLUSTER>
 __global__ void __launch_bounds__(kTileThreads, 2) int4_tiles_kernel(const Int4Attn p) {
   constexpr int NG = D / 32, PITCH = kPitch<D>, STAGES = kTileStages<T, R>, HALVES = kHalves<T>, STAGE = kStage<D>, PARTS = kParts<D>;
