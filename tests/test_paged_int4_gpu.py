@@ -347,6 +347,32 @@ def test_half_precision_over_many_keys(B, W, H, Hkv, D, positions):
     assert float((got.double() - want).norm() / want.norm()) < 2.0 ** -11 / 3 ** 0.5
 
 
+@pytest.mark.parametrize("W", [1, 5, 200])
+def test_pages_behind_4_gigabytes(W):
+    """The last pages of a pool of 4.3 GB of codes: written, read back and attended to as the same pages of a small pool, bit by bit (200 tokens: unpacked)."""
+    ps, H, Hkv, D, n = 16, 16, 2, 128, 2 ** 21 + 64
+    d = make(7, "cuda", BF16, 1, W, H, Hkv, D, ps, [700])
+    used, at = d["k_pages"].codes.shape[0], n - d["k_pages"].codes.shape[0]
+    assert at * ps * Hkv * D // 2 > 2 ** 32 and used <= 64
+    d["table"] = torch.cat([d["table"], torch.full((1, 4000 - d["table"].shape[1]), -1, dtype=torch.int32, device="cuda")], 1)
+    slots = (d["table"][:, 700 // ps:].repeat_interleave(ps, 1) * ps + torch.arange(ps, device="cuda").repeat(4000 - 700 // ps))[:, 700 % ps:][:, :W].int()
+    small = [Pages(*(t.clone() for t in p)) for p in (d["k_pages"], d["v_pages"])]
+    large = [ops.paged_int4.new_pages(n, ps, Hkv, D, device="cuda") for _ in "kv"]
+    for p, from_ in zip(large, small):
+        for t, x in zip(p, from_):
+            t[at:] = x
+    angles = torch.rand(1000, D // 2, device="cuda")
+    out = []
+    for pages, off in ((small, 0), (large, at)):
+        table = torch.where(d["table"] >= 0, d["table"] + off, -1)
+        q = ops.paged_int4.append(d["q"], d["k"], d["v"], d["positions"], angles.cos(), angles.sin(), *pages, slots + off * ps)
+        out.append([q, *ops.paged_int4.gather(*pages, slots + off * ps, F32), ops.paged_int4.attention(q, *pages, table, d["positions"])])
+    assert all(torch.equal(a, b) for a, b in zip(*out)) and bool(out[0][3].isfinite().all())
+    for p, from_ in zip(large, small):
+        for t, x in zip(p, from_):
+            assert torch.equal(t[at:].nan_to_num(), x.nan_to_num()) and not bool(t[:64].any())
+
+
 def test_refusals():
     refusals("cuda")
     d = make(1, "cuda", BF16, 2, 3, 4, 2, 64, 16, [3, 20])
