@@ -207,35 +207,56 @@ __global__ void __launch_bounds__(kAppendThreads, ROLE == kQuery ? 12 : 8) int4_
 
 // ---------------------------------------------------------------------------------------------------------------- gather
 constexpr int kGatherThreads = 128;
-// Tokens at slots as numbers of T: a block has a token's keys or values (or, with many heads, a part of them), a thread eight numbers at a time.  Bound by the start of many
-// small blocks: 4 x 2000 tokens of 8 heads 17 us, where the 43 MB that move would take 7.
-template <typename T, int D0>
-__global__ void __launch_bounds__(kGatherThreads) int4_gather_kernel(const Int4Pages kp, const Int4Pages vp, const int* slots, T* k, T* v, int Hkv, int D1, int ps, long tokens) {
+// Tokens at slots as numbers of T: a block has the keys or the values of TOKENS tokens (with many heads a part of them, with few as many times TOKENS as there are threads for), a
+// thread eight numbers of TOKENS tokens at a time, which are asked for together.  Where all blocks are on the GPU at once anyway, one token is quicker (us, one / four: 1 token
+// of 32 heads 1.6 / 1.7, 240 of 8 heads of 64 1.9 / 2.5, 500 of 8 heads 2.8 / 3.0; but 2000 5.3 / 5.0, 8000 17.0 / 12.6, 8000 of 32 heads 67 / 47).  Bound by the start of its
+// blocks and two dependent loads each: 8000 tokens of 8 heads at 0.52 of the copy rate.
+template <typename T, int D0, int TOKENS>
+__global__ void __launch_bounds__(kGatherThreads) int4_gather_kernel(const Int4Pages kp, const Int4Pages vp, const int* slots, T* k, T* v, long n, int Hkv, int D1, int ps, long tokens, int abreast) {
   const int D = D0 ? D0 : D1, items = Hkv * (D / 8);
   pdl_trigger();
   pdl_wait();
   const bool key = blockIdx.z == 0;
   const Int4Pages& from = key ? kp : vp;
-  const int slot = slots[blockIdx.x];
-  const bool there = slot >= 0 && slot < tokens;
-  const int page = there ? slot / ps : 0, row = there ? slot - page * ps : 0;
-  const uint8_t* const codes = from.codes + page * from.c_sp + row * from.c_sr;
-  const uint16_t* const steps = from.steps + page * from.s_sp + row * from.s_sr;
-  T* const to = (key ? k : v) + (long)blockIdx.x * Hkv * D;
-  for (int i = blockIdx.y * kGatherThreads + threadIdx.x; i < items; i += gridDim.y * kGatherThreads) {
+  const int mine = abreast > 1 ? (int)(threadIdx.x / (unsigned)items) : 0;       // which of the tokens
+  const long t0 = (long)blockIdx.x * TOKENS * abreast + mine;
+  if (mine >= abreast || t0 >= n) return;
+  auto here = [&](int t) { return t0 + t * abreast < n; };
+  const uint8_t* codes[TOKENS];
+  const uint16_t* steps[TOKENS];
+#pragma unroll
+  for (int t = 0; t < TOKENS; ++t) {
+    const int slot = here(t) ? slots[t0 + t * abreast] : -1;
+    const bool there = slot >= 0 && slot < tokens;
+    const int page = there ? slot / ps : 0, row = there ? slot - page * ps : 0;
+    codes[t] = there ? from.codes + page * from.c_sp + row * from.c_sr : nullptr;
+    steps[t] = from.steps + page * from.s_sp + row * from.s_sr;
+  }
+  T* const to = (key ? k : v) + t0 * Hkv * D;
+  for (int i = blockIdx.y * kGatherThreads + threadIdx.x - mine * items; i < items; i += gridDim.y * kGatherThreads) {
     const int head = i / (D / 8), c = (i - head * (D / 8)) * 8;
-    Eight<T> out;
-    if (there) {
-      const uint32_t word = *reinterpret_cast<const uint32_t*>(codes + head * from.c_sh + c / 2);
-      const uint16_t* const st = steps + head * from.s_sh + c / 32;
-      const float s = __half2float(__ushort_as_half(st[0])), m = __half2float(__ushort_as_half(st[D / 32]));
+    uint32_t word[TOKENS];
+    uint16_t s16[TOKENS], m16[TOKENS];
 #pragma unroll
-      for (int j = 0; j < 8; ++j) out.set(j, fmaf(__uint_as_float(0x4b000000u | (word >> (4 * j) & 15)) - 0x1p23f, s, m));
-    } else {
-#pragma unroll
-      for (int j = 0; j < 8; ++j) out.set(j, 0.f);
+    for (int t = 0; t < TOKENS; ++t) {
+      word[t] = 0;
+      s16[t] = m16[t] = 0;
+      if (codes[t]) {
+        word[t] = *reinterpret_cast<const uint32_t*>(codes[t] + head * from.c_sh + c / 2);
+        const uint16_t* const st = steps[t] + head * from.s_sh + c / 32;
+        s16[t] = st[0];
+        m16[t] = st[D / 32];
+      }
     }
-    out.store(to + (long)i * 8);
+#pragma unroll
+    for (int t = 0; t < TOKENS; ++t) {
+      if (!here(t)) break;
+      const float s = __half2float(__ushort_as_half(s16[t])), m = __half2float(__ushort_as_half(m16[t]));
+      Eight<T> out;                                        // without a slot: zeros
+#pragma unroll
+      for (int j = 0; j < 8; ++j) out.set(j, fmaf(__uint_as_float(0x4b000000u | (word[t] >> (4 * j) & 15)) - 0x1p23f, s, m));
+      out.store(to + ((long)t * abreast * items + i) * 8);
+    }
   }
 }
 
@@ -843,12 +864,15 @@ int int4_append(const Int4Append& p, int dt, cudaStream_t st) {
 void int4_gather(const Int4Pages& kp, const Int4Pages& vp, const int* slots, void* k, void* v, long n, int Hkv, int D, int ps, long tokens, int dt, cudaStream_t st) {
   if (n == 0) return;
   if (n >= (1l << 31)) nxd_throw("int4_gather: too many tokens", __FILE__, __LINE__);
-  const dim3 grid((unsigned)n, std::min(64, (Hkv * (D / 8) + kGatherThreads - 1) / kGatherThreads), 2);
-  auto go = [&](auto* k, auto* v, auto kernel) { launch_dependent(kernel, grid, kGatherThreads, 0, st, kp, vp, slots, k, v, Hkv, D, ps, tokens); };
+  const int items = Hkv * (D / 8), abreast = std::max(1, kGatherThreads / items), parts = std::min(64, (items + kGatherThreads - 1) / kGatherThreads);
+  const bool one = (n + abreast - 1) / abreast * parts * 2 <= 16l * device_sm_count();
+  const int tokens_at = (one ? 1 : 4) * abreast;
+  const dim3 grid((unsigned)((n + tokens_at - 1) / tokens_at), parts, 2);
+  auto go = [&](auto* k, auto* v, auto kernel) { launch_dependent(kernel, grid, kGatherThreads, 0, st, kp, vp, slots, k, v, n, Hkv, D, ps, tokens, abreast); };
   auto typed = [&](auto zero) {
     using T = decltype(zero);
-    if (D == 128) go((T*)k, (T*)v, int4_gather_kernel<T, 128>);
-    else go((T*)k, (T*)v, int4_gather_kernel<T, 0>);
+    if (one) D == 128 ? go((T*)k, (T*)v, int4_gather_kernel<T, 128, 1>) : go((T*)k, (T*)v, int4_gather_kernel<T, 0, 1>);
+    else D == 128 ? go((T*)k, (T*)v, int4_gather_kernel<T, 128, 4>) : go((T*)k, (T*)v, int4_gather_kernel<T, 0, 4>);
   };
   if (dt == kBF16) typed(__nv_bfloat16());
   else if (dt == kF16) typed(__half());

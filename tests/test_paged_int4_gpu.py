@@ -373,6 +373,23 @@ def test_pages_behind_4_gigabytes(W):
             assert torch.equal(t[at:].nan_to_num(), x.nan_to_num()) and not bool(t[:64].any())
 
 
+@pytest.mark.parametrize("n, Hkv, D", [(30000, 1, 32), (20011, 1, 64), (9001, 3, 96), (4003, 9, 128), (2500, 40, 64), (130, 1100, 128)])
+def test_gather_of_many_tokens(n, Hkv, D):
+    g = torch.Generator(device="cuda").manual_seed(n)
+    pages = [ops.paged_int4.new_pages(24, 16, Hkv, D, device="cuda") for _ in "kv"]
+    for p in pages:
+        p.codes.copy_(torch.randint(0, 256, p.codes.shape, generator=g, device="cuda", dtype=torch.uint8))
+        p.steps.copy_(torch.randn(p.steps.shape, generator=g, device="cuda"))
+    slots = torch.randint(-1, 24 * 16 + 1, (1, n), generator=g, device="cuda", dtype=torch.int32)
+    at, there = slots.long().clamp(0, 24 * 16 - 1), (slots >= 0) & (slots < 24 * 16)
+    for x, p in zip(ops.paged_int4.gather(*pages, slots, BF16), pages):
+        assert x.shape == (1, n, Hkv, D)
+        for lo in range(0, n, 4000):
+            a = at[:, lo:lo + 4000]
+            want = values(Pages(*(t[a // 16, a % 16] for t in p))) * there[:, lo:lo + 4000, None, None]
+            assert bool(((x[:, lo:lo + 4000].double() - want).abs() <= (2.0 ** -8 + 2.0 ** -24) * want.abs() + 2.0 ** -25).all())
+
+
 def test_refusals():
     refusals("cuda")
     d = make(1, "cuda", BF16, 2, 3, 4, 2, 64, 16, [3, 20])
