@@ -38,7 +38,8 @@ def assign(page_table: torch.Tensor, held: torch.Tensor, free: torch.Tensor, spa
     there is no page, have slot -1.  ``short [1]`` int32 becomes 1 where a row that needed pages took none, or a token that counts has no slot (and stays
     as it is otherwise).
 
-    ``in_place``: the state's own tensors are changed and returned; otherwise they stay, and new ones are returned."""
+    ``in_place``: the state's own tensors are changed and returned (rows of the table may not share memory, and calls that change one state go one after the
+    other); otherwise they stay, and new ones are returned."""
     if _ext.use_cuda(page_table):
         return Tables(*_ext.ext().assign_pages(page_table, held, free, span, positions, new, page_size, lens, lengths, shared, trim, short, in_place))
     return _assign_plain(page_table, held, free, span, positions, new, page_size, lens, lengths, shared, trim, short, in_place)

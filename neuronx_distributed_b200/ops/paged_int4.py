@@ -172,7 +172,7 @@ def attention(q: torch.Tensor, k_pages: Pages, v_pages: Pages, page_table: torch
     of the numbers that the codes stand for, with its arguments.  ``page_table [B, n]`` int32 (entries outside the pool are holes, whose keys nobody
     sees), ``positions [B]`` of the rows' first new tokens (negative: an idle row), ``lens [B]`` new tokens that count.  ``shared_pages [n]`` int32 stand in
     place of the first ``n`` columns of every row's table; each row reads them for itself.  Keys and values that some token of a row sees have to be
-    finite, and so have queries.
+    finite, and so have queries.  The kernels take pools whose codes span less than 64 GB, and tables of less than 2^31 tokens.
 
     Sums and statistics are in 32 bits, codes and steps enter them as they are."""
     _no_gradient("attention in 4 bits", q)
