@@ -15,7 +15,7 @@ def cuda(*t):
     return [None if x is None else x.cuda() for x in t]
 
 
-@pytest.mark.parametrize("case", CASES + [(2500, 9, 9000, 16, 1, 2), (1, 5000, 8000, 16, 0, 3)])
+@pytest.mark.parametrize("case", CASES + [(2500, 9, 9000, 16, 1, 2), (1, 5000, 8000, 16, 0, 3), (3, 1301, 1500, 16, 5, 40), (37, 257, 4000, 16, 3, 9), (130, 64, 3000, 16, 0, 20)])
 @pytest.mark.parametrize("mode", ["tokens", "turnover"])
 @pytest.mark.parametrize("in_place", [False, True])
 def test_assign(case, mode, in_place):
