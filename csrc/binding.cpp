@@ -523,7 +523,8 @@ static std::vector<Tensor> moe_block_tkg(const Tensor& x, const c10::optional<Te
   return {out, logits, idx, w};
 }
 // a [M,K], b [N,K]: fp8 bytes; sfa [ceil(M/128), K/128, 512], sfb [ceil(N/128), K/128, 512]: tiled E8M0 scales → [M,N] bf16
-static Tensor gemm_mxfp8(const Tensor& a, const Tensor& b, const Tensor& sfa, const Tensor& sfb, int64_t a_fmt, int64_t b_fmt) {
+static Tensor gemm_mxfp8(const Tensor& a, const Tensor& b, const Tensor& sfa, const Tensor& sfb, int64_t a_fmt, int64_t b_fmt,
+                         int64_t wait_ns) {
   CHECK_IN(a); CHECK_IN(b); CHECK_IN(sfa); CHECK_IN(sfb);
   TORCH_CHECK(a.dim() == 2 && b.dim() == 2 && a.element_size() == 1 && b.element_size() == 1);
   // byte tensors: K bytes per row for fp8 formats, K/2 for packed e2m1 (format 5)
@@ -535,12 +536,12 @@ static Tensor gemm_mxfp8(const Tensor& a, const Tensor& b, const Tensor& sfa, co
               "gemm_mxfp8: scale tensors must be tiled [rows/128, K/128, 512]");
   c10::cuda::CUDAGuard guard(a.device());
   Tensor out = at::empty({M, N}, a.options().dtype(at::kBFloat16));
-  nxd::gemm_mxfp8(a.data_ptr(), b.data_ptr(), sfa.data_ptr(), sfb.data_ptr(), out.data_ptr(), M, N, K, (int)a_fmt, (int)b_fmt, stream());
+  nxd::gemm_mxfp8(a.data_ptr(), b.data_ptr(), sfa.data_ptr(), sfb.data_ptr(), out.data_ptr(), M, N, K, (int)a_fmt, (int)b_fmt, wait_ns, stream());
   return out;
 }
 // a [M,K/2], b [N,K/2]: packed e2m1 bytes; sfa [ceil(M/128), K/(4·vs), 512], sfb likewise: tiled scales (E8M0 for vs 32, UE4M3 for
 // vs 16) → alpha · product, [M,N] bf16
-static Tensor gemm_f4(const Tensor& a, const Tensor& b, const Tensor& sfa, const Tensor& sfb, int64_t vec_size, double alpha) {
+static Tensor gemm_f4(const Tensor& a, const Tensor& b, const Tensor& sfa, const Tensor& sfb, int64_t vec_size, double alpha, int64_t wait_ns) {
   CHECK_IN(a); CHECK_IN(b); CHECK_IN(sfa); CHECK_IN(sfb);
   TORCH_CHECK(a.dim() == 2 && b.dim() == 2 && a.element_size() == 1 && b.element_size() == 1);
   const int M = a.size(0), N = b.size(0), K = 2 * a.size(1);
@@ -553,7 +554,7 @@ static Tensor gemm_f4(const Tensor& a, const Tensor& b, const Tensor& sfa, const
               "gemm_f4: scale tensors must be tiled [rows/128, K/(4*vec_size), 512]");
   c10::cuda::CUDAGuard guard(a.device());
   Tensor out = at::empty({M, N}, a.options().dtype(at::kBFloat16));
-  nxd::gemm_f4(a.data_ptr(), b.data_ptr(), sfa.data_ptr(), sfb.data_ptr(), out.data_ptr(), M, N, K, (int)vec_size, (float)alpha, stream());
+  nxd::gemm_f4(a.data_ptr(), b.data_ptr(), sfa.data_ptr(), sfb.data_ptr(), out.data_ptr(), M, N, K, (int)vec_size, (float)alpha, wait_ns, stream());
   return out;
 }
 // x [M<=8, K] bf16; w = MX byte stream of [N, K] (fp4: K/2 bytes per row, fp8: K), any integer dtype view; scale [N, K/32] uint8
@@ -1074,8 +1075,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("nvls_all_to_all", &nvls_all_to_all);
   m.def("gemv_mx", &gemv_mx);
   m.def("gemv_mx_grouped", &gemv_mx_grouped);
-  m.def("gemm_mxfp8", &gemm_mxfp8);
-  m.def("gemm_f4", &gemm_f4);
+  m.def("gemm_mxfp8", &gemm_mxfp8, py::arg("a"), py::arg("b"), py::arg("sfa"), py::arg("sfb"), py::arg("a_fmt"), py::arg("b_fmt"),
+        py::arg("wait_ns") = 2000000000);
+  m.def("gemm_f4", &gemm_f4, py::arg("a"), py::arg("b"), py::arg("sfa"), py::arg("sfb"), py::arg("vec_size"), py::arg("alpha"), py::arg("wait_ns") = 2000000000);
   m.def("moe_block_tkg", &moe_block_tkg);
   m.def("moe_block_tkg_supported", [](int64_t T, int64_t H, int64_t E, int64_t I, int64_t K) {
     return nxd::moe_block_tkg_supported((int)T, (int)H, (int)E, (int)I, (int)K);

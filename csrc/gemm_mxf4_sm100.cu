@@ -84,14 +84,16 @@ __host__ __device__ constexpr uint32_t make_idesc_f4() {
 template <int VS>
 __global__ void __launch_bounds__(kThreads, 1)
 gemm_f4_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant__ CUtensorMap tma_b, const uint8_t* __restrict__ sfa,
-               const uint8_t* __restrict__ sfb, __nv_bfloat16* __restrict__ out, int M, int N, int K, float alpha) {
+               const uint8_t* __restrict__ sfb, __nv_bfloat16* __restrict__ out, int M, int N, int K, float alpha, long wait_ns) {
   constexpr int CH = BK / (4 * VS);                      // scale chunks per operand per k-block: 2 (MXFP4) / 4 (NVFP4)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint64_t* bars = (uint64_t*)(smem + kBarOffset);
-  uint32_t* tmem_slot = (uint32_t*)(bars + 2 * kStages + 2 * kAcc);
+  uint32_t* tmem_slot = (uint32_t*)(bars + 2 * kStages + 2 * kAcc + 1);
   const uint32_t bar_full = smem_u32(bars), bar_empty = smem_u32(bars + kStages);
   const uint32_t bar_tfull = smem_u32(bars + 2 * kStages), bar_tempty = smem_u32(bars + 2 * kStages + kAcc);
+  const uint32_t bar_end = smem_u32(bars + 2 * kStages + 2 * kAcc), gave_up = smem_u32(tmem_slot + 1);
+  const uint64_t limit = wait_ns < 0 ? -wait_ns : wait_ns;  // negative: nothing is loaded (tests)
   const uint32_t smem_base = smem_u32(smem);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int tiles_m = (M + BM - 1) / BM, tiles_n = (N + BN - 1) / BN, num_tiles = tiles_m * tiles_n;
@@ -102,6 +104,8 @@ gemm_f4_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant_
     prefetch_tmap(&tma_b);
     for (int i = 0; i < kStages; ++i) { mbar_init(bar_full + 8 * i, 1); mbar_init(bar_empty + 8 * i, 1); }
     for (int i = 0; i < kAcc; ++i) { mbar_init(bar_tfull + 8 * i, 1); mbar_init(bar_tempty + 8 * i, kEpiThreads); }
+    mbar_init(bar_end, 1);
+    tmem_slot[1] = 0;
     fence_barrier_init();
   }
   if (warp == 1) { tcgen05_alloc(smem_u32(tmem_slot), kTmemCols); tcgen05_relinquish(); }
@@ -109,15 +113,20 @@ gemm_f4_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant_
   __syncthreads();
   tcgen05_fence_after();
   const uint32_t tmem_base = *tmem_slot;
+  // A wait that takes longer than the limit is an error in here: the block's roles leave their loops, wait (a while) for what they have in flight, and the block's
+  // tiles from there on are NaN.
+  auto wait = [&](uint32_t bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, limit, gave_up); };
+  constexpr uint64_t kInFlight = 100000000;               // ns; copies and products take microseconds
+  bool ok = true;
 
   if (warp == 0) {
     // ===== producer: packed operand tiles by TMA, the k-block's CH scale chunks per operand as one bulk copy each =====
     if (lane == 0) {
       int stage = 0; uint32_t phase = 0;
-      for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x) {
+      for (int tile = wait_ns < 0 ? num_tiles : blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
         const int m_blk = tile % tiles_m, n_blk = tile / tiles_m;
         for (int kb = 0; kb < num_kb; ++kb) {
-          mbar_wait_bounded(bar_empty + 8 * stage, phase ^ 1);
+          if (!(ok = wait(bar_empty + 8 * stage, phase ^ 1))) break;
           const uint32_t full = bar_full + 8 * stage;
           mbar_expect_tx(full, kTileBytes + 2 * CH * kSfChunk);
           const uint32_t sa = smem_base + stage * kTileBytes, sb = sa + kABytes;
@@ -129,6 +138,8 @@ gemm_f4_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant_
           if (++stage == kStages) { stage = 0; phase ^= 1; }
         }
       }
+      // the last copies into every stage: this lap's in front of `stage`, the one before's behind it (none yet: passed)
+      for (int i = 0; i < kStages; ++i) mbar_wait_bounded(bar_full + 8 * i, i < stage ? phase : phase ^ 1, kInFlight, 0);
     }
     __syncwarp();
   } else if (warp == 1) {
@@ -137,11 +148,11 @@ gemm_f4_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant_
       constexpr uint32_t idesc0 = make_idesc_f4<VS>();
       int stage = 0; uint32_t phase = 0; int as = 0; uint32_t aphase = 0;
       for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x) {
-        mbar_wait_bounded(bar_tempty + 8 * as, aphase ^ 1);
+        if (!(ok = wait(bar_tempty + 8 * as, aphase ^ 1))) break;
         tcgen05_fence_after();
         const uint32_t tmem_d = tmem_base + as * BN;
         for (int kb = 0; kb < num_kb; ++kb) {
-          mbar_wait_bounded(bar_full + 8 * stage, phase);
+          if (!(ok = wait(bar_full + 8 * stage, phase))) break;
           tcgen05_fence_after();
           const uint32_t sa = smem_base + stage * kTileBytes, sb = sa + kABytes;
           const uint32_t ssf = smem_base + kSfOffset + stage * kSfStage;
@@ -164,8 +175,13 @@ gemm_f4_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant_
           tcgen05_commit(bar_empty + 8 * stage);
           if (++stage == kStages) { stage = 0; phase ^= 1; }
         }
+        if (!ok) break;
         tcgen05_commit(bar_tfull + 8 * as);
         if (++as == kAcc) { as = 0; aphase ^= 1; }
+      }
+      if (!ok) {                                         // products in flight
+        tcgen05_commit(bar_end);
+        mbar_wait_bounded(bar_end, 0, kInFlight, 0);
       }
     }
     __syncwarp();
@@ -175,15 +191,20 @@ gemm_f4_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_constant_
     int as = 0; uint32_t aphase = 0;
     for (int tile = blockIdx.x; tile < num_tiles; tile += gridDim.x) {
       const int m_blk = tile % tiles_m, n_blk = tile / tiles_m;
-      mbar_wait_bounded(bar_tfull + 8 * as, aphase);
+      ok = __all_sync(0xffffffffu, ok && wait(bar_tfull + 8 * as, aphase));
       tcgen05_fence_after();
       const int row = m_blk * BM + q * 32 + lane;
       __nv_bfloat16* orow = out + (size_t)row * N;
 #pragma unroll 1
       for (int c = 0; c < BN / 32; ++c) {
         uint32_t r[32];
-        tcgen05_ld_32x32(tmem_base + ((uint32_t)(q * 32) << 16) + as * BN + c * 32, r);
-        tcgen05_wait_ld();
+        if (ok) {
+          tcgen05_ld_32x32(tmem_base + ((uint32_t)(q * 32) << 16) + as * BN + c * 32, r);
+          tcgen05_wait_ld();
+        } else {
+#pragma unroll
+          for (int j = 0; j < 32; ++j) r[j] = 0x7fffffffu;
+        }
         const int col0 = n_blk * BN + c * 32;
         if (row < M && col0 < N) {
           if (col0 + 32 <= N) {
@@ -219,7 +240,7 @@ int device_sm_count();
 // a [M,K], b [N,K]: packed e2m1 (K/2 bytes per row); sfa / sfb: scale chunks tiled [rows/128][K/(4·VS)][512] (E8M0 for
 // vec_size 32, UE4M3 for vec_size 16); out [M,N] bf16 = alpha · product.  K % 256 == 0, N % 8 == 0.
 void gemm_f4(const void* a, const void* b, const void* sfa, const void* sfb, void* out, int M, int N, int K, int vec_size, float alpha,
-             cudaStream_t st) {
+             long wait_ns, cudaStream_t st) {
   if (K % mxf4::BK || N % 8) nxd_throw("gemm_f4: K % 256 == 0 and N % 8 == 0", __FILE__, __LINE__);
   if (vec_size != 32 && vec_size != 16) nxd_throw("gemm_f4: scale vector size 32 (MXFP4) or 16 (NVFP4)", __FILE__, __LINE__);
   const CUtensorMap ta = make_tmap_u4_packed_box(a, M, K, mxf4::BM);
@@ -234,10 +255,10 @@ void gemm_f4(const void* a, const void* b, const void* sfa, const void* sfb, voi
   }
   if (vec_size == 32)
     mxf4::gemm_f4_kernel<32><<<grid, mxf4::kThreads, mxf4::kSmem, st>>>(ta, tb, (const uint8_t*)sfa, (const uint8_t*)sfb,
-                                                                         (__nv_bfloat16*)out, M, N, K, alpha);
+                                                                         (__nv_bfloat16*)out, M, N, K, alpha, wait_ns);
   else
     mxf4::gemm_f4_kernel<16><<<grid, mxf4::kThreads, mxf4::kSmem, st>>>(ta, tb, (const uint8_t*)sfa, (const uint8_t*)sfb,
-                                                                         (__nv_bfloat16*)out, M, N, K, alpha);
+                                                                         (__nv_bfloat16*)out, M, N, K, alpha, wait_ns);
   NXD_CUDA_CHECK(cudaGetLastError());
 }
 

@@ -161,14 +161,15 @@ void moe_block_tkg(const void* x, const void* gamma, const void* router_w, const
                    int act_over_topk, int normalize, int pre_scale, int round_logits, int act, float act_alpha, float act_beta,
                    float gate_lo, float gate_hi, float up_lo, float up_hi, bool cooperative, cudaStream_t st);
 
-// ---- block-scaled MXFP8 GEMM on tcgen05 (gemm_mx_sm100.cu); a_fmt / b_fmt: 0 = e4m3, 1 = e5m2
+// ---- block-scaled MXFP8 GEMM on tcgen05 (gemm_mx_sm100.cu); a_fmt / b_fmt: 0 = e4m3, 1 = e5m2, 5 = e2m1; wait_ns: after which a wait in the kernel gives up (its
+// block's tiles are NaN from there on); negative: after so many, and nothing is loaded (tests)
 void gemm_mxfp8(const void* a, const void* b, const void* sfa, const void* sfb, void* out, int M, int N, int K, int a_fmt,
-                int b_fmt, cudaStream_t st);
+                int b_fmt, long wait_ns, cudaStream_t st);
 
 // ---- 4-bit block-scaled GEMM at the FP4 rate (gemm_mxf4_sm100.cu): packed e2m1 operands; vec_size 32 = MXFP4 (E8M0 scales),
 // 16 = NVFP4 (UE4M3 scales, alpha = product of the per-tensor factors)
 void gemm_f4(const void* a, const void* b, const void* sfa, const void* sfb, void* out, int M, int N, int K, int vec_size, float alpha,
-             cudaStream_t st);
+             long wait_ns, cudaStream_t st);
 
 // ---- decode GEMV on MX (block-scaled fp4 / fp8) weights (gemv_mx.cu)
 void gemv_mx(const void* x, const void* w, const void* scale, const void* residual, void* y, int M, int N, int K, int fmt,

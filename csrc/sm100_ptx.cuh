@@ -31,12 +31,12 @@ NXD_DEVICE void mbar_wait(uint32_t bar, uint32_t parity) {
         : "memory");
   } while (!done);
 }
-// Same wait with a wall-clock bound: a kernel whose producer never arrives (wrong expected-byte count, rejected tensor map)
-// traps after ~4 s instead of spinning until the host gives up.  Used by kernels that have not had a hardware run yet.
-NXD_DEVICE void mbar_wait_bounded(uint32_t bar, uint32_t parity) {
+// Same wait with an end: after `limit` ns it gives up, and so do the block's other waits, by the word `gave_up` of its shared memory (0: nobody is told).
+// → whether the barrier was passed.  For kernels whose producer might never arrive (a wrong count of expected bytes, a rejected tensor map).
+NXD_DEVICE bool mbar_wait_bounded(uint32_t bar, uint32_t parity, uint64_t limit, uint32_t gave_up) {
   uint32_t done, it = 0;
   uint64_t t0 = 0;
-  do {
+  while (true) {
     asm volatile(
         "{\n\t.reg .pred p;\n\t"
         "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
@@ -44,13 +44,19 @@ NXD_DEVICE void mbar_wait_bounded(uint32_t bar, uint32_t parity) {
         : "=r"(done)
         : "r"(bar), "r"(parity)
         : "memory");
-    if (!done && (++it & 0x3ffu) == 0) {
-      uint64_t t;
-      asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-      if (t0 == 0) t0 = t;
-      else if (t - t0 > 4000000000ull) __trap();
+    if (done) return true;
+    if ((++it & 63u) != 0) continue;
+    uint32_t over = 0;
+    if (gave_up) asm volatile("ld.volatile.shared.u32 %0, [%1];" : "=r"(over) : "r"(gave_up) : "memory");
+    if (over) return false;
+    uint64_t t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    if (t0 == 0) t0 = t;
+    else if (t - t0 > limit) {
+      if (gave_up) asm volatile("st.volatile.shared.u32 [%0], %1;" ::"r"(gave_up), "r"(1u) : "memory");
+      return false;
     }
-  } while (!done);
+  }
 }
 NXD_DEVICE void fence_barrier_init() { asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory"); }
 
