@@ -74,8 +74,10 @@ NXD_DEVICE void unpack8(const uint4& raw, float (&f)[8]) {
 }
 NXD_DEVICE float bf16_round(float v) { return __bfloat162float(__float2bfloat16_rn(v)); }
 
-// All CTAs of the (co-resident) grid meet; `target` = barriers passed so far × gridDim.x.
-NXD_DEVICE void grid_barrier(unsigned* ctr, unsigned target) {
+// All CTAs of the (co-resident) grid meet; `target` = barriers passed so far × gridDim.x.  → false where they did not within 4 s: the others miss this CTA at the next
+// one then, and give up there.
+NXD_DEVICE bool grid_barrier(unsigned* ctr, unsigned target) {
+  int late = 0;
   __syncthreads();
   if (threadIdx.x == 0) {
     __threadfence();
@@ -84,16 +86,16 @@ NXD_DEVICE void grid_barrier(unsigned* ctr, unsigned target) {
     uint64_t t0 = 0;
     while (ld_acquire_gpu_u32(ctr) < target) {
       __nanosleep(32);
-      if ((++it & 0x3fffu) == 0) {                       // a grid that is not co-resident would wait forever: trap after ~4 s
+      if ((++it & 0x3fffu) == 0) {                       // a grid that is not co-resident would wait forever
         uint64_t t;
         asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
         if (t0 == 0) t0 = t;
-        else if (t - t0 > 4000000000ull) __trap();
+        else if (t - t0 > 4000000000ull) { late = 1; break; }
       }
     }
     __threadfence();
   }
-  __syncthreads();
+  return !__syncthreads_or(late);
 }
 
 NXD_DEVICE float glu_act(const TkgParams& p, float g, float u) {
@@ -136,6 +138,14 @@ __global__ void __launch_bounds__(kTkgThreads) moe_block_tkg_kernel(const TkgPar
   const int T = p.T, H = p.H, E = p.E, I = p.I, K = p.K, N2 = 2 * p.I;
   const int gw = blockIdx.x * kTkgWarps + warp, GW = gridDim.x * kTkgWarps;
   const long gtid = (long)blockIdx.x * kTkgThreads + tid, gthreads = (long)gridDim.x * kTkgThreads;
+
+  // this CTA's part of the output where a barrier gave up
+  auto not_there = [&] {
+    const uint32_t nan = 0x7fff7fffu;
+    for (long i = gtid * 8; i < (long)T * H; i += gthreads * 8) *reinterpret_cast<uint4*>(p.out + i) = make_uint4(nan, nan, nan, nan);
+    if (blockIdx.x == 0)
+      for (int i = tid; i < T * K; i += kTkgThreads) { p.topk_idx[i] = 0; p.topk_w[i] = __int_as_float(0x7fffffff); }
+  };
 
   // ---- phase A: zero the scratch, RMSNorm every token into shared memory (each CTA keeps its own copy) ----------------
   for (long i = gtid; i < (long)T * K * N2; i += gthreads) p.gu[i] = 0.f;
@@ -198,7 +208,7 @@ __global__ void __launch_bounds__(kTkgThreads) moe_block_tkg_kernel(const TkgPar
       }
     }
   }
-  grid_barrier(p.barrier, 1u * gridDim.x);
+  if (!grid_barrier(p.barrier, 1u * gridDim.x)) return not_there();
 
   // ---- phase C: activation, top-k, normalisation — every CTA computes the same routing table ----------------------------
   for (int t = warp; t < T; t += kTkgWarps) {
@@ -351,7 +361,7 @@ __global__ void __launch_bounds__(kTkgThreads) moe_block_tkg_kernel(const TkgPar
       }
     }
   }
-  grid_barrier(p.barrier, 2u * gridDim.x);
+  if (!grid_barrier(p.barrier, 2u * gridDim.x)) return not_there();
 
   // ---- phase E: GLU activation on the fly + down GEMV: item = (active expert, 256-column chunk of H, 64-row slice of I) --
   {
@@ -421,7 +431,7 @@ __global__ void __launch_bounds__(kTkgThreads) moe_block_tkg_kernel(const TkgPar
       }
     }
   }
-  grid_barrier(p.barrier, 3u * gridDim.x);
+  if (!grid_barrier(p.barrier, 3u * gridDim.x)) return not_there();
 
   // ---- phase F: fp32 accumulators → bf16 output ------------------------------------------------------------------------
   for (long i = gtid * 8; i < (long)T * H; i += gthreads * 8) {
