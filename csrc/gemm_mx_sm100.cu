@@ -109,13 +109,15 @@ gemm_mxfp8_kernel(const __grid_constant__ CUtensorMap tma_a, const __grid_consta
   if (warp == 0) {
     // ===== producer: operand tiles by TMA, scale chunks by bulk copy, all on the stage's full barrier =====
     if (lane == 0) {
+      // a copy that spreads 4-bit numbers over 16-byte containers counts the bytes that it reads, half a tile
+      const uint32_t arriving = (a_fmt == 5 ? kABytes / 2 : kABytes) + (b_fmt == 5 ? kBBytes / 2 : kBBytes) + 2 * kSfBytes;
       int stage = 0; uint32_t phase = 0;
       for (int tile = wait_ns < 0 ? num_tiles : blockIdx.x; ok && tile < num_tiles; tile += gridDim.x) {
         const int m_blk = tile % tiles_m, n_blk = tile / tiles_m;
         for (int kb = 0; kb < num_kb; ++kb) {
           if (!(ok = wait(bar_empty + 8 * stage, phase ^ 1))) break;
           const uint32_t full = bar_full + 8 * stage;
-          mbar_expect_tx(full, kTileBytes + 2 * kSfBytes);
+          mbar_expect_tx(full, arriving);
           const uint32_t sa = smem_base + stage * kTileBytes, sb = sa + kABytes;
           const uint32_t ssf = smem_base + kSfOffset + stage * 2 * kSfBytes;
           tma_load_2d(sa, &tma_a, full, kb * BK, m_blk * BM);

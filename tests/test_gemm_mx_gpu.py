@@ -37,3 +37,11 @@ def test_waits_that_run_out(M, N, K):
     call = [a, b] + [gemm_mx.tile_scales(t) for t in (sa, sb)] + [32, 1.0]
     assert bool(_ext.ext().gemm_f4(*call, wait_ns=-20000000).isnan().all())
     close(_ext.ext().gemm_f4(*call), gemm_mx.matmul_f4_reference(a, sa, b, sb))
+
+
+@pytest.mark.parametrize("a_kind, b_kind", [("mxfp8", "mxfp4"), ("mxfp4", "mxfp8"), ("mxfp4", "mxfp4")])
+@pytest.mark.parametrize("M, N, K", [(1, 8, 128), (128, 128, 128), (300, 520, 1024), (1000, 2000, 2048)])
+def test_operands_of_four_bits(a_kind, b_kind, M, N, K):
+    """Numbers of 4 bits, which copies spread over containers of 8: beside 8-bit ones, on either side, and on both."""
+    a, b = (f(M, N, K)[i:i + 2] for f, i in ((eights if a_kind == "mxfp8" else fours, 0), (eights if b_kind == "mxfp8" else fours, 2)))
+    close(gemm_mx.matmul_mxfp8(*a, *b, a_kind, b_kind), gemm_mx.matmul_mxfp8_reference(*a, *b, a_kind, b_kind))
