@@ -225,7 +225,7 @@ struct PagedAttn {
   long k_sp, k_sr, k_sh, v_sp, v_sr, v_sh;        // strides of pages, rows in a page, heads
   float scale_log2;
   int wait_ns;                       // after which a wait in the tile kernel gives up; negative: after so many, and no keys are loaded (tests)
-  const float* units;                // tiles: what the scores of a query row are multiplied by, beside the scale, or null: 1
+  const float* units;                // tiles whose output has another type: what the scores of a query row are multiplied by, beside the scale
   long u_sb, u_sw;                   // their strides of sequences and tokens
 };
 // How a launch is dealt out (rows: few, the kernel of paged.cu, or tiles of 64, 128 or 256, paged_attention_sm100.cu); workspaces follow from it

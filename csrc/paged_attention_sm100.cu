@@ -19,6 +19,7 @@
 
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "attention_sm100.cuh"
 #include "common.cuh"
@@ -601,6 +602,10 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
     const uint32_t tS = tmem_S + t * 128 + lane_base, tO = tmem_O + t * 128 + lane_base;
     const uint32_t my_s = bar_s + 8 * t, my_p = bar_p + 8 * t;
     constexpr int Q = KEYS / 32;
+    // rows have scales of their own where queries were made another type; a number of the launch otherwise (windows 42.4 us, 46.0 with one read for every row)
+    constexpr bool UNITS = !std::is_same<T, O>::value;
+    float sl2 = p.scale_log2;
+    uint64_t sl2_2 = pack2(sl2, sl2);
     int g = 0, items = 0, pos0 = 0, tile0 = 0;
     // A piece of one step in front of the first works on whatever there is and leaves nothing behind (its weights go over the sums, which the first
     // product does not add to): a step's 10 KB of instructions come from memory, a part by each warp, while the place is found and the first keys
@@ -616,8 +621,10 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         int b = 0, w = 0;
         const int row = first_row(it) + (PAIR ? t * kRows : 0) + own, n = SHARED ? shared_keys : it.keys;
         const bool live = !dry && row_token(it, row, b, w);
-        const float sl2 = live && p.units ? p.scale_log2 * p.units[b * p.u_sb + w * p.u_sw + it.head * p.G + row % p.G] : p.scale_log2;
-        const uint64_t sl2_2 = pack2(sl2, sl2);
+        if constexpr (UNITS) {
+          sl2 = live ? p.scale_log2 * p.units[b * p.u_sb + w * p.u_sw + it.head * p.G + row % p.G] : p.scale_log2;
+          sl2_2 = pack2(sl2, sl2);
+        }
         // keys that this row sees (one that does not count: all, whatever comes of it), and the fewest of the warp's rows
         const int sees = live ? min(visible_keys(p, b, w), n) : 0x7fffffff;
         const int sees_lo = __reduce_min_sync(0xffffffffu, sees);
