@@ -18,6 +18,7 @@
 #include <cuda.h>
 
 #include <algorithm>
+#include <cfloat>
 #include <string>
 #include <type_traits>
 
@@ -622,7 +623,8 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         const int row = first_row(it) + (PAIR ? t * kRows : 0) + own, n = SHARED ? shared_keys : it.keys;
         const bool live = !dry && row_token(it, row, b, w);
         if constexpr (UNITS) {
-          sl2 = live ? p.scale_log2 * p.units[b * p.u_sb + w * p.u_sw + it.head * p.G + row % p.G] : p.scale_log2;
+          // not 0, which the -inf of what nobody sees makes NaN: scores that small are alike in any case
+          sl2 = live ? fmaxf(p.scale_log2 * p.units[b * p.u_sb + w * p.u_sw + it.head * p.G + row % p.G], FLT_MIN) : p.scale_log2;
           sl2_2 = pack2(sl2, sl2);
         }
         // keys that this row sees (one that does not count: all, whatever comes of it), and the fewest of the warp's rows

@@ -1,6 +1,8 @@
 // Bindings of the paged key/value cache and of the verification of drafted tokens: checks of arguments, workspaces, launches.
+#include <algorithm>
 #include <atomic>
 #include <cmath>
+#include <limits>
 
 #include "paged_checks.h"
 
@@ -114,7 +116,7 @@ c10::optional<Tensor> paged_attention(const Tensor& q_, const Tensor& kc, const 
   p.part_ml = p.pre_o + plan.pre_slots * D;
   p.pre_ml = p.part_ml + plan.slots * 2;
   p.wait_ns = wait_ns.load();
-  p.scale_log2 = (float)(scale * 1.4426950408889634);
+  p.scale_log2 = std::max((float)(scale * 1.4426950408889634), std::numeric_limits<float>::min());        // kernels count less as 0
   count_launches(nxd::paged_attention(p, plan, (int)D, dt_code(q), stream()));
   return out;
 }

@@ -225,7 +225,7 @@ c10::optional<Tensor> int4_attention(const Tensor& q_, const Tensor& kc, const T
   p.v_sp = vc.stride(0) / 16; p.v_sr = vc.stride(1) / 16; p.v_sh = vc.stride(2) / 16;
   p.ks_sp = ks.stride(0) / row; p.ks_sr = ks.stride(1) / row; p.ks_sh = ks.stride(2) / row;
   p.vs_sp = vs.stride(0) / row; p.vs_sr = vs.stride(1) / row; p.vs_sh = vs.stride(2) / row;
-  p.scale_log2 = (float)(scale * 1.4426950408889634);
+  p.scale_log2 = std::max((float)(scale * 1.4426950408889634), std::numeric_limits<float>::min());        // kernels count less as 0
   if (p.cols == 0) return out.zero_();               // nobody sees a key
   const nxd::PagedPlan plan = nxd::int4_plan(p, dt_code(q));
   if (plan.tiles) {
