@@ -3,7 +3,7 @@ import pytest
 import torch
 
 from paged_cases import make as make16
-from paged_int4_cases import attention, bound, make
+from paged_int4_cases import attention, bound, make, values
 from paged_oracle import attention as oracle16
 
 from neuronx_distributed_b200 import ops
@@ -54,3 +54,92 @@ def test_scales_below_the_normal_numbers_over_16_bit_pages(dtype, W):
     got = ops.paged.attention(d["q"], d["k_cache"], d["v_cache"], d["table"], d["positions"], scale=1e-39)
     want, size = oracle16(d["q"], d["k_cache"], d["v_cache"], d["table"], d["positions"], 1e-39)
     assert bool(((got.double() - want).abs() <= torch.finfo(dtype).eps / 2 * (want.abs() + size) + 2.0 ** -13 * size + 1e-7).all())
+
+
+def key_roundings(d, scale=None):
+    """What unpacked keys, rounded to halves, do to the weights.  Each number is off by 2^-11 of itself at most, evenly spread and for itself, a score by six standard deviations of their
+    sum; by that a weight, and by that the sum of all."""
+    D = d["q"].shape[-1]
+    scale = D ** -0.5 if scale is None else scale
+    k, most = values(d["k_pages"]), 0.0
+    for b in range(d["q"].shape[0]):
+        table = d["table"][b].clone()
+        if d["shared_pages"] is not None:
+            table[:len(d["shared_pages"])] = d["shared_pages"]
+        keys = k[table[(table >= 0) & (table < k.shape[0])].long()].flatten(0, 1).nan_to_num(0.0)
+        q = d["q"][b].double().unflatten(1, (keys.shape[1], -1))
+        most = max([most, *(float(torch.einsum("wgd,nd->wgn", q[:, h] ** 2, keys[:, h] ** 2).amax()) for h in range(keys.shape[1]))])
+    return 2 * 6 * 2.0 ** -11 / 3 ** 0.5 * scale * most ** 0.5
+
+
+@pytest.mark.parametrize("layout", ["heads", "rows", "slice"])
+@pytest.mark.parametrize("D, B, W, H, Hkv, ps, positions, lens", [
+    (64, 2, 300, 8, 2, 64, [500, 30], [300, 111]),
+    (128, 2, 300, 8, 2, 64, [500, 30], [300, 111]),
+    (64, 3, 128, 6, 1, 16, [-1, 0, 700], None),
+    (128, 3, 100, 4, 4, 48, [64, -1, 511], [100, 50, 0]),
+    (64, 1, 257, 24, 8, 128, [1000], None),
+    (128, 4, 33, 32, 4, 32, [0, 1, 127, 900], [1, 33, 32, 7]),
+])
+def test_portions(D, B, W, H, Hkv, ps, positions, lens, layout):
+    """Heads of either size, in groups and alone, rows that are idle or count in part, pages laid out in every way."""
+    d = wide(make(B * W + H, "cuda", BF16, B, W, H, Hkv, D, ps, positions, lens, layout=layout), 40000)
+    got = attend(d, True)
+    check(d, got, more=key_roundings(d))
+    assert torch.equal(got, attend(d, True))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("k_factor, v_factor, v_add, scale", [(6, 1, 0, None), (0, 1, 0, None), (1, 1000, 0, None), (1, 1e-3, 0, None), (1, 1, 300, None), (1, 0, 0, None), (1, 4000, -20000, None),
+                                                              (1, 1, 0, 0.01), (1, 1, 0, 0.5), (30, 1, 0, 0.003)])
+def test_portions_of_other_sizes(D, k_factor, v_factor, v_add, scale):
+    d = wide(make(6, "cuda", BF16, 2, 70, 8, 2, D, 16, [400, 37], k_factor=k_factor, v_factor=v_factor, v_add=v_add), 20000)
+    check(d, attend(d, True, scale=scale), scale, key_roundings(d, scale))
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_shared_pages_and_holes_in_portions(D):
+    d = wide(make(10, "cuda", BF16, 3, 70, 8, 2, D, 16, [64, 90, 33], [70, 1, 0], shared=2), 20000)
+    check(d, attend(d, True), more=key_roundings(d))
+    d["table"][0, :2] = 1 << 30                              # not looked at
+    check(d, attend(d, True), more=key_roundings(d))
+    d["table"][1, 3] = -7
+    d["table"][0, 4:6] = -1
+    d["shared_pages"][1] = d["k_pages"].codes.shape[0]
+    check(d, attend(d, True), more=key_roundings(d))
+    assert not bool(attend({**d, "table": torch.full_like(d["table"], -1), "shared_pages": None}, True).any())
+
+
+@pytest.mark.parametrize("factor", [1e-30, 1e-8, 1e4, 1e6])
+def test_portions_of_other_queries(factor):
+    d = wide(make(8, "cuda", BF16, 2, 80, 8, 2, 128, 16, [100, 37]), 20000)
+    d["q"] = d["q"] * factor
+    check(d, attend(d, True, scale=0.1 / factor), 0.1 / factor, key_roundings(d, 0.1 / factor))
+
+
+def test_a_query_of_nan_is_its_own_in_portions():
+    d = wide(make(9, "cuda", BF16, 2, 80, 8, 2, 128, 16, [100, 37]), 20000)
+    clean = attend(d, True)
+    d["q"] = d["q"].clone()
+    d["q"][0, 11, 3] = float("nan")
+    got = attend(d, True)
+    assert bool(got[0, 11, 3].isnan().all())
+    got[0, 11, 3] = clean[0, 11, 3]
+    assert torch.equal(got, clean)
+
+
+@pytest.mark.parametrize("W, H, Hkv, cols", [(1, 8, 8, 2100), (3, 8, 8, 2100), (2, 8, 1, 2100), (5, 16, 8, 2100)])
+def test_many_pairs_behind_wide_tables(W, H, Hkv, cols):
+    """More pairs than blocks, dealt out because the table is wide: cut pairs are joined by the block in front of whose share they are cut."""
+    B = 300 // Hkv + 1
+    positions = [(37 * i) % 900 for i in range(B)]
+    positions[3], positions[7], positions[11] = -1, 33000, 0
+    d = make(W + H, "cuda", BF16, B, W, H, Hkv, 64, 16, [p if p < 5000 else 900 for p in positions])
+    d["table"] = torch.cat([d["table"], torch.full((B, cols - d["table"].shape[1]), -1, dtype=torch.int32, device="cuda")], 1)
+    long = d["table"][7, :50].repeat(cols // 50 + 1)[:cols]                    # a long sequence, whose pages stand in its table again and again
+    d["table"][7] = long
+    d["positions"][7] = 33000
+    n = _ext.launches()
+    got = attend(d)
+    assert _ext.launches() == n + 2
+    check(d, got)
