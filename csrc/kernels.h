@@ -285,7 +285,7 @@ struct Int4Attn : PagedAttn {        // k, v: codes, their strides in units of 1
 };
 PagedPlan int4_plan(Int4Attn& p, int dt);            // fills in p's cuts; tiles: the pages are better unpacked
 int int4_attention(const Int4Attn& p, const PagedPlan& plan, int D, int dt, cudaStream_t st);          // → launches
-// The pages of p's sequences as half-precision numbers that `to` reads: k, v [p.B * p.cols][Hkv][ps][D], a table of them, and queries of halves with their units
+// The pages of p's sequences as numbers in half precision, half their size: k, v [p.B * p.cols][Hkv][ps][D], a table of them, and queries of halves with their units
 void int4_unpack(const Int4Attn& p, void* k, void* v, int* table, int D, cudaStream_t st);
 void int4_queries(const void* q, void* out, float* units, int B, int W, int H, int D, long q_sb, long q_sw, long q_sh, cudaStream_t st);
 

@@ -161,7 +161,7 @@ NXD_DEVICE long begin_share(const PagedAttn& p, const Place& at, Walk& w) {
 // PAIR: a step of two row tiles and 128 keys takes 2.2 us: exponentials 1.05, products 1.05 (heads of 128 numbers), which overlap little.  2 x 1000 tokens (a
 // quarter padding) behind 6000 keys, 48 heads of 64 on 8: 158 us, 470 TFLOP/s.  Otherwise: two tiles of 64 keys in 1.7 us, 5 TB/s over the GPU; windows of 5
 // tokens of 8 sequences to 6000 keys, 64 heads on 8: 43 us, of which 7 are the start and 5 the launch that joins parts.
-// O: of what comes out, T or another 16-bit type.
+// O: of what comes out, T or another 16-bit type; then rows have units of their own and values are half their size (paged_int4.cu).
 template <typename T, int D, bool PAIR, int ROWS, bool SHARED, typename O>
 __global__ void __launch_bounds__(kRowsThreads, 1)
 paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant__ CUtensorMap tv, const PagedAttn p, int box) {
@@ -720,7 +720,8 @@ paged_tiles_kernel(const __grid_constant__ CUtensorMap tk, const __grid_constant
         if (!dry) {
           wait(bar_le + 8 * t, (uint32_t)((items & 1) ^ 1));
           ++items;
-          asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(sStat + t * 1024 + own * 8), "f"(m_ref * sl2), "f"(l) : "memory");
+          asm volatile("st.shared.v2.f32 [%0], {%1, %2};" ::"r"(sStat + t * 1024 + own * 8), "f"(m_ref * sl2),
+                       "f"(UNITS ? 0.5f * l : l) : "memory");          // such caches' values are halved
           mbar_arrive(bar_lf + 8 * t);
         }
       }

@@ -262,8 +262,8 @@ __global__ void __launch_bounds__(kGatherThreads) int4_gather_kernel(const Int4P
 
 // ----------------------------------------------------------------------------------------------- numbers for portions of prompts
 constexpr int kUnpackThreads = 128, kUnpackEach = 4;       // packets of a thread at a time
-// Pages of all sequences as halves, for the attention of many rows (paged_attention_sm100.cu), which the unpacked numbers serve many times: m + s c rounded
-// once.  Block (column of a sequence, head, keys or values), a thread 16 bytes at a time.  Keys that nobody sees are left as they are.  Bound by the start of its many
+// Pages of all sequences as halves, for the attention of many rows (paged_attention_sm100.cu), which the unpacked numbers serve many times: half of m + s c rounded
+// once, so that a group whose ends are halves has none that is infinite; the units of the queries and the sums of the weights have the other factor.  Block (column of a sequence, head, keys or values), a thread 16 bytes at a time.  Keys that nobody sees are left as they are.  Bound by the start of its many
 // small blocks: 2 sequences of 6000 keys, 8 heads of 64, 10 us, 25 MB written (16 numbers a thread: 12).
 template <int D>
 __global__ void __launch_bounds__(kUnpackThreads) int4_unpack_kernel(const Int4Attn p, __half* k, __half* v, int* table) {
@@ -296,19 +296,19 @@ __global__ void __launch_bounds__(kUnpackThreads) int4_unpack_kernel(const Int4A
     for (int y = 0; y < kUnpackEach; ++y) {
       const int i = i0 + y * kUnpackThreads;
       if (i >= items) break;
-      const __half2 s2 = __half2half2(s[y]), m2 = __half2half2(m[y]);
+      const __half2 half2x = __float2half2_rn(0.5f), s2 = __half2half2(s[y]), m2 = __hmul2(__half2half2(m[y]), half2x);
       uint32_t o[4];
 #pragma unroll
       for (int x = 0; x < 4; ++x) {
         const uint32_t two = word[y] >> (8 * x);           // numbers 2 x and 2 x + 1
-        o[x] = as_u32(__hfma2(__hsub2(as_half2((two & 0xfu) | (two & 0xf0u) << 12 | 0x64006400u), __float2half2_rn(1024.f)), s2, m2));
+        o[x] = as_u32(__hfma2(__hfma2(as_half2((two & 0xfu) | (two & 0xf0u) << 12 | 0x64006400u), half2x, __float2half2_rn(-512.f)), s2, m2));
       }
       *reinterpret_cast<uint4*>(to + (long)i * 8) = make_uint4(o[0], o[1], o[2], o[3]);
     }
   }
 }
 
-// Queries as halves: a row is multiplied by a power of two that brings its largest number to 2^14; the row's unit takes that back.  A thread has
+// Queries as halves: a row is multiplied by a power of two that brings its largest number to 2^14; the row's unit takes that back, and that keys are halved.  A thread has
 // eight numbers.  2 x 1000 tokens of 48 heads of 64: 6 us, 25 MB.
 template <int D>
 __global__ void __launch_bounds__(128) int4_queries_kernel(const __nv_bfloat16* q, __half* out, float* units, unsigned rows, unsigned W, unsigned H, long q_sb, long q_sw,
@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(128) int4_queries_kernel(const __nv_bfloat16* 
 #pragma unroll
   for (int k = 0; k < 4; ++k) o[k] = pack_half(x.f(2 * k) * up, x.f(2 * k + 1) * up);
   reinterpret_cast<uint4*>(out)[(size_t)r * C + c] = make_uint4(o[0], o[1], o[2], o[3]);
-  if (c == 0) units[r] = __uint_as_float((uint32_t)(e - 14) << 23);
+  if (c == 0) units[r] = __uint_as_float((uint32_t)(e - 13) << 23);
 }
 
 // ------------------------------------------------------------------------------------------------------- attention, up to eight rows

@@ -4,7 +4,8 @@ the codes (kernels: ``csrc/paged_int4.cu``).  What ``ops.paged`` does for 16-bit
 
 Format: 32 numbers ``x`` of a token's head, one after the other, are held as ``m + s c``: ``m`` is their least and ``s`` a fifteenth of what the largest
 is above ``m``, both rounded to half precision, and ``c`` is ``(x - m) / s`` rounded to the nearest of 0 … 15 (0 where ``s`` is 0 or not finite).  A number
-is off by ``s / 2`` at most, and by what the roundings of ``m`` and ``s`` do at the ends.  Numbers beyond half precision make their 32 infinite or NaN.
+is off by ``s / 2`` at most, and by what the roundings of ``m`` and ``s`` do at the ends.  A least number beyond half precision, or a range of 15 times that, makes its 32 infinite
+or NaN; a largest one that is does not by itself.
 
 Layout (:class:`Pages`): ``codes [pages, page_size, Hkv, D / 2]`` uint8, number ``2 i`` of a head in the low half of byte ``i``; ``steps [pages, page_size,
 Hkv, 2, D / 32]`` float16, first ``s``, then ``m``.  A page has a multiple of 16 tokens.  :func:`new_pages` lays a head's rows of a page beside one another.
@@ -172,7 +173,7 @@ def attention(q: torch.Tensor, k_pages: Pages, v_pages: Pages, page_table: torch
     of the numbers that the codes stand for, with its arguments.  ``page_table [B, n]`` int32 (entries outside the pool are holes, whose keys nobody
     sees), ``positions [B]`` of the rows' first new tokens (negative: an idle row), ``lens [B]`` new tokens that count.  ``shared_pages [n]`` int32 stand in
     place of the first ``n`` columns of every row's table; each row reads them for itself.  Keys and values that some token of a row sees have to be
-    finite, and so have queries.  The kernels take pools whose codes span less than 64 GB, and tables of less than 2^31 tokens.
+    131008 at most in magnitude (twice the largest half), queries finite and below 1e35.  The kernels take pools whose codes span less than 64 GB, and tables of less than 2^31 tokens.
 
     Sums and statistics are in 32 bits, codes and steps enter them as they are."""
     _no_gradient("attention in 4 bits", q)

@@ -143,3 +143,22 @@ def test_many_pairs_behind_wide_tables(W, H, Hkv, cols):
     got = attend(d)
     assert _ext.launches() == n + 2
     check(d, got)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("W, tokens, unpacked", [(1, 0, False), (6, 0, False), (70, 20000, True)])
+def test_numbers_next_to_and_beyond_the_largest_half(D, W, tokens, unpacked):
+    """Groups from 0 to the largest half, whose last code stands for more than that, and groups that reach beyond it: finite, and what they are, however many rows there are."""
+    d = wide(make(31, "cuda", BF16, 2, W, 8, 2, D, 16, [300, 37]), tokens)
+    for n in ("k_pages", "v_pages"):
+        steps = d[n].steps
+        s, m = steps[..., 0, :].float(), steps[..., 1, :].float()
+        far = torch.arange(s.shape[-1], device="cuda") % 2 == 1
+        # of 2.2 below and above: 0 to 65520, and 40000 to 75000 and more
+        steps[..., 0, :] = torch.where(s.isnan(), s, torch.where(far, s * 8000, 4368.0)).half()
+        steps[..., 1, :] = torch.where(m.isnan(), m, torch.where(far, m * 8000 + 56000, 0.0)).half()
+    most = float(values(d["v_pages"]).nan_to_num(0.0).max())
+    assert 70000 < most < 131008
+    got = attend(d, unpacked, scale=1e-5)
+    # scores are sums of up to 128 products whose magnitudes add up to 100 here: off by 128 * 2^-24 * 100 < 2^-10 of the weights at most
+    check(d, got, 1e-5, key_roundings(d, 1e-5) + 2.0 ** -10)
