@@ -197,7 +197,8 @@ class PagedKVCacheManager:
 class DevicePagedKVCacheManager(PagedKVCacheManager):
     """Pages handed out on the device, by ``ops.page_tables.assign``: :meth:`slots` gives the rows of a step what pages they are short of, from positions
     that the host does not look at, in captured and recorded programs as outside.  A pool that runs short, and positions without a page, are noted in ``lost``
-    and said by :meth:`check` (which the end of a sequence does not wait for).  Rows of a prompt get pages for the tokens that count."""
+    and said by :meth:`check`, which the end of a sequence does not wait for; whoever calls a model's steps in a loop of their own calls it behind the last one, at the end of
+    :meth:`reserved_ahead` it is called.  Rows of a prompt get pages for the tokens that count."""
 
     def __init__(self, *args, **kwargs):
         super().__init__(*args, **kwargs)
@@ -249,10 +250,15 @@ class DevicePagedKVCacheManager(PagedKVCacheManager):
 
     @contextmanager
     def reserved_ahead(self, rows: int, tokens: int) -> Iterator[None]:
-        """Rows get their pages when they need them, and nothing ahead."""
+        """Rows get their pages when they need them, and nothing ahead: what had no page is said at the end (:meth:`check`, which waits for the device; what was lost
+        before, at the beginning)."""
         if tokens > self.max_seq_len:
             raise ValueError(f"a sequence of {tokens} tokens is longer than max_seq_len {self.max_seq_len}")
+        if not self.in_program():
+            self.check()
         yield
+        if not self.in_program():
+            self.check()
 
     def release(self, row: int) -> None:
         self._assign(self.batch_size, self._row, lengths=torch.where(self._row == row, 0, -1))

@@ -292,7 +292,8 @@ class LlamaForInference(nn.Module):
     @torch.no_grad()
     def token_generation(self, input_ids: torch.Tensor, positions: torch.Tensor, kv_len: Optional[int] = None) -> torch.Tensor:
         """``input_ids`` [B, 1], ``positions`` [B] → next token ids [B].  Positions count the shared prefix of a paged cache; its rows get
-        pages for them (a captured program takes none: ``kv.reserve`` them before), and one at -1 is idle."""
+        pages for them (a captured program takes none: ``kv.reserve`` them before), and one at -1 is idle.  With ``device_tables`` a pool that runs short is said
+        by ``kv.check()``, not here, as with :meth:`speculation_forward` and :meth:`context_encoding`."""
         if self.paged:
             self._take_slots(positions, 1)
         try:
