@@ -283,7 +283,7 @@ struct Int4Attn : PagedAttn {        // k, v: codes, their strides in units of 1
   const void *ks, *vs;               // steps, strides in rows of them (D / 8 bytes), below 2^32 alike
   long ks_sp, ks_sr, ks_sh, vs_sp, vs_sr, vs_sh;
 };
-PagedPlan int4_plan(Int4Attn& p, int dt);            // fills in p's cuts; tiles: the pages are better unpacked
+PagedPlan int4_plan(Int4Attn& p, int D, int dt);     // fills in p's cuts; tiles: the pages are better unpacked
 int int4_attention(const Int4Attn& p, const PagedPlan& plan, int D, int dt, cudaStream_t st);          // → launches
 // The pages of p's sequences as numbers in half precision, half their size: k, v [p.B * p.cols][Hkv][ps][D], a table of them, and queries of halves with their units
 void int4_unpack(const Int4Attn& p, void* k, void* v, int* table, int D, cudaStream_t st);

@@ -772,7 +772,7 @@ int launch(const Int4Attn& p, const PagedPlan& plan, int dt, cudaStream_t st) {
 
 }  // namespace
 
-PagedPlan int4_plan(Int4Attn& p, int dt) {
+PagedPlan int4_plan(Int4Attn& p, int D, int dt) {
   PagedPlan plan{};
   const int sms = device_sm_count();
   const long rows = (long)p.W * p.G;
@@ -790,8 +790,8 @@ PagedPlan int4_plan(Int4Attn& p, int dt) {
   // takes 0.19 us for 1000 and 18 us in all (us, row tiles / unpacked: 8 sequences to 6000 keys, 8 heads, 64 rows 81 / 93, 96 rows 134 / 96; 2 to 3000, 8
   // heads, 128 rows 30 / 36, 256 rows 54 / 40; 1 to 1000, 40 heads, 200 rows 26 / 31; 2 x 1000 tokens to 6000, 48 heads of 64 on 8, 504 / 169).
   // Results in half precision would show that keys, values and weights are rounded to halves there (0.0004 against 64 bits, where rounding the result costs 0.00021; row tiles
-  // 0.00028), those in bf16 do not (0.0017 either way).
-  plan.tiles = dt == kBF16 && (23l * p.row_tiles - 38) * heads * cap > 3600000;
+  // 0.00028), those in bf16 do not (0.0017 either way).  A head whose table alone would take more than 1 GB of memory (2 million tokens of 128 numbers) is not unpacked.
+  plan.tiles = dt == kBF16 && cap <= (1l << 28) / D && (23l * p.row_tiles - 38) * heads * cap > 3600000;
   if (plan.tiles) return plan;
   plan.grid = each * sms;
   // A cluster per pair, as many blocks in it as the GPU takes at once, has neither a search for places nor a second launch, but the longest sequence lasts as long as

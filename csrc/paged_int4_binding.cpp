@@ -137,7 +137,7 @@ c10::optional<std::vector<Tensor>> int4_gather(const Tensor& kc, const Tensor& k
   return std::vector<Tensor>{k, v};
 }
 
-// Bytes of unpacked keys and values at a time: sequences, then key/value heads, in turns where there are more
+// Bytes of unpacked keys and values at a time: sequences, then key/value heads, in turns where there are more (one head of one sequence may take more, int4_plan)
 constexpr int64_t kUnpacked = 256ll << 20;
 
 // Many rows of bf16: their sequences' pages are unpacked to halves, which the attention on the tensor memory reads
@@ -227,7 +227,7 @@ c10::optional<Tensor> int4_attention(const Tensor& q_, const Tensor& kc, const T
   p.vs_sp = vs.stride(0) / row; p.vs_sr = vs.stride(1) / row; p.vs_sh = vs.stride(2) / row;
   p.scale_log2 = std::max((float)(scale * 1.4426950408889634), std::numeric_limits<float>::min());        // kernels count less as 0
   if (p.cols == 0) return out.zero_();               // nobody sees a key
-  const nxd::PagedPlan plan = nxd::int4_plan(p, dt_code(q));
+  const nxd::PagedPlan plan = nxd::int4_plan(p, (int)D, dt_code(q));
   if (plan.tiles) {
     attend_portion(p, q, D);
     return out;

@@ -162,3 +162,15 @@ def test_numbers_next_to_and_beyond_the_largest_half(D, W, tokens, unpacked):
     got = attend(d, unpacked, scale=1e-5)
     # scores are sums of up to 128 products whose magnitudes add up to 100 here: off by 128 * 2^-24 * 100 < 2^-10 of the weights at most
     check(d, got, 1e-5, key_roundings(d, 1e-5) + 2.0 ** -10)
+
+
+@pytest.mark.parametrize("tokens, unpacked", [(1 << 21, True), ((1 << 21) + 16, False), (1 << 28, False)])
+def test_portions_behind_tables_of_millions_of_tokens(tokens, unpacked):
+    """Unpacked heads take 1 GB at most, however wide the table is."""
+    d = wide(make(41, "cuda", BF16, 1, 60, 4, 1, 128, 16, [100]), tokens)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    got = attend(d, unpacked)
+    assert torch.cuda.max_memory_allocated() - before < 1.1 * 2 ** 30
+    check(d, got, more=key_roundings(d))
