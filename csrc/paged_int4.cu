@@ -354,8 +354,9 @@ template <int D, bool CLUSTER> constexpr int rows_smem = kQueries<D, 1> + (CLUST
 // most 2^15 (`room` below), so that they are halves of all their bits: 11 of each product's.  Where the output is in half precision too, weights
 // are two halves, the rounded one and what that left (22 bits).
 //
-// Bound by instructions: some 220 of a warp for 16 keys, 18 of them products of 8 cycles each, 1030 cycles an SM for 128 keys where memory would take 650 (16 sequences of 8192
-// keys, 8 heads: 37 us, 3.4 TB/s; copies alone take 26).
+// Bound by how few warps hide one another's latencies: some 220 instructions of a warp for 16 keys, 18 of them products of 8 cycles each, from four warps a scheduler (127
+// registers), which issue in 53 of 100 cycles and wait for fixed latencies most; the pipes of logic and of products are busy for 40 and 21 of 100.  1030 cycles an SM for 128
+// keys where memory would take 650 (16 sequences of 8192 keys, 8 heads: 37 us, 3.4 TB/s; copies alone take 26).
 template <typename T, int D, bool CLUSTER>
 __global__ void __launch_bounds__(kRowWarps * 32, 2) int4_rows_kernel(const Int4Attn p) {
   constexpr bool TWO = std::is_same<T, __half>::value;     // weights as two halves
@@ -790,7 +791,7 @@ PagedPlan int4_plan(Int4Attn& p, int D, int dt) {
   // takes 0.19 us for 1000 and 18 us in all (us, row tiles / unpacked: 8 sequences to 6000 keys, 8 heads, 64 rows 81 / 93, 96 rows 134 / 96; 2 to 3000, 8
   // heads, 128 rows 30 / 36, 256 rows 54 / 40; 1 to 1000, 40 heads, 200 rows 26 / 31; 2 x 1000 tokens to 6000, 48 heads of 64 on 8, 504 / 169).
   // Results in half precision would show that keys, values and weights are rounded to halves there (0.0004 against 64 bits, where rounding the result costs 0.00021; row tiles
-  // 0.00028), those in bf16 do not (0.0017 either way).  A head whose table alone would take more than 1 GB of memory (2 million tokens of 128 numbers) is not unpacked.
+  // 0.00028), those in bf16 hardly do (0.00169 and 0.00168, where rounding the result costs 0.00166; with keys of six times that size 0.00177 and 0.00167).  A head whose table alone would take more than 1 GB of memory (2 million tokens of 128 numbers) is not unpacked.
   plan.tiles = dt == kBF16 && cap <= (1l << 28) / D && (23l * p.row_tiles - 38) * heads * cap > 3600000;
   if (plan.tiles) return plan;
   plan.grid = each * sms;

@@ -68,7 +68,7 @@ def matmul_mxfp8_reference(a_q: torch.Tensor, a_scale: torch.Tensor, b_q: torch.
 
 
 def gemm_mx_eligible(x2d: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor, kind: str) -> bool:
-    if os.environ.get("NXD_GEMM_MX", "0") != "1":                 # opt-in until the kernel has run on hardware
+    if os.environ.get("NXD_GEMM_MX", "0") != "1":                 # opt-in: activations in 8 bits, and no timing yet
         return False
     return (x2d.is_cuda and kind in _MMA_FMT and x2d.shape[1] % 128 == 0 and scale.shape[0] % 8 == 0
             and weight.is_contiguous() and _ext.use_cuda(x2d, weight, scale) and hasattr(_ext.ext(), "gemm_mxfp8"))
@@ -141,7 +141,7 @@ def matmul_f4_reference(a_q, a_scale, b_q, b_scale, vec_size: int = 32, a_global
 
 
 def gemm_f4_eligible(M: int, N: int, K: int, *tensors: torch.Tensor) -> bool:
-    if os.environ.get("NXD_GEMM_F4", "0") != "1":                 # opt-in: W4A4 numerics, and the kernel has not run on hardware yet
+    if os.environ.get("NXD_GEMM_F4", "0") != "1":                 # opt-in: W4A4 numerics, and no timing yet
         return False
     return (K % 256 == 0 and N % 8 == 0 and all(t.is_cuda for t in tensors) and _ext.use_cuda(*tensors)
             and hasattr(_ext.ext(), "gemm_f4"))
@@ -161,7 +161,7 @@ def matmul_f4(a_q: torch.Tensor, a_scale: torch.Tensor, b_q: torch.Tensor, b_sca
 
 
 def gemv_eligible(x2d: torch.Tensor, weight: torch.Tensor, scale: torch.Tensor) -> bool:
-    if os.environ.get("NXD_GEMV_MX", "0") != "1":                 # opt-in until the kernel has run on hardware
+    if os.environ.get("NXD_GEMV_MX", "0") != "1":                 # opt-in: no timing yet
         return False
     return (x2d.is_cuda and x2d.dtype == torch.bfloat16 and x2d.dim() == 2 and 1 <= x2d.shape[0] <= 8 and x2d.shape[1] % 32 == 0
             and x2d.is_contiguous() and weight.is_contiguous() and scale.is_contiguous() and scale.dtype == torch.uint8

@@ -84,7 +84,7 @@ def moe_block_tkg_reference(x, gamma, router_w, router_bias, w_gu, w_dn, e0: int
 def kernel_eligible(x: torch.Tensor, router_w: torch.Tensor, w_gu: torch.Tensor, w_dn: torch.Tensor, top_k: int) -> bool:
     if not (_ext.use_cuda(x, router_w, w_gu, w_dn) and hasattr(_ext.ext(), "moe_block_tkg")):
         return False
-    if os.environ.get("NXD_MOE_TKG_KERNEL", "0") != "1":      # opt-in until the kernel has run on hardware (tests/test_zz_late_gpu.py)
+    if os.environ.get("NXD_MOE_TKG_KERNEL", "0") != "1":      # opt-in: no timing yet
         return False
     if not all(t.dtype == torch.bfloat16 and t.is_contiguous() for t in (x, router_w, w_gu, w_dn)):
         return False

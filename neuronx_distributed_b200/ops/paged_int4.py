@@ -103,7 +103,7 @@ def append(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, positions: torch.T
     the codes of ``k`` and ``v`` to the tokens' slots, in one launch.  ``cos`` / ``sin [positions, r / 2]`` fp32 (``ops.rope.rope_tables``): the first ``r``
     numbers of a head turn, number ``i`` with ``i + r / 2``, or with ``interleaved`` number ``2 i`` with ``2 i + 1``; the others stay.  Tokens without a
     slot, or that stand outside the rotation tables, come back as zeros and are not written.  ``lost [1]`` int32 becomes 1 where a token that has a slot
-    stands outside the tables (and stays as it is otherwise).  Two tokens with one slot leave numbers of either.
+    stands outside the tables (and stays as it is otherwise).  What a slot holds that two tokens of a call have is not defined.
 
     Codes are those of the rotated numbers before any rounding: next to a border they are found in 64 bits."""
     _no_gradient("append", q, k, v)
@@ -175,7 +175,10 @@ def attention(q: torch.Tensor, k_pages: Pages, v_pages: Pages, page_table: torch
     place of the first ``n`` columns of every row's table; each row reads them for itself.  Keys and values that some token of a row sees have to be
     131008 at most in magnitude (twice the largest half), queries finite and below 1e35.  The kernels take pools whose codes span less than 64 GB, and tables of less than 2^31 tokens.
 
-    Sums and statistics are in 32 bits, codes and steps enter them as they are."""
+    Scaled scores stay below 2^24 in magnitude.  Sums and statistics are in 32 bits.  Where a sequence has up to 8 query rows for a key/value head (tokens times heads of a
+    group), codes and steps enter as they are; weights, and their products with the steps of the values, are rounded to halves, to two halves each where the result is in half
+    precision.  With more rows values are rounded to halves before they meet such weights; and portions of prompts in bf16 read pages that were unpacked to halves before, keys as
+    well, and weights of one half: the error of a score is that of its keys.  The sizes of tables, not positions, say which kernel it is."""
     _no_gradient("attention in 4 bits", q)
     e = _ext._load() if _ext._PLAN_PROXY is None and _ext.use_cuda(q) else _kernels(q, "int4_attention_ok", q, *k_pages, *v_pages)
     if e is not None:
