@@ -765,7 +765,8 @@ def record(model: Callable, example_inputs: Sequence[torch.Tensor], input_names:
 def save_plans(path: str, plans: Dict[str, LaunchPlan], rank: int = 0, extra: Optional[Dict[str, Any]] = None,
                save_weights: bool = True) -> None:
     """``<path>/plans_rank<r>.json`` (all buckets) + ``<path>/constants_rank<r>.safetensors`` (one copy of every named
-    constant — buckets share them — and each bucket's anonymous captures under ``<key>::<name>``).  Derived constants
+    constant — buckets share them — and each bucket's anonymous captures under ``<key>::<name>``, one copy of what several
+    buckets captured: a key/value cache, page tables).  Derived constants
     (outputs of a layout transformer) are not stored: they are recomputed at load.  ``save_weights=False`` leaves out the
     ``state_dict`` entries that no bucket writes to (the checkpoint weights: supply them with ``set_weights`` after loading);
     non-persistent buffers and captured tables are always stored."""
@@ -774,6 +775,8 @@ def save_plans(path: str, plans: Dict[str, LaunchPlan], rank: int = 0, extra: Op
     os.makedirs(path, exist_ok=True)
     tensors: Dict[str, torch.Tensor] = {}
     state: Set[str] = set()
+    first: Dict[Tuple, str] = {}                                   # where a capture lies → its name, the first bucket's
+    shared: Dict[str, str] = {}                                    # other buckets' names of it
     for plan in plans.values():
         state.update(plan.state_names())
     for key, plan in plans.items():
@@ -787,13 +790,17 @@ def save_plans(path: str, plans: Dict[str, LaunchPlan], rank: int = 0, extra: Op
                 raise PlanError(f"bucket {key}: constant {c.name} has no tensor to save")
             name = c.name if c.named else f"{key}::{c.name}"
             t = plan.tensors[vid]
+            where = _Recorder._mem_key(t)
+            if not c.named and where[0] and first.setdefault(where, name) != name:
+                shared[name] = first[where]
+                continue
             if name in tensors and tensors[name].data_ptr() != t.data_ptr():
                 raise PlanError(f"two different tensors are named {name!r}")
             tensors[name] = t
     save_state_dict_safetensors({k: v.detach().contiguous() for k, v in tensors.items()},
                                 os.path.join(path, f"constants_rank{rank}.safetensors"))
     with open(os.path.join(path, f"plans_rank{rank}.json"), "w") as f:
-        json.dump({"plans": {k: p.to_json() for k, p in plans.items()}, "extra": extra or {}}, f)
+        json.dump({"plans": {k: p.to_json() for k, p in plans.items()}, "shared": shared, "extra": extra or {}}, f)
 
 
 def load_plans(path: str, rank: int = 0, device: Optional[torch.device] = None
@@ -805,16 +812,22 @@ def load_plans(path: str, rank: int = 0, device: Optional[torch.device] = None
     dev = device or (torch.device("cuda", torch.cuda.current_device()) if torch.cuda.is_available() else torch.device("cpu"))
     raw = load_state_dict_safetensors(os.path.join(path, f"constants_rank{rank}.safetensors"))
     plans = {k: LaunchPlan.from_json(p) for k, p in blob["plans"].items()}
+    shared: Dict[str, str] = blob.get("shared", {})
+
+    def stored(key: str, c: ConstInfo) -> str:
+        name = c.name if c.named else f"{key}::{c.name}"
+        return shared.get(name, name)
+
     host: Set[str] = set()                                         # constants that lived on the host in a device plan
     for key, plan in plans.items():
         for c in plan.constants.values():
             if c.device_type and c.device_type != plan.device_type:
-                host.add(c.name if c.named else f"{key}::{c.name}")
+                host.add(stored(key, c))
     tensors: Dict[str, torch.Tensor] = {name: (t if name in host else t.to(dev)) for name, t in raw.items()}
     for key, plan in plans.items():
         mine = {}
         for c in plan.constants.values():
-            n = c.name if c.named else f"{key}::{c.name}"
+            n = stored(key, c)
             if n in tensors:
                 mine[c.name] = tensors[n]
         plan.bind(mine, strict=False)
