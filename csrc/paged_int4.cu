@@ -263,8 +263,9 @@ __global__ void __launch_bounds__(kGatherThreads) int4_gather_kernel(const Int4P
 // ----------------------------------------------------------------------------------------------- numbers for portions of prompts
 constexpr int kUnpackThreads = 128, kUnpackEach = 4;       // packets of a thread at a time
 // Pages of all sequences as halves, for the attention of many rows (paged_attention_sm100.cu), which the unpacked numbers serve many times: half of m + s c rounded
-// once, so that a group whose ends are halves has none that is infinite; the units of the queries and the sums of the weights have the other factor.  Block (column of a sequence, head, keys or values), a thread 16 bytes at a time.  Keys that nobody sees are left as they are.  Bound by the start of its many
-// small blocks: 2 sequences of 6000 keys, 8 heads of 64, 10 us, 25 MB written (16 numbers a thread: 12).
+// once, so that a group whose ends are halves has none that is infinite; the units of the queries and the sums of the weights have the other factor.  Block (column of a
+// sequence, head, keys or values), a thread 16 bytes at a time.  Keys that nobody sees are left as they are.  Bound by the start of its many small blocks:
+// 2 sequences of 6000 keys, 8 heads of 64, 10 us, 25 MB written (16 numbers a thread: 12).
 template <int D>
 __global__ void __launch_bounds__(kUnpackThreads) int4_unpack_kernel(const Int4Attn p, __half* k, __half* v, int* table) {
   constexpr int C = D / 8;
@@ -791,7 +792,8 @@ PagedPlan int4_plan(Int4Attn& p, int D, int dt) {
   // takes 0.19 us for 1000 and 18 us in all (us, row tiles / unpacked: 8 sequences to 6000 keys, 8 heads, 64 rows 81 / 93, 96 rows 134 / 96; 2 to 3000, 8
   // heads, 128 rows 30 / 36, 256 rows 54 / 40; 1 to 1000, 40 heads, 200 rows 26 / 31; 2 x 1000 tokens to 6000, 48 heads of 64 on 8, 504 / 169).
   // Results in half precision would show that keys, values and weights are rounded to halves there (0.0004 against 64 bits, where rounding the result costs 0.00021; row tiles
-  // 0.00028), those in bf16 hardly do (0.00169 and 0.00168, where rounding the result costs 0.00166; with keys of six times that size 0.00177 and 0.00167).  A head whose table alone would take more than 1 GB of memory (2 million tokens of 128 numbers) is not unpacked.
+  // 0.00028), those in bf16 hardly do (0.00169 and 0.00168, where rounding the result costs 0.00166; with keys of six times that size 0.00177 and 0.00167).
+  // A head whose table alone would take more than 1 GB of memory (2 million tokens of 128 numbers) is not unpacked.
   plan.tiles = dt == kBF16 && cap <= (1l << 28) / D && (23l * p.row_tiles - 38) * heads * cap > 3600000;
   if (plan.tiles) return plan;
   plan.grid = each * sms;

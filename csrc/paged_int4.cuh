@@ -240,7 +240,8 @@ struct Ring {
 
 // A warp makes a row of queries ready: number d of a group at (d % 4) 8 + d / 4, so that four 8 x 8 matrices of a group are the operands of its two products; odd
 // numbers, which meet codes that lie one place up, a sixteenth.  The row is multiplied by a power of two that brings its largest number to 2^14; unit: what
-// brings scores back (codes are 2^-24 of themselves), not 0, which would make NaN of the -inf of what nobody sees.  sums: of the groups, 2^-5 of them, as two halves each, the rounded ones, then what that left.
+// brings scores back (codes are 2^-24 of themselves), not 0, which would make NaN of the -inf of what nobody sees.
+// sums: of the groups, 2^-5 of them, as two halves each, the rounded ones, then what that left.
 template <typename T, int D>
 NXD_DEVICE void ready_query(const T* row, bool live, uint32_t to, uint32_t sums, float* unit, float scale_log2, int lane) {
   constexpr int N = D / 32, NG = D / 32;                   // numbers of a lane, groups

@@ -174,3 +174,27 @@ def test_portions_behind_tables_of_millions_of_tokens(tokens, unpacked):
     got = attend(d, unpacked)
     assert torch.cuda.max_memory_allocated() - before < 1.1 * 2 ** 30
     check(d, got, more=key_roundings(d))
+
+
+def test_portions_captured_twice_on_another_stream():
+    """Two captured portions whose pages are unpacked, one in several turns, replayed after each other on a stream of their own, give what the calls give."""
+    a = wide(make(51, "cuda", BF16, 2, 70, 8, 2, 64, 16, [100, 50]), 20000)
+    b = wide(make(52, "cuda", BF16, 3, 48, 2, 1, 128, 128, [300, 17, 411]), 200000)
+    want = attend(a, True), attend(b, True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        graphs, outs = [], []
+        for d in (a, b):
+            attend(d)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph, stream=side):
+                outs.append(attend(d))
+            graphs.append(graph)
+        for _ in range(3):
+            for o in outs:
+                o.fill_(float("nan"))
+            for graph in graphs:
+                graph.replay()
+            assert all(torch.equal(o, w) for o, w in zip(outs, want))
+    torch.cuda.current_stream().wait_stream(side)
